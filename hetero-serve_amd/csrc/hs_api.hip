@@ -1,4 +1,5 @@
-// extern "C" entry points of libhsattn.so (declared in include/hsattn.h).
+// extern "C" entry points of libhsattn.so (declared in include/hsattn.h and
+// include/hsattn_ops.h).
 //
 // This layer validates arguments with the reference's error messages where it
 // has one, sizes grids and workspaces, and hands off to the kernel launchers.
@@ -9,6 +10,7 @@
 #include <string>
 #include <unordered_map>
 
+#include "../../include/hsattn_ops.h"
 #include "hs_kernels.h"
 #include "hs_private.h"
 
@@ -932,6 +934,166 @@ int hs_block_tables(const int32_t* packed, int B, int width, int32_t* out, void*
   if ((int64_t)B * width == 0) return HS_OK;
   if (!packed || !out) return fail(HS_EINVAL, "null pointer");
   return launch_block_tables(packed, B, width, out, static_cast<hipStream_t>(stream));
+}
+
+static int rotary(Rotary w, void* stream) {
+  if (w.n < 0 || w.H <= 0 || w.Hkv <= 0 || w.D <= 0 || w.axes <= 0 || w.pairs <= 0)
+    return fail(HS_EINVAL, "rotary sizes must be positive");
+  if (w.pairs > w.D / 2) return fail(HS_EINVAL, "more rotary pairs than head_dim / 2");
+  if (!valid_dtype(w.src_dtype) || !valid_dtype(w.out_dtype) || !valid_dtype(w.kv_dtype))
+    return fail(HS_EINVAL, "unsupported dtype code");
+  if (w.q_row < (int64_t)w.H * w.D || w.k_row < (int64_t)w.Hkv * w.D ||
+      w.v_row < (int64_t)w.Hkv * w.D)
+    return fail(HS_EINVAL, "source row stride is smaller than a row");
+  if (w.n == 0) return HS_OK;
+  if (!w.q || !w.k || !w.positions || !w.inv_freq || !w.q_out) return fail(HS_EINVAL, "null pointer");
+  return launch_rotary(w, static_cast<hipStream_t>(stream), current_cus());
+}
+
+int hs_rotary(const void* q, const void* k, int src_dtype, int64_t q_row_stride, int64_t k_row_stride,
+              const int32_t* positions, int axes, const float* inv_freq, const int32_t* pair_axis,
+              int pairs, int interleaved, int64_t n, int H, int Hkv, int D, void* q_out, void* k_out,
+              int out_dtype, void* stream) {
+  if (n > 0 && !k_out) return fail(HS_EINVAL, "null pointer");
+  Rotary w{};
+  w.q = q;
+  w.k = k;
+  w.src_dtype = src_dtype;
+  w.q_row = q_row_stride;
+  w.k_row = k_row_stride;
+  w.v_row = (int64_t)Hkv * D;
+  w.positions = positions;
+  w.axes = axes;
+  w.inv_freq = inv_freq;
+  w.pair_axis = pair_axis;
+  w.pairs = pairs;
+  w.interleaved = interleaved;
+  w.n = n;
+  w.H = H;
+  w.Hkv = Hkv;
+  w.D = D;
+  w.q_out = q_out;
+  w.k_out = k_out;
+  w.out_dtype = out_dtype;
+  w.kv_dtype = src_dtype;
+  return rotary(w, stream);
+}
+
+int hs_rotary_append(const void* q, const void* k, const void* v, int src_dtype,
+                     int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
+                     const int32_t* positions, int axes, const float* inv_freq,
+                     const int32_t* pair_axis, int pairs, int interleaved, int64_t n, int H, int Hkv,
+                     int D, void* q_out, void* k_out, int out_dtype, void* k_cache, void* v_cache,
+                     int kv_dtype, int NB, int BS, const int32_t* block_tables, int B, int MB,
+                     const int32_t* cache_positions, const int32_t* seq_ids, void* stream) {
+  if (NB <= 0 || BS <= 0 || B <= 0 || MB <= 0)
+    return fail(HS_EINVAL, "append sizes must be positive");
+  if (n > 0 && (!v || !k_cache || !v_cache || !block_tables || !cache_positions))
+    return fail(HS_EINVAL, "null pointer");
+  return rotary({q, k, v, src_dtype, q_row_stride, k_row_stride, v_row_stride, positions, axes, inv_freq,
+                 pair_axis, pairs, interleaved, n, H, Hkv, D, q_out, k_out, out_dtype, k_cache, v_cache,
+                 kv_dtype, NB, BS, block_tables, B, MB, cache_positions, seq_ids},
+                stream);
+}
+
+int hs_prompt_attention(const void* q, const void* k, const void* v, int dtype, int64_t q_row_stride,
+                        int64_t q_head_stride, int64_t k_row_stride, int64_t k_head_stride,
+                        int64_t v_row_stride, int64_t v_head_stride, const int32_t* cu_seqlens, int B,
+                        int64_t total, int max_seqlen, int H, int Hkv, int D, float scale, void* out,
+                        void* stream) {
+  if (!valid_dtype(dtype)) return fail(HS_EINVAL, "unknown dtype code " + std::to_string(dtype));
+  if (B < 0 || total < 0 || max_seqlen < 0 || H <= 0 || Hkv <= 0 || D <= 0)
+    return fail(HS_EINVAL, "sizes must be positive");
+  if (H % Hkv != 0) return fail(HS_EINVAL, "n_head must be divisible by n_kv_head");
+  if (!valid_row_head_dim(D))
+    return fail(HS_EUNSUPPORTED, "unsupported head_dim " + std::to_string(D));
+  if (total > 0x7fffffffLL) return fail(HS_EUNSUPPORTED, "too many rows: cu_seqlens is 32-bit");
+  if (H > 65535) return fail(HS_EUNSUPPORTED, "too many heads for one launch");
+  const int64_t sizes[6] = {q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride,
+                            v_head_stride};
+  const int64_t unit = dtype == HS_DTYPE_F32 ? 4 : 8;   // elements of 16 bytes
+  for (int64_t s : sizes) {
+    if (s < 0) return fail(HS_EINVAL, "strides must not be negative");
+    if (s % unit != 0) return fail(HS_EINVAL, "strides must be multiples of 16 bytes");
+    if (sat_mul(std::max(total, (int64_t)H), s, 4) >= INT64_MAX / 4)
+      return fail(HS_EUNSUPPORTED, "strides too large for 64-bit offsets");
+  }
+  if (B == 0 || total == 0 || max_seqlen == 0) return HS_OK;
+  if (!q || !k || !v || !cu_seqlens || !out) return fail(HS_EINVAL, "null tensor pointer");
+  for (const void* p : {q, k, v, (const void*)out})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return fail(HS_EINVAL, "tensors must be 16-byte aligned");
+  return launch_prompt({q, k, v, dtype, q_row_stride, q_head_stride, k_row_stride, k_head_stride,
+                        v_row_stride, v_head_stride, cu_seqlens, B, total, max_seqlen, H, Hkv, D, scale,
+                        out},
+                       static_cast<hipStream_t>(stream));
+}
+
+static int copy_blocks(void* pool, int L, int NB, int64_t page_bytes, const int64_t* src,
+                       const int64_t* dst, int n, bool host_ids, void* stream) {
+  if (n < 0 || L <= 0 || NB <= 0 || page_bytes <= 0)
+    return fail(HS_EINVAL, "page copy sizes must be positive");
+  if (n == 0) return HS_OK;
+  if (!pool || !src || !dst) return fail(HS_EINVAL, "null pointer");
+  const auto launch = host_ids ? launch_copy_blocks_host_ids : launch_copy_blocks;
+  return launch(pool, L, NB, page_bytes, src, dst, n, static_cast<hipStream_t>(stream));
+}
+
+int hs_kv_copy(void* pool, int L, int NB, int64_t page_bytes, const int64_t* src_ids,
+               const int64_t* dst_ids, int n, void* stream) {
+  return copy_blocks(pool, L, NB, page_bytes, src_ids, dst_ids, n, false, stream);
+}
+
+int hs_kv_copy_host_ids(void* pool, int L, int NB, int64_t page_bytes, const int64_t* host_src,
+                        const int64_t* host_dst, int n, void* stream) {
+  return copy_blocks(pool, L, NB, page_bytes, host_src, host_dst, n, true, stream);
+}
+
+int hs_kv_find_free(const int32_t* ref_counts, int NB, int32_t* out, int n, void* stream) {
+  if (n < 0 || NB <= 0) return fail(HS_EINVAL, "free block search sizes must be positive");
+  if (n == 0) return HS_OK;
+  if (!ref_counts || !out) return fail(HS_EINVAL, "null pointer");
+  return launch_find_free(ref_counts, NB, out, n, static_cast<hipStream_t>(stream));
+}
+
+int hs_kv_fork(void* pool, int L, int NB, int64_t page_bytes, int BS, int32_t* block_tables, int B,
+               int MB, int32_t* context_lens, int32_t* ref_counts, const int32_t* parents,
+               const int32_t* children, const int32_t* fresh, int n, int32_t* forked, void* stream) {
+  if (n < 0 || L <= 0 || NB <= 0 || page_bytes <= 0 || BS <= 0 || B <= 0 || MB <= 0)
+    return fail(HS_EINVAL, "fork sizes must be positive");
+  if (page_bytes % BS != 0) return fail(HS_EINVAL, "page_bytes must be a multiple of block_size");
+  if (n == 0) return HS_OK;
+  if (!pool || !block_tables || !context_lens || !ref_counts || !parents || !children || !fresh || !forked)
+    return fail(HS_EINVAL, "null pointer");
+  return launch_fork(pool, L, NB, page_bytes, BS, block_tables, B, MB, context_lens, ref_counts, parents,
+                     children, fresh, n, forked, static_cast<hipStream_t>(stream));
+}
+
+int hs_kv_free(int32_t* block_tables, int B, int MB, int32_t* context_lens, int32_t* ref_counts, int NB,
+               const int32_t* rows, int n, void* stream) {
+  if (n < 0 || NB <= 0 || B <= 0 || MB <= 0) return fail(HS_EINVAL, "free sizes must be positive");
+  if (n == 0) return HS_OK;
+  if (!block_tables || !context_lens || !ref_counts || !rows) return fail(HS_EINVAL, "null pointer");
+  return launch_free(block_tables, B, MB, context_lens, ref_counts, NB, rows, n,
+                     static_cast<hipStream_t>(stream));
+}
+
+size_t hs_kv_compact_workspace_bytes(int NB) {
+  return NB > 0 ? (size_t)compact_workspace_bytes(NB) : 0;
+}
+
+int hs_kv_compact(void* pool, int L, int NB, int64_t page_bytes, int32_t* block_tables, int B, int MB,
+                  int32_t* ref_counts, int32_t* moved_to, int32_t* live, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  if (L <= 0 || NB <= 0 || page_bytes <= 0 || B < 0 || MB < 0)
+    return fail(HS_EINVAL, "compaction sizes must be positive");
+  if (!pool || !ref_counts || !moved_to || !live || ((int64_t)B * MB > 0 && !block_tables))
+    return fail(HS_EINVAL, "null pointer");
+  const size_t need = hs_kv_compact_workspace_bytes(NB);
+  if (!workspace || workspace_bytes < need)
+    return fail(HS_EWORKSPACE, "compaction needs " + std::to_string(need) + " workspace bytes, got " +
+                                   std::to_string(workspace ? workspace_bytes : 0));
+  return launch_compact(pool, L, NB, page_bytes, block_tables, B, MB, ref_counts, moved_to, live, workspace,
+                        current_cus(), static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -188,6 +188,58 @@ int launch_prefill_mfma(const float* q, const int32_t* cu_q, int S, int max_rows
                         int MB, float scale, void* workspace, size_t workspace_bytes,
                         hipStream_t stream);
 
+// Rotary positions and the cache write (hs_rotary.hip); v null: no cache.
+// Strides in elements.
+struct Rotary {
+  const void *q, *k, *v;
+  int src_dtype;
+  int64_t q_row, k_row, v_row;
+  const int32_t* positions;
+  int axes;
+  const float* inv_freq;
+  const int32_t* pair_axis;
+  int pairs, interleaved;
+  int64_t n;
+  int H, Hkv, D;
+  void *q_out, *k_out;
+  int out_dtype;
+  void *k_cache, *v_cache;
+  int kv_dtype, NB, BS;
+  const int32_t* bt;
+  int B, MB;
+  const int32_t *cache_positions, *seq_ids;
+};
+int launch_rotary(const Rotary& w, hipStream_t stream, int cus);
+
+// Causal attention over packed prompts (hs_prompt.hip).  Strides in elements.
+struct Prompt {
+  const void *q, *k, *v;
+  int dtype;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const int32_t* cu;
+  int B;
+  int64_t T;
+  int max_len, H, Hkv, D;
+  float scale;
+  void* out;
+};
+int launch_prompt(const Prompt& w, hipStream_t stream);
+
+// Pages inside one pool [L, 2, NB, page] (hs_pages.hip).
+int launch_copy_blocks(void* pool, int L, int NB, int64_t page, const int64_t* src,
+                       const int64_t* dst, int n, hipStream_t stream);
+int launch_copy_blocks_host_ids(void* pool, int L, int NB, int64_t page, const int64_t* src,
+                                const int64_t* dst, int n, hipStream_t stream);
+int launch_find_free(const int32_t* refs, int NB, int32_t* out, int n, hipStream_t stream);
+int launch_fork(void* pool, int L, int NB, int64_t page, int BS, int32_t* bt, int B, int MB,
+                int32_t* ctx, int32_t* refs, const int32_t* parents, const int32_t* children,
+                const int32_t* fresh, int n, int32_t* forked, hipStream_t stream);
+int launch_free(int32_t* bt, int B, int MB, int32_t* ctx, int32_t* refs, int NB, const int32_t* rows,
+                int n, hipStream_t stream);
+int64_t compact_workspace_bytes(int NB);
+int launch_compact(void* pool, int L, int NB, int64_t page, int32_t* bt, int B, int MB, int32_t* refs,
+                   int32_t* moved_to, int32_t* live, void* workspace, int cus, hipStream_t stream);
+
 // Launch shape of the MFMA prefill (workgroup width, key-range parts) and the
 // workspace a split needs (0 without one).
 struct PrefillPlan {

@@ -42,6 +42,10 @@ int hs_kv_pack_host_ids(const void* pool, int L, int NB, int64_t page_bytes,
 int hs_kv_unpack_host_ids(void* pool, int L, int NB, int64_t page_bytes, const int64_t* host_ids,
                           int n, const void* in, void* stream);
 
+/* hs_kv_copy with at most HS_KV_HOST_IDS / 2 pairs of ids in host memory. */
+int hs_kv_copy_host_ids(void* pool, int L, int NB, int64_t page_bytes, const int64_t* host_src,
+                        const int64_t* host_dst, int n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

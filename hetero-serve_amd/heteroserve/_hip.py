@@ -81,6 +81,29 @@ _SIGNATURES = {
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
+# must match include/hsattn_ops.h
+_OPERATORS = {
+    "hs_rotary": (_c_int, [_c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_vp, _c_int, _c_vp, _c_vp, _c_int,
+                           _c_int, _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_int, _c_vp]),
+    "hs_rotary_append": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_int,
+                                  _c_vp, _c_vp, _c_int, _c_int, _c_i64, _c_int, _c_int, _c_int,
+                                  _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp,
+                                  _c_int, _c_int, _c_vp, _c_vp, _c_vp]),
+    "hs_prompt_attention": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int] + [_c_i64] * 6
+                            + [_c_vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_float,
+                               _c_vp, _c_vp]),
+    "hs_kv_copy": (_c_int, [_c_vp, _c_int, _c_int, _c_i64, _c_vp, _c_vp, _c_int, _c_vp]),
+    "hs_kv_find_free": (_c_int, [_c_vp, _c_int, _c_vp, _c_int, _c_vp]),
+    "hs_kv_fork": (_c_int, [_c_vp, _c_int, _c_int, _c_i64, _c_int, _c_vp, _c_int, _c_int, _c_vp,
+                            _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp]),
+    "hs_kv_free": (_c_int, [_c_vp, _c_int, _c_int, _c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_vp]),
+    "hs_kv_compact_workspace_bytes": (_c_size, [_c_int]),
+    "hs_kv_compact": (_c_int, [_c_vp, _c_int, _c_int, _c_i64, _c_vp, _c_int, _c_int, _c_vp, _c_vp,
+                               _c_vp, _c_vp, _c_size, _c_vp]),
+}
+
+OPERATOR_SYMBOLS = tuple(_OPERATORS)
+
 # entry points of this layer's own; must match csrc/hs_private.h
 _PRIVATE = {
     "hs_kv_pack_host_ids": (_c_int, [_c_vp, _c_int, _c_int, _c_i64, _c_vp, _c_int, _c_vp, _c_vp]),
@@ -88,6 +111,7 @@ _PRIVATE = {
     "hs_kv_scatter_layers": (_c_int, [_c_vp, _c_vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_i64,
                                       _c_vp, _c_i64, _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_i64,
                                       _c_vp]),
+    "hs_kv_copy_host_ids": (_c_int, [_c_vp, _c_int, _c_int, _c_i64, _c_vp, _c_vp, _c_int, _c_vp]),
 }
 
 
@@ -114,7 +138,7 @@ def open_library(path: Optional[Path] = None) -> ctypes.CDLL:
     got = bind("hs_abi_version", *_SIGNATURES["hs_abi_version"])()
     if got != ABI_VERSION:
         raise OSError(f"libhsattn ABI version {got}, expected {ABI_VERSION}")
-    for name, (res, args) in {**_SIGNATURES, **_PRIVATE}.items():
+    for name, (res, args) in {**_SIGNATURES, **_PRIVATE, **_OPERATORS}.items():
         bind(name, res, args)
     return lib
 
@@ -614,3 +638,234 @@ def block_tables(packed_dev, B: int, width: int, out) -> None:
     with _DeviceGuard(out.get_device()):
         check(L.hs_block_tables(packed_dev.data_ptr(), B, width, out.data_ptr(),
                                 _stream_at(out.get_device())))
+
+
+# ---------------------------------------------------------------------------
+# rotary positions, whole prompts, pages in place
+# ---------------------------------------------------------------------------
+
+
+def _rotary_head(q, k, positions, inv_freq, axes, interleaved):
+    """What both rotary calls pass first: (q, k, their row strides, the device index,
+    the arguments from positions to D, and the tensors those point to)."""
+    if q.dim() != 3 or k.dim() != 3:
+        raise RuntimeError("q must be [n, H, D] and k [n, Hkv, D]")
+    n, H, D = q.shape
+    Hkv = k.shape[1]
+    index = q.get_device()
+    if index < 0 or k.get_device() != index:
+        raise RuntimeError("q and k must be on CUDA, on the same device")
+    if k.shape[0] != n or k.shape[2] != D or k.dtype is not q.dtype:
+        raise RuntimeError("k must have the rows, the head_dim and the dtype of q")
+    pos = _int32_on(positions, q.device)
+    n_axes = 1 if pos.dim() <= 1 else pos.shape[0]
+    if pos.dim() > 2 or pos.numel() != n_axes * n:
+        raise RuntimeError(f"positions must be [axes, {n}] or [{n}], got {tuple(positions.shape)}")
+    freq = inv_freq
+    if freq.dtype is not torch.float32 or freq.get_device() != index or not freq.is_contiguous():
+        freq = freq.to(device=q.device, dtype=torch.float32).contiguous()
+    pairs = freq.numel()
+    if not 0 < pairs <= D // 2:
+        raise RuntimeError(f"inv_freq must have 1 to head_dim / 2 = {D // 2} entries, got {pairs}")
+    pa = None if axes is None else _int32_on(axes, q.device)
+    if pa is not None and pa.numel() != pairs:
+        raise RuntimeError(f"{pa.numel()} axes for {pairs} rotary pairs")
+    q, q_row = _rows(q, H, D)
+    k, k_row = _rows(k, Hkv, D)
+    middle = (pos.data_ptr(), n_axes, freq.data_ptr(), None if pa is None else pa.data_ptr(), pairs,
+              int(bool(interleaved)), n, H, Hkv, D)
+    return q, k, (q_row, k_row), index, middle, (pos, freq, pa)
+
+
+def rotary(q, k, positions, inv_freq, axes, interleaved, out_dtype):
+    """(q, k) turned by hs_rotary, contiguous, of out_dtype (q's when None)."""
+    L = lib("rotary HIP kernel")
+    out_dtype = out_dtype or q.dtype
+    q, k, strides, index, middle, keep = _rotary_head(q, k, positions, inv_freq, axes, interleaved)
+    q_out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=out_dtype, device=q.device)
+    with _DeviceGuard(index):
+        check(L.hs_rotary(q.data_ptr(), k.data_ptr(), dtype_code(q.dtype), *strides, *middle,
+                          q_out.data_ptr(), k_out.data_ptr(), dtype_code(out_dtype),
+                          _stream_at(index)))
+    return q_out, k_out
+
+
+def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, block_tables, cache_positions,
+                  seq_ids, axes, interleaved, out_dtype, keep_k):
+    """(q, k or None) turned by hs_rotary_append, which writes k and v into the caches."""
+    L = lib("rotary HIP kernel")
+    out_dtype = out_dtype or q.dtype
+    q, k, strides, index, middle, keep = _rotary_head(q, k, positions, inv_freq, axes, interleaved)
+    n, Hkv, D = k.shape
+    (NB, BS, cache_heads, cache_dim), cache_index = _check_write(k_cache, v_cache, k, v)
+    if cache_index != index:
+        raise RuntimeError("kv cache and new rows must be on the same device")
+    if (cache_heads, cache_dim) != (Hkv, D):
+        raise RuntimeError(f"K/V rows must be [n, {cache_heads}, {cache_dim}], got {tuple(k.shape)}")
+    v, v_row = _rows(v, Hkv, D)
+    if v.shape[0] != n or v.dtype is not k.dtype:
+        raise RuntimeError("k and v rows must have the same count and dtype")
+    bt = _int32_on(block_tables, q.device)
+    at = _int32_on(cache_positions, q.device)
+    sid = None if seq_ids is None else _int32_on(seq_ids, q.device)
+    if bt.dim() != 2:
+        raise RuntimeError("block_tables must be [B, max_blocks]")
+    if at.numel() != n:
+        raise RuntimeError(f"{at.numel()} positions for {n} rows")
+    if sid is not None and sid.numel() != n:
+        raise RuntimeError(f"{sid.numel()} sequence ids for {n} rows")
+    if sid is None and n > bt.shape[0]:
+        raise RuntimeError("without seq_ids, row i uses table row i: more rows than tables")
+    q_out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=out_dtype, device=q.device) if keep_k else None
+    with _DeviceGuard(index):
+        check(L.hs_rotary_append(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype_code(q.dtype), *strides, v_row, *middle,
+            q_out.data_ptr(), None if k_out is None else k_out.data_ptr(), dtype_code(out_dtype),
+            k_cache.data_ptr(), v_cache.data_ptr(), dtype_code(k_cache.dtype), NB, BS, bt.data_ptr(),
+            bt.shape[0], bt.shape[1], at.data_ptr(), None if sid is None else sid.data_ptr(),
+            _stream_at(index)))
+    return q_out, k_out
+
+
+def _heads(x, name: str):
+    """(tensor, row stride, head stride): rows and heads any multiple of 16 bytes
+    apart, D elements of a head contiguous; a contiguous copy of anything else."""
+    unit = 16 // x.element_size()
+
+    def fits(t):
+        return t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
+            t.shape[i] == 1 or (t.stride(i) >= 0 and t.stride(i) % unit == 0) for i in (0, 1))
+
+    if not fits(x):
+        x = x.contiguous()
+    # a dim of one index has no stride of its own
+    return x, x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0
+
+
+def prompt_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float, out=None):
+    """out[T, H, D] of q's dtype via hs_prompt_attention."""
+    L = lib("prompt attention kernel")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise RuntimeError("q must be [total_tokens, H, D], k and v [total_tokens, Hkv, D]")
+    index = q.get_device()
+    if index < 0 or k.get_device() != index or v.get_device() != index:
+        raise RuntimeError("q, k and v must be on CUDA, on the same device")
+    T, H, D = q.shape
+    Hkv = k.shape[1]
+    if k.shape != (T, Hkv, D) or v.shape != k.shape:
+        raise RuntimeError(f"k and v must be [{T}, Hkv, {D}], got {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise RuntimeError("q, k and v must have the same dtype")
+    cu = _int32_on(cu_seqlens, q.device)
+    if cu.dim() != 1 or cu.numel() < 1:
+        raise RuntimeError("cu_seqlens must be [B + 1]")
+    if out is None:
+        out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
+    elif (out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != index
+          or not out.is_contiguous() or out.data_ptr() % 16):
+        raise RuntimeError("out must be a contiguous, 16-byte aligned tensor like q")
+    q, qr, qh = _heads(q, "q")
+    k, kr, kh = _heads(k, "k")
+    v, vr, vh = _heads(v, "v")
+    with _DeviceGuard(index):
+        check(L.hs_prompt_attention(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype_code(q.dtype), qr, qh, kr, kh, vr, vh,
+            cu.data_ptr(), cu.numel() - 1, T, int(max_seqlen), H, Hkv, D, float(scale),
+            out.data_ptr(), _stream_at(index)))
+    return out
+
+
+def _check_state(name: str, t, dim: int, index: int):
+    """A tensor that a page operation changes in place."""
+    if t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of {dim} dim(s): it is "
+                           "written in place")
+    if t.get_device() != index or index < 0:
+        raise RuntimeError(f"{name} must be on CUDA, on the device of the others")
+
+
+def kv_copy(pool, src_dev, dst_dev) -> None:
+    """pool[:, :, dst] = pool[:, :, src]  (bitwise, device int64 ids)."""
+    L = lib("KV copy HIP kernel")
+    index = pool.get_device()
+    with _DeviceGuard(index):
+        check(L.hs_kv_copy(pool.data_ptr(), *_pages(pool), src_dev.data_ptr(), dst_dev.data_ptr(),
+                           src_dev.numel(), _stream_at(index)))
+
+
+def kv_copy_host_ids(pool, src, dst) -> None:
+    """kv_copy with at most HOST_IDS / 2 pairs in contiguous int64 numpy arrays."""
+    L = lib("KV copy HIP kernel")
+    index = pool.get_device()
+    with _DeviceGuard(index):
+        check(L.hs_kv_copy_host_ids(pool.data_ptr(), *_pages(pool), src.ctypes.data, dst.ctypes.data,
+                                    src.size, _stream_at(index)))
+
+
+def kv_find_free(ref_counts, n: int):
+    """int32 [n]: the lowest free blocks, -1 past the last."""
+    L = lib("free block search HIP kernel")
+    index = ref_counts.get_device()
+    _check_state("ref_counts", ref_counts, 1, index)
+    out = torch.empty(n, dtype=torch.int32, device=ref_counts.device)
+    with _DeviceGuard(index):
+        check(L.hs_kv_find_free(ref_counts.data_ptr(), ref_counts.numel(), out.data_ptr(), n,
+                                _stream_at(index)))
+    return out
+
+
+def kv_fork(pool, block_tables, context_lens, ref_counts, parents, children, fresh):
+    """int32 [n], 1 where row children[i] became a fork of row parents[i]."""
+    L = lib("KV fork HIP kernel")
+    index = pool.get_device()
+    _check_state("block_tables", block_tables, 2, index)
+    _check_state("context_lens", context_lens, 1, index)
+    _check_state("ref_counts", ref_counts, 1, index)
+    B, MB = block_tables.shape
+    n = parents.numel()
+    if context_lens.numel() != B or ref_counts.numel() != pool.shape[2]:
+        raise RuntimeError("context_lens must have one entry per table row, ref_counts one per block")
+    if children.numel() != n or fresh.numel() != n:
+        raise RuntimeError("parents, children and fresh must have the same length")
+    forked = torch.empty(n, dtype=torch.int32, device=pool.device)
+    with _DeviceGuard(index):
+        check(L.hs_kv_fork(pool.data_ptr(), *_pages(pool), pool.shape[3], block_tables.data_ptr(), B, MB,
+                           context_lens.data_ptr(), ref_counts.data_ptr(), parents.data_ptr(),
+                           children.data_ptr(), fresh.data_ptr(), n, forked.data_ptr(),
+                           _stream_at(index)))
+    return forked
+
+
+def kv_free(block_tables, context_lens, ref_counts, rows) -> None:
+    L = lib("KV free HIP kernel")
+    index = ref_counts.get_device()
+    _check_state("block_tables", block_tables, 2, index)
+    _check_state("context_lens", context_lens, 1, index)
+    _check_state("ref_counts", ref_counts, 1, index)
+    B, MB = block_tables.shape
+    if context_lens.numel() != B:
+        raise RuntimeError("context_lens must have one entry per table row")
+    with _DeviceGuard(index):
+        check(L.hs_kv_free(block_tables.data_ptr(), B, MB, context_lens.data_ptr(), ref_counts.data_ptr(),
+                           ref_counts.numel(), rows.data_ptr(), rows.numel(), _stream_at(index)))
+
+
+def kv_compact(pool, block_tables, ref_counts):
+    """(moved_to int32 [NB], live int32 [1])."""
+    L = lib("KV compaction HIP kernel")
+    index = pool.get_device()
+    _check_state("block_tables", block_tables, 2, index)
+    _check_state("ref_counts", ref_counts, 1, index)
+    NB = pool.shape[2]
+    if ref_counts.numel() != NB:
+        raise RuntimeError("ref_counts must have one entry per block")
+    need = L.hs_kv_compact_workspace_bytes(NB)
+    made = torch.empty(NB + 1 + (need + 3) // 4, dtype=torch.int32, device=pool.device)
+    moved_to, live, ws = made[:NB], made[NB:NB + 1], made[NB + 1:]
+    with _DeviceGuard(index):
+        check(L.hs_kv_compact(pool.data_ptr(), *_pages(pool), block_tables.data_ptr(),
+                              *block_tables.shape, ref_counts.data_ptr(), moved_to.data_ptr(),
+                              live.data_ptr(), ws.data_ptr(), need, _stream_at(index)))
+    return moved_to, live

@@ -311,5 +311,10 @@ class HipKVMixin:
     def write_kv(self, block_ids, start_pos, k, v) -> None:
         write_kv(self.pool, block_ids, start_pos, k, v)
 
+    def copy_blocks(self, src_ids, dst_ids) -> None:
+        from .pages import copy_blocks
+
+        copy_blocks(self.pool, src_ids, dst_ids)
+
     def block_table_tensor(self, tables, pad_to=None):
         return block_table_tensor(tables, pad_to, self.device)

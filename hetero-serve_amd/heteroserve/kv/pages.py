@@ -1,0 +1,133 @@
+"""Pages of the paged cache while its sequences live: copies, forks, frees, compaction.
+
+    copy_blocks        pool[:, :, dst] = pool[:, :, src], all layers, one launch
+    find_free_blocks   the lowest blocks that nobody holds
+    fork_blocks        children share their parent's full blocks and get a copy of
+                       the last, unfinished one (parallel samples, beams)
+    free_blocks        finished sequences give their blocks back
+    compact_blocks     live blocks move into the lowest ids
+
+The reference keeps counts and tables on the host (heteroserve/kv/blocks.py:62)
+and copies pages between pools only.  Here the state is three int32 tensors that
+stay on the device beside the pool, and every call runs in stream order without a
+copy to the host, so a step that forks or frees can be captured in a graph:
+
+    block_tables   [B, MB], -1 padded, as the attention reads them
+    context_lens   [B]
+    ref_counts     [num_blocks]: how many table rows (or other holders, such as a
+                   prefix cache) keep a block; a block is free at 0
+
+Row indexes and block ids come as device tensors, which are not read back (one
+that names no row or block is skipped), or from the host, where they follow torch
+indexing and mistakes raise before anything is launched.
+"""
+
+from __future__ import annotations
+
+from .. import _hip
+from .pack import _check_pool, _ids_array, _ids_tensor, _normalise_ids
+
+
+def copy_blocks(pool, src_ids, dst_ids) -> None:
+    """pool[:, :, dst_ids[i]] = pool[:, :, src_ids[i]], bit for bit.  Ids follow
+    torch indexing; a destination may not repeat nor be a source."""
+    import numpy as np
+
+    _hip.lib("KV copy HIP kernel")
+    _check_pool(pool)
+    src = _normalise_ids(src_ids, pool.shape[2])
+    dst = _normalise_ids(dst_ids, pool.shape[2])
+    n = len(src)
+    if len(dst) != n:
+        raise RuntimeError(f"{n} source blocks for {len(dst)} destinations")
+    if n == 0:
+        return
+    if len(np.unique(dst)) != n:
+        raise RuntimeError("a destination block repeats")
+    if np.isin(dst, src).any():
+        raise RuntimeError("a block is both source and destination")
+    if 2 * n <= _hip.HOST_IDS:
+        _hip.kv_copy_host_ids(pool, _ids_array(src), _ids_array(dst))
+    else:
+        both = _ids_tensor(np.concatenate([src, dst]), pool.device)
+        _hip.kv_copy(pool, both[:n], both[n:])
+
+
+def find_free_blocks(ref_counts, n: int):
+    """int32 [n] on the device: the lowest blocks with a count of 0, ascending, -1
+    past the last one.  Nothing is reserved until a count goes up."""
+    n = int(n)
+    if n < 0:
+        raise RuntimeError("n must not be negative")
+    return _hip.kv_find_free(ref_counts, n)
+
+
+def _indexes(values, size: int, what: str, device):
+    """(int32 device tensor, host array or None): host values are checked and
+    wrapped as torch indexing does."""
+    import numpy as np
+    import torch
+
+    if torch.is_tensor(values) and values.is_cuda:
+        return _hip._int32_on(values.reshape(-1), device), None
+    host = np.asarray(values.tolist() if torch.is_tensor(values) else values).reshape(-1)
+    if host.size and host.dtype.kind not in "iu":
+        raise RuntimeError(f"{what} must be integers, got {host.dtype}")
+    host = host.astype(np.int64)
+    bad = (host < -size) | (host >= size)
+    if bad.any():
+        i = int(host[int(np.argmax(bad))])
+        raise IndexError(f"{what} index {i} is out of bounds for size {size}")
+    host = np.where(host < 0, host + size, host)
+    return torch.from_numpy(host.astype(np.int32)).to(device), host
+
+
+def fork_blocks(pool, block_tables, context_lens, ref_counts, parents, children, fresh):
+    """Row children[i] becomes a fork of row parents[i]: the full blocks are shared
+    (counts up by 1), the tokens of the last, unfinished block are copied to block
+    fresh[i] (count up by 1; unused where the parent's context ends with a
+    block).  Changes block_tables, context_lens and ref_counts in place and returns
+    int32 [n]: 1, or 0 where the fork could not be made (fresh[i] is -1 because
+    the pool is full, or the parent's table has no last block), which leaves the
+    child empty.
+
+    A parent may have several children.  Children must be rows that hold no
+    blocks, and must not repeat nor be parents; fresh blocks must not repeat."""
+    import numpy as np
+
+    _hip.lib("KV fork HIP kernel")
+    _check_pool(pool)
+    if block_tables.dim() != 2:
+        raise RuntimeError("block_tables must be [B, max_blocks]")
+    B, dev = block_tables.shape[0], pool.device
+    parents, host_p = _indexes(parents, B, "parent row", dev)
+    children, host_c = _indexes(children, B, "child row", dev)
+    fresh, host_f = _indexes(fresh, pool.shape[2], "fresh block", dev)
+    if host_c is not None and len(np.unique(host_c)) != len(host_c):
+        raise RuntimeError("a child row repeats")
+    if host_f is not None and len(np.unique(host_f)) != len(host_f):
+        raise RuntimeError("a fresh block repeats")
+    if host_c is not None and host_p is not None and np.isin(host_c, host_p).any():
+        raise RuntimeError("a row is both parent and child")
+    return _hip.kv_fork(pool, block_tables, context_lens, ref_counts, parents, children, fresh)
+
+
+def free_blocks(block_tables, context_lens, ref_counts, rows) -> None:
+    """Table rows `rows` give up their blocks: counts go down by 1 (never below 0),
+    the rows become -1 and their context lengths 0, all in place.  A row that
+    repeats is freed once."""
+    _hip.lib("KV free HIP kernel")
+    if block_tables.dim() != 2:
+        raise RuntimeError("block_tables must be [B, max_blocks]")
+    rows, _ = _indexes(rows, block_tables.shape[0], "row", ref_counts.device)
+    _hip.kv_free(block_tables, context_lens, ref_counts, rows)
+
+
+def compact_blocks(pool, block_tables, ref_counts):
+    """The live blocks move into blocks [0, live), the highest into the lowest hole
+    and so on, for all layers; block_tables and ref_counts follow in place.  Returns
+    (moved_to int32 [num_blocks], live int32 [1]): every live block's new id, -1
+    for the free ones, for whoever else keeps ids (a prefix cache's hashes)."""
+    _hip.lib("KV compaction HIP kernel")
+    _check_pool(pool)
+    return _hip.kv_compact(pool, block_tables, ref_counts)

@@ -9,6 +9,9 @@
  * pybind types: tensors cross as plain device pointers plus sizes, and the
  * stream crosses as an opaque hipStream_t handle (void*).
  *
+ * Entry points without a counterpart on that path (rotary positions, whole
+ * prompts, pages in place) are in hsattn_ops.h, under the same conventions.
+ *
  * Conventions shared by every entry point
  *   - All pointers are device pointers on the current HIP device, except
  *     where a comment says otherwise.
