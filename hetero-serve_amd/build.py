@@ -69,6 +69,7 @@ PER_FILE_FLAGS = {
     "hs_decode_gqa.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "hs_prefill_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "hs_decode_splitmm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+    "hs_prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
 }
 
 

@@ -1007,7 +1007,8 @@ int hs_prompt_attention(const void* q, const void* k, const void* v, int dtype, 
   if (H % Hkv != 0) return fail(HS_EINVAL, "n_head must be divisible by n_kv_head");
   if (!valid_row_head_dim(D))
     return fail(HS_EUNSUPPORTED, "unsupported head_dim " + std::to_string(D));
-  if (total > 0x7fffffffLL) return fail(HS_EUNSUPPORTED, "too many rows: cu_seqlens is 32-bit");
+  if (total > 0x7fffffffLL || std::min(total, (int64_t)max_seqlen) > (1 << 30))
+    return fail(HS_EUNSUPPORTED, "too many rows for 32-bit offsets");
   if (H > 65535) return fail(HS_EUNSUPPORTED, "too many heads for one launch");
   const int64_t sizes[6] = {q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride,
                             v_head_stride};
@@ -1023,8 +1024,8 @@ int hs_prompt_attention(const void* q, const void* k, const void* v, int dtype, 
   for (const void* p : {q, k, v, (const void*)out})
     if (reinterpret_cast<uintptr_t>(p) & 15) return fail(HS_EINVAL, "tensors must be 16-byte aligned");
   return launch_prompt({q, k, v, dtype, q_row_stride, q_head_stride, k_row_stride, k_head_stride,
-                        v_row_stride, v_head_stride, cu_seqlens, B, total, max_seqlen, H, Hkv, D, scale,
-                        out},
+                        v_row_stride, v_head_stride, cu_seqlens, B, total,
+                        (int)std::min(total, (int64_t)max_seqlen), H, Hkv, D, scale, out},
                        static_cast<hipStream_t>(stream));
 }
 
