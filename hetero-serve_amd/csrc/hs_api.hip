@@ -1016,8 +1016,7 @@ int hs_prompt_attention(const void* q, const void* k, const void* v, int dtype, 
   for (int64_t s : sizes) {
     if (s < 0) return fail(HS_EINVAL, "strides must not be negative");
     if (s % unit != 0) return fail(HS_EINVAL, "strides must be multiples of 16 bytes");
-    if (sat_mul(std::max(total, (int64_t)H), s, 4) >= INT64_MAX / 4)
-      return fail(HS_EUNSUPPORTED, "strides too large for 64-bit offsets");
+    if (s > (1 << 22)) return fail(HS_EUNSUPPORTED, "strides too large: at most 2^22 elements");
   }
   if (B == 0 || total == 0 || max_seqlen == 0) return HS_OK;
   if (!q || !k || !v || !cu_seqlens || !out) return fail(HS_EINVAL, "null tensor pointer");
@@ -1026,7 +1025,7 @@ int hs_prompt_attention(const void* q, const void* k, const void* v, int dtype, 
   return launch_prompt({q, k, v, dtype, q_row_stride, q_head_stride, k_row_stride, k_head_stride,
                         v_row_stride, v_head_stride, cu_seqlens, B, total,
                         (int)std::min(total, (int64_t)max_seqlen), H, Hkv, D, scale, out},
-                       static_cast<hipStream_t>(stream));
+                       current_cus(), static_cast<hipStream_t>(stream));
 }
 
 static int copy_blocks(void* pool, int L, int NB, int64_t page_bytes, const int64_t* src,

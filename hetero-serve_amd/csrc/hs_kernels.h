@@ -223,7 +223,7 @@ struct Prompt {
   float scale;
   void* out;
 };
-int launch_prompt(const Prompt& w, hipStream_t stream);
+int launch_prompt(const Prompt& w, int cus, hipStream_t stream);
 
 // Pages inside one pool [L, 2, NB, page] (hs_pages.hip).
 int launch_copy_blocks(void* pool, int L, int NB, int64_t page, const int64_t* src,

@@ -3,6 +3,35 @@
 //
 //   out[i, h] = sum_{j <= i} p_ij v[j, h'],  p_i = softmax_j(scale q[i, h] . k[j, h'])
 // over the rows j <= i of row i's own sequence, h' = h / (H / Hkv).
+//
+// A workgroup of 4 waves takes 128 query rows of one (sequence, head), 32 a wave, and
+// walks the keys once with a running maximum and sum.  K and V tiles go from global
+// memory straight to LDS (two of each; the next ones are on their way while one is
+// used), swizzled by permuting the addresses that the lanes load from, since the LDS
+// side of such a load is linear.  S^T = K Q^T and O^T = V^T P^T: a lane holds one
+// query's scores, so its maximum and sum need one exchange of the two lane halves,
+// and the probabilities are the second product's operand where they stand.  Rows
+// are 128 and not 256 a workgroup because two workgroups then share a CU: one's
+// set-up and barriers pass beside the other's products.  us at 256 / 128 rows, bf16:
+// one prompt of 2048 tokens, 32 / 8 heads, D 128 55 / 49, 32 of 128 tokens 50 / 27, one
+// of 8192 493 / 496.
+//
+// What bounds it: the matrix cores' power.  One prompt of 8192 tokens, 32 / 8 heads,
+// D 128, bf16: 496 us, 1108 TFLOP/s of useful products at 1.9 GHz (2.5 PFLOP/s
+// nominal at 2.4).  The same loop without softmax and without LDS reads reached
+// 1534, without softmax 1347, without barriers and loads 1129.
+//
+// Numerics.  16-bit inputs are multiplied in their own type, the probabilities
+// rounded to it (relative to a maximum that is at most 2^8 too low, so none
+// overflows), and the sum adds the rounded ones, so that the rounding cancels where
+// one key dominates; scores, maxima, sums and O are fp32.  fp32 inputs use the fp32
+// matrix cores.  Scores are scaled in fp32 behind the product, not in the query's type
+// before it.
+//
+// Masked keys.  A score that a row does not see is -inf and its probability 0, but 0
+// times an infinite or NaN value is NaN in a product.  A row whose result is not
+// finite is therefore computed again by a walk that never touches the keys behind
+// it (row_walk); rows that hold such values by right pay for it too.
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
 
@@ -21,6 +50,7 @@ struct PromptArgs {
   int64_t T;
   int max_len;
   float qscale;               // scale * log2(e)
+  int by_level;               // order of the tiles: see find_tile
 };
 
 // First row and rows of sequence b, whatever cu holds: rows of [0, T), at most
@@ -97,24 +127,7 @@ __device__ inline void row_walk(const PromptArgs& a, int64_t row0, int i, int h)
     Codec<T>::store8(dst, acc);
 }
 
-// A wave per (row, head): grid (rows / 4, H).
-template <typename T, int D>
-__global__ __launch_bounds__(256) void prompt_rows_kernel(PromptArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.T) return;
-  int lo = 0, hi = a.B;   // cu[lo] <= row < cu[hi], where cu ascends
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu[mid] <= row) lo = mid; else hi = mid;
-  }
-  int64_t row0;
-  int len;
-  seq_rows(a, lo, row0, len);
-  if (row < row0 || row >= row0 + len) return;
-  row_walk<T, D>(a, row0, (int)(row - row0), blockIdx.y);
-}
-
-// ---- matrix cores, 16-bit types ---------------------------------------------
+// ---- the matrix-core kernels ------------------------------------------------
 
 constexpr float kSlack = 8.0f;   // lazy raise of the running max, log2 units
 
@@ -131,6 +144,11 @@ template <typename T>
 struct Half;
 template <>
 struct Half<Bf16> {
+  // acc + both halves' values, in fp32
+  __device__ static float sum2(uint32_t w, float acc) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w),
+                                           __builtin_bit_cast(bf16x2, 0x3f803f80u), acc, false);
+  }
   __device__ static float16x mma(short8x a, short8x b, float16x c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -141,6 +159,10 @@ struct Half<Bf16> {
 };
 template <>
 struct Half<_Float16> {
+  __device__ static float sum2(uint32_t w, float acc) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3c003c00u),
+                                  acc, false);
+  }
   __device__ static float16x mma(short8x a, short8x b, float16x c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -162,55 +184,166 @@ __device__ inline float both_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// 16 bytes from every lane's address to LDS, at the wave's byte offset `to` + 16 lane;
+// 16 bytes from base + every lane's offset to LDS, at the wave's byte offset `to` + 16 lane;
 // counted by vmcnt.  As a builtin, the compiler waits for all such loads before every
 // transposing read.  No output register is in flight, and nothing else here uses m0.
-__device__ inline void load_to_lds(const uint8_t* p, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p)
+__device__ inline void load_to_lds(const uint8_t* base, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to),
+               "v"(offset), "s"(base)
                : "memory");
 }
 
-// Where the 16-byte chunk c of row r lies in its LDS row of kC chunks: K rows are
-// read 16 at a time at one chunk, V rows 4 at a time at 4 neighbouring chunks, and
-// each pattern shall cover all 64 banks.
+// Where the 16-byte chunk c of row r lies in its LDS row of kC chunks, so that each
+// reading pattern covers all 64 banks: K rows are read 16 at a time at one chunk, V
+// rows of 16-bit elements 4 at a time at 4 neighbouring chunks, of fp32 elements 2 at
+// a time, 4 rows apart, at 8 neighbouring chunks (which rows of 8 chunks cannot).
 template <int kC>
-__device__ inline int k_place(int r, int c) {
-  if constexpr (kC >= 16) return c ^ (r & 15);
-  else if constexpr (kC == 8) return c ^ ((r >> 1) & 7);
-  else return c ^ ((r >> 2) & 3);
-}
+struct KPlace {
+  static constexpr int kPeriod = 16;   // rows
+  __device__ static int at(int r, int c) {
+    if constexpr (kC >= 16) return c ^ (r & 15);
+    else if constexpr (kC == 8) return c ^ ((r >> 1) & 7);
+    else return c ^ ((r >> 2) & 3);
+  }
+};
 template <int kC>
-__device__ inline int v_place(int r, int c) {
-  if constexpr (kC >= 16) return c ^ ((r & 3) << 2);
-  else if constexpr (kC == 8) return c ^ (((r >> 1) & 1) << 2);
-  else return c;
+struct VPlace16 {
+  static constexpr int kPeriod = 4;
+  __device__ static int at(int r, int c) {
+    if constexpr (kC >= 16) return c ^ ((r & 3) << 2);
+    else if constexpr (kC == 8) return c ^ (((r >> 1) & 1) << 2);
+    else return c;
+  }
+};
+template <int kC>
+struct VPlace32 {
+  static constexpr int kPeriod = 8;
+  __device__ static int at(int r, int c) {
+    if constexpr (kC >= 16) return c ^ (((r >> 2) & 1) << 3);
+    else return c;
+  }
+};
+
+constexpr int kThreads = 256;
+
+// The loads of K's or V's rows, kKeys at a time; rows past the sequence are read as
+// its last one (and masked), and behind the last tile it is read again.  A load of the
+// workgroup covers kStep rows; the swizzle repeats after kOff of them, so those many
+// offsets per lane serve all.
+template <int kC, int kKeys, typename Place>
+struct TileLoads {
+  static constexpr int kLoads = kKeys * kC / kThreads, kStep = kThreads / kC;
+  static constexpr int kOff = Place::kPeriod > kStep ? Place::kPeriod / kStep : 1;
+  static_assert(kLoads >= 1 && kLoads * kThreads == kKeys * kC, "tile / thread split");
+  const uint8_t* base;    // of the next tile
+  int64_t stride;         // bytes between rows
+  int left;               // rows of the sequence from the next tile on
+  uint32_t lds;           // this wave's part of the first of two tiles
+  uint32_t off[kOff];
+
+  __device__ void init(const uint8_t* first, int64_t row_stride, int len, uint32_t to, int wave) {
+    base = first;
+    stride = row_stride;
+    left = len;
+    lds = __builtin_amdgcn_readfirstlane(to + wave * 1024);
+    const int r = threadIdx.x / kC, c = threadIdx.x % kC;
+#pragma unroll
+    for (int u = 0; u < kOff; ++u)
+      off[u] = (uint32_t)r * (uint32_t)stride + 16 * Place::at(u * kStep + r, c);
+  }
+  __device__ void load(int odd) {
+    const uint32_t to = lds + odd * (kKeys * kC * 16);
+    if (left >= kKeys) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u)
+        load_to_lds(base + u * kStep * stride, off[u % kOff], to + u * kThreads * 16);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const int r = u * kStep + threadIdx.x / kC;
+        load_to_lds(base, (uint32_t)min(r, left - 1) * (uint32_t)stride + 16 * Place::at(r, threadIdx.x % kC),
+                    to + u * kThreads * 16);
+      }
+    }
+    if (left > kKeys) {
+      base += stride * kKeys;
+      left -= kKeys;
+    }
+  }
+};
+
+// Sum over the wave, in every lane.
+__device__ inline int wave_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, kDppQuadXor1, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, kDppQuadXor2, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, kDppRowHalfMirror, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, kDppRowMirror, 0xF, 0xF, false);
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = r[0] + r[1];
+  const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return s[0] + s[1];
 }
 
-// The tile of query rows that workgroup `i` takes: tiles of all sequences, those
-// that walk the most keys first.  nt_b tiles of `rows` rows in sequence b; tile
-// qt of it walks qt + 1 tiles of keys, so the tiles go by falling qt, and by b
-// among equals: with F(l) = sum_b max(0, nt_b - l) tiles from level l on, i lies
-// on the highest level l with F(l) > i.  Every wave finds it by itself.  False:
-// there is no such tile.
-__device__ inline bool find_tile(const PromptArgs& a, int rows, int64_t i, int& b, int& qt) {
+// The tile of query rows that workgroup `i` takes, nt_b tiles of `rows` rows in
+// sequence b, of which tile qt walks the keys of qt + 1.  Every wave finds it by
+// itself.  False: there is no such tile.
+//   by_level  tiles by falling qt, and by b among equals, so that the longest walks
+//             begin first: with F(l) = sum_b max(0, nt_b - l) tiles from level l on, i
+//             lies on the highest level l with F(l) > i
+//   else      a sequence's tiles are neighbours, the last one first, so that its keys
+//             are read again from the L2 of the XCD that its heads run on, and
+//             sequences go by falling nt_b
+// More than 64 sequences go in their order, a sequence's tiles as neighbours.
+__device__ inline bool find_tile(const PromptArgs& a, int rows, int i, int& b, int& qt) {
   const int lane = threadIdx.x & 63;
-  auto tiles = [&](int s) {
+  auto tiles_of = [&](int s) {
     int64_t row0;
-    int len;
-    if (s >= a.B) return 0;
-    seq_rows(a, s, row0, len);
+    int len = 0;
+    if (s < a.B) seq_rows(a, s, row0, len);
     return (len + rows - 1) / rows;
   };
-  auto from_level = [&](int l) {
-    int64_t f = 0;
+  if (a.B > 64) {
+    int total = 0;
     for (int s0 = 0; s0 < a.B; s0 += 64) {
-      int x = max(0, tiles(s0 + lane) - l);
+      const int nt = tiles_of(s0 + lane);
+      int inc = nt;
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-      f += x;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(inc, o);
+        if (lane >= o) inc += x;
+      }
+      const uint64_t m = __builtin_amdgcn_ballot_w64(i < total + inc);
+      if (m != 0) {
+        const int at = __builtin_ctzll(m);
+        b = s0 + at;
+        qt = total + __builtin_amdgcn_readlane(inc, at) - 1 - i;
+        return true;
+      }
+      total += __builtin_amdgcn_readlane(inc, 63);
     }
-    return f;
-  };
+    return false;
+  }
+  const int nt = tiles_of(lane);
+  if (a.B == 1) {
+    b = 0;
+    qt = __builtin_amdgcn_readlane(nt, 0) - 1 - i;
+    return qt >= 0;
+  }
+  if (!a.by_level) {
+    // the tiles of the sequences in front of this lane's
+    const int64_t key = (int64_t)nt << 6 | (63 - lane);
+    int before = 0;
+    for (int s = 0; s < a.B; ++s) {
+      const int x = __builtin_amdgcn_readlane(nt, s);
+      before += ((int64_t)x << 6 | (63 - s)) > key ? x : 0;
+    }
+    const uint64_t m = __builtin_amdgcn_ballot_w64(i >= before && i < before + nt);
+    if (m == 0) return false;
+    b = __builtin_ctzll(m);
+    qt = __builtin_amdgcn_readlane(nt + before, b) - 1 - i;
+    return true;
+  }
+  auto from_level = [&](int l) { return wave_sum(max(0, nt - l)); };
   if (from_level(0) <= i) return false;
   int lo = 0, hi = (a.max_len + rows - 1) / rows;   // F(lo) > i >= F(hi) = 0
   while (hi - lo > 1) {
@@ -218,71 +351,154 @@ __device__ inline bool find_tile(const PromptArgs& a, int rows, int64_t i, int& 
     if (from_level(mid) > i) lo = mid; else hi = mid;
   }
   qt = lo;
-  int64_t k = i - from_level(lo + 1);               // the k-th sequence with nt_b > lo
-  for (int s0 = 0; s0 < a.B; s0 += 64) {
-    uint64_t m = __builtin_amdgcn_ballot_w64(tiles(s0 + lane) > lo);
-    const int n = __builtin_popcountll(m);
-    if (k < n) {
-      for (; k > 0; --k) m &= m - 1;
-      b = s0 + __builtin_ctzll(m);
-      return true;
-    }
-    k -= n;
-  }
-  return false;
+  uint64_t m = __builtin_amdgcn_ballot_w64(nt > lo);
+  for (int k = i - from_level(lo + 1); k > 0; --k) m &= m - 1;   // the k-th with nt_b > lo
+  b = __builtin_ctzll(m);
+  return true;
 }
 
-// A workgroup: W waves of 32 query rows of one (sequence, head).  It walks the keys
-// in tiles of kBN, K and V going from global memory straight to LDS, kStages tiles
-// deep.  S^T = K Q^T and O^T = V^T P^T on 32x32x16 products, so that a lane holds one
-// query's scores and the probabilities are the second product's operand where they
-// stand: accumulator register r of lane half h is row 8 (r / 4) + 4 h + r % 4, the
-// operand wants 8 h + r % 8 (+ 16 (r / 8)), and lane j reading key swap23(j) turns
-// the one into the other.
-template <typename T, int D, int W, int kBN, int kStages>
-__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_mma_kernel(PromptArgs a) {
-  constexpr int kRows = 32 * W, kC = D / 8, kThreads = 64 * W;
-  constexpr int kRowBytes = 2 * D, kTile = kBN * kRowBytes;
-  constexpr int kLoads = kTile / (16 * kThreads);   // 16-byte loads of a thread, K and V each
+// What a workgroup of R waves of rows works on.
+struct Task {
+  int h, kvh, q0, len;
+  int64_t row0;
+  __device__ bool find(const PromptArgs& a, int rows) {
+    // neighbouring workgroups: the heads of one tile, a KV head's group on one XCD
+    const int p = blockIdx.x % a.H;
+    kvh = p % a.Hkv;
+    h = kvh * (a.H / a.Hkv) + p / a.Hkv;
+    int b, qt;
+    if (!find_tile(a, rows, (int)(blockIdx.x / a.H), b, qt)) return false;
+    // wave-uniform, and the loop's bounds with them
+    seq_rows(a, __builtin_amdgcn_readfirstlane(b), row0, len);
+    q0 = __builtin_amdgcn_readfirstlane(qt) * rows;
+    return true;
+  }
+};
+
+// The softmax state of a wave's 32 rows, lane (j, hh): row j, accumulator register r
+// of o[d] dim 32 d + 8 (r / 4) + 4 hh + r % 4; l over this lane's keys.
+template <typename T, int D>
+__device__ void walk_rows(const PromptArgs& a, const Task& t, uint32_t bad, int first_row) {
+  for (; bad; bad &= bad - 1) {
+    const int i = first_row + __builtin_ctz(bad);
+    if (i < t.len) row_walk<T, D>(a, t.row0, i, t.h);
+  }
+}
+
+template <int kDB>
+struct State {
+  static constexpr int kFloats = 64 * kDB * 16 + 128;   // of a wave, in LDS
+  float m, l;
+  float16x o[kDB];
+
+  __device__ void clear() {
+    m = kNegBig;
+    l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kDB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+  }
+  // The maximum of this lane's new scores, times qs; the running one is only raised
+  // where some row's lies more than kSlack above it.
+  __device__ void raise(float mx, float qs) {
+    mx = both_max(mx) * qs;
+    if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+      const float m_new = fmaxf(m, mx), keep = fast_exp2(m - m_new);
+      m = m_new;
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < kDB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= keep;
+    }
+  }
+  __device__ void put(float* to) const {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 0; d < kDB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(to + ((d * 4 + g) * 64 + lane) * 4) =
+            make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+    *reinterpret_cast<float2*>(to + 64 * kDB * 16 + 2 * lane) = make_float2(m, l);
+  }
+  __device__ void add(const float* from) {
+    const int lane = threadIdx.x & 63;
+    const float2 ml = *reinterpret_cast<const float2*>(from + 64 * kDB * 16 + 2 * lane);
+    const float mm = fmaxf(m, ml.x), w_s = fast_exp2(m - mm), w_o = fast_exp2(ml.x - mm);
+    m = mm;
+    l = l * w_s + ml.y * w_o;
+#pragma unroll
+    for (int d = 0; d < kDB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 x = *reinterpret_cast<const float4*>(from + ((d * 4 + g) * 64 + lane) * 4);
+        o[d][4 * g] = o[d][4 * g] * w_s + x.x * w_o;
+        o[d][4 * g + 1] = o[d][4 * g + 1] * w_s + x.y * w_o;
+        o[d][4 * g + 2] = o[d][4 * g + 2] * w_s + x.z * w_o;
+        o[d][4 * g + 3] = o[d][4 * g + 3] * w_s + x.w * w_o;
+      }
+  }
+  // O over its sum; rows (a bit each) that are not finite.
+  __device__ uint32_t normalise() {
+    const float inv = 1.0f / both_sum(l);
+    bool fine = true;
+#pragma unroll
+    for (int d = 0; d < kDB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        o[d][r] *= inv;
+        fine = fine && fabsf(o[d][r]) < INFINITY;
+      }
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(!fine);
+    return (uint32_t)bad | (uint32_t)(bad >> 32);
+  }
+};
+
+// This wave's loads have landed, but for the last `kLater`; behind the barrier
+// everybody's have.
+template <int kLater>
+__device__ inline void landed() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLater) : "memory");
+}
+
+// 16-bit types.  KS groups of 4 / KS waves take KS neighbouring tiles of kBN keys each
+// step, for the same rows, and put their states together at the end: twice the
+// workgroups, each half as long, where there are few.
+//
+// A 32x32x16 product's accumulator register r of lane half h is row 8 (r / 4) + 4 h +
+// r % 4, its operand wants 8 h + r % 8 (+ 16 (r / 8)); lane j of K's operand reading key
+// swap23(j) turns the one into the other for the probabilities.
+template <typename T, int D, int kBN, int KS>
+__global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : D == 64 ? 3 : 2) void prompt_mma_kernel(
+    PromptArgs a) {
+  constexpr int R = 4 / KS, kC = D / 8, kKeys = KS * kBN, kRowBytes = 2 * D;
   constexpr int kKB = kBN / 32, kDC = D / 16, kDB = D / 32;
-  static_assert(kLoads >= 1 && kLoads * 16 * kThreads == kTile, "tile / thread split");
-  __shared__ __align__(1024) uint8_t lds[kStages][2][kTile];
+  using KLoads = TileLoads<kC, kKeys, KPlace<kC>>;
+  using VLoads = TileLoads<kC, kKeys, VPlace16<kC>>;
+  __shared__ __align__(1024) uint8_t lds[2][2][kKeys * kRowBytes];   // [K, V][even, odd tiles]
 
   const int lane = threadIdx.x & 63, j = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // neighbouring workgroups: the heads of one tile, a KV head's group on one XCD
-  const int hp = blockIdx.x % a.H;
-  const int h = hp % a.Hkv * (a.H / a.Hkv) + hp / a.Hkv, kvh = hp % a.Hkv;
-  int b, qt;
-  if (!find_tile(a, kRows, blockIdx.x / a.H, b, qt)) return;
-  b = __builtin_amdgcn_readfirstlane(b);
-  int64_t row0;
-  int len;
-  seq_rows(a, b, row0, len);
-  const int q0 = qt * kRows;
-  const int n_kt = (min(q0 + kRows, len) + kBN - 1) / kBN;
+  Task t;
+  if (!t.find(a, 32 * R)) return;
+  const int n_kt = (min(t.q0 + 32 * R, t.len) + kKeys - 1) / kKeys;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  KLoads kl;
+  VLoads vl;
+  kl.init(a.k + t.row0 * a.k_row + t.kvh * a.k_head, a.k_row, t.len, lds0, wave);
+  vl.init(a.v + t.row0 * a.v_row + t.kvh * a.v_head, a.v_row, t.len, lds0 + sizeof(lds[0]), wave);
+  kl.load(0);
+  kl.load(1);
+  vl.load(0);
 
-  const uint8_t* kbase = a.k + row0 * a.k_row + kvh * a.k_head;
-  const uint8_t* vbase = a.v + row0 * a.v_row + kvh * a.v_head;
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
-      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds);
-  // Keys past the sequence are read as its last one (and masked).
-  auto load_tile = [&](int kt, int stage) {
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      const int at = (u * W + wave) * 64 + lane;      // 16-byte place in the tile
-      const int r = at / kC, p = at % kC;
-      const int64_t key = min(kt * kBN + r, len - 1);
-      const uint32_t to = lds0 + (uint32_t)(2 * stage * kTile + (u * W + wave) * 1024);
-      load_to_lds(kbase + key * a.k_row + 16 * k_place<kC>(r, p), to);
-      load_to_lds(vbase + key * a.v_row + 16 * v_place<kC>(r, p), to + kTile);
-    }
-  };
-
-  const int qrow = q0 + 32 * wave + j;   // of the sequence
+  const int kg = wave / R;                      // which of the step's tiles
+  const int first_row = t.q0 + 32 * (wave % R);
+  const int qrow = first_row + j;               // of the sequence
   short8x qf[kDC];
   {
-    const uint8_t* src = a.q + (row0 + min(qrow, len - 1)) * a.q_row + h * a.q_head + 16 * hh;
+    const uint8_t* src = a.q + (t.row0 + min(qrow, t.len - 1)) * a.q_row + t.h * a.q_head + 16 * hh;
 #pragma unroll
     for (int c = 0; c < kDC; ++c)
       qf[c] = *reinterpret_cast<const short8x*>(src + 32 * c);
@@ -297,121 +513,146 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_mma_kernel(Pr
   for (int c = 0; c < kDC; ++c) asm volatile("" : "+v"(qf[c]));
   // above 0, so that the -inf of a key behind the row stays one
   const float qs = fmaxf(fabsf(a.qscale), 1e-30f);
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) load_tile(s, s);
+  State<kDB> st;
+  st.clear();
+  const int last_kt = min(first_row / kKeys, n_kt - 1);   // the only step with keys behind some row
 
-  float m = kNegBig, l = 0.0f;
-  float16x o[kDB];
+  // Tile kt's turn: its V and the next tile's K have landed, behind the barrier
+  // everybody's part of them; and everybody is done with what the next loads replace
+  // (K of tile kt, V of the tile before).
+  auto arrive = [&](int odd) {
+    landed<0>();
+    kl.load(odd);
+    vl.load(1 - odd);
+  };
+  // Fragments: lane (j, hh) of K's gets elements 16 c + 8 hh .. of key swap23(j) of the
+  // 32 of block kb; of V^T's V[key0 + 8 hh + e][32 d + j], where the transposing read
+  // takes 8 bytes of row i / 4 from lane i of 16 and gives it column i.  The swizzles
+  // depend on the lane alone, so every read is a lane's offset and a constant.
+  const int kr = swap23(j), vi = j & 15;
+  auto k_frag = [&](int odd, int i) {               // i = c kKB + kb
+    const int c = i / kKB, kb = i % kKB;
+    return *reinterpret_cast<const short8x*>(lds[0][odd] + 32 * kb * kRowBytes + (kg * kBN + kr) * kRowBytes +
+                                             16 * KPlace<kC>::at(kr, 2 * c + hh));
+  };
+  auto v_frag = [&](int odd, int i) {               // i = (kb 2 + c) kDB + d
+    typedef __attribute__((address_space(3))) short4x lshort4x;
+    const int d = i % kDB, r = 8 * hh + (vi >> 2), e0 = 32 * d + (j & 16) + 4 * (vi & 3);
+    const uint8_t* p = lds[1][odd] + 16 * (i / kDB) * kRowBytes;
+    const short4x lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lshort4x*)(p + ((kg * kBN + r) * kRowBytes + 16 * VPlace16<kC>::at(r, e0 / 8) + 2 * (e0 % 8))));
+    const short4x hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lshort4x*)(p + 4 * kRowBytes + ((kg * kBN + r) * kRowBytes + 16 * VPlace16<kC>::at(r + 4, e0 / 8) + 2 * (e0 % 8))));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  // Keys behind the row, in the wave's last tile.
+  auto mask = [&](float16x (&s)[kKB]) {
 #pragma unroll
-  for (int d = 0; d < kDB; ++d)
+    for (int kb = 0; kb < kKB; ++kb)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+      for (int r = 0; r < 16; ++r)
+        if (last_kt * kKeys + kg * kBN + 32 * kb + 16 * (r / 8) + 8 * hh + r % 8 > qrow) s[kb][r] = -INFINITY;
+  };
+  constexpr int kQk = kKB * kDC, kPv = kKB * 2 * kDB;      // products of a tile
+  constexpr int kPairs = kKB * 8;                          // pairs of scores of a lane
+  constexpr int kAhead = kQk < 3 ? kQk : 3;                // fragments read ahead
+  uint32_t pw[kPairs];                                     // probabilities, two a word
+  auto prob = [&](float16x (&s)[kKB], int e) {
+    const float x = fast_exp2(fmaf(s[e / 8][2 * (e % 8)], qs, -st.m));
+    const float y = fast_exp2(fmaf(s[e / 8][2 * (e % 8) + 1], qs, -st.m));
+    pw[e] = Half<T>::pack(x, y);
+    st.l = Half<T>::sum2(pw[e], st.l);
+  };
+  auto pv = [&](short8x v, int i) {
+    const int g = 4 * (i / kDB);
+    st.o[i % kDB] = Half<T>::mma(v, __builtin_bit_cast(short8x, make_uint4(pw[g], pw[g + 1], pw[g + 2], pw[g + 3])),
+                                 st.o[i % kDB]);
+  };
 
-  const int first_row = q0 + 32 * wave;
-  int stage = 0;
-  for (int kt = 0; kt < n_kt; ++kt) {
-    // this wave's loads of tile kt have landed (those of later tiles may be on
-    // their way); behind the barrier everybody's have, and everybody is done with
-    // tile kt - 1, whose place the next loads take
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * kLoads * (kStages - 2)) : "memory");
-    {
-      int next = stage + kStages - 1;
-      if (next >= kStages) next -= kStages;
-      load_tile(kt + kStages - 1, next);
+  // One tile: S^T of the next one beside this one's exponentials, then O^T beside the
+  // next one's maxima, product by product in this order (the barriers keep the compiler
+  // from gathering them).
+  float mx = 0.0f;
+  auto step = [&](int odd, int kt, float16x (&sc)[kKB], float16x (&sn)[kKB]) {
+    st.raise(mx, qs);
+    arrive(odd);
+    short8x kf[kQk], vf[kPv];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) kf[i] = k_frag(1 - odd, i);
+#pragma unroll
+    for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sn[kb][r] = 0.0f;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kQk; ++i) {
+      const int n = i + kAhead;
+      if (n < kQk) kf[n] = k_frag(1 - odd, n);
+      else if (n - kQk < kPv) vf[n - kQk] = v_frag(odd, n - kQk);
+      sn[i % kKB] = Half<T>::mma(kf[i], qf[i / kKB], sn[i % kKB]);
+#pragma unroll
+      for (int e = i * kPairs / kQk; e < (i + 1) * kPairs / kQk; ++e) prob(sc, e);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    const uint8_t* ks = lds[stage][0];
-    const uint8_t* vs = lds[stage][1];
-    if (++stage == kStages) stage = 0;
-    const int k0 = kt * kBN;
-    if (k0 > first_row + 31) continue;   // every key lies behind this wave's rows
+    if (kt + 1 == last_kt) mask(sn);
+    mx = sn[0][0];
+#pragma unroll
+    for (int i = 0; i < kPv; ++i) {
+      if (i + kAhead < kPv) vf[i + kAhead] = v_frag(odd, i + kAhead);
+      pv(vf[i], i);
+#pragma unroll
+      for (int e = i * kPairs / kPv; e < (i + 1) * kPairs / kPv; ++e)
+        mx = fmaxf(fmaxf(mx, sn[e / 8][2 * (e % 8)]), sn[e / 8][2 * (e % 8) + 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto finish = [&](int odd, float16x (&sc)[kKB]) {
+    st.raise(mx, qs);
+    arrive(odd);
+#pragma unroll
+    for (int e = 0; e < kPairs; ++e) prob(sc, e);
+#pragma unroll
+    for (int i = 0; i < kPv; ++i) pv(v_frag(odd, i), i);
+  };
 
-    float16x s[kKB];
+  float16x sa[kKB], sb[kKB];
+  landed<KLoads::kLoads + VLoads::kLoads>();
 #pragma unroll
-    for (int kb = 0; kb < kKB; ++kb)
+  for (int kb = 0; kb < kKB; ++kb)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[kb][r] = 0.0f;
-    const int kr = swap23(j);
+    for (int r = 0; r < 16; ++r) sa[kb][r] = 0.0f;
 #pragma unroll
-    for (int c = 0; c < kDC; ++c)
+  for (int i = 0; i < kQk; ++i) sa[i % kKB] = Half<T>::mma(k_frag(0, i), qf[i / kKB], sa[i % kKB]);
+  if (last_kt == 0) mask(sa);
+  mx = sa[0][0];
 #pragma unroll
-      for (int kb = 0; kb < kKB; ++kb) {
-        const short8x kf = *reinterpret_cast<const short8x*>(
-            ks + (32 * kb + kr) * kRowBytes + 16 * k_place<kC>(kr, 2 * c + hh));
-        s[kb] = Half<T>::mma(kf, qf[c], s[kb]);
-      }
-    if (k0 + kBN - 1 > first_row) {      // some row does not see some key
-#pragma unroll
-      for (int kb = 0; kb < kKB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (k0 + 32 * kb + 16 * (r / 8) + 8 * hh + r % 8 > qrow) s[kb][r] = -INFINITY;
-    }
-    float mx = s[0][0];
-#pragma unroll
-    for (int kb = 0; kb < kKB; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
-    mx = both_max(mx) * qs;
-    if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
-      const float m_new = fmaxf(m, mx), keep = fast_exp2(m - m_new);
-      m = m_new;
-      l *= keep;
-#pragma unroll
-      for (int d = 0; d < kDB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] *= keep;
-    }
-    short8x pf[kKB][2];
-#pragma unroll
-    for (int kb = 0; kb < kKB; ++kb)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = fast_exp2(fmaf(s[kb][8 * c + 2 * e], qs, -m));
-          const float y = fast_exp2(fmaf(s[kb][8 * c + 2 * e + 1], qs, -m));
-          l += x + y;
-          w[e] = Half<T>::pack(x, y);
-        }
-        pf[kb][c] = __builtin_bit_cast(short8x, make_uint4(w[0], w[1], w[2], w[3]));
-      }
-    // V^T: lane (j, hh) gets V[key0 + 8 hh + e][32 d + j]; the transposing read takes
-    // 8 bytes of row i / 4 from lane i of 16 and gives it column i
-    const int vi = j & 15;
-#pragma unroll
-    for (int kb = 0; kb < kKB; ++kb)
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int d = 0; d < kDB; ++d) {
-          const int r = 32 * kb + 16 * c + 8 * hh + (vi >> 2);
-          const int e0 = 32 * d + (j & 16) + 4 * (vi & 3);   // element of the row
-          typedef __attribute__((address_space(3))) short4x lshort4x;
-          const short4x lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lshort4x*)(vs + r * kRowBytes + 16 * v_place<kC>(r, e0 / 8) + 2 * (e0 % 8)));
-          const short4x hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lshort4x*)(vs + (r + 4) * kRowBytes + 16 * v_place<kC>(r + 4, e0 / 8) + 2 * (e0 % 8)));
-          o[d] = Half<T>::mma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf[kb][c], o[d]);
-        }
+  for (int e = 0; e < kPairs; ++e) mx = fmaxf(fmaxf(mx, sa[e / 8][2 * (e % 8)]), sa[e / 8][2 * (e % 8) + 1]);
+  int kt = 0;
+  for (; kt + 1 < last_kt; kt += 2) {
+    step(0, kt, sa, sb);
+    step(1, kt + 1, sb, sa);
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last loads land before the LDS is given up
+  if (kt < last_kt) {
+    step(0, kt, sa, sb);
+    ++kt;
+    finish(1, sb);
+  } else {
+    finish(0, sa);
+  }
+  while (++kt < n_kt) arrive(kt & 1);                     // the other waves' last tiles
+  landed<0>();   // the last loads, before the LDS is used again or given up
+  if constexpr (KS == 2) {
+    float* other = reinterpret_cast<float*>(&lds[0][0][0]) + wave % R * State<kDB>::kFloats;
+    static_assert(R * State<kDB>::kFloats * 4 <= (int)sizeof(lds), "states fit the LDS");
+    if (kg > 0) st.put(other);
+    __syncthreads();
+    if (kg > 0) return;
+    st.add(other);
+  }
 
-  // A value behind a row that is infinite or NaN has been added times 0: rows that
-  // are not finite are computed again, without those keys.
-  const float inv = 1.0f / both_sum(l);
-  bool fine = true;
-  uint8_t* dst = a.out + (((row0 + qrow) * a.H + h) * (int64_t)D) * 2;
-#pragma unroll
-  for (int d = 0; d < kDB; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      o[d][r] *= inv;
-      fine = fine && fabsf(o[d][r]) < INFINITY;
-    }
-  uint64_t bad = __builtin_amdgcn_ballot_w64(!fine && qrow < len);
-  uint32_t bad_rows = (uint32_t)bad | (uint32_t)(bad >> 32);
-  if (qrow < len && !((bad_rows >> j) & 1)) {
+  const uint32_t bad = st.normalise();
+  uint8_t* dst = a.out + (((t.row0 + qrow) * a.H + t.h) * (int64_t)D) * 2;
+  if (qrow < t.len && !((bad >> j) & 1)) {
 #pragma unroll
     for (int d = 0; d < kDB; ++d)
 #pragma unroll
@@ -419,48 +660,184 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_mma_kernel(Pr
         // lane halves hold 4 dims each of two groups of 8: swapped into one group each
         uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = Half<T>::pack(o[d][8 * g + 2 * e], o[d][8 * g + 2 * e + 1]);
+        for (int e = 0; e < 4; ++e)
+          w[e] = Half<T>::pack(st.o[d][8 * g + 2 * e], st.o[d][8 * g + 2 * e + 1]);
         const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
         const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
         *reinterpret_cast<uint4*>(dst + 64 * d + 32 * g + 16 * hh) = make_uint4(x[0], y[0], x[1], y[1]);
       }
   }
-  for (; bad_rows; bad_rows &= bad_rows - 1)
-    row_walk<T, D>(a, row0, first_row + __builtin_ctz(bad_rows), h);
+  walk_rows<T, D>(a, t, bad, first_row);
+}
+
+// fp32 on v_mfma_f32_32x32x2_f32, 64 cycles each: a tile's products take 8 times as
+// long as in 16-bit types, and the softmax and LDS reads pass beside the other wave's.
+// Lane (j, hh) holds dims 8 c + 4 hh .. + 3 of its key and its query, four products'
+// operands (any order of the dims serves, if both have it); the probability in
+// register r is key 8 (r / 4) + 4 hh + r % 4 of the 32, so that product reads that key's
+// row of V.
+template <int D, int kBN, int KS>
+__global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : 2) void prompt_f32_kernel(PromptArgs a) {
+  constexpr int R = 4 / KS, kC = D / 4, kKeys = KS * kBN, kRowBytes = 4 * D;
+  constexpr int kKB = kBN / 32, kDC = D / 8, kDB = D / 32;
+  using KLoads = TileLoads<kC, kKeys, KPlace<kC>>;
+  using VLoads = TileLoads<kC, kKeys, VPlace32<kC>>;
+  __shared__ __align__(1024) uint8_t lds[2][2][kKeys * kRowBytes];   // [K, V][even, odd tiles]
+
+  const int lane = threadIdx.x & 63, j = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Task t;
+  if (!t.find(a, 32 * R)) return;
+  const int n_kt = (min(t.q0 + 32 * R, t.len) + kKeys - 1) / kKeys;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  KLoads kl;
+  VLoads vl;
+  kl.init(a.k + t.row0 * a.k_row + t.kvh * a.k_head, a.k_row, t.len, lds0, wave);
+  vl.init(a.v + t.row0 * a.v_row + t.kvh * a.v_head, a.v_row, t.len, lds0 + sizeof(lds[0]), wave);
+  kl.load(0);
+  vl.load(0);
+
+  const int kg = wave / R, first_row = t.q0 + 32 * (wave % R);
+  const int qrow = first_row + j;   // of the sequence
+  float4 qf[kDC];
+  const uint8_t* src = a.q + (t.row0 + min(qrow, t.len - 1)) * a.q_row + t.h * a.q_head + 16 * hh;
+#pragma unroll
+  for (int c = 0; c < kDC; ++c) qf[c] = *reinterpret_cast<const float4*>(src + 32 * c);
+  if (a.qscale < 0) {   // the running max is of scores times |scale|
+#pragma unroll
+    for (int c = 0; c < kDC; ++c) qf[c] = make_float4(-qf[c].x, -qf[c].y, -qf[c].z, -qf[c].w);
+  }
+#pragma unroll
+  for (int c = 0; c < kDC; ++c)
+    asm volatile("" : "+v"(qf[c].x), "+v"(qf[c].y), "+v"(qf[c].z), "+v"(qf[c].w));
+  const float qs = fmaxf(fabsf(a.qscale), 1e-30f);
+
+  State<kDB> st;
+  st.clear();
+  const int last_kt = min(first_row / kKeys, n_kt - 1);   // the only step with keys behind some row
+  for (int kt = 0; kt < n_kt; ++kt) {
+    const int odd = kt & 1;
+    landed<0>();                       // and everybody is done with the tile before
+    kl.load(1 - odd);
+    vl.load(1 - odd);
+    if (kt > last_kt) continue;        // the other waves' last steps
+    float16x s[kKB];
+    const uint8_t* ks = lds[0][odd] + (kg * kBN + j) * kRowBytes;
+#pragma unroll
+    for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kDC; ++c)
+#pragma unroll
+      for (int kb = 0; kb < kKB; ++kb) {
+        const float4 kf = *reinterpret_cast<const float4*>(ks + 32 * kb * kRowBytes +
+                                                           16 * KPlace<kC>::at(j, 2 * c + hh));
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.x, qf[c].x, s[kb], 0, 0, 0);
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.y, qf[c].y, s[kb], 0, 0, 0);
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.z, qf[c].z, s[kb], 0, 0, 0);
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.w, qf[c].w, s[kb], 0, 0, 0);
+      }
+    if (kt == last_kt) {
+#pragma unroll
+      for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (kt * kKeys + kg * kBN + 32 * kb + 8 * (r / 4) + 4 * hh + r % 4 > qrow) s[kb][r] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+    st.raise(mx, qs);
+#pragma unroll
+    for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[kb][r] = fast_exp2(fmaf(s[kb][r], qs, -st.m));
+        st.l += s[kb][r];
+      }
+#pragma unroll
+    for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = 8 * (r / 4) + 4 * hh + r % 4;   // its swizzle depends on hh alone
+        const uint8_t* vs = lds[1][odd] + (kg * kBN + 32 * kb + key) * kRowBytes + 4 * (j & 3);
+#pragma unroll
+        for (int d = 0; d < kDB; ++d)
+          st.o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+              *reinterpret_cast<const float*>(vs + 16 * VPlace32<kC>::at(4 * hh, 8 * d + (j >> 2))), s[kb][r],
+              st.o[d], 0, 0, 0);
+      }
+  }
+  landed<0>();   // the last loads, before the LDS is used again or given up
+  if constexpr (KS == 2) {
+    float* other = reinterpret_cast<float*>(&lds[0][0][0]) + wave % R * State<kDB>::kFloats;
+    static_assert(R * State<kDB>::kFloats * 4 <= (int)sizeof(lds), "states fit the LDS");
+    if (kg > 0) st.put(other);
+    __syncthreads();
+    if (kg > 0) return;
+    st.add(other);
+  }
+  const uint32_t bad = st.normalise();
+  uint8_t* dst = a.out + (((t.row0 + qrow) * a.H + t.h) * (int64_t)D) * 4;
+  if (qrow < t.len && !((bad >> j) & 1)) {
+#pragma unroll
+    for (int d = 0; d < kDB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(dst + 128 * d + 32 * g + 16 * hh) =
+            make_float4(st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]);
+  }
+  walk_rows<float, D>(a, t, bad, first_row);
+}
+
+template <typename T, int D, int kBN, int KS>
+void launch_one(const PromptArgs& a, int64_t grid, hipStream_t stream) {
+  if constexpr (sizeof(T) == 4)
+    hipLaunchKernelGGL((prompt_f32_kernel<D, kBN, KS>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((prompt_mma_kernel<T, D, kBN, KS>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+}
+
+// Tiles of 32 R rows of all sequences, at most.
+int64_t tiles_of(const PromptArgs& a, int rows) {
+  return std::min(sat_mul(a.B, ceil_div(a.max_len, rows)), a.T / rows + a.B);
+}
+
+template <typename T, int D>
+int launch_dim(const PromptArgs& a, int cus, hipStream_t stream) {
+  constexpr int kBN = D * sizeof(T) >= 512 ? 32 : 64;
+  constexpr bool kSplits = 2 * 4 * kBN * D * sizeof(T) <= 160 * 1024;   // two tiles of keys a step fit the LDS
+  const bool split = kSplits && sat_mul(tiles_of(a, 128), a.H) <= cus;
+  const int64_t grid = sat_mul(tiles_of(a, split ? 64 : 128), a.H);
+  if (grid > 0x7fffffffLL) return fail(HS_EUNSUPPORTED, "prompt grid too large");
+  if constexpr (kSplits) {
+    if (split) {
+      launch_one<T, D, kBN, 2>(a, grid, stream);
+      return HS_OK;
+    }
+  }
+  launch_one<T, D, kBN, 1>(a, grid, stream);
+  return HS_OK;
 }
 
 template <typename T>
-int launch_dim(const PromptArgs& a, int D, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2) {
-    const int W = D == 256 || D == 32 ? 4 : 8, rows = 32 * W;
-    const int64_t tiles = std::min(sat_mul(a.B, ceil_div(a.max_len, rows)), a.T / rows + a.B);
-    const int64_t grid = sat_mul(tiles, a.H);
-    if (grid > 0x7fffffffLL) return fail(HS_EUNSUPPORTED, "prompt grid too large");
-    const dim3 g((unsigned)grid), t(64 * W);
-    switch (D) {
-      case 32: hipLaunchKernelGGL((prompt_mma_kernel<T, 32, 4, 64, 3>), g, t, 0, stream, a); break;
-      case 64: hipLaunchKernelGGL((prompt_mma_kernel<T, 64, 8, 64, 3>), g, t, 0, stream, a); break;
-      case 128: hipLaunchKernelGGL((prompt_mma_kernel<T, 128, 8, 64, 3>), g, t, 0, stream, a); break;
-      case 256: hipLaunchKernelGGL((prompt_mma_kernel<T, 256, 4, 32, 3>), g, t, 0, stream, a); break;
-      default: return fail(HS_EUNSUPPORTED, "unsupported head_dim " + std::to_string(D));
-    }
-    return HS_OK;
-  }
-  const dim3 g((unsigned)ceil_div(a.T, 4), (unsigned)a.H), t(256);
+int launch_type(const PromptArgs& a, int D, int cus, hipStream_t stream) {
   switch (D) {
-    case 32: hipLaunchKernelGGL((prompt_rows_kernel<T, 32>), g, t, 0, stream, a); break;
-    case 64: hipLaunchKernelGGL((prompt_rows_kernel<T, 64>), g, t, 0, stream, a); break;
-    case 128: hipLaunchKernelGGL((prompt_rows_kernel<T, 128>), g, t, 0, stream, a); break;
-    case 256: hipLaunchKernelGGL((prompt_rows_kernel<T, 256>), g, t, 0, stream, a); break;
+    case 32: return launch_dim<T, 32>(a, cus, stream);
+    case 64: return launch_dim<T, 64>(a, cus, stream);
+    case 128: return launch_dim<T, 128>(a, cus, stream);
+    case 256: return launch_dim<T, 256>(a, cus, stream);
     default: return fail(HS_EUNSUPPORTED, "unsupported head_dim " + std::to_string(D));
   }
-  return HS_OK;
 }
 
 }  // namespace
 
 // Strides in elements; the sizes and pointers are checked (hs_api.hip).
-int launch_prompt(const Prompt& w, hipStream_t stream) {
+int launch_prompt(const Prompt& w, int cus, hipStream_t stream) {
   const int64_t sb = dtype_bytes(w.dtype);
   PromptArgs a{};
   a.q = static_cast<const uint8_t*>(w.q);
@@ -480,11 +857,13 @@ int launch_prompt(const Prompt& w, hipStream_t stream) {
   a.T = w.T;
   a.max_len = w.max_len;
   a.qscale = w.scale * kLog2e;
+  // the keys and values of all heads stay in the XCDs' L2s (4 MB each)
+  a.by_level = sat_mul(w.T, w.Hkv, w.D, 2 * sb) <= 8 * (4 << 20);
   profile_begin(stream);
   int rc;
-  if (w.dtype == HS_DTYPE_F32) rc = launch_dim<float>(a, w.D, stream);
-  else if (w.dtype == HS_DTYPE_F16) rc = launch_dim<_Float16>(a, w.D, stream);
-  else rc = launch_dim<Bf16>(a, w.D, stream);
+  if (w.dtype == HS_DTYPE_F32) rc = launch_type<float>(a, w.D, cus, stream);
+  else if (w.dtype == HS_DTYPE_F16) rc = launch_type<_Float16>(a, w.D, cus, stream);
+  else rc = launch_type<Bf16>(a, w.D, cus, stream);
   profile_end(stream);
   return rc == HS_OK ? check_launch("prompt attention") : rc;
 }

@@ -736,7 +736,7 @@ def _heads(x, name: str):
 
     def fits(t):
         return t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
-            t.shape[i] == 1 or (t.stride(i) >= 0 and t.stride(i) % unit == 0) for i in (0, 1))
+            t.shape[i] == 1 or (0 <= t.stride(i) <= 1 << 22 and t.stride(i) % unit == 0) for i in (0, 1))
 
     if not fits(x):
         x = x.contiguous()

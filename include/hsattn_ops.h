@@ -68,8 +68,9 @@ int hs_rotary_append(const void* q, const void* k, const void* v, int src_dtype,
  * hold behind a row never reaches it, infinities and NaN included.
  * No reference counterpart (its engine prefills through the cache).
  *   q, k, v     [total, H, D], [total, Hkv, D] twice, of dtype; rows and
- *               heads are the given strides apart (elements; multiples of 16
- *               bytes), D elements of a head contiguous, 16-byte aligned
+ *               heads are the given strides apart (elements, at most 2^22;
+ *               multiples of 16 bytes), D elements of a head contiguous,
+ *               16-byte aligned
  *   out         [total, H, D] of dtype, contiguous, 16-byte aligned; must not
  *               overlap the inputs
  *   D           32, 64, 128 or 256;  H % Hkv == 0
