@@ -645,35 +645,44 @@ def block_tables(packed_dev, B: int, width: int, out) -> None:
 # ---------------------------------------------------------------------------
 
 
+def _head_rows(x, heads: int, D: int):
+    """_rows of a tensor whose last two dims are known to be (heads, D)."""
+    s = x.stride()
+    if s[2] == 1 and (s[1] == D or heads == 1) and s[0] >= heads * D:
+        return x, s[0]
+    return _rows(x, heads, D)
+
+
 def _rotary_head(q, k, positions, inv_freq, axes, interleaved):
     """What both rotary calls pass first: (q, k, their row strides, the device index,
     the arguments from positions to D, and the tensors those point to)."""
     if q.dim() != 3 or k.dim() != 3:
         raise RuntimeError("q must be [n, H, D] and k [n, Hkv, D]")
     n, H, D = q.shape
-    Hkv = k.shape[1]
+    k_rows, Hkv, k_dim = k.shape
     index = q.get_device()
     if index < 0 or k.get_device() != index:
         raise RuntimeError("q and k must be on CUDA, on the same device")
-    if k.shape[0] != n or k.shape[2] != D or k.dtype is not q.dtype:
+    if k_rows != n or k_dim != D or k.dtype is not q.dtype:
         raise RuntimeError("k must have the rows, the head_dim and the dtype of q")
-    pos = _int32_on(positions, q.device)
+    dev = q.device
+    pos = _int32_on(positions, dev)
     n_axes = 1 if pos.dim() <= 1 else pos.shape[0]
     if pos.dim() > 2 or pos.numel() != n_axes * n:
         raise RuntimeError(f"positions must be [axes, {n}] or [{n}], got {tuple(positions.shape)}")
     freq = inv_freq
     if freq.dtype is not torch.float32 or freq.get_device() != index or not freq.is_contiguous():
-        freq = freq.to(device=q.device, dtype=torch.float32).contiguous()
+        freq = freq.to(device=dev, dtype=torch.float32).contiguous()
     pairs = freq.numel()
     if not 0 < pairs <= D // 2:
         raise RuntimeError(f"inv_freq must have 1 to head_dim / 2 = {D // 2} entries, got {pairs}")
-    pa = None if axes is None else _int32_on(axes, q.device)
+    pa = None if axes is None else _int32_on(axes, dev)
     if pa is not None and pa.numel() != pairs:
         raise RuntimeError(f"{pa.numel()} axes for {pairs} rotary pairs")
-    q, q_row = _rows(q, H, D)
-    k, k_row = _rows(k, Hkv, D)
+    q, q_row = _head_rows(q, H, D)
+    k, k_row = _head_rows(k, Hkv, D)
     middle = (pos.data_ptr(), n_axes, freq.data_ptr(), None if pa is None else pa.data_ptr(), pairs,
-              int(bool(interleaved)), n, H, Hkv, D)
+              1 if interleaved else 0, n, H, Hkv, D)
     return q, k, (q_row, k_row), index, middle, (pos, freq, pa)
 
 
@@ -681,13 +690,13 @@ def rotary(q, k, positions, inv_freq, axes, interleaved, out_dtype):
     """(q, k) turned by hs_rotary, contiguous, of out_dtype (q's when None)."""
     L = lib("rotary HIP kernel")
     out_dtype = out_dtype or q.dtype
+    out_code = dtype_code(out_dtype)
     q, k, strides, index, middle, keep = _rotary_head(q, k, positions, inv_freq, axes, interleaved)
-    q_out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=out_dtype, device=q.device)
+    q_out = q.new_empty(q.shape, dtype=out_dtype)
+    k_out = q.new_empty(k.shape, dtype=out_dtype)
     with _DeviceGuard(index):
         check(L.hs_rotary(q.data_ptr(), k.data_ptr(), dtype_code(q.dtype), *strides, *middle,
-                          q_out.data_ptr(), k_out.data_ptr(), dtype_code(out_dtype),
-                          _stream_at(index)))
+                          q_out.data_ptr(), k_out.data_ptr(), out_code, _stream_at(index)))
     return q_out, k_out
 
 
@@ -696,52 +705,55 @@ def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, block_tables, 
     """(q, k or None) turned by hs_rotary_append, which writes k and v into the caches."""
     L = lib("rotary HIP kernel")
     out_dtype = out_dtype or q.dtype
+    out_code = dtype_code(out_dtype)
     q, k, strides, index, middle, keep = _rotary_head(q, k, positions, inv_freq, axes, interleaved)
     n, Hkv, D = k.shape
     (NB, BS, cache_heads, cache_dim), cache_index = _check_write(k_cache, v_cache, k, v)
     if cache_index != index:
         raise RuntimeError("kv cache and new rows must be on the same device")
-    if (cache_heads, cache_dim) != (Hkv, D):
+    if cache_heads != Hkv or cache_dim != D:
         raise RuntimeError(f"K/V rows must be [n, {cache_heads}, {cache_dim}], got {tuple(k.shape)}")
-    v, v_row = _rows(v, Hkv, D)
-    if v.shape[0] != n or v.dtype is not k.dtype:
+    if v.dtype is not k.dtype or v.shape[0] != n:
         raise RuntimeError("k and v rows must have the same count and dtype")
-    bt = _int32_on(block_tables, q.device)
-    at = _int32_on(cache_positions, q.device)
-    sid = None if seq_ids is None else _int32_on(seq_ids, q.device)
+    v, v_row = _head_rows(v, Hkv, D) if v.shape == k.shape else _rows(v, Hkv, D)
+    dev = q.device
+    bt = _int32_on(block_tables, dev)
+    at = _int32_on(cache_positions, dev)
+    sid = None if seq_ids is None else _int32_on(seq_ids, dev)
     if bt.dim() != 2:
         raise RuntimeError("block_tables must be [B, max_blocks]")
+    B, MB = bt.shape
     if at.numel() != n:
         raise RuntimeError(f"{at.numel()} positions for {n} rows")
     if sid is not None and sid.numel() != n:
         raise RuntimeError(f"{sid.numel()} sequence ids for {n} rows")
-    if sid is None and n > bt.shape[0]:
+    if sid is None and n > B:
         raise RuntimeError("without seq_ids, row i uses table row i: more rows than tables")
-    q_out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=out_dtype, device=q.device) if keep_k else None
+    q_out = q.new_empty(q.shape, dtype=out_dtype)
+    k_out = q.new_empty(k.shape, dtype=out_dtype) if keep_k else None
     with _DeviceGuard(index):
         check(L.hs_rotary_append(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype_code(q.dtype), *strides, v_row, *middle,
-            q_out.data_ptr(), None if k_out is None else k_out.data_ptr(), dtype_code(out_dtype),
+            q_out.data_ptr(), None if k_out is None else k_out.data_ptr(), out_code,
             k_cache.data_ptr(), v_cache.data_ptr(), dtype_code(k_cache.dtype), NB, BS, bt.data_ptr(),
-            bt.shape[0], bt.shape[1], at.data_ptr(), None if sid is None else sid.data_ptr(),
-            _stream_at(index)))
+            B, MB, at.data_ptr(), None if sid is None else sid.data_ptr(), _stream_at(index)))
     return q_out, k_out
 
 
-def _heads(x, name: str):
-    """(tensor, row stride, head stride): rows and heads any multiple of 16 bytes
-    apart, D elements of a head contiguous; a contiguous copy of anything else."""
-    unit = 16 // x.element_size()
-
-    def fits(t):
-        return t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
-            t.shape[i] == 1 or (0 <= t.stride(i) <= 1 << 22 and t.stride(i) % unit == 0) for i in (0, 1))
-
-    if not fits(x):
+def _heads(x):
+    """(tensor, pointer, row stride, head stride): rows and heads any multiple of 16
+    bytes apart, D elements of a head contiguous; a contiguous copy of anything else."""
+    s0, s1, s2 = x.stride()
+    ptr = x.data_ptr()
+    unit = 15 // x.element_size()      # a mask: 3 or 7
+    if (s2 != 1 or ptr & 15 or (s0 | s1) & unit or not 0 <= s0 <= 1 << 22
+            or not 0 <= s1 <= 1 << 22):
         x = x.contiguous()
-    # a dim of one index has no stride of its own
-    return x, x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0
+        if x.data_ptr() & 15:
+            x = x.clone(memory_format=torch.contiguous_format)
+        # (a dim of one index may still have any stride of its own)
+        ptr, s0, s1 = x.data_ptr(), x.shape[1] * x.shape[2], x.shape[2]
+    return x, ptr, s0, s1
 
 
 def prompt_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float, out=None):
@@ -752,38 +764,41 @@ def prompt_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float, out=Non
     index = q.get_device()
     if index < 0 or k.get_device() != index or v.get_device() != index:
         raise RuntimeError("q, k and v must be on CUDA, on the same device")
-    T, H, D = q.shape
-    Hkv = k.shape[1]
-    if k.shape != (T, Hkv, D) or v.shape != k.shape:
+    shape, kv_shape, dtype = q.shape, k.shape, q.dtype
+    T, H, D = shape
+    Hkv = kv_shape[1]
+    if kv_shape != (T, Hkv, D) or v.shape != kv_shape:
         raise RuntimeError(f"k and v must be [{T}, Hkv, {D}], got {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.dtype is not q.dtype or v.dtype is not q.dtype:
+    if k.dtype is not dtype or v.dtype is not dtype:
         raise RuntimeError("q, k and v must have the same dtype")
+    code = dtype_code(dtype)
     cu = _int32_on(cu_seqlens, q.device)
-    if cu.dim() != 1 or cu.numel() < 1:
+    B = cu.numel() - 1
+    if cu.dim() != 1 or B < 0:
         raise RuntimeError("cu_seqlens must be [B + 1]")
     if out is None:
-        out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
-    elif (out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != index
+        out = q.new_empty(shape)
+    elif (out.shape != shape or out.dtype is not dtype or out.get_device() != index
           or not out.is_contiguous() or out.data_ptr() % 16):
         raise RuntimeError("out must be a contiguous, 16-byte aligned tensor like q")
-    q, qr, qh = _heads(q, "q")
-    k, kr, kh = _heads(k, "k")
-    v, vr, vh = _heads(v, "v")
+    q, qp, qr, qh = _heads(q)
+    k, kp, kr, kh = _heads(k)
+    v, vp, vr, vh = _heads(v)
     with _DeviceGuard(index):
-        check(L.hs_prompt_attention(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype_code(q.dtype), qr, qh, kr, kh, vr, vh,
-            cu.data_ptr(), cu.numel() - 1, T, int(max_seqlen), H, Hkv, D, float(scale),
-            out.data_ptr(), _stream_at(index)))
+        check(L.hs_prompt_attention(qp, kp, vp, code, qr, qh, kr, kh, vr, vh, cu.data_ptr(), B, T,
+                                    int(max_seqlen), H, Hkv, D, float(scale), out.data_ptr(),
+                                    _stream_at(index)))
     return out
 
 
 def _check_state(name: str, t, dim: int, index: int):
     """A tensor that a page operation changes in place."""
+    if t.dtype is torch.int32 and t.dim() == dim and t.get_device() == index >= 0 and t.is_contiguous():
+        return
     if t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous():
         raise RuntimeError(f"{name} must be a contiguous int32 tensor of {dim} dim(s): it is "
                            "written in place")
-    if t.get_device() != index or index < 0:
-        raise RuntimeError(f"{name} must be on CUDA, on the device of the others")
+    raise RuntimeError(f"{name} must be on CUDA, on the device of the others")
 
 
 def kv_copy(pool, src_dev, dst_dev) -> None:
@@ -809,7 +824,7 @@ def kv_find_free(ref_counts, n: int):
     L = lib("free block search HIP kernel")
     index = ref_counts.get_device()
     _check_state("ref_counts", ref_counts, 1, index)
-    out = torch.empty(n, dtype=torch.int32, device=ref_counts.device)
+    out = ref_counts.new_empty(n)
     with _DeviceGuard(index):
         check(L.hs_kv_find_free(ref_counts.data_ptr(), ref_counts.numel(), out.data_ptr(), n,
                                 _stream_at(index)))
@@ -829,7 +844,7 @@ def kv_fork(pool, block_tables, context_lens, ref_counts, parents, children, fre
         raise RuntimeError("context_lens must have one entry per table row, ref_counts one per block")
     if children.numel() != n or fresh.numel() != n:
         raise RuntimeError("parents, children and fresh must have the same length")
-    forked = torch.empty(n, dtype=torch.int32, device=pool.device)
+    forked = ref_counts.new_empty(n)
     with _DeviceGuard(index):
         check(L.hs_kv_fork(pool.data_ptr(), *_pages(pool), pool.shape[3], block_tables.data_ptr(), B, MB,
                            context_lens.data_ptr(), ref_counts.data_ptr(), parents.data_ptr(),
@@ -862,7 +877,7 @@ def kv_compact(pool, block_tables, ref_counts):
     if ref_counts.numel() != NB:
         raise RuntimeError("ref_counts must have one entry per block")
     need = L.hs_kv_compact_workspace_bytes(NB)
-    made = torch.empty(NB + 1 + (need + 3) // 4, dtype=torch.int32, device=pool.device)
+    made = ref_counts.new_empty(NB + 1 + (need + 3) // 4)
     moved_to, live, ws = made[:NB], made[NB:NB + 1], made[NB + 1:]
     with _DeviceGuard(index):
         check(L.hs_kv_compact(pool.data_ptr(), *_pages(pool), block_tables.data_ptr(),

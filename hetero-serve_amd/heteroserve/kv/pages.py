@@ -42,9 +42,9 @@ def copy_blocks(pool, src_ids, dst_ids) -> None:
         raise RuntimeError(f"{n} source blocks for {len(dst)} destinations")
     if n == 0:
         return
-    if len(np.unique(dst)) != n:
+    if _repeats(dst):
         raise RuntimeError("a destination block repeats")
-    if np.isin(dst, src).any():
+    if not set(dst.tolist()).isdisjoint(src.tolist()):
         raise RuntimeError("a block is both source and destination")
     if 2 * n <= _hip.HOST_IDS:
         _hip.kv_copy_host_ids(pool, _ids_array(src), _ids_array(dst))
@@ -65,11 +65,12 @@ def find_free_blocks(ref_counts, n: int):
 def _indexes(values, size: int, what: str, device):
     """(int32 device tensor, host array or None): host values are checked and
     wrapped as torch indexing does."""
-    import numpy as np
     import torch
 
     if torch.is_tensor(values) and values.is_cuda:
-        return _hip._int32_on(values.reshape(-1), device), None
+        return _hip._int32_on(values if values.dim() == 1 else values.reshape(-1), device), None
+    import numpy as np
+
     host = np.asarray(values.tolist() if torch.is_tensor(values) else values).reshape(-1)
     if host.size and host.dtype.kind not in "iu":
         raise RuntimeError(f"{what} must be integers, got {host.dtype}")
@@ -80,6 +81,10 @@ def _indexes(values, size: int, what: str, device):
         raise IndexError(f"{what} index {i} is out of bounds for size {size}")
     host = np.where(host < 0, host + size, host)
     return torch.from_numpy(host.astype(np.int32)).to(device), host
+
+
+def _repeats(ids) -> bool:
+    return len(set(ids.tolist())) != len(ids)
 
 
 def fork_blocks(pool, block_tables, context_lens, ref_counts, parents, children, fresh):
@@ -93,8 +98,6 @@ def fork_blocks(pool, block_tables, context_lens, ref_counts, parents, children,
 
     A parent may have several children.  Children must be rows that hold no
     blocks, and must not repeat nor be parents; fresh blocks must not repeat."""
-    import numpy as np
-
     _hip.lib("KV fork HIP kernel")
     _check_pool(pool)
     if block_tables.dim() != 2:
@@ -103,11 +106,11 @@ def fork_blocks(pool, block_tables, context_lens, ref_counts, parents, children,
     parents, host_p = _indexes(parents, B, "parent row", dev)
     children, host_c = _indexes(children, B, "child row", dev)
     fresh, host_f = _indexes(fresh, pool.shape[2], "fresh block", dev)
-    if host_c is not None and len(np.unique(host_c)) != len(host_c):
+    if host_c is not None and _repeats(host_c):
         raise RuntimeError("a child row repeats")
-    if host_f is not None and len(np.unique(host_f)) != len(host_f):
+    if host_f is not None and _repeats(host_f):
         raise RuntimeError("a fresh block repeats")
-    if host_c is not None and host_p is not None and np.isin(host_c, host_p).any():
+    if host_c is not None and host_p is not None and not set(host_c.tolist()).isdisjoint(host_p.tolist()):
         raise RuntimeError("a row is both parent and child")
     return _hip.kv_fork(pool, block_tables, context_lens, ref_counts, parents, children, fresh)
 
