@@ -10,11 +10,12 @@
 // the highest live blocks into the lowest holes.  Counts change by integer
 // atomics, whose order changes no result.
 //
-// The copies are HBM-bound, 4 KiB a workgroup at a time as in the migration's
-// pack (hs_pack.hip); everything else is a few microseconds of latency, so each
-// operation is one launch (a compaction two).  The scans need each chunk's number
+// The copies are HBM-bound (copies of 128 blocks of 32 layers, 537 MB read and written:
+// 95.6 us, 5.6 TB/s; a large copy reaches 6.6); everything else is a few microseconds
+// of latency, so each operation is one launch (a compaction two).  The scans need each chunk's number
 // of blocks before it: every workgroup counts them itself, a stream of reads
-// from L2, which is shorter than a second launch would be.
+// from L2, which is shorter than a second launch would be (131072 blocks: 8.7 us in
+// all, 18 with one load in flight a thread).
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
 #include "hs_private.h"
@@ -46,6 +47,33 @@ __device__ inline void copy_piece(const uint8_t* src, uint8_t* dst, int64_t byte
   }
 }
 
+// Workgroup b of n runs on XCD b % 8: each XCD takes one contiguous run of the jobs
+// (128 blocks of 32 layers, 32-KB pages: 100.9 us in grid order, 95.6 so; whole pages a
+// workgroup 101.2; stores without the streaming hint 101.2).
+__device__ inline int64_t xcd_run(int64_t b, int64_t n) {
+  const int64_t x = b % 8, q = n / 8, r = n % 8;
+  return x * q + (x < r ? x : r) + b / 8;
+}
+
+// `bytes` by one workgroup, 8 loads of a thread at a time.
+template <bool kVec>
+__device__ inline void copy_bytes(const uint8_t* src, uint8_t* dst, int64_t bytes) {
+  if constexpr (kVec) {
+    constexpr int kU = 8;
+    for (int64_t base = (int64_t)threadIdx.x * 16; base < bytes; base += kU * kPiece) {
+      uint4 v[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (base + u * kPiece < bytes) v[u] = load16_stream(src + base + u * kPiece);
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (base + u * kPiece < bytes) store16_stream(dst + base + u * kPiece, v[u]);
+    }
+  } else {
+    for (int64_t off = threadIdx.x; off < bytes; off += kCopyThreads) dst[off] = src[off];
+  }
+}
+
 // ---- copies inside the pool -------------------------------------------------
 
 struct PairsInMemory {
@@ -64,7 +92,7 @@ template <bool kVec, typename Pairs>
 __global__ __launch_bounds__(kCopyThreads) void copy_blocks_kernel(uint8_t* pool, Pairs ids, int L2,
                                                                    int NB, int64_t page,
                                                                    int64_t pieces) {
-  const int64_t w = blockIdx.x;
+  const int64_t w = xcd_run(blockIdx.x, gridDim.x);
   const int64_t pg = w / pieces, piece = w - pg * pieces;
   const int64_t i = pg / L2, lc = pg - i * L2;
   const int64_t s = ids.from(i), d = ids.to(i);
@@ -108,20 +136,30 @@ __device__ inline int block_scan(int x, int* part, int& total) {
   return before + inc - x;
 }
 
-// Live blocks among the first `n` (n a multiple of kScanChunk or NB), this
-// thread's share.
-__device__ inline int count_live(const int32_t* refs, int n) {
+// Live blocks among [first, end), this thread's share; first is a multiple of
+// kScanChunk, so 16-byte loads start as aligned as refs does (vec).
+__device__ inline int count_live(const int32_t* refs, int first, int end, bool vec) {
   int live = 0;
-  for (int i = threadIdx.x; i < n; i += kScanThreads) live += refs[i] > 0;
+  int i = first;
+  if (vec) {
+    const int4* v = reinterpret_cast<const int4*>(refs) + threadIdx.x;
+#pragma unroll 8
+    for (; i + kScanChunk <= end; i += kScanChunk) {
+      const int4 x = v[i / 4];
+      live += (x.x > 0) + (x.y > 0) + (x.z > 0) + (x.w > 0);
+    }
+  }
+#pragma unroll 4
+  for (i += threadIdx.x; i < end; i += kScanThreads) live += refs[i] > 0;
   return live;
 }
 
 // out[0 .. n): the lowest free blocks, -1 past the last.
 __global__ __launch_bounds__(kScanThreads) void find_free_kernel(const int32_t* refs, int NB,
-                                                                 int32_t* out, int n) {
+                                                                 int32_t* out, int n, bool vec) {
   __shared__ int part[kScanThreads / 64];
   const int first = blockIdx.x * kScanChunk;
-  const int before = first - block_sum(count_live(refs, first), part);   // free blocks
+  const int before = first - block_sum(count_live(refs, 0, first, vec), part);   // free blocks
   const bool last = blockIdx.x == gridDim.x - 1;
   if (before >= n && !last) return;
   const int i0 = first + threadIdx.x * kScanPer;
@@ -181,19 +219,20 @@ __device__ inline bool fork_plan(const ForkArgs& a, int i, ForkPlan& p) {
   return true;
 }
 
-// y 0: the child's table row and the counts; y 1 + (l, c) * pieces + piece: a
-// piece of the tokens of the last block.
+// y 0: the child's table row and the counts; y 1 + (l, c): the tokens of the last
+// block's page, whose loads are all on their way behind one walk of dependent reads
+// (us, a workgroup per 4 KB / per page: 16 children, 32 layers, 32-KB pages 12.5 / 5.7, 64
+// children 42 / 27).
 template <bool kVec>
-__global__ __launch_bounds__(kCopyThreads) void fork_kernel(ForkArgs a, int pieces) {
+__global__ __launch_bounds__(kCopyThreads) void fork_kernel(ForkArgs a) {
   const int i = blockIdx.x;
   ForkPlan p;
   const bool ok = fork_plan(a, i, p);
   if (blockIdx.y > 0) {
     if (!ok || !p.rem) return;
-    const int job = blockIdx.y - 1;
-    const int64_t lc = job / pieces;
-    copy_piece(a.pool + (lc * a.NB + p.last) * a.page, a.pool + (lc * a.NB + p.fresh) * a.page,
-               a.page / a.BS * p.rem, job % pieces, kVec);
+    const int64_t lc = blockIdx.y - 1;
+    copy_bytes<kVec>(a.pool + (lc * a.NB + p.last) * a.page, a.pool + (lc * a.NB + p.fresh) * a.page,
+                     a.page / a.BS * p.rem);
     return;
   }
   if (threadIdx.x == 0) a.forked[i] = ok;
@@ -240,12 +279,12 @@ struct CompactPlan {
 };
 
 __global__ __launch_bounds__(kScanThreads) void compact_plan_kernel(const int32_t* refs, int NB,
-                                                                    CompactPlan p, int32_t* live_out) {
+                                                                    CompactPlan p, int32_t* live_out,
+                                                                    bool vec) {
   __shared__ int part[kScanThreads / 64];
   const int first = blockIdx.x * kScanChunk;
-  const int own_before = count_live(refs, first);
-  int rest = 0;
-  for (int i = first + threadIdx.x; i < NB; i += kScanThreads) rest += refs[i] > 0;
+  const int own_before = count_live(refs, 0, first, vec);
+  const int rest = count_live(refs, first, NB, vec);
   const int before = block_sum(own_before, part);
   const int live = before + block_sum(rest, part);
   const int i0 = first + threadIdx.x * kScanPer;
@@ -286,8 +325,7 @@ __global__ __launch_bounds__(kScanThreads) void compact_plan_kernel(const int32_
 
 template <bool kVec>
 __global__ __launch_bounds__(kCopyThreads) void compact_move_kernel(uint8_t* pool, int L2, int NB,
-                                                                    int64_t page, int64_t pieces,
-                                                                    int32_t* bt, int64_t entries,
+                                                                    int64_t page, int32_t* bt, int64_t entries,
                                                                     int32_t* refs, CompactPlan p,
                                                                     int32_t* moved_to) {
   const int moves = *p.n;
@@ -307,12 +345,10 @@ __global__ __launch_bounds__(kCopyThreads) void compact_move_kernel(uint8_t* poo
     refs[p.hole[i]] = refs[m];
     refs[m] = 0;
   }
-  const int64_t jobs = (int64_t)moves * L2 * pieces;
+  const int64_t jobs = (int64_t)moves * L2;
   for (int64_t w = blockIdx.x; w < jobs; w += gridDim.x) {
-    const int64_t pg = w / pieces, piece = w - pg * pieces;
-    const int64_t i = pg / L2, lc = pg - i * L2;
-    copy_piece(pool + (lc * NB + p.mover[i]) * page, pool + (lc * NB + p.hole[i]) * page, page, piece,
-               kVec);
+    const int64_t i = w / L2, lc = w - i * L2;
+    copy_bytes<kVec>(pool + (lc * NB + p.mover[i]) * page, pool + (lc * NB + p.hole[i]) * page, page);
   }
 }
 
@@ -361,25 +397,23 @@ int launch_find_free(const int32_t* refs, int NB, int32_t* out, int n, hipStream
   if (NB > kMaxScan)
     return fail(HS_EUNSUPPORTED, "at most " + std::to_string(kMaxScan) + " blocks in a scan");
   hipLaunchKernelGGL(find_free_kernel, dim3((unsigned)chunks), dim3(kScanThreads), 0, stream, refs, NB,
-                     out, n);
+                     out, n, aligned16(refs));
   return check_launch("free block search");
 }
 
 int launch_fork(void* pool, int L, int NB, int64_t page, int BS, int32_t* bt, int B, int MB,
                 int32_t* ctx, int32_t* refs, const int32_t* parents, const int32_t* children,
                 const int32_t* fresh, int n, int32_t* forked, hipStream_t stream) {
-  const int64_t pieces = ceil_div(page, kPiece);
-  const int64_t jobs = sat_mul(2, L, pieces);
   if (!pool_fits(L, NB, page)) return fail(HS_EUNSUPPORTED, "pool too large for 64-bit offsets");
-  if (jobs > 65534) return fail(HS_EUNSUPPORTED, "fork grid too large");
+  if (L > 32767) return fail(HS_EUNSUPPORTED, "fork grid too large");
   ForkArgs a{static_cast<uint8_t*>(pool), 2 * L, NB, BS, page, bt, ctx, refs, parents, children, fresh,
              forked, B, MB};
-  const dim3 g((unsigned)n, (unsigned)(1 + jobs)), t(kCopyThreads);
+  const dim3 g((unsigned)n, (unsigned)(1 + 2 * L)), t(kCopyThreads);
   profile_begin(stream);
   if (pool_vec(pool, page) && page / BS % 16 == 0)
-    hipLaunchKernelGGL(fork_kernel<true>, g, t, 0, stream, a, (int)pieces);
+    hipLaunchKernelGGL(fork_kernel<true>, g, t, 0, stream, a);
   else
-    hipLaunchKernelGGL(fork_kernel<false>, g, t, 0, stream, a, (int)pieces);
+    hipLaunchKernelGGL(fork_kernel<false>, g, t, 0, stream, a);
   profile_end(stream);
   return check_launch("kv fork");
 }
@@ -397,25 +431,27 @@ int64_t compact_workspace_bytes(int NB) { return sat_mul(sat_add(sat_mul(3, NB),
 
 int launch_compact(void* pool, int L, int NB, int64_t page, int32_t* bt, int B, int MB, int32_t* refs,
                    int32_t* moved_to, int32_t* live, void* workspace, int cus, hipStream_t stream) {
-  const int64_t pieces = ceil_div(page, kPiece);
-  if (!pool_fits(L, NB, page) || sat_mul(NB, 2, L, pieces) == INT64_MAX)
+  if (!pool_fits(L, NB, page))
     return fail(HS_EUNSUPPORTED, "pool too large for 64-bit offsets");
   if (NB > kMaxScan)
     return fail(HS_EUNSUPPORTED, "at most " + std::to_string(kMaxScan) + " blocks in a scan");
   int32_t* ws = static_cast<int32_t*>(workspace);
   const CompactPlan p{ws, ws + 64, ws + 64 + (int64_t)NB, ws + 64 + 2 * (int64_t)NB};
   hipLaunchKernelGGL(compact_plan_kernel, dim3((unsigned)ceil_div(NB, kScanChunk)), dim3(kScanThreads), 0,
-                     stream, refs, NB, p, live);
-  // the number of moves stays on the device: resident workgroups take them in turn
-  const dim3 g((unsigned)(8 * cus)), t(kCopyThreads);
+                     stream, refs, NB, p, live, aligned16(refs));
+  // The number of moves, at most NB / 2, stays on the device, so up to 64 workgroups a CU
+  // take the pages in turn.  32 layers, 432 moves of 32-KB pages, us at 8 / 64 / 512: 190 /
+  // 173 / 166; without a move 7 / 10 / 35.
+  const int64_t most = sat_mul((NB + 1) / 2, 2, L);
+  const dim3 g((unsigned)std::min((int64_t)64 * cus, std::max((int64_t)cus, most))), t(kCopyThreads);
   uint8_t* pl = static_cast<uint8_t*>(pool);
   const int64_t entries = (int64_t)B * MB;
   profile_begin(stream);
   if (pool_vec(pool, page))
-    hipLaunchKernelGGL(compact_move_kernel<true>, g, t, 0, stream, pl, 2 * L, NB, page, pieces, bt, entries,
+    hipLaunchKernelGGL(compact_move_kernel<true>, g, t, 0, stream, pl, 2 * L, NB, page, bt, entries,
                        refs, p, moved_to);
   else
-    hipLaunchKernelGGL(compact_move_kernel<false>, g, t, 0, stream, pl, 2 * L, NB, page, pieces, bt,
+    hipLaunchKernelGGL(compact_move_kernel<false>, g, t, 0, stream, pl, 2 * L, NB, page, bt,
                        entries, refs, p, moved_to);
   profile_end(stream);
   return check_launch("kv compaction");
