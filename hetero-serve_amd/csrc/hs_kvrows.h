@@ -124,6 +124,11 @@ struct RowMap {
   }
 };
 
+// A launch holds fewer than 2^32 work-items along x.
+inline bool grid_fits(int64_t workgroups, int threads) {
+  return workgroups < ((int64_t)1 << 32) / threads;
+}
+
 inline int dtype_bytes(int code) { return code == HS_DTYPE_F32 ? 4 : 2; }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -89,13 +89,13 @@ struct PairsInArguments {
 
 // Workgroup w copies piece (w % pieces) of page (w / pieces) = (i * 2 L) + (l, c).
 template <bool kVec, typename Pairs>
-__global__ __launch_bounds__(kCopyThreads) void copy_blocks_kernel(uint8_t* pool, Pairs ids, int L2,
-                                                                   int NB, int64_t page,
+__global__ __launch_bounds__(kCopyThreads) void copy_blocks_kernel(uint8_t* pool, Pairs ids, int first,
+                                                                   int L2, int NB, int64_t page,
                                                                    int64_t pieces) {
   const int64_t w = xcd_run(blockIdx.x, gridDim.x);
   const int64_t pg = w / pieces, piece = w - pg * pieces;
   const int64_t i = pg / L2, lc = pg - i * L2;
-  const int64_t s = ids.from(i), d = ids.to(i);
+  const int64_t s = ids.from(first + i), d = ids.to(first + i);
   if (s < 0 || s >= NB || d < 0 || d >= NB) return;
   copy_piece(pool + (lc * NB + s) * page, pool + (lc * NB + d) * page, page, piece, kVec);
 }
@@ -359,16 +359,22 @@ bool pool_vec(const void* pool, int64_t page) { return page % 16 == 0 && aligned
 template <typename Pairs>
 int launch_copy(void* pool, int L, int NB, int64_t page, const Pairs& ids, int n, hipStream_t stream) {
   const int64_t pieces = ceil_div(page, kPiece);
-  const int64_t grid = sat_mul(n, L, 2, pieces);
-  if (grid > 0x7fffffffLL) return fail(HS_EUNSUPPORTED, "page copy grid too large");
+  const int64_t per_block = sat_mul(2, L, pieces);
+  if (!grid_fits(per_block, kCopyThreads)) return fail(HS_EUNSUPPORTED, "page copy grid too large");
   if (!pool_fits(L, NB, page)) return fail(HS_EUNSUPPORTED, "pool too large for 64-bit offsets");
   uint8_t* p = static_cast<uint8_t*>(pool);
-  const dim3 g((unsigned)grid), t(kCopyThreads);
+  // as many blocks as one launch holds (64 GiB of copies)
+  const int most = (int)std::min((int64_t)n, (((int64_t)1 << 32) / kCopyThreads - 1) / per_block);
   profile_begin(stream);
-  if (pool_vec(pool, page))
-    hipLaunchKernelGGL((copy_blocks_kernel<true, Pairs>), g, t, 0, stream, p, ids, 2 * L, NB, page, pieces);
-  else
-    hipLaunchKernelGGL((copy_blocks_kernel<false, Pairs>), g, t, 0, stream, p, ids, 2 * L, NB, page, pieces);
+  for (int first = 0; first < n; first += std::min(most, n - first)) {
+    const dim3 g((unsigned)(std::min(most, n - first) * per_block)), t(kCopyThreads);
+    if (pool_vec(pool, page))
+      hipLaunchKernelGGL((copy_blocks_kernel<true, Pairs>), g, t, 0, stream, p, ids, first, 2 * L, NB, page,
+                         pieces);
+    else
+      hipLaunchKernelGGL((copy_blocks_kernel<false, Pairs>), g, t, 0, stream, p, ids, first, 2 * L, NB, page,
+                         pieces);
+  }
   profile_end(stream);
   return check_launch("kv copy");
 }
@@ -405,7 +411,7 @@ int launch_fork(void* pool, int L, int NB, int64_t page, int BS, int32_t* bt, in
                 int32_t* ctx, int32_t* refs, const int32_t* parents, const int32_t* children,
                 const int32_t* fresh, int n, int32_t* forked, hipStream_t stream) {
   if (!pool_fits(L, NB, page)) return fail(HS_EUNSUPPORTED, "pool too large for 64-bit offsets");
-  if (L > 32767) return fail(HS_EUNSUPPORTED, "fork grid too large");
+  if (L > 32767 || !grid_fits(n, kCopyThreads)) return fail(HS_EUNSUPPORTED, "fork grid too large");
   ForkArgs a{static_cast<uint8_t*>(pool), 2 * L, NB, BS, page, bt, ctx, refs, parents, children, fresh,
              forked, B, MB};
   const dim3 g((unsigned)n, (unsigned)(1 + 2 * L)), t(kCopyThreads);
@@ -421,7 +427,8 @@ int launch_fork(void* pool, int L, int NB, int64_t page, int BS, int32_t* bt, in
 int launch_free(int32_t* bt, int B, int MB, int32_t* ctx, int32_t* refs, int NB, const int32_t* rows,
                 int n, hipStream_t stream) {
   const int64_t chunks = ceil_div(MB, kCopyThreads);
-  if (chunks > 65535) return fail(HS_EUNSUPPORTED, "block table too wide for one launch");
+  if (chunks > 65535 || !grid_fits(n, kCopyThreads))
+    return fail(HS_EUNSUPPORTED, "block table too wide, or too many rows, for one launch");
   hipLaunchKernelGGL(free_kernel, dim3((unsigned)n, (unsigned)chunks), dim3(kCopyThreads), 0, stream, bt,
                      ctx, refs, rows, B, MB, NB);
   return check_launch("kv free");

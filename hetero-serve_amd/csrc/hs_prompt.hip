@@ -370,8 +370,9 @@ struct Task {
     if (!find_tile(a, rows, (int)(blockIdx.x / a.H), b, qt)) return false;
     // wave-uniform, and the loop's bounds with them
     seq_rows(a, __builtin_amdgcn_readfirstlane(b), row0, len);
-    q0 = __builtin_amdgcn_readfirstlane(qt) * rows;
-    return true;
+    qt = __builtin_amdgcn_readfirstlane(qt);
+    q0 = qt * rows;
+    return qt >= 0 && q0 < len;   // (cu that overlaps can count past 32 bits)
   }
 };
 
@@ -812,7 +813,7 @@ int launch_dim(const PromptArgs& a, int cus, hipStream_t stream) {
   constexpr bool kSplits = 2 * 4 * kBN * D * sizeof(T) <= 160 * 1024;   // two tiles of keys a step fit the LDS
   const bool split = kSplits && sat_mul(tiles_of(a, 128), a.H) <= cus;
   const int64_t grid = sat_mul(tiles_of(a, split ? 64 : 128), a.H);
-  if (grid > 0x7fffffffLL) return fail(HS_EUNSUPPORTED, "prompt grid too large");
+  if (!grid_fits(grid, kThreads)) return fail(HS_EUNSUPPORTED, "prompt grid too large");
   if constexpr (kSplits) {
     if (split) {
       launch_one<T, D, kBN, 2>(a, grid, stream);

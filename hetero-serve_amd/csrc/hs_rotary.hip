@@ -17,9 +17,14 @@
 //
 // A workgroup takes a few rows (tokens).  Its threads first fill LDS with the
 // sines and cosines, one (row, pair) each, which all heads of a row then share;
-// then each thread turns 8 pairs at a time (two 16-byte loads of a 16-bit
-// source).  Sizes or addresses that are no multiples of 16 bytes take one pair
+// then each thread turns the pairs of two 16-byte loads.  Sizes or addresses that are no multiples of 16 bytes take one pair
 // at a time.
+//
+// Bound by HBM: 8192 rows of 32 / 8 heads, D 128, bf16 in and out (218 MB), 39 us,
+// 5.6 TB/s (a large copy reaches 6.6), with loads that leave the cache in front of
+// HBM to what is written, 47 without that hint.  A decode step's few rows take 4.3 us,
+// a launch and two dependent reads.  A thread per unit of a row, with several rows'
+// loads in flight, was no faster (50 us).
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
 
@@ -65,97 +70,113 @@ __device__ inline void fill_angles(const RotaryArgs& a, int64_t row0, int rows, 
   __syncthreads();
 }
 
+__device__ inline void turn(float& a, float& b, float c, float s) {
+  const float p = a;
+  a = p * c - b * s;
+  b = b * c + p * s;
+}
+
+// N elements (4 or 8) from fp32, each rounded once.
+template <typename T, int N>
+__device__ inline void store(uint8_t* p, const float* x) {
+  if constexpr (N == 8) {
+    Codec<T>::store8(p, x);
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    float y[8] = {x[0], x[1], x[2], x[3], 0.0f, 0.0f, 0.0f, 0.0f};
+    uint4 w;
+    Codec<T>::store8(reinterpret_cast<uint8_t*>(&w), y);
+    *reinterpret_cast<uint2*>(p) = make_uint2(w.x, w.y);
+  }
+}
+
+// A unit is two 16-byte loads: the same place in both halves of a head's turned part
+// (which pairs up the elements, or, interleaved, holds whole pairs), of the part that
+// passes, or of a value's head.  Neighbouring lanes read neighbouring 16 bytes.
 template <typename S, typename O, typename C>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotaryArgs a) {
   extern __shared__ __align__(16) uint8_t lds[];
+  constexpr int kV = Elem<S>::kVec, kS = Codec<S>::kBytes, kO = Codec<O>::kBytes, kC = Codec<C>::kBytes;
   const int64_t row0 = (int64_t)blockIdx.x * a.rows;
   const int rows = (int)min((int64_t)a.rows, a.n - row0);
   float2* cs = reinterpret_cast<float2*>(lds);                          // [rows, pairs]
   int64_t* slot = reinterpret_cast<int64_t*>(cs + a.rows * a.pairs);   // [rows]
   fill_angles(a, row0, rows, cs, slot);
 
-  const uint32_t per_head = (uint32_t)a.D / 16;   // groups of 16 elements
+  const uint32_t per_head = (uint32_t)a.D / (2 * kV);
   const uint32_t heads = (uint32_t)(a.H + (a.v ? 2 : 1) * a.Hkv);
   const uint32_t per_row = heads * per_head;
+  const int turned_units = a.pairs / kV;
   for (uint32_t u = blockIdx.y * kRotThreads + threadIdx.x; u < per_row * (uint32_t)rows;
        u += gridDim.y * kRotThreads) {
     const uint32_t r = u / per_row, in_row = u - r * per_row;
-    const uint32_t head = in_row / per_head, g = in_row - head * per_head;
+    const uint32_t head = in_row / per_head;
+    const int g = (int)(in_row - head * per_head);
     const int64_t row = row0 + r;
     if (head >= (uint32_t)(a.H + a.Hkv)) {   // a value: cast (or copied) into the cache
       const int64_t sl = slot[r];
       if (sl < 0) continue;
-      const int64_t e = (int64_t)(head - a.H - a.Hkv) * a.D + 16 * g;
-      const uint8_t* src = a.v + row * a.v_row + e * Codec<S>::kBytes;
-      uint8_t* dst = a.v_cache + (sl * ((int64_t)a.Hkv * a.D) + e) * Codec<C>::kBytes;
-      if constexpr (std::is_same<S, C>::value) {   // a bit copy (NaN payloads included)
-        uint4 w[Codec<S>::kBytes];
+      const uint32_t h = head - a.H - a.Hkv;
+      const uint8_t* src = a.v + row * a.v_row + ((int64_t)h * a.D + kV * g) * kS;
+      uint8_t* dst = a.v_cache + ((sl * a.Hkv + h) * (int64_t)a.D + kV * g) * kC;
+      const uint4 w[2] = {load16_stream(src), load16_stream(src + a.D / 2 * kS)};
 #pragma unroll
-        for (int b = 0; b < Codec<S>::kBytes; ++b) w[b] = load16(src + 16 * b);
-#pragma unroll
-        for (int b = 0; b < Codec<S>::kBytes; ++b) *reinterpret_cast<uint4*>(dst + 16 * b) = w[b];
-      } else {
-        float x[16];
-        Codec<S>::load8(src, x);
-        Codec<S>::load8(src + 8 * Codec<S>::kBytes, x + 8);
-        Codec<C>::store8(dst, x);
-        Codec<C>::store8(dst + 8 * Codec<C>::kBytes, x + 8);
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (std::is_same<S, C>::value) {   // a bit copy (NaN payloads included)
+          *reinterpret_cast<uint4*>(dst + i * (a.D / 2) * kC) = w[i];
+        } else {
+          float x[kV];
+          Elem<S>::to_f32(w[i], x);
+          store<C, kV>(dst + i * (a.D / 2) * kC, x);
+        }
       }
       continue;
     }
-    const bool is_q = head < (uint32_t)a.H;
+    const bool is_q = head < (uint32_t)a.H, turned = g < turned_units;
     const uint32_t h = is_q ? head : head - a.H;
-    const bool turned = g < (uint32_t)a.pairs / 8;
-    int e0, e1;   // the two groups of 8 elements
-    if (turned && !a.interleaved) {
-      e0 = 8 * g;
-      e1 = a.pairs + e0;
-    } else {
-      e0 = turned ? 16 * g : 2 * a.pairs + 16 * (g - a.pairs / 8);
-      e1 = e0 + 8;
+    const int e0 = kV * g + (turned ? 0 : a.pairs);   // behind both halves of the turned part
+    const int e1 = e0 + (turned ? a.pairs : a.D / 2 - a.pairs);
+    const uint8_t* src = (is_q ? a.q + row * a.q_row : a.k + row * a.k_row) + (int64_t)h * a.D * kS;
+    float x[kV], y[kV];
+    {
+      const uint4 w0 = load16_stream(src + e0 * kS), w1 = load16_stream(src + e1 * kS);
+      Elem<S>::to_f32(w0, x);
+      Elem<S>::to_f32(w1, y);
     }
-    const uint8_t* src = (is_q ? a.q + row * a.q_row : a.k + row * a.k_row) +
-                         (int64_t)h * a.D * Codec<S>::kBytes;
-    float x[8], y[8];
-    Codec<S>::load8(src + e0 * Codec<S>::kBytes, x);
-    Codec<S>::load8(src + e1 * Codec<S>::kBytes, y);
     if (turned) {
-      float2 t[8];
-      const float4* c4 = reinterpret_cast<const float4*>(cs + r * a.pairs + 8 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 w = c4[i];
-        t[2 * i] = make_float2(w.x, w.y);
-        t[2 * i + 1] = make_float2(w.z, w.w);
-      }
+      const float2* t = cs + r * a.pairs;
       if (a.interleaved) {
+        const float4* t0 = reinterpret_cast<const float4*>(t + e0 / 2);
+        const float4* t1 = reinterpret_cast<const float4*>(t + e1 / 2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = x[2 * i], q = x[2 * i + 1], v = y[2 * i], w = y[2 * i + 1];
-          x[2 * i] = p * t[i].x - q * t[i].y;
-          x[2 * i + 1] = q * t[i].x + p * t[i].y;
-          y[2 * i] = v * t[4 + i].x - w * t[4 + i].y;
-          y[2 * i + 1] = w * t[4 + i].x + v * t[4 + i].y;
+        for (int i = 0; i < kV / 4; ++i) {
+          const float4 c0 = t0[i], c1 = t1[i];
+          turn(x[4 * i], x[4 * i + 1], c0.x, c0.y);
+          turn(x[4 * i + 2], x[4 * i + 3], c0.z, c0.w);
+          turn(y[4 * i], y[4 * i + 1], c1.x, c1.y);
+          turn(y[4 * i + 2], y[4 * i + 3], c1.z, c1.w);
         }
       } else {
+        const float4* t0 = reinterpret_cast<const float4*>(t + e0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = x[i], q = y[i];
-          x[i] = p * t[i].x - q * t[i].y;
-          y[i] = q * t[i].x + p * t[i].y;
+        for (int i = 0; i < kV / 2; ++i) {
+          const float4 c = t0[i];
+          turn(x[2 * i], y[2 * i], c.x, c.y);
+          turn(x[2 * i + 1], y[2 * i + 1], c.z, c.w);
         }
       }
     }
     uint8_t* out = is_q ? a.q_out : a.k_out;
     if (out) {
-      uint8_t* dst = out + ((row * (is_q ? a.H : a.Hkv) + h) * (int64_t)a.D) * Codec<O>::kBytes;
-      Codec<O>::store8(dst + e0 * Codec<O>::kBytes, x);
-      Codec<O>::store8(dst + e1 * Codec<O>::kBytes, y);
+      uint8_t* dst = out + ((row * (is_q ? a.H : a.Hkv) + h) * (int64_t)a.D) * kO;
+      store<O, kV>(dst + e0 * kO, x);
+      store<O, kV>(dst + e1 * kO, y);
     }
     if (!is_q && a.v && slot[r] >= 0) {
-      uint8_t* dst = a.k_cache + (slot[r] * ((int64_t)a.Hkv * a.D) + (int64_t)h * a.D) * Codec<C>::kBytes;
-      Codec<C>::store8(dst + e0 * Codec<C>::kBytes, x);
-      Codec<C>::store8(dst + e1 * Codec<C>::kBytes, y);
+      uint8_t* dst = a.k_cache + ((slot[r] * a.Hkv + h) * (int64_t)a.D) * kC;
+      store<C, kV>(dst + e0 * kC, x);
+      store<C, kV>(dst + e1 * kC, y);
     }
   }
 }
@@ -201,10 +222,9 @@ __global__ __launch_bounds__(kRotThreads) void rotary_scalar_kernel(RotaryArgs a
                          (int64_t)h * a.D * Codec<S>::kBytes;
     float x = Codec<S>::load1(src + e0 * Codec<S>::kBytes), y = x;
     if (turned) {
-      const float p = x, q = Codec<S>::load1(src + e1 * Codec<S>::kBytes);
       const float2 t = cs[r * a.pairs + i];
-      x = p * t.x - q * t.y;
-      y = q * t.x + p * t.y;
+      y = Codec<S>::load1(src + e1 * Codec<S>::kBytes);
+      turn(x, y, t.x, t.y);
     }
     uint8_t* out = is_q ? a.q_out : a.k_out;
     if (out) {
@@ -295,15 +315,14 @@ int launch_rotary(const Rotary& w, hipStream_t stream, int cus) {
   l.vec = w.D % 16 == 0 && w.pairs % 8 == 0 && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) &&
           a.q_row % 16 == 0 && a.k_row % 16 == 0 && a.v_row % 16 == 0 && aligned16(a.q_out) &&
           aligned16(a.k_out) && aligned16(a.k_cache) && aligned16(a.v_cache);
-  // Rows of a workgroup: as many as give its threads one (row, pair) each, where
-  // that leaves every CU several workgroups; single rows, spread over several
-  // workgroups, otherwise.
-  const int64_t units = l.vec ? per_row / 16 : per_row;
-  const int together = std::max(1, std::min(8, kRotThreads / w.pairs));
-  a.rows = w.n >= (int64_t)together * 4 * cus ? together : 1;
+  // Two rows share a workgroup's set-up where that leaves every CU several
+  // workgroups (8192 rows, 32 / 8 heads, D 128, bf16, us at 1 / 2 / 4 / 8: 46 / 38 / 41 / 44);
+  // otherwise one row is spread over several workgroups.
+  const int64_t units = l.vec ? per_row / (32 / sb) : per_row;
+  a.rows = w.n >= (int64_t)8 * cus ? 2 : 1;
   const int64_t parts = a.rows > 1 ? 1 : std::min((int64_t)64, ceil_div(units, kRotThreads));
   const int64_t groups = ceil_div(w.n, a.rows);
-  if (groups > 0x7fffffffLL) return fail(HS_EUNSUPPORTED, "too many rows for one launch");
+  if (!grid_fits(groups, kRotThreads)) return fail(HS_EUNSUPPORTED, "too many rows for one launch");
   l.grid = dim3((unsigned)groups, (unsigned)parts);
   l.lds = (size_t)a.rows * (8 + 8 * (size_t)w.pairs);
   profile_begin(stream);
