@@ -8,7 +8,7 @@
 // walks the keys once with a running maximum and sum.  K and V tiles go from global
 // memory straight to LDS (two of each; the next ones are on their way while one is
 // used), swizzled by permuting the addresses that the lanes load from, since the LDS
-// side of such a load is linear.  S^T = K Q^T and O^T = V^T P^T: a lane holds one
+// side of such a load is linear (fp32 tiles pass through registers, see Split3).  S^T = K Q^T and O^T = V^T P^T: a lane holds one
 // query's scores, so its maximum and sum need one exchange of the two lane halves,
 // and the probabilities are the second product's operand where they stand.  Rows
 // are 128 and not 256 a workgroup because two workgroups then share a CU: one's
@@ -24,9 +24,9 @@
 // Numerics.  16-bit inputs are multiplied in their own type, the probabilities
 // rounded to it (relative to a maximum that is at most 2^8 too low, so none
 // overflows), and the sum adds the rounded ones, so that the rounding cancels where
-// one key dominates; scores, maxima, sums and O are fp32.  fp32 inputs use the fp32
-// matrix cores.  Scores are scaled in fp32 behind the product, not in the query's type
-// before it.
+// one key dominates; scores, maxima, sums and O are fp32.  fp32 inputs are split into
+// three bf16 terms, which keeps fp32's accuracy (see Split3).  Scores are scaled in fp32
+// behind the product, not in the query's type before it.
 //
 // Masked keys.  A score that a row does not see is -inf and its probability 0, but 0
 // times an infinite or NaN value is NaN in a product.  A row whose result is not
@@ -195,8 +195,7 @@ __device__ inline void load_to_lds(const uint8_t* base, uint32_t offset, uint32_
 
 // Where the 16-byte chunk c of row r lies in its LDS row of kC chunks, so that each
 // reading pattern covers all 64 banks: K rows are read 16 at a time at one chunk, V
-// rows of 16-bit elements 4 at a time at 4 neighbouring chunks, of fp32 elements 2 at
-// a time, 4 rows apart, at 8 neighbouring chunks (which rows of 8 chunks cannot).
+// rows 4 at a time at 4 neighbouring chunks.
 template <int kC>
 struct KPlace {
   static constexpr int kPeriod = 16;   // rows
@@ -207,7 +206,7 @@ struct KPlace {
   }
 };
 template <int kC>
-struct VPlace16 {
+struct VPlace {
   static constexpr int kPeriod = 4;
   __device__ static int at(int r, int c) {
     if constexpr (kC >= 16) return c ^ ((r & 3) << 2);
@@ -215,15 +214,6 @@ struct VPlace16 {
     else return c;
   }
 };
-template <int kC>
-struct VPlace32 {
-  static constexpr int kPeriod = 8;
-  __device__ static int at(int r, int c) {
-    if constexpr (kC >= 16) return c ^ (((r >> 2) & 1) << 3);
-    else return c;
-  }
-};
-
 constexpr int kThreads = 256;
 
 // The loads of K's or V's rows, kKeys at a time; rows past the sequence are read as
@@ -477,7 +467,7 @@ __global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : D == 64 ? 3 : 2)
   constexpr int R = 4 / KS, kC = D / 8, kKeys = KS * kBN, kRowBytes = 2 * D;
   constexpr int kKB = kBN / 32, kDC = D / 16, kDB = D / 32;
   using KLoads = TileLoads<kC, kKeys, KPlace<kC>>;
-  using VLoads = TileLoads<kC, kKeys, VPlace16<kC>>;
+  using VLoads = TileLoads<kC, kKeys, VPlace<kC>>;
   __shared__ __align__(1024) uint8_t lds[2][2][kKeys * kRowBytes];   // [K, V][even, odd tiles]
 
   const int lane = threadIdx.x & 63, j = lane & 31, hh = lane >> 5;
@@ -541,9 +531,9 @@ __global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : D == 64 ? 3 : 2)
     const int d = i % kDB, r = 8 * hh + (vi >> 2), e0 = 32 * d + (j & 16) + 4 * (vi & 3);
     const uint8_t* p = lds[1][odd] + 16 * (i / kDB) * kRowBytes;
     const short4x lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lshort4x*)(p + ((kg * kBN + r) * kRowBytes + 16 * VPlace16<kC>::at(r, e0 / 8) + 2 * (e0 % 8))));
+        (lshort4x*)(p + ((kg * kBN + r) * kRowBytes + 16 * VPlace<kC>::at(r, e0 / 8) + 2 * (e0 % 8))));
     const short4x hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lshort4x*)(p + 4 * kRowBytes + ((kg * kBN + r) * kRowBytes + 16 * VPlace16<kC>::at(r + 4, e0 / 8) + 2 * (e0 % 8))));
+        (lshort4x*)(p + 4 * kRowBytes + ((kg * kBN + r) * kRowBytes + 16 * VPlace<kC>::at(r + 4, e0 / 8) + 2 * (e0 % 8))));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
   // Keys behind the row, in the wave's last tile.
@@ -671,59 +661,116 @@ __global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : D == 64 ? 3 : 2)
   walk_rows<T, D>(a, t, bad, first_row);
 }
 
-// fp32 on v_mfma_f32_32x32x2_f32, 64 cycles each: a tile's products take 8 times as
-// long as in 16-bit types, and the softmax and LDS reads pass beside the other wave's.
-// Lane (j, hh) holds dims 8 c + 4 hh .. + 3 of its key and its query, four products'
-// operands (any order of the dims serves, if both have it); the probability in
-// register r is key 8 (r / 4) + 4 hh + r % 4 of the 32, so that product reads that key's
-// row of V.
-template <int D, int kBN, int KS>
-__global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : 2) void prompt_f32_kernel(PromptArgs a) {
-  constexpr int R = 4 / KS, kC = D / 4, kKeys = KS * kBN, kRowBytes = 4 * D;
-  constexpr int kKB = kBN / 32, kDC = D / 8, kDB = D / 32;
-  using KLoads = TileLoads<kC, kKeys, KPlace<kC>>;
-  using VLoads = TileLoads<kC, kKeys, VPlace32<kC>>;
-  __shared__ __align__(1024) uint8_t lds[2][2][kKeys * kRowBytes];   // [K, V][even, odd tiles]
+// fp32 on the bf16 matrix cores.  An fp32 number is the sum of three bf16 ones, each
+// the leading 8 bits of what is left (cutting, not rounding, makes the remainders
+// exact), so a product of two is six bf16 products,
+//   hh + hm + mh + mm + hl + lh,
+// the three left out being 2^-23 of it on average and 2^-21 at most, no more than what
+// adding 32 products in fp32 may lose.  Numbers below 2^-102 keep fewer bits, bf16 having
+// no smaller terms.  Six 32x32x16 products take 192 cycles
+// where the fp32 ones of the same size (8 of v_mfma_f32_32x32x2_f32) take 512.  K and V
+// are split once for the workgroup, from registers into three planes each in LDS; Q
+// stays split in registers, and the probabilities are split where they stand.  An
+// infinity splits into NaNs: its rows are not finite, and computed again (row_walk).
+// One prompt of 2048 tokens, 32 / 8 heads, D 128: 202 us, 170 TFLOP/s of fp32 products
+// (with the fp32 ones 377); 334 and 1001 tokens, 12 heads, D 64: 26.7 us.
+struct Split3 {
+  uint32_t h, m, l;   // two numbers each
+  __device__ Split3(float x, float y) {
+    const uint32_t xh = __float_as_uint(x) & 0xffff0000u, yh = __float_as_uint(y) & 0xffff0000u;
+    x -= __uint_as_float(xh);
+    y -= __uint_as_float(yh);
+    const uint32_t xm = __float_as_uint(x) & 0xffff0000u, ym = __float_as_uint(y) & 0xffff0000u;
+    x -= __uint_as_float(xm);
+    y -= __uint_as_float(ym);
+    h = __builtin_amdgcn_perm(yh, xh, 0x07060302u);
+    m = __builtin_amdgcn_perm(ym, xm, 0x07060302u);
+    l = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+  }
+};
+
+// acc + a . b, planes h, m, l, the small terms first.
+__device__ inline float16x mma3(const short8x (&a)[3], const short8x (&b)[3], float16x acc) {
+  acc = Half<Bf16>::mma(a[2], b[0], acc);
+  acc = Half<Bf16>::mma(a[0], b[2], acc);
+  acc = Half<Bf16>::mma(a[1], b[1], acc);
+  acc = Half<Bf16>::mma(a[1], b[0], acc);
+  acc = Half<Bf16>::mma(a[0], b[1], acc);
+  return Half<Bf16>::mma(a[0], b[0], acc);
+}
+
+template <int D, int kBN, int KS, int W>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_f32_kernel(PromptArgs a) {
+  constexpr int kThreads = 64 * W, R = W / KS, kC = D / 8, kKeys = KS * kBN, kRowBytes = 2 * D;
+  constexpr int kKB = kBN / 32, kDC = D / 16, kDB = D / 32;
+  constexpr int kLoads = kKeys * D / 4 / kThreads;   // of 4 elements, a thread, K and V each
+  static_assert(kLoads >= 1 && kLoads * kThreads * 4 == kKeys * D, "tile / thread split");
+  __shared__ __align__(1024) uint8_t lds[2][3][kKeys * kRowBytes];   // [K, V][planes]
 
   const int lane = threadIdx.x & 63, j = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Task t;
   if (!t.find(a, 32 * R)) return;
   const int n_kt = (min(t.q0 + 32 * R, t.len) + kKeys - 1) / kKeys;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  KLoads kl;
-  VLoads vl;
-  kl.init(a.k + t.row0 * a.k_row + t.kvh * a.k_head, a.k_row, t.len, lds0, wave);
-  vl.init(a.v + t.row0 * a.v_row + t.kvh * a.v_head, a.v_row, t.len, lds0 + sizeof(lds[0]), wave);
-  kl.load(0);
-  vl.load(0);
-
   const int kg = wave / R, first_row = t.q0 + 32 * (wave % R);
   const int qrow = first_row + j;   // of the sequence
-  float4 qf[kDC];
-  const uint8_t* src = a.q + (t.row0 + min(qrow, t.len - 1)) * a.q_row + t.h * a.q_head + 16 * hh;
+
+  // This thread's part of a tile: rows lr, lr + kStep, .. at elements 4 lc .. + 3.
+  constexpr int kStep = kThreads / (D / 4);
+  const int lr = threadIdx.x / (D / 4), lc = threadIdx.x % (D / 4);
+  const uint8_t* kbase = a.k + t.row0 * a.k_row + t.kvh * a.k_head + 16 * lc;
+  const uint8_t* vbase = a.v + t.row0 * a.v_row + t.kvh * a.v_head + 16 * lc;
+  float4 kr[kLoads], vr[kLoads];
+  auto load = [&](int kt) {
 #pragma unroll
-  for (int c = 0; c < kDC; ++c) qf[c] = *reinterpret_cast<const float4*>(src + 32 * c);
-  if (a.qscale < 0) {   // the running max is of scores times |scale|
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t key = min(kt * kKeys + u * kStep + lr, t.len - 1);   // (past the last: masked)
+      kr[u] = *reinterpret_cast<const float4*>(kbase + key * a.k_row);
+      vr[u] = *reinterpret_cast<const float4*>(vbase + key * a.v_row);
+    }
+  };
+  auto put = [&](uint8_t (*to)[kKeys * kRowBytes], int at, const float4& x) {
+    const Split3 p(x.x, x.y), q(x.z, x.w);
+    *reinterpret_cast<uint2*>(to[0] + at) = make_uint2(p.h, q.h);
+    *reinterpret_cast<uint2*>(to[1] + at) = make_uint2(p.m, q.m);
+    *reinterpret_cast<uint2*>(to[2] + at) = make_uint2(p.l, q.l);
+  };
+  load(0);
+
+  short8x qf[kDC][3];
+  {
+    const uint8_t* src = a.q + (t.row0 + min(qrow, t.len - 1)) * a.q_row + t.h * a.q_head + 32 * hh;
+    const float sign = a.qscale < 0 ? -1.0f : 1.0f;   // the running max is of scores times |scale|
 #pragma unroll
-    for (int c = 0; c < kDC; ++c) qf[c] = make_float4(-qf[c].x, -qf[c].y, -qf[c].z, -qf[c].w);
+    for (int c = 0; c < kDC; ++c) {
+      const float4 x = *reinterpret_cast<const float4*>(src + 64 * c);
+      const float4 y = *reinterpret_cast<const float4*>(src + 64 * c + 16);
+      const Split3 p0(sign * x.x, sign * x.y), p1(sign * x.z, sign * x.w), p2(sign * y.x, sign * y.y),
+          p3(sign * y.z, sign * y.w);
+      qf[c][0] = __builtin_bit_cast(short8x, make_uint4(p0.h, p1.h, p2.h, p3.h));
+      qf[c][1] = __builtin_bit_cast(short8x, make_uint4(p0.m, p1.m, p2.m, p3.m));
+      qf[c][2] = __builtin_bit_cast(short8x, make_uint4(p0.l, p1.l, p2.l, p3.l));
+    }
   }
-#pragma unroll
-  for (int c = 0; c < kDC; ++c)
-    asm volatile("" : "+v"(qf[c].x), "+v"(qf[c].y), "+v"(qf[c].z), "+v"(qf[c].w));
   const float qs = fmaxf(fabsf(a.qscale), 1e-30f);
 
   State<kDB> st;
   st.clear();
+  const int kl = swap23(j), vi = j & 15;
   const int last_kt = min(first_row / kKeys, n_kt - 1);   // the only step with keys behind some row
   for (int kt = 0; kt < n_kt; ++kt) {
-    const int odd = kt & 1;
-    landed<0>();                       // and everybody is done with the tile before
-    kl.load(1 - odd);
-    vl.load(1 - odd);
+    __syncthreads();                   // everybody is done with the tile before
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int r = u * kStep + lr;
+      put(lds[0], r * kRowBytes + 16 * KPlace<kC>::at(r, lc / 2) + 8 * (lc & 1), kr[u]);
+      put(lds[1], r * kRowBytes + 16 * VPlace<kC>::at(r, lc / 2) + 8 * (lc & 1), vr[u]);
+    }
+    if (kt + 1 < n_kt) load(kt + 1);
+    // the tile is there; the next one's loads stay on their way
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (kt > last_kt) continue;        // the other waves' last steps
     float16x s[kKB];
-    const uint8_t* ks = lds[0][odd] + (kg * kBN + j) * kRowBytes;
 #pragma unroll
     for (int kb = 0; kb < kKB; ++kb)
 #pragma unroll
@@ -732,19 +779,19 @@ __global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : 2) void prompt_f
     for (int c = 0; c < kDC; ++c)
 #pragma unroll
       for (int kb = 0; kb < kKB; ++kb) {
-        const float4 kf = *reinterpret_cast<const float4*>(ks + 32 * kb * kRowBytes +
-                                                           16 * KPlace<kC>::at(j, 2 * c + hh));
-        s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.x, qf[c].x, s[kb], 0, 0, 0);
-        s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.y, qf[c].y, s[kb], 0, 0, 0);
-        s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.z, qf[c].z, s[kb], 0, 0, 0);
-        s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.w, qf[c].w, s[kb], 0, 0, 0);
+        short8x kf[3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          kf[p] = *reinterpret_cast<const short8x*>(lds[0][p] + (kg * kBN + 32 * kb + kl) * kRowBytes +
+                                                    16 * KPlace<kC>::at(kl, 2 * c + hh));
+        s[kb] = mma3(kf, qf[c], s[kb]);
       }
     if (kt == last_kt) {
 #pragma unroll
       for (int kb = 0; kb < kKB; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (kt * kKeys + kg * kBN + 32 * kb + 8 * (r / 4) + 4 * hh + r % 4 > qrow) s[kb][r] = -INFINITY;
+          if (kt * kKeys + kg * kBN + 32 * kb + 16 * (r / 8) + 8 * hh + r % 8 > qrow) s[kb][r] = -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
@@ -752,34 +799,56 @@ __global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : 2) void prompt_f
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
     st.raise(mx, qs);
+    short8x pf[kKB * 2][3];
 #pragma unroll
-    for (int kb = 0; kb < kKB; ++kb)
+    for (int g = 0; g < kKB * 2; ++g) {
+      uint32_t w[3][4];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[kb][r] = fast_exp2(fmaf(s[kb][r], qs, -st.m));
-        st.l += s[kb][r];
+      for (int e = 0; e < 4; ++e) {
+        const float x = fast_exp2(fmaf(s[g / 2][8 * (g % 2) + 2 * e], qs, -st.m));
+        const float y = fast_exp2(fmaf(s[g / 2][8 * (g % 2) + 2 * e + 1], qs, -st.m));
+        st.l += x + y;
+        const Split3 p(x, y);
+        w[0][e] = p.h;
+        w[1][e] = p.m;
+        w[2][e] = p.l;
       }
 #pragma unroll
-    for (int kb = 0; kb < kKB; ++kb)
+      for (int p = 0; p < 3; ++p)
+        pf[g][p] = __builtin_bit_cast(short8x, make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]));
+    }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = 8 * (r / 4) + 4 * hh + r % 4;   // its swizzle depends on hh alone
-        const uint8_t* vs = lds[1][odd] + (kg * kBN + 32 * kb + key) * kRowBytes + 4 * (j & 3);
+    for (int g = 0; g < kKB * 2; ++g)
 #pragma unroll
-        for (int d = 0; d < kDB; ++d)
-          st.o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(
-              *reinterpret_cast<const float*>(vs + 16 * VPlace32<kC>::at(4 * hh, 8 * d + (j >> 2))), s[kb][r],
-              st.o[d], 0, 0, 0);
+      for (int d = 0; d < kDB; ++d) {
+        typedef __attribute__((address_space(3))) short4x lshort4x;
+        const int r = 8 * hh + (vi >> 2), e0 = 32 * d + (j & 16) + 4 * (vi & 3);
+        short8x vf[3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          const uint8_t* at = lds[1][p] + (kg * kBN + 16 * g + r) * kRowBytes + 2 * (e0 % 8);
+          vf[p] = __builtin_shufflevector(
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lshort4x*)(at + 16 * VPlace<kC>::at(r, e0 / 8))),
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lshort4x*)(at + 4 * kRowBytes + 16 * VPlace<kC>::at(r + 4, e0 / 8))),
+              0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        st.o[d] = mma3(vf, pf[g], st.o[d]);
       }
   }
-  landed<0>();   // the last loads, before the LDS is used again or given up
-  if constexpr (KS == 2) {
-    float* other = reinterpret_cast<float*>(&lds[0][0][0]) + wave % R * State<kDB>::kFloats;
+  __syncthreads();
+  if constexpr (KS > 1) {
+    // the groups' states, one after the other through one place in the LDS
+    float* place = reinterpret_cast<float*>(&lds[0][0][0]) + wave % R * State<kDB>::kFloats;
     static_assert(R * State<kDB>::kFloats * 4 <= (int)sizeof(lds), "states fit the LDS");
-    if (kg > 0) st.put(other);
-    __syncthreads();
+#pragma unroll
+    for (int k = 1; k < KS; ++k) {
+      if (kg == k) st.put(place);
+      __syncthreads();
+      if (kg == 0) st.add(place);
+      __syncthreads();
+    }
     if (kg > 0) return;
-    st.add(other);
   }
   const uint32_t bad = st.normalise();
   uint8_t* dst = a.out + (((t.row0 + qrow) * a.H + t.h) * (int64_t)D) * 4;
@@ -794,34 +863,46 @@ __global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : 2) void prompt_f
   walk_rows<float, D>(a, t, bad, first_row);
 }
 
-template <typename T, int D, int kBN, int KS>
-void launch_one(const PromptArgs& a, int64_t grid, hipStream_t stream) {
-  if constexpr (sizeof(T) == 4)
-    hipLaunchKernelGGL((prompt_f32_kernel<D, kBN, KS>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((prompt_mma_kernel<T, D, kBN, KS>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
-}
-
-// Tiles of 32 R rows of all sequences, at most.
+// Tiles of `rows` rows of all sequences, at most.
 int64_t tiles_of(const PromptArgs& a, int rows) {
   return std::min(sat_mul(a.B, ceil_div(a.max_len, rows)), a.T / rows + a.B);
 }
 
+// Workgroups of 32 W / KS rows.
+template <typename T, int D, int kBN, int KS, int W>
+int launch_one(const PromptArgs& a, hipStream_t stream) {
+  const int64_t grid = sat_mul(tiles_of(a, 32 * W / KS), a.H);
+  if (!grid_fits(grid, 64 * W)) return fail(HS_EUNSUPPORTED, "prompt grid too large");
+  if constexpr (sizeof(T) == 4)
+    hipLaunchKernelGGL((prompt_f32_kernel<D, kBN, KS, W>), dim3((unsigned)grid), dim3(64 * W), 0, stream, a);
+  else
+    hipLaunchKernelGGL((prompt_mma_kernel<T, D, kBN, KS>), dim3((unsigned)grid), dim3(64 * W), 0, stream, a);
+  return HS_OK;
+}
+
+// Few workgroups of 128 rows (no more than CUs) split the keys over their waves.  us, one
+// group of waves / 16-bit types: 2 groups of 2, fp32 at head dims 32 and 64: 4 groups of 2:
+//   bf16  1 prompt of 512 tokens, 32 heads, D 128 (128 workgroups) 15.3 / 13.1; 1000, 12 heads,
+//         D 64 (96) 16.1 / 11.7; 4 of 1024, 12 heads, D 64 (384) 19.8 / 21.4; 2048, 32 heads, D 128
+//         (512) 51 / 70
+//   fp32  334 and 1001, 12 heads, D 64 (144) 46 / 28.5; 3 of 1024 (288) 57 / 56; 4 (384) 61 / 64;
+//         8 (768) 111 / 130
+// fp32 at head dim 128: the tiles fill the LDS of a CU, so it holds one workgroup, and
+// that has 2 groups of 4 waves, but for short prompts: one group / two, 2048 tokens, 32 / 8
+// heads 233 / 207; 300 and 700 tokens 74 / 59; 16 prompts of 128 32 / 47.
 template <typename T, int D>
 int launch_dim(const PromptArgs& a, int cus, hipStream_t stream) {
-  constexpr int kBN = D * sizeof(T) >= 512 ? 32 : 64;
-  constexpr bool kSplits = 2 * 4 * kBN * D * sizeof(T) <= 160 * 1024;   // two tiles of keys a step fit the LDS
-  const bool split = kSplits && sat_mul(tiles_of(a, 128), a.H) <= cus;
-  const int64_t grid = sat_mul(tiles_of(a, split ? 64 : 128), a.H);
-  if (!grid_fits(grid, kThreads)) return fail(HS_EUNSUPPORTED, "prompt grid too large");
-  if constexpr (kSplits) {
-    if (split) {
-      launch_one<T, D, kBN, 2>(a, grid, stream);
-      return HS_OK;
-    }
+  const bool few = sat_mul(tiles_of(a, 128), a.H) <= cus;
+  if constexpr (sizeof(T) == 2) {
+    constexpr int kBN = D >= 256 ? 32 : 64;
+    return few ? launch_one<T, D, kBN, 2, 4>(a, stream) : launch_one<T, D, kBN, 1, 4>(a, stream);
+  } else if constexpr (D <= 64) {
+    return few ? launch_one<T, D, 32, 4, 8>(a, stream) : launch_one<T, D, 64, 1, 4>(a, stream);
+  } else if constexpr (D == 128) {
+    return a.max_len > 256 ? launch_one<T, D, 32, 2, 8>(a, stream) : launch_one<T, D, 32, 1, 4>(a, stream);
+  } else {
+    return launch_one<T, D, 32, 1, 4>(a, stream);
   }
-  launch_one<T, D, kBN, 1>(a, grid, stream);
-  return HS_OK;
 }
 
 template <typename T>
