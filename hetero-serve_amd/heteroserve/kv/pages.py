@@ -17,9 +17,11 @@ copy to the host, so a step that forks or frees can be captured in a graph:
     ref_counts     [num_blocks]: how many table rows (or other holders, such as a
                    prefix cache) keep a block; a block is free at 0
 
-Row indexes and block ids come as device tensors, which are not read back (one
+Row indexes and fresh blocks come as device tensors, which are not read back (one
 that names no row or block is skipped), or from the host, where they follow torch
-indexing and mistakes raise before anything is launched.
+indexing (but a fresh block of -1 is none, as from find_free_blocks) and mistakes
+raise before anything is launched.  copy_blocks reads its ids back, as the pack calls
+do.
 """
 
 from __future__ import annotations
@@ -59,12 +61,15 @@ def find_free_blocks(ref_counts, n: int):
     n = int(n)
     if n < 0:
         raise RuntimeError("n must not be negative")
+    if n >= 1 << 31:
+        raise RuntimeError(f"n must be below 2^31, got {n}")
     return _hip.kv_find_free(ref_counts, n)
 
 
-def _indexes(values, size: int, what: str, device):
+def _indexes(values, size: int, what: str, device, none: bool = False):
     """(int32 device tensor, host array or None): host values are checked and
-    wrapped as torch indexing does."""
+    wrapped as torch indexing does, or, with none, -1 is kept and the only value
+    below 0."""
     import torch
 
     if torch.is_tensor(values) and values.is_cuda:
@@ -75,11 +80,12 @@ def _indexes(values, size: int, what: str, device):
     if host.size and host.dtype.kind not in "iu":
         raise RuntimeError(f"{what} must be integers, got {host.dtype}")
     host = host.astype(np.int64)
-    bad = (host < -size) | (host >= size)
+    bad = (host < (-1 if none else -size)) | (host >= size)
     if bad.any():
         i = int(host[int(np.argmax(bad))])
         raise IndexError(f"{what} index {i} is out of bounds for size {size}")
-    host = np.where(host < 0, host + size, host)
+    if not none:
+        host = np.where(host < 0, host + size, host)
     return torch.from_numpy(host.astype(np.int32)).to(device), host
 
 
@@ -105,10 +111,10 @@ def fork_blocks(pool, block_tables, context_lens, ref_counts, parents, children,
     B, dev = block_tables.shape[0], pool.device
     parents, host_p = _indexes(parents, B, "parent row", dev)
     children, host_c = _indexes(children, B, "child row", dev)
-    fresh, host_f = _indexes(fresh, pool.shape[2], "fresh block", dev)
+    fresh, host_f = _indexes(fresh, pool.shape[2], "fresh block", dev, none=True)
     if host_c is not None and _repeats(host_c):
         raise RuntimeError("a child row repeats")
-    if host_f is not None and _repeats(host_f):
+    if host_f is not None and _repeats(host_f[host_f >= 0]):
         raise RuntimeError("a fresh block repeats")
     if host_c is not None and host_p is not None and not set(host_c.tolist()).isdisjoint(host_p.tolist()):
         raise RuntimeError("a row is both parent and child")

@@ -276,3 +276,26 @@ def test_refusals():
     refused("one entry per block", pages.compact_blocks, pool, t, r[:7])
     refused("contiguous", pages.compact_blocks, pool[:, :, ::2], t, r)
     assert (t.cpu() == -1).all() and (r.cpu() == 0).all()
+
+
+def test_no_fresh_block_from_the_host_is_no_block():
+    """-1 of find_free_blocks, brought to the host and back, is not the last block."""
+    from heteroserve.kv import pages
+
+    rng = np.random.default_rng(3)
+    tables, ctx, refs = _batch(rng, 8, [20, 32], 3, 5, 16, share=False)
+    refs[:] = np.maximum(refs, (np.arange(5) < 4))          # a full pool but for one block or none
+    pool = _pool(1, 5, 16, 2, 64)
+    want = [_words(pool).copy(), tables.copy(), ctx.copy(), refs.copy()]
+    fresh = [-1, -1, -1]
+    done = ops.fork(*want, [0, 0, 1], [4, 5, 6], fresh)
+    assert done.tolist() == [0, 0, 1]
+    t, c, r = _dev(tables), _dev(ctx), _dev(refs)
+    got = pages.fork_blocks(pool, t, c, r, [0, 0, 1], [4, 5, 6], fresh)
+    assert got.tolist() == done.tolist()
+    for x, w in zip((_words(pool), t.cpu(), c.cpu(), r.cpu()), want):
+        assert np.array_equal(np.asarray(x), w)
+    with pytest.raises(IndexError, match="fresh block index -2"):
+        pages.fork_blocks(pool, t, c, r, [0], [4], [-2])
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        pages.find_free_blocks(r, 2 ** 31)
