@@ -756,6 +756,16 @@ def _heads(x):
     return x, ptr, s0, s1
 
 
+def _overlap(out, x) -> bool:
+    """Whether contiguous `out` and the range from x's first to its last element share
+    a byte."""
+    if not x.numel():
+        return False
+    p, size = x.data_ptr(), x.element_size()
+    end = p + size * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
+    return p < out.data_ptr() + size * out.numel() and out.data_ptr() < end
+
+
 def prompt_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float, out=None):
     """out[T, H, D] of q's dtype via hs_prompt_attention."""
     L = lib("prompt attention kernel")
@@ -781,12 +791,19 @@ def prompt_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float, out=Non
     elif (out.shape != shape or out.dtype is not dtype or out.get_device() != index
           or not out.is_contiguous() or out.data_ptr() % 16):
         raise RuntimeError("out must be a contiguous, 16-byte aligned tensor like q")
+    elif _overlap(out, q) or _overlap(out, k) or _overlap(out, v):
+        raise RuntimeError("out must not overlap q, k or v")
+    max_len = int(max_seqlen)
+    if max_len > T:        # (the library takes 32 bits)
+        max_len = T
+    elif max_len < 0:
+        raise RuntimeError("max_seqlen must be positive or 0")
     q, qp, qr, qh = _heads(q)
     k, kp, kr, kh = _heads(k)
     v, vp, vr, vh = _heads(v)
     with _DeviceGuard(index):
         check(L.hs_prompt_attention(qp, kp, vp, code, qr, qh, kr, kh, vr, vh, cu.data_ptr(), B, T,
-                                    int(max_seqlen), H, Hkv, D, float(scale), out.data_ptr(),
+                                    max_len, H, Hkv, D, float(scale), out.data_ptr(),
                                     _stream_at(index)))
     return out
 

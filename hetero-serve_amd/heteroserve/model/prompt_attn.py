@@ -17,7 +17,7 @@ paged_attn_prefill.paged_attention_prefill_varlen.
 Slices of a fused QKV output are read in place where rows and heads lie
 multiples of 16 bytes (at most 2^22 elements) apart; other layouts are copied
 first.  Rows behind the last sequence are left as they were in ``out`` (not set
-where the call makes it).  Products run on the matrix cores, of 16-bit inputs in
+where the call makes it), which must be contiguous and no part of q, k or v.  Products run on the matrix cores, of 16-bit inputs in
 their own type, the probabilities rounded to it, of float32 ones in three bf16
 terms a number, as accurate as float32; scores, softmax and sums are fp32.
 """

@@ -314,3 +314,24 @@ def test_refusals():
         prompt_attention(q, k, v, torch.zeros(0, dtype=torch.int32), 8, 0.1)
     with pytest.raises(RuntimeError, match="positive"):
         prompt_attention(q, k, v, cu, -1, 0.1)
+
+
+def test_out_that_is_an_input_and_lengths_past_32_bits():
+    from heteroserve.model.prompt_attn import prompt_attention
+
+    q, k, v, cu = _rows([30, 12], 4, 2, 64, BF16, 1)
+    cu = torch.tensor(cu, device=DEV)
+    want = prompt_attention(q, k, v, cu, 30, 0.1)
+    for longest in (42, 2 ** 32, 2 ** 40 + 1):
+        assert torch.equal(prompt_attention(q, k, v, cu, longest, 0.1), want)
+    with pytest.raises(RuntimeError, match="positive"):
+        prompt_attention(q, k, v, cu, -2 ** 32, 0.1)
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    both = torch.empty(2 * 42, 4, 64, dtype=BF16, device=DEV)
+    both[42:] = q
+    with pytest.raises(RuntimeError, match="overlap"):
+        prompt_attention(q, k, v, cu, 30, 0.1, out=q)
+    with pytest.raises(RuntimeError, match="overlap"):
+        prompt_attention(both[42:], k, v, cu, 30, 0.1, out=both[1:43])
+    got = prompt_attention(both[42:], k, v, cu, 30, 0.1, out=both[:42])
+    assert torch.equal(got, want)
