@@ -266,3 +266,35 @@ def test_refusals():
     refused("at least|positions for", q, k, v, pos, f, kc, vc, bt, pos[:2])
     with pytest.raises(RuntimeError, match="sections"):
         rotary.axes_of([-1, 2])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D,pairs,interleaved", [(64, 32, False), (64, 16, True), (80, 20, False),
+                                                 (128, 24, False), (7, 3, True)])
+@pytest.mark.parametrize("n", [3, 2100])
+def test_outputs_that_are_their_sources(dtype, D, pairs, interleaved, n):
+    """hs_rotary and hs_rotary_append in place, as the header allows them."""
+    from heteroserve import _hip
+    from heteroserve.kv import rotary
+
+    lib = _hip.lib()
+    H, Hkv = 3, 2
+    q, k, v = [x.contiguous() for x in _inputs(n, H, Hkv, D, dtype, 5)]
+    at, freq = torch.arange(n, dtype=torch.int32, device=DEV), _freq(pairs)
+    want = rotary.rotate_qk(q, k, at, freq, interleaved=interleaved)
+    code, stream = _hip.dtype_code(dtype), _hip.stream_of(q.device)
+    a, b = q.clone(), k.clone()
+    turn = (at.data_ptr(), 1, freq.data_ptr(), None, pairs, int(interleaved), n, H, Hkv, D)
+    _hip.check(lib.hs_rotary(a.data_ptr(), b.data_ptr(), code, H * D, Hkv * D, *turn, a.data_ptr(),
+                             b.data_ptr(), code, stream))
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+    a, b = q.clone(), k.clone()
+    kc, vc = torch.zeros(2, -(-n // 16), 16, Hkv, D, dtype=dtype, device=DEV)
+    table = torch.arange(-(-n // 16), dtype=torch.int32, device=DEV)
+    seq = torch.zeros(n, dtype=torch.int32, device=DEV)
+    _hip.check(lib.hs_rotary_append(
+        a.data_ptr(), b.data_ptr(), v.data_ptr(), code, H * D, Hkv * D, Hkv * D, *turn, a.data_ptr(),
+        b.data_ptr(), code, kc.data_ptr(), vc.data_ptr(), code, kc.shape[0], 16, table.data_ptr(), 1,
+        table.numel(), at.data_ptr(), seq.data_ptr(), stream))
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+    assert torch.equal(kc.view(-1, Hkv, D)[:n], want[1]) and torch.equal(vc.view(-1, Hkv, D)[:n], v)
