@@ -12,10 +12,10 @@
 //
 // The copies are HBM-bound (copies of 128 blocks of 32 layers, 537 MB read and written:
 // 95.6 us, 5.6 TB/s; a large copy reaches 6.6); everything else is a few microseconds
-// of latency, so each operation is one launch (a compaction two).  The scans need each chunk's number
-// of blocks before it: every workgroup counts them itself, a stream of reads
-// from L2, which is shorter than a second launch would be (131072 blocks: 8.7 us in
-// all, 18 with one load in flight a thread).
+// of latency, so each operation is one launch (a compaction two).  The scans need each
+// chunk's number of blocks before it: every workgroup counts them itself, a stream of
+// reads from L2, which is shorter than a second launch would be (131072 blocks: 8.7 us
+// in all, 18 with one load in flight a thread).
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
 #include "hs_private.h"

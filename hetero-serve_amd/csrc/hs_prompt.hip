@@ -8,9 +8,10 @@
 // walks the keys once with a running maximum and sum.  K and V tiles go from global
 // memory straight to LDS (two of each; the next ones are on their way while one is
 // used), swizzled by permuting the addresses that the lanes load from, since the LDS
-// side of such a load is linear (fp32 tiles pass through registers, see Split3).  S^T = K Q^T and O^T = V^T P^T: a lane holds one
-// query's scores, so its maximum and sum need one exchange of the two lane halves,
-// and the probabilities are the second product's operand where they stand.  Rows
+// side of such a load is linear (fp32 tiles pass through registers, see Split3).
+// S^T = K Q^T and O^T = V^T P^T: a lane holds one query's scores, so its maximum and sum
+// need one exchange of the two lane halves, and the probabilities are the second
+// product's operand where they stand.  Short prompts take a wave each instead.  Rows
 // are 128 and not 256 a workgroup because two workgroups then share a CU: one's
 // set-up and barriers pass beside the other's products.  us at 256 / 128 rows, bf16:
 // one prompt of 2048 tokens, 32 / 8 heads, D 128 55 / 49, 32 of 128 tokens 50 / 27, one
@@ -50,7 +51,7 @@ struct PromptArgs {
   int64_t T;
   int max_len;
   float qscale;               // scale * log2(e)
-  int by_level;               // order of the tiles: see find_tile
+  int by_level, per;          // order of the tiles: see find_tile
 };
 
 // First row and rows of sequence b, whatever cu holds: rows of [0, T), at most
@@ -172,6 +173,11 @@ struct Half<_Float16> {
   }
 };
 
+__device__ inline int64_t readlane64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
+
 __device__ inline int swap23(int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); }
 
 // Both lane halves' larger value, and sum.
@@ -274,16 +280,30 @@ __device__ inline int wave_sum(int x) {
   return s[0] + s[1];
 }
 
+// Sum of this lane's and the lanes' before it.
+__device__ inline int wave_scan(int x) {
+  constexpr int kRowShr = 0x110, kBcast15 = 0x142, kBcast31 = 0x143;
+  x += __builtin_amdgcn_update_dpp(0, x, kRowShr + 1, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, kRowShr + 2, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, kRowShr + 4, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, kRowShr + 8, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, kBcast15, 0xA, 0xF, false);   // rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, kBcast31, 0xC, 0xF, false);   // rows 2 and 3
+  return x;
+}
+
 // The tile of query rows that workgroup `i` takes, nt_b tiles of `rows` rows in
 // sequence b, of which tile qt walks the keys of qt + 1.  Every wave finds it by
 // itself.  False: there is no such tile.
+//   per       `per` tiles a sequence, some of which may not be, in the sequences' order
 //   by_level  tiles by falling qt, and by b among equals, so that the longest walks
 //             begin first: with F(l) = sum_b max(0, nt_b - l) tiles from level l on, i
 //             lies on the highest level l with F(l) > i
 //   else      a sequence's tiles are neighbours, the last one first, so that its keys
 //             are read again from the L2 of the XCD that its heads run on, and
 //             sequences go by falling nt_b
-// More than 64 sequences go in their order, a sequence's tiles as neighbours.
+// More than 64 sequences go in their order, a sequence's tiles as neighbours, the last
+// one first.
 __device__ inline bool find_tile(const PromptArgs& a, int rows, int i, int& b, int& qt) {
   const int lane = threadIdx.x & 63;
   auto tiles_of = [&](int s) {
@@ -292,24 +312,31 @@ __device__ inline bool find_tile(const PromptArgs& a, int rows, int i, int& b, i
     if (s < a.B) seq_rows(a, s, row0, len);
     return (len + rows - 1) / rows;
   };
+  if (a.per) {
+    b = i / a.per;
+    qt = a.per - 1 - (i - b * a.per);
+    return b < a.B;
+  }
   if (a.B > 64) {
-    int total = 0;
-    for (int s0 = 0; s0 < a.B; s0 += 64) {
-      const int nt = tiles_of(s0 + lane);
-      int inc = nt;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(inc, o);
-        if (lane >= o) inc += x;
+    // every lane adds up a run of sequences; the run that holds tile i is then looked at
+    // by itself
+    for (int first = 0, n = a.B; n > 0;) {
+      const int run = (n + 63) / 64;
+      int nt = 0;
+#pragma unroll 4
+      for (int s = lane * run; s < min((lane + 1) * run, n); ++s) nt += tiles_of(first + s);
+      const int inc = wave_scan(nt);
+      const uint64_t m = __builtin_amdgcn_ballot_w64(i < inc);
+      if (m == 0) return false;
+      const int at = __builtin_ctzll(m);
+      i -= __builtin_amdgcn_readlane(inc, at) - __builtin_amdgcn_readlane(nt, at);
+      first += at * run;
+      if (run == 1) {
+        b = first;
+        qt = __builtin_amdgcn_readlane(nt, at) - 1 - i;
+        return b < a.B;
       }
-      const uint64_t m = __builtin_amdgcn_ballot_w64(i < total + inc);
-      if (m != 0) {
-        const int at = __builtin_ctzll(m);
-        b = s0 + at;
-        qt = total + __builtin_amdgcn_readlane(inc, at) - 1 - i;
-        return true;
-      }
-      total += __builtin_amdgcn_readlane(inc, 63);
+      n = min(run, n - at * run);
     }
     return false;
   }
@@ -447,6 +474,42 @@ struct State {
   }
 };
 
+// The normalised rows of a wave, but for the bad ones.
+template <typename T, int D>
+__device__ inline void store_rows(const PromptArgs& a, const Task& t, int qrow, const State<D / 32>& st,
+                                  uint32_t bad) {
+  constexpr int kDB = D / 32;
+  const int lane = threadIdx.x & 63, j = lane & 31, hh = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    uint8_t* dst = a.out + (((t.row0 + qrow) * a.H + t.h) * (int64_t)D) * 2;
+    if (qrow < t.len && !((bad >> j) & 1)) {
+  #pragma unroll
+      for (int d = 0; d < kDB; ++d)
+  #pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          // lane halves hold 4 dims each of two groups of 8: swapped into one group each
+          uint32_t w[4];
+  #pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = Half<T>::pack(st.o[d][8 * g + 2 * e], st.o[d][8 * g + 2 * e + 1]);
+          const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+          const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+          *reinterpret_cast<uint4*>(dst + 64 * d + 32 * g + 16 * hh) = make_uint4(x[0], y[0], x[1], y[1]);
+        }
+    }
+  } else {
+    uint8_t* dst = a.out + (((t.row0 + qrow) * a.H + t.h) * (int64_t)D) * 4;
+    if (qrow < t.len && !((bad >> j) & 1)) {
+  #pragma unroll
+      for (int d = 0; d < kDB; ++d)
+  #pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(dst + 128 * d + 32 * g + 16 * hh) =
+              make_float4(st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]);
+    }
+  }
+}
+
 // This wave's loads have landed, but for the last `kLater`; behind the barrier
 // everybody's have.
 template <int kLater>
@@ -533,7 +596,8 @@ __global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : D == 64 ? 3 : 2)
     const short4x lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
         (lshort4x*)(p + ((kg * kBN + r) * kRowBytes + 16 * VPlace<kC>::at(r, e0 / 8) + 2 * (e0 % 8))));
     const short4x hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lshort4x*)(p + 4 * kRowBytes + ((kg * kBN + r) * kRowBytes + 16 * VPlace<kC>::at(r + 4, e0 / 8) + 2 * (e0 % 8))));
+        (lshort4x*)(p + 4 * kRowBytes +
+                    ((kg * kBN + r) * kRowBytes + 16 * VPlace<kC>::at(r + 4, e0 / 8) + 2 * (e0 % 8))));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
   // Keys behind the row, in the wave's last tile.
@@ -642,22 +706,7 @@ __global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : D == 64 ? 3 : 2)
   }
 
   const uint32_t bad = st.normalise();
-  uint8_t* dst = a.out + (((t.row0 + qrow) * a.H + t.h) * (int64_t)D) * 2;
-  if (qrow < t.len && !((bad >> j) & 1)) {
-#pragma unroll
-    for (int d = 0; d < kDB; ++d)
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        // lane halves hold 4 dims each of two groups of 8: swapped into one group each
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[e] = Half<T>::pack(st.o[d][8 * g + 2 * e], st.o[d][8 * g + 2 * e + 1]);
-        const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-        const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-        *reinterpret_cast<uint4*>(dst + 64 * d + 32 * g + 16 * hh) = make_uint4(x[0], y[0], x[1], y[1]);
-      }
-  }
+  store_rows<T, D>(a, t, qrow, st, bad);
   walk_rows<T, D>(a, t, bad, first_row);
 }
 
@@ -688,6 +737,15 @@ struct Split3 {
     l = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
   }
 };
+
+// The three planes of sign times 8 numbers.
+__device__ inline void split8(const float4& x, const float4& y, float sign, short8x (&to)[3]) {
+  const Split3 a(sign * x.x, sign * x.y), b(sign * x.z, sign * x.w), c(sign * y.x, sign * y.y),
+      d(sign * y.z, sign * y.w);
+  to[0] = __builtin_bit_cast(short8x, make_uint4(a.h, b.h, c.h, d.h));
+  to[1] = __builtin_bit_cast(short8x, make_uint4(a.m, b.m, c.m, d.m));
+  to[2] = __builtin_bit_cast(short8x, make_uint4(a.l, b.l, c.l, d.l));
+}
 
 // acc + a . b, planes h, m, l, the small terms first.
 __device__ inline float16x mma3(const short8x (&a)[3], const short8x (&b)[3], float16x acc) {
@@ -745,11 +803,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_f32_kernel(Pr
     for (int c = 0; c < kDC; ++c) {
       const float4 x = *reinterpret_cast<const float4*>(src + 64 * c);
       const float4 y = *reinterpret_cast<const float4*>(src + 64 * c + 16);
-      const Split3 p0(sign * x.x, sign * x.y), p1(sign * x.z, sign * x.w), p2(sign * y.x, sign * y.y),
-          p3(sign * y.z, sign * y.w);
-      qf[c][0] = __builtin_bit_cast(short8x, make_uint4(p0.h, p1.h, p2.h, p3.h));
-      qf[c][1] = __builtin_bit_cast(short8x, make_uint4(p0.m, p1.m, p2.m, p3.m));
-      qf[c][2] = __builtin_bit_cast(short8x, make_uint4(p0.l, p1.l, p2.l, p3.l));
+      split8(x, y, sign, qf[c]);
     }
   }
   const float qs = fmaxf(fabsf(a.qscale), 1e-30f);
@@ -851,16 +905,161 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_f32_kernel(Pr
     if (kg > 0) return;
   }
   const uint32_t bad = st.normalise();
-  uint8_t* dst = a.out + (((t.row0 + qrow) * a.H + t.h) * (int64_t)D) * 4;
-  if (qrow < t.len && !((bad >> j) & 1)) {
-#pragma unroll
-    for (int d = 0; d < kDB; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<float4*>(dst + 128 * d + 32 * g + 16 * hh) =
-            make_float4(st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]);
-  }
+  store_rows<float, D>(a, t, qrow, st, bad);
   walk_rows<float, D>(a, t, bad, first_row);
+}
+
+// ---- short prompts: a wave by itself ----------------------------------------
+
+// A wave takes 32 rows of one (sequence, head) and shares nothing: the workgroup's waves
+// are just neighbours (heads of a KV group, whose keys the L1 then holds; us at 1 / 2 / 4
+// waves: 8 of 64 tokens, 8 / 4 heads, D 256 9.8 / 11.2 / 14.9, 300 of 100 on average, 32 / 8
+// heads, D 128 268 / 253 / 232).  Its tile's number says which sequence and rows it is, `per`
+// tiles a sequence, so nothing is searched for, and many fit a CU, so their loads hide one
+// another: 512 prompts of 16 tokens, 32 / 8 heads, D 128, bf16 54 us, 3.1 TB/s.  K's operands come
+// straight from memory (a lane's 16 bytes of one key).  V's: 16-bit types pass through
+// 32 rows of LDS, for the transposing read; of fp32 a lane loads 8 keys' numbers of
+// one dim, 128 neighbouring bytes a half wave.
+constexpr int kWaves = 2;
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWaves) void prompt_wave_kernel(PromptArgs a) {
+  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr int kC = D / 8, kDC = D / 16, kDB = D / 32, kRowBytes = 2 * D;
+  __shared__ __align__(1024) uint8_t lds[kWaves][kF32 ? 16 : 32 * kRowBytes];
+  const int lane = threadIdx.x & 63, j = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t item = (int64_t)blockIdx.x * kWaves + wave;
+  const int64_t tile = item / a.H;
+  const int64_t b = tile / a.per;
+  if (b >= a.B) return;
+  Task t;
+  t.h = (int)(item - tile * a.H);
+  t.kvh = t.h / (a.H / a.Hkv);
+  seq_rows(a, (int)b, t.row0, t.len);
+  t.row0 = readlane64(t.row0);
+  t.len = __builtin_amdgcn_readfirstlane(t.len);
+  const int qt = a.per - 1 - (int)(tile - b * a.per);
+  t.q0 = 32 * qt;
+  if (t.q0 >= t.len) return;
+  const int qrow = t.q0 + j;
+  const uint8_t* qp = a.q + (t.row0 + min(qrow, t.len - 1)) * a.q_row + t.h * a.q_head;
+  const uint8_t* kb = a.k + t.row0 * a.k_row + t.kvh * a.k_head;
+  const uint8_t* vb = a.v + t.row0 * a.v_row + t.kvh * a.v_head;
+  const int kl = swap23(j), vi = j & 15;
+  const float sign = a.qscale < 0 ? -1.0f : 1.0f;
+  const float qs = fmaxf(fabsf(a.qscale), 1e-30f);
+  const uint32_t to = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds[wave]);
+  State<kDB> st;
+  st.clear();
+  short8x qf[kF32 ? 1 : kDC];
+  if constexpr (!kF32) {
+#pragma unroll
+    for (int c = 0; c < kDC; ++c) {
+      qf[c] = *reinterpret_cast<const short8x*>(qp + 32 * c + 16 * hh);
+      if (a.qscale < 0) qf[c] ^= (short)0x8000;
+    }
+  }
+  for (int kt = 0; kt <= qt; ++kt) {
+    const uint8_t* krow = kb + (int64_t)min(32 * kt + kl, t.len - 1) * a.k_row;
+    float16x s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+    if constexpr (kF32) {
+#pragma unroll
+      for (int c = 0; c < kDC; ++c) {
+        const float4 x = *reinterpret_cast<const float4*>(krow + 64 * c + 32 * hh);
+        const float4 y = *reinterpret_cast<const float4*>(krow + 64 * c + 32 * hh + 16);
+        const float4 u = *reinterpret_cast<const float4*>(qp + 64 * c + 32 * hh);
+        const float4 w = *reinterpret_cast<const float4*>(qp + 64 * c + 32 * hh + 16);
+        short8x kf[3], qk[3];
+        split8(x, y, 1.0f, kf);
+        split8(u, w, sign, qk);
+        s = mma3(kf, qk, s);
+      }
+    } else {
+      short8x kf[kDC];
+#pragma unroll
+      for (int c = 0; c < kDC; ++c) kf[c] = *reinterpret_cast<const short8x*>(krow + 32 * c + 16 * hh);
+      constexpr int kStep = 64 / kC;   // rows of a load
+      const uint8_t* base = vb + (int64_t)32 * kt * a.v_row;
+      const int left = t.len - 32 * kt;
+#pragma unroll
+      for (int u = 0; u < 32 / kStep; ++u) {
+        const int r = u * kStep + lane / kC;
+        load_to_lds(base, (uint32_t)min(r, left - 1) * (uint32_t)a.v_row + 16 * VPlace<kC>::at(r, lane % kC),
+                    to + u * 1024);
+      }
+#pragma unroll
+      for (int c = 0; c < kDC; ++c) s = Half<T>::mma(kf[c], qf[c], s);
+    }
+    if (kt == qt) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (32 * kt + 16 * (r / 8) + 8 * hh + r % 8 > qrow) s[r] = -INFINITY;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    st.raise(mx, qs);
+    if constexpr (kF32) {
+      float p[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p[r] = fast_exp2(fmaf(s[r], qs, -st.m));
+        st.l += p[r];
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        short8x pf[3];
+        split8(make_float4(p[8 * g], p[8 * g + 1], p[8 * g + 2], p[8 * g + 3]),
+               make_float4(p[8 * g + 4], p[8 * g + 5], p[8 * g + 6], p[8 * g + 7]), 1.0f, pf);
+        const int key0 = 32 * kt + 16 * g + 8 * hh;
+#pragma unroll
+        for (int d = 0; d < kDB; ++d) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] = *reinterpret_cast<const float*>(vb + (int64_t)min(key0 + e, t.len - 1) * a.v_row +
+                                                   128 * d + 4 * j);
+          short8x vf[3];
+          split8(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), 1.0f, vf);
+          st.o[d] = mma3(vf, pf, st.o[d]);
+        }
+      }
+    } else {
+      uint32_t pw[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        pw[e] = Half<T>::pack(fast_exp2(fmaf(s[2 * e], qs, -st.m)), fast_exp2(fmaf(s[2 * e + 1], qs, -st.m)));
+        st.l = Half<T>::sum2(pw[e], st.l);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const short8x pf = __builtin_bit_cast(
+            short8x, make_uint4(pw[4 * g], pw[4 * g + 1], pw[4 * g + 2], pw[4 * g + 3]));
+#pragma unroll
+        for (int d = 0; d < kDB; ++d) {
+          typedef __attribute__((address_space(3))) short4x lshort4x;
+          const int r = 8 * hh + (vi >> 2), e0 = 32 * d + (j & 16) + 4 * (vi & 3);
+          const uint8_t* at = lds[wave] + (16 * g + r) * kRowBytes + 2 * (e0 % 8);
+          const short8x vf = __builtin_shufflevector(
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lshort4x*)(at + 16 * VPlace<kC>::at(r, e0 / 8))),
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lshort4x*)(at + 4 * kRowBytes + 16 * VPlace<kC>::at(r + 4, e0 / 8))),
+              0, 1, 2, 3, 4, 5, 6, 7);
+          st.o[d] = Half<T>::mma(vf, pf, st.o[d]);
+        }
+      }
+      // the reads are done before the next tile's loads replace what they read
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  }
+  const uint32_t bad = st.normalise();
+  store_rows<T, D>(a, t, qrow, st, bad);
+  walk_rows<T, D>(a, t, bad, t.q0);
 }
 
 // Tiles of `rows` rows of all sequences, at most.
@@ -870,13 +1069,29 @@ int64_t tiles_of(const PromptArgs& a, int rows) {
 
 // Workgroups of 32 W / KS rows.
 template <typename T, int D, int kBN, int KS, int W>
-int launch_one(const PromptArgs& a, hipStream_t stream) {
-  const int64_t grid = sat_mul(tiles_of(a, 32 * W / KS), a.H);
+int launch_one(PromptArgs a, hipStream_t stream) {
+  constexpr int rows = 32 * W / KS;
+  const int64_t per = ceil_div(a.max_len, rows), fewest = tiles_of(a, rows);
+  // Tiles by their number where that launches no empty workgroups, or saves the search
+  // through a thousand sequences.  us, searched for / by number: 1024 prompts of 100 tokens,
+  // 32 / 8 heads, D 128 903 / 655; 4000 of 1 to 300, 8 heads, D 64 2207 / 719; 400 of 128 to
+  // 1000, 8 / 4 heads, D 256 1600 / 1800.
+  a.per = a.B > 64 && sat_mul(a.B, per) <= (a.B < 1024 ? 1 : 2) * fewest ? (int)per : 0;
+  const int64_t grid = sat_mul(a.per ? a.B * per : fewest, a.H);
   if (!grid_fits(grid, 64 * W)) return fail(HS_EUNSUPPORTED, "prompt grid too large");
   if constexpr (sizeof(T) == 4)
     hipLaunchKernelGGL((prompt_f32_kernel<D, kBN, KS, W>), dim3((unsigned)grid), dim3(64 * W), 0, stream, a);
   else
     hipLaunchKernelGGL((prompt_mma_kernel<T, D, kBN, KS>), dim3((unsigned)grid), dim3(64 * W), 0, stream, a);
+  return HS_OK;
+}
+
+template <typename T, int D>
+int launch_waves(PromptArgs a, hipStream_t stream) {
+  a.per = (int)ceil_div(a.max_len, 32);
+  const int64_t grid = ceil_div(sat_mul(a.B, a.per, a.H), kWaves);
+  if (!grid_fits(grid, 64 * kWaves)) return fail(HS_EUNSUPPORTED, "prompt grid too large");
+  hipLaunchKernelGGL((prompt_wave_kernel<T, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, stream, a);
   return HS_OK;
 }
 
@@ -890,8 +1105,17 @@ int launch_one(const PromptArgs& a, hipStream_t stream) {
 // fp32 at head dim 128: the tiles fill the LDS of a CU, so it holds one workgroup, and
 // that has 2 groups of 4 waves, but for short prompts: one group / two, 2048 tokens, 32 / 8
 // heads 233 / 207; 300 and 700 tokens 74 / 59; 16 prompts of 128 32 / 47.
+//
+// Short prompts take a wave each.  us, workgroups as above / waves: 512 of 16 tokens, 32 / 8
+// heads, D 128 253 / 54; 8 of 64 10.6 / 8.7; 256 of 64 154 / 108; 256 of 128 194 / 255; fp32, 12
+// heads, D 64, 512 of 16 115 / 26; 256 of 64 64 / 45.  fp32 heads of 128 and more need more of a
+// wave than it can hide: 32 / 8 heads, D 128, 512 of 16 359 / 139, 16 of 24 13.5 / 12.2, 1 of 24
+// 9.5 / 12.2, 256 of 64 271 / 277.
 template <typename T, int D>
 int launch_dim(const PromptArgs& a, int cus, hipStream_t stream) {
+  constexpr bool kLarge = sizeof(T) == 4 && D >= 128;
+  if (a.max_len <= (kLarge ? 32 : 64) && (!kLarge || sat_mul(a.B, a.H) >= 2 * cus))
+    return launch_waves<T, D>(a, stream);
   const bool few = sat_mul(tiles_of(a, 128), a.H) <= cus;
   if constexpr (sizeof(T) == 2) {
     constexpr int kBN = D >= 256 ? 32 : 64;

@@ -17,8 +17,8 @@
 //
 // A workgroup takes a few rows (tokens).  Its threads first fill LDS with the
 // sines and cosines, one (row, pair) each, which all heads of a row then share;
-// then each thread turns the pairs of two 16-byte loads.  Sizes or addresses that are no multiples of 16 bytes take one pair
-// at a time.
+// then each thread turns the pairs of two 16-byte loads.  Sizes or addresses that are no
+// multiples of 16 bytes take one pair at a time.
 //
 // Bound by HBM: 8192 rows of 32 / 8 heads, D 128, bf16 in and out (218 MB), 39 us,
 // 5.6 TB/s (a large copy reaches 6.6), with loads that leave the cache in front of

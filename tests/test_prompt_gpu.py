@@ -335,3 +335,110 @@ def test_out_that_is_an_input_and_lengths_past_32_bits():
         prompt_attention(both[42:], k, v, cu, 30, 0.1, out=both[1:43])
     got = prompt_attention(both[42:], k, v, cu, 30, 0.1, out=both[:42])
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D,H,Hkv", [(32, 4, 4), (64, 6, 2), (128, 8, 2), (256, 4, 1)])
+def test_many_short_prompts(dtype, D, H, Hkv):
+    """A wave each: odd counts of heads and prompts, none and one token, whole tiles and
+    one row more, few and many (fp32 heads of 128 and more differ by their number)."""
+    gen = np.random.default_rng(D + H)
+    for lens in ([1, 32, 0, 31, 17], [33, 64, 63, 1], [int(x) for x in gen.integers(0, 33, 150)],
+                 [int(x) for x in gen.integers(0, 65, 40)]):
+        _check(*_rows(lens, H, Hkv, D, dtype, D + len(lens)), dtype)
+    q, k, v, cu = _rows([20, 40, 30], H, Hkv, D, dtype, 3, extra=2)
+    for scale in (0.0, -0.2, 30.0 / D):
+        _check(q[:90], k[:90], v[:90], cu, dtype, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B", [65, 300, 1100, 4200])
+def test_many_sequences_by_number_and_searched_for(dtype, B):
+    """More sequences than lanes: one length but for one (tiles by their number from a
+    thousand on) and lengths of which most are short (searched for, in one or two steps).
+    Tolerance as of test_long."""
+    from heteroserve.model.prompt_attn import prompt_attention
+
+    gen = np.random.default_rng(B)
+    for lens in ([70 if B < 1000 else 66] * B,
+                 np.where(gen.random(B) < 40 / B, gen.integers(100, 420, B), gen.integers(0, 9, B)).tolist()):
+        lens[B // 2] = 130
+        q, k, v, cu = _rows(lens, 2, 1, 32, dtype, B)
+        got = prompt_attention(q, k, v, torch.tensor(cu, device=DEV), max(lens), 0.2)
+        want = _dense_each(q, k, v, cu, 0.2)
+        tol = 64 * 2.0 ** -24 + (0 if dtype is F32 else 2 * torch.finfo(dtype).eps / 2)
+        rel = ((got.double() - want).norm(dim=-1) / want.norm(dim=-1)).max().item()
+        assert rel <= tol, (rel, tol)
+
+
+def _dense_each(q, k, v, cu, scale):
+    """_dense over padded batches: float64 [T, H, D]."""
+    lens = np.diff(cu)
+    n, B = int(lens.max()), len(lens)
+    at = torch.tensor(cu[:-1].astype(np.int64), device=DEV)[:, None] + torch.arange(n, device=DEV)
+    here = torch.arange(n, device=DEV) < torch.tensor(lens, device=DEV)[:, None]
+    at = torch.where(here, at, 0)
+    out = torch.empty(q.shape, dtype=torch.float64, device=DEV)
+    g = q.shape[1] // k.shape[1]
+    later = torch.ones(n, n, dtype=torch.bool, device=DEV).triu(1)
+    for h in range(q.shape[1]):
+        for b0 in range(0, B, 256):
+            i = at[b0:b0 + 256]
+            x, y, z = q[i, h].double(), k[i, h // g].double(), v[i, h // g].double()
+            s = torch.bmm(x, y.transpose(1, 2).contiguous()) * scale
+            o = torch.bmm(torch.softmax(s.masked_fill(later, -np.inf), -1), z)
+            m = here[b0:b0 + 256]
+            out[i[m], h] = o[m]
+    return out
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("D,B", [(64, 3), (256, 3), (128, 130)])
+def test_what_lies_behind_a_short_prompts_row(dtype, bad, D, B):
+    from heteroserve.model.prompt_attn import prompt_attention
+
+    lens = [30] * B
+    q, k, v, cu = _rows(lens, 4, 2, D, dtype, 11)
+    q, k, v = q.clone(), k.clone(), v.clone()
+    cu_d = torch.tensor(cu, device=DEV)
+    for dirty in (k, v):
+        clean = prompt_attention(q, k, v, cu_d, 30, D ** -0.5)
+        kept, dirty[47, 0, 5] = dirty[47, 0, 5].clone(), bad
+        got = prompt_attention(q, k, v, cu_d, 30, D ** -0.5)
+        assert torch.equal(got[:, 2:], clean[:, 2:])
+        assert torch.equal(got[60:], clean[60:]) and torch.equal(got[:30], clean[:30])
+        assert torch.isfinite(got[:47]).all()
+        tol = 2.0 ** -16 if dtype is F32 else 4 * torch.finfo(dtype).eps
+        assert ((got[30:47] - clean[30:47]).float().abs() <= tol * clean[30:47].float().abs().max()).all()
+        want = _dense(q[30:60], k[30:60], v[30:60], [0, 30], D ** -0.5)[17:, :2]
+        assert torch.equal(torch.isnan(want), torch.isnan(got[47:60, :2]))
+        assert torch.equal(want == np.inf, got[47:60, :2] == np.inf)
+        dirty[47, 0, 5] = kept
+
+
+def test_short_prompts_replayed_and_laid_out_otherwise():
+    """Strided, transposed and expanded rows, rows of no sequence, and a replayed graph."""
+    from heteroserve.model.prompt_attn import prompt_attention
+
+    for dtype in (F32, F16):
+        q, k, v, cu = _rows([33, 0, 50, 7], 4, 2, 64, dtype, 8, extra=3)
+        cu = torch.tensor(cu, device=DEV)
+        out = torch.full((93, 4, 64), 5.0, dtype=dtype, device=DEV)
+        want = prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu, 50, 0.125, out=out)
+        assert (want[90:] == 5.0).all()
+        flipped = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+        for x in ((q, k, v), flipped):
+            assert torch.equal(prompt_attention(*x, cu, 50, 0.125)[:90], want[:90])
+        cut = prompt_attention(q, k, v, cu, 40, 0.125, out=torch.full_like(out, 6.0))
+        assert torch.equal(cut[:73], want[:73]) and (cut[73:83] == 6.0).all()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = prompt_attention(q, k, v, cu, 50, 0.125)
+        for _ in range(3):
+            got.fill_(float("nan"))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got[:90], want[:90])
