@@ -18,8 +18,8 @@
 // of 8192 493 / 496.
 //
 // What bounds it: the matrix cores' power.  One prompt of 8192 tokens, 32 / 8 heads,
-// D 128, bf16: 496 us, 1108 TFLOP/s of useful products at 1.9 GHz (2.5 PFLOP/s
-// nominal at 2.4).  The same loop without softmax and without LDS reads reached
+// D 128, bf16: 491 us, 1120 TFLOP/s of useful products at 1.9 GHz (2.5 PFLOP/s
+// nominal at 2.4; the library's product of two 8192 x 8192 matrices reaches 1226).  The same loop without softmax and without LDS reads reached
 // 1534, without softmax 1347, without barriers and loads 1129.
 //
 // Numerics.  16-bit inputs are multiplied in their own type, the probabilities
@@ -51,7 +51,7 @@ struct PromptArgs {
   int64_t T;
   int max_len;
   float qscale;               // scale * log2(e)
-  int by_level, per;          // order of the tiles: see find_tile
+  int by_level, per;          // order of the tiles: see Task
 };
 
 // First row and rows of sequence b, whatever cu holds: rows of [0, T), at most
@@ -292,89 +292,7 @@ __device__ inline int wave_scan(int x) {
   return x;
 }
 
-// The tile of query rows that workgroup `i` takes, nt_b tiles of `rows` rows in
-// sequence b, of which tile qt walks the keys of qt + 1.  Every wave finds it by
-// itself.  False: there is no such tile.
-//   per       `per` tiles a sequence, some of which may not be, in the sequences' order
-//   by_level  tiles by falling qt, and by b among equals, so that the longest walks
-//             begin first: with F(l) = sum_b max(0, nt_b - l) tiles from level l on, i
-//             lies on the highest level l with F(l) > i
-//   else      a sequence's tiles are neighbours, the last one first, so that its keys
-//             are read again from the L2 of the XCD that its heads run on, and
-//             sequences go by falling nt_b
-// More than 64 sequences go in their order, a sequence's tiles as neighbours, the last
-// one first.
-__device__ inline bool find_tile(const PromptArgs& a, int rows, int i, int& b, int& qt) {
-  const int lane = threadIdx.x & 63;
-  auto tiles_of = [&](int s) {
-    int64_t row0;
-    int len = 0;
-    if (s < a.B) seq_rows(a, s, row0, len);
-    return (len + rows - 1) / rows;
-  };
-  if (a.per) {
-    b = i / a.per;
-    qt = a.per - 1 - (i - b * a.per);
-    return b < a.B;
-  }
-  if (a.B > 64) {
-    // every lane adds up a run of sequences; the run that holds tile i is then looked at
-    // by itself
-    for (int first = 0, n = a.B; n > 0;) {
-      const int run = (n + 63) / 64;
-      int nt = 0;
-#pragma unroll 4
-      for (int s = lane * run; s < min((lane + 1) * run, n); ++s) nt += tiles_of(first + s);
-      const int inc = wave_scan(nt);
-      const uint64_t m = __builtin_amdgcn_ballot_w64(i < inc);
-      if (m == 0) return false;
-      const int at = __builtin_ctzll(m);
-      i -= __builtin_amdgcn_readlane(inc, at) - __builtin_amdgcn_readlane(nt, at);
-      first += at * run;
-      if (run == 1) {
-        b = first;
-        qt = __builtin_amdgcn_readlane(nt, at) - 1 - i;
-        return b < a.B;
-      }
-      n = min(run, n - at * run);
-    }
-    return false;
-  }
-  const int nt = tiles_of(lane);
-  if (a.B == 1) {
-    b = 0;
-    qt = __builtin_amdgcn_readlane(nt, 0) - 1 - i;
-    return qt >= 0;
-  }
-  if (!a.by_level) {
-    // the tiles of the sequences in front of this lane's
-    const int64_t key = (int64_t)nt << 6 | (63 - lane);
-    int before = 0;
-    for (int s = 0; s < a.B; ++s) {
-      const int x = __builtin_amdgcn_readlane(nt, s);
-      before += ((int64_t)x << 6 | (63 - s)) > key ? x : 0;
-    }
-    const uint64_t m = __builtin_amdgcn_ballot_w64(i >= before && i < before + nt);
-    if (m == 0) return false;
-    b = __builtin_ctzll(m);
-    qt = __builtin_amdgcn_readlane(nt + before, b) - 1 - i;
-    return true;
-  }
-  auto from_level = [&](int l) { return wave_sum(max(0, nt - l)); };
-  if (from_level(0) <= i) return false;
-  int lo = 0, hi = (a.max_len + rows - 1) / rows;   // F(lo) > i >= F(hi) = 0
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (from_level(mid) > i) lo = mid; else hi = mid;
-  }
-  qt = lo;
-  uint64_t m = __builtin_amdgcn_ballot_w64(nt > lo);
-  for (int k = i - from_level(lo + 1); k > 0; --k) m &= m - 1;   // the k-th with nt_b > lo
-  b = __builtin_ctzll(m);
-  return true;
-}
-
-// What a workgroup of R waves of rows works on.
+// What a workgroup works on: rows q0 .. of a sequence, for one head.
 struct Task {
   int h, kvh, q0, len;
   int64_t row0;
@@ -383,13 +301,109 @@ struct Task {
     const int p = blockIdx.x % a.H;
     kvh = p % a.Hkv;
     h = kvh * (a.H / a.Hkv) + p / a.Hkv;
-    int b, qt;
-    if (!find_tile(a, rows, (int)(blockIdx.x / a.H), b, qt)) return false;
+    int qt = 0;
+    row0 = len = 0;
+    const bool there = find_tile(a, rows, (int)(blockIdx.x / a.H), qt);
     // wave-uniform, and the loop's bounds with them
-    seq_rows(a, __builtin_amdgcn_readfirstlane(b), row0, len);
+    row0 = readlane64(row0);
+    len = __builtin_amdgcn_readfirstlane(len);
     qt = __builtin_amdgcn_readfirstlane(qt);
     q0 = qt * rows;
-    return qt >= 0 && q0 < len;   // (cu that overlaps can count past 32 bits)
+    return there && qt >= 0 && q0 < len;   // (cu that overlaps can count past 32 bits)
+  }
+
+ private:
+  __device__ void take(int64_t lane_row0, int lane_len, int lane) {
+    row0 = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(lane_row0 >> 32), lane) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)lane_row0, lane));
+    len = __builtin_amdgcn_readlane(lane_len, lane);
+  }
+
+  // The tile of query rows that workgroup `i` takes, nt_b tiles of `rows` rows in
+  // sequence b, of which tile qt walks the keys of qt + 1; sets row0 and len.  Every wave
+  // finds it by itself, with the lengths of up to 64 sequences in its lanes.  False: there
+  // is no such tile.
+  //   by_level  tiles by falling qt, and by b among equals, so that the longest walks
+  //             begin first: with F(l) = sum_b max(0, nt_b - l) tiles from level l on, i
+  //             lies on the highest level l with F(l) > i
+  //   else      a sequence's tiles are neighbours, the last one first, so that its keys
+  //             are read again from the L2 of the XCD that its heads run on, and
+  //             sequences go by falling nt_b
+  //   per       `per` tiles a sequence, some of which may not be: no search, the sequences
+  //             in their order
+  // More than 64 sequences that are searched go in their order too.  A search costs a
+  // workgroup 1 to 4 us, which two others on its CU do not hide where walks are short.
+  __device__ bool find_tile(const PromptArgs& a, int rows, int i, int& qt) {
+    const int lane = threadIdx.x & 63;
+    auto tiles = [&](int n) { return (n + rows - 1) / rows; };
+    if (a.per) {
+      const int b = a.by_level ? i % a.B : i / a.per;
+      qt = a.per - 1 - (a.by_level ? i / a.B : i % a.per);
+      if (b >= a.B) return false;
+      seq_rows(a, __builtin_amdgcn_readfirstlane(b), row0, len);
+      return true;
+    }
+    int64_t r0 = 0;
+    int n = 0;
+    if (a.B > 64) {
+      // every lane adds up a run of sequences; the run that holds tile i is then looked
+      // at by itself
+      for (int first = 0, left = a.B; left > 0;) {
+        const int run = (left + 63) / 64;
+        int nt = 0;
+#pragma unroll 4
+        for (int s = lane * run; s < min((lane + 1) * run, left); ++s) {
+          seq_rows(a, first + s, r0, n);
+          nt += tiles(n);
+        }
+        const int inc = wave_scan(nt);
+        const uint64_t m = __builtin_amdgcn_ballot_w64(i < inc);
+        if (m == 0) return false;
+        const int at = __builtin_ctzll(m);
+        i -= __builtin_amdgcn_readlane(inc, at) - __builtin_amdgcn_readlane(nt, at);
+        if (run == 1) {
+          qt = __builtin_amdgcn_readlane(nt, at) - 1 - i;
+          take(r0, n, at);
+          return at < left;
+        }
+        first += at * run;
+        left = min(run, left - at * run);
+      }
+      return false;
+    }
+    if (lane < a.B) seq_rows(a, lane, r0, n);
+    const int nt = tiles(n);
+    if (!a.by_level) {
+      // the tiles of the sequences in front of this lane's
+      const int64_t key = (int64_t)nt << 6 | (63 - lane);
+      int before = 0;
+      for (int s = 0; s < a.B; ++s) {
+        const int x = __builtin_amdgcn_readlane(nt, s);
+        before += ((int64_t)x << 6 | (63 - s)) > key ? x : 0;
+      }
+      const uint64_t m = __builtin_amdgcn_ballot_w64(i >= before && i < before + nt);
+      if (m == 0) return false;
+      const int b = __builtin_ctzll(m);
+      qt = __builtin_amdgcn_readlane(nt + before, b) - 1 - i;
+      take(r0, n, b);
+      return true;
+    }
+    auto from_level = [&](int l) { return wave_sum(max(0, nt - l)); };
+    if (from_level(0) <= i) return false;
+    int lo = 0, hi = tiles(a.max_len);   // F(lo) > i >= F(hi) = 0
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (from_level(mid) > i) lo = mid; else hi = mid;
+    }
+    qt = lo;
+    // the lane of rank i - F(lo + 1) among those with nt_b > lo (the sum by all lanes)
+    const int want = i - from_level(lo + 1);
+    const uint64_t m = __builtin_amdgcn_ballot_w64(nt > lo);
+    const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+    const uint64_t it = __builtin_amdgcn_ballot_w64(nt > lo && rank == want);
+    if (it == 0) return false;
+    take(r0, n, __builtin_ctzll(it));
+    return true;
   }
 };
 
@@ -1073,10 +1087,10 @@ int launch_one(PromptArgs a, hipStream_t stream) {
   constexpr int rows = 32 * W / KS;
   const int64_t per = ceil_div(a.max_len, rows), fewest = tiles_of(a, rows);
   // Tiles by their number where that launches no empty workgroups, or saves the search
-  // through a thousand sequences.  us, searched for / by number: 1024 prompts of 100 tokens,
-  // 32 / 8 heads, D 128 903 / 655; 4000 of 1 to 300, 8 heads, D 64 2207 / 719; 400 of 128 to
-  // 1000, 8 / 4 heads, D 256 1600 / 1800.
-  a.per = a.B > 64 && sat_mul(a.B, per) <= (a.B < 1024 ? 1 : 2) * fewest ? (int)per : 0;
+  // through a thousand sequences.  us, searched for / by number: 64 prompts of 200 tokens,
+  // 32 / 8 heads, D 128 117 / 92; 1024 of 100 903 / 650; 4000 of 1 to 300, 8 heads, D 64
+  // 2207 / 719; 400 of 128 to 1000, 8 / 4 heads, D 256 1600 / 1800.
+  a.per = sat_mul(a.B, per) <= (a.B < 1024 ? 1 : 2) * fewest ? (int)per : 0;
   const int64_t grid = sat_mul(a.per ? a.B * per : fewest, a.H);
   if (!grid_fits(grid, 64 * W)) return fail(HS_EUNSUPPORTED, "prompt grid too large");
   if constexpr (sizeof(T) == 4)
