@@ -736,7 +736,7 @@ __global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : D == 64 ? 3 : 2)
 // stays split in registers, and the probabilities are split where they stand.  An
 // infinity splits into NaNs: its rows are not finite, and computed again (row_walk).
 // One prompt of 2048 tokens, 32 / 8 heads, D 128: 202 us, 170 TFLOP/s of fp32 products
-// (with the fp32 ones 377); 334 and 1001 tokens, 12 heads, D 64: 26.7 us.
+// (with the fp32 ones 377); 500 and 834 tokens, 12 heads, D 64: 26.3 us (37).
 struct Split3 {
   uint32_t h, m, l;   // two numbers each
   __device__ Split3(float x, float y) {
@@ -1114,7 +1114,7 @@ int launch_waves(PromptArgs a, hipStream_t stream) {
 //   bf16  1 prompt of 512 tokens, 32 heads, D 128 (128 workgroups) 15.3 / 13.1; 1000, 12 heads,
 //         D 64 (96) 16.1 / 11.7; 4 of 1024, 12 heads, D 64 (384) 19.8 / 21.4; 2048, 32 heads, D 128
 //         (512) 51 / 70
-//   fp32  334 and 1001, 12 heads, D 64 (144) 46 / 28.5; 3 of 1024 (288) 57 / 56; 4 (384) 61 / 64;
+//   fp32  500 and 834, 12 heads, D 64 (132) 46 / 28.5; 3 of 1024 (288) 57 / 56; 4 (384) 61 / 64;
 //         8 (768) 111 / 130
 // fp32 at head dim 128: the tiles fill the LDS of a CU, so it holds one workgroup, and
 // that has 2 groups of 4 waves, but for short prompts: one group / two, 2048 tokens, 32 / 8

@@ -24,4 +24,6 @@ builder, which this image does not have.
     kvpack        export_blocks, write_blocks (numpy and torch forms),
                   gather_kv_batch, KV-row writes, block tables
     splits        choose_num_splits
+    operators     rotary positions, whole prompts, pages (no reference
+                  counterpart: from their definitions, in 64 bits)
 """
