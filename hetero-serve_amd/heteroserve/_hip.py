@@ -215,6 +215,8 @@ def check(rc: int) -> None:
 _DTYPE_CODES = {} if torch is None else {
     torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 _raw_stream = getattr(getattr(torch, "_C", None), "_cuda_getCurrentRawStream", None)
+_device = getattr(getattr(torch, "_C", None), "_cuda_getDevice", None)   # once HIP is up
+_INT32 = getattr(torch, "int32", None)
 
 
 def dtype_code(dt) -> int:
@@ -240,7 +242,7 @@ def _stream_at(index: int) -> int:
 def _int32_on(t, device):
     if not torch.is_tensor(t):
         t = torch.as_tensor(t)
-    if t.dtype is torch.int32 and t.get_device() == device.index and t.is_contiguous():
+    if t.dtype is _INT32 and t.get_device() == device.index and t.is_contiguous():
         return t
     return t.to(device=device, dtype=torch.int32).contiguous()
 
@@ -287,7 +289,7 @@ class _DeviceGuard:
         self._prev = None
 
     def __enter__(self):
-        cur = torch.cuda.current_device()
+        cur = _device() if _device is not None else torch.cuda.current_device()
         if cur != self._index:
             self._prev = cur
             torch.cuda.set_device(self._index)
@@ -653,6 +655,10 @@ def _head_rows(x, heads: int, D: int):
     return _rows(x, heads, D)
 
 
+def _contiguous_like(x, dtype):
+    return torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _rotary_head(q, k, positions, inv_freq, axes, interleaved):
     """What both rotary calls pass first: (q, k, their row strides, the device index,
     the arguments from positions to D, and the tensors those point to)."""
@@ -692,8 +698,8 @@ def rotary(q, k, positions, inv_freq, axes, interleaved, out_dtype):
     out_dtype = out_dtype or q.dtype
     out_code = dtype_code(out_dtype)
     q, k, strides, index, middle, keep = _rotary_head(q, k, positions, inv_freq, axes, interleaved)
-    q_out = q.new_empty(q.shape, dtype=out_dtype)
-    k_out = q.new_empty(k.shape, dtype=out_dtype)
+    q_out = _contiguous_like(q, out_dtype)
+    k_out = _contiguous_like(k, out_dtype)
     with _DeviceGuard(index):
         check(L.hs_rotary(q.data_ptr(), k.data_ptr(), dtype_code(q.dtype), *strides, *middle,
                           q_out.data_ptr(), k_out.data_ptr(), out_code, _stream_at(index)))
@@ -729,8 +735,8 @@ def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, block_tables, 
         raise RuntimeError(f"{sid.numel()} sequence ids for {n} rows")
     if sid is None and n > B:
         raise RuntimeError("without seq_ids, row i uses table row i: more rows than tables")
-    q_out = q.new_empty(q.shape, dtype=out_dtype)
-    k_out = q.new_empty(k.shape, dtype=out_dtype) if keep_k else None
+    q_out = _contiguous_like(q, out_dtype)
+    k_out = _contiguous_like(k, out_dtype) if keep_k else None
     with _DeviceGuard(index):
         check(L.hs_rotary_append(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype_code(q.dtype), *strides, v_row, *middle,
@@ -787,7 +793,7 @@ def prompt_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float, out=Non
     if cu.dim() != 1 or B < 0:
         raise RuntimeError("cu_seqlens must be [B + 1]")
     if out is None:
-        out = q.new_empty(shape)
+        out = _contiguous_like(q, dtype)
     elif (out.shape != shape or out.dtype is not dtype or out.get_device() != index
           or not out.is_contiguous() or out.data_ptr() % 16):
         raise RuntimeError("out must be a contiguous, 16-byte aligned tensor like q")
