@@ -1109,13 +1109,28 @@ int launch_waves(PromptArgs a, hipStream_t stream) {
   return HS_OK;
 }
 
-// Few workgroups of 128 rows (no more than CUs) split the keys over their waves.  us, one
-// group of waves / 16-bit types: 2 groups of 2, fp32 at head dims 32 and 64: 4 groups of 2:
-//   bf16  1 prompt of 512 tokens, 32 heads, D 128 (128 workgroups) 15.3 / 13.1; 1000, 12 heads,
-//         D 64 (96) 16.1 / 11.7; 4 of 1024, 12 heads, D 64 (384) 19.8 / 21.4; 2048, 32 heads, D 128
-//         (512) 51 / 70
-//   fp32  500 and 834, 12 heads, D 64 (132) 46 / 28.5; 3 of 1024 (288) 57 / 56; 4 (384) 61 / 64;
-//         8 (768) 111 / 130
+// Few workgroups of 128 rows split the keys over their waves: the longest walk, which the
+// others' CUs would wait for, is half as long, for twice the set-up and a merge.  How many
+// are few depends on how many fit a CU and on the walk's length.  us, one group of waves /
+// two (fp32, D 32 and 64: four of half as many waves):
+//   D 128  2 at a time a CU: 1 prompt of 512 tokens, 32 / 8 heads (128 workgroups) 16.0 / 14.3,
+//          640 (160) 18.2 / 18.2, 3 of 200, 32 heads (192) 11.7 / 16.7, 1024 (256) 24.1 / 26.3
+//   D 256  1 at a time: 8 / 4 heads, 1 of 4096 (256) 134 / 114, 4 of 1024 (256) 43.2 / 45.6, 4736
+//          (296) 147 / 153
+//   D 64   12 heads, 4 of 640 (240) 13.1 / 11.7, 16 of 256 (384) 10.4 / 14.0; long walks: 2 of 1536
+//          (288) 23.0 / 18.1, 2 of 2048 (384) 29.9 / 28.1, 2 of 2688 (504) 40.1 / 39.9
+//   D 32   8 heads, 4 of 1024 (256) 14.2 / 11.0, 64 of 512 (2048) 36 / 73; long walks: 2 of 4096
+//          (512) 41.2 / 37.5, 4 of 3200 (800) 46.0 / 44.6, 8 of 4096 (2048) 118 / 148
+//   fp32   12 heads, D 64, 500 and 834 (132) 46 / 28.5, 3 of 1024 (288) 57 / 56, 4 (384) 61 / 64
+template <typename T, int D>
+bool few(const PromptArgs& a, int cus) {
+  const int64_t n = sat_mul(tiles_of(a, 128), a.H);
+  const bool long_walks = a.max_len >= 1536;
+  if (sizeof(T) == 2 && D == 128) return n <= (int64_t)cus * 5 / 8;
+  if (sizeof(T) == 2 && D <= 64 && long_walks) return n <= (int64_t)cus * (D == 64 ? 3 : 6) / 2;
+  return n <= cus;
+}
+
 // fp32 at head dim 128: the tiles fill the LDS of a CU, so it holds one workgroup, and
 // that has 2 groups of 4 waves, but for short prompts: one group / two, 2048 tokens, 32 / 8
 // heads 233 / 207; 300 and 700 tokens 74 / 59; 16 prompts of 128 32 / 47.
@@ -1130,12 +1145,12 @@ int launch_dim(const PromptArgs& a, int cus, hipStream_t stream) {
   constexpr bool kLarge = sizeof(T) == 4 && D >= 128;
   if (a.max_len <= (kLarge ? 32 : 64) && (!kLarge || sat_mul(a.B, a.H) >= 2 * cus))
     return launch_waves<T, D>(a, stream);
-  const bool few = sat_mul(tiles_of(a, 128), a.H) <= cus;
+  const bool split = few<T, D>(a, cus);
   if constexpr (sizeof(T) == 2) {
     constexpr int kBN = D >= 256 ? 32 : 64;
-    return few ? launch_one<T, D, kBN, 2, 4>(a, stream) : launch_one<T, D, kBN, 1, 4>(a, stream);
+    return split ? launch_one<T, D, kBN, 2, 4>(a, stream) : launch_one<T, D, kBN, 1, 4>(a, stream);
   } else if constexpr (D <= 64) {
-    return few ? launch_one<T, D, 32, 4, 8>(a, stream) : launch_one<T, D, 64, 1, 4>(a, stream);
+    return split ? launch_one<T, D, 32, 4, 8>(a, stream) : launch_one<T, D, 64, 1, 4>(a, stream);
   } else if constexpr (D == 128) {
     return a.max_len > 256 ? launch_one<T, D, 32, 2, 8>(a, stream) : launch_one<T, D, 32, 1, 4>(a, stream);
   } else {
