@@ -1111,8 +1111,8 @@ int launch_waves(PromptArgs a, hipStream_t stream) {
 
 // Few workgroups of 128 rows split the keys over their waves: the longest walk, which the
 // others' CUs would wait for, is half as long, for twice the set-up and a merge.  How many
-// are few depends on how many fit a CU and on the walk's length.  us, one group of waves /
-// two (fp32, D 32 and 64: four of half as many waves):
+// are few depends on how many fit a CU and on the walk's length.  us, one group of 4 waves /
+// two of 2 (fp32: four of 2, at D 128 two of 4), workgroups in brackets:
 //   D 128  2 at a time a CU: 1 prompt of 512 tokens, 32 / 8 heads (128 workgroups) 16.0 / 14.3,
 //          640 (160) 18.2 / 18.2, 3 of 200, 32 heads (192) 11.7 / 16.7, 1024 (256) 24.1 / 26.3
 //   D 256  1 at a time: 8 / 4 heads, 1 of 4096 (256) 134 / 114, 4 of 1024 (256) 43.2 / 45.6, 4736
@@ -1121,20 +1121,24 @@ int launch_waves(PromptArgs a, hipStream_t stream) {
 //          (288) 23.0 / 18.1, 2 of 2048 (384) 29.9 / 28.1, 2 of 2688 (504) 40.1 / 39.9
 //   D 32   8 heads, 4 of 1024 (256) 14.2 / 11.0, 64 of 512 (2048) 36 / 73; long walks: 2 of 4096
 //          (512) 41.2 / 37.5, 4 of 3200 (800) 46.0 / 44.6, 8 of 4096 (2048) 118 / 148
-//   fp32   12 heads, D 64, 500 and 834 (132) 46 / 28.5, 3 of 1024 (288) 57 / 56, 4 (384) 61 / 64
+//   fp32   D 64, 12 heads: 500 and 834 (132) 46 / 28.5, 16 of 256 (384) 24 / 36; long walks: 3 of
+//          1024 (288) 54 / 51, 2 of 2048 (384) 106 / 100, 1 of 6784 (636) 406 / 450
+//          D 32, 8 heads, long walks: 1 of 8192 (512) 242 / 230, 2 of 6400 (800) 264 / 268
+//          D 128 (2 at a time a CU, with 2 groups of 4 waves 1), 32 / 8 heads: 1 of 300 (96) 36 / 31,
+//          4 of 300 (384) 48 / 55; long walks: 2048 (512) 233 / 202, 3200 (800) 441 / 468
 template <typename T, int D>
 bool few(const PromptArgs& a, int cus) {
   const int64_t n = sat_mul(tiles_of(a, 128), a.H);
-  const bool long_walks = a.max_len >= 1536;
-  if (sizeof(T) == 2 && D == 128) return n <= (int64_t)cus * 5 / 8;
-  if (sizeof(T) == 2 && D <= 64 && long_walks) return n <= (int64_t)cus * (D == 64 ? 3 : 6) / 2;
+  if constexpr (sizeof(T) == 2) {
+    if (D == 128) return n <= (int64_t)cus * 5 / 8;
+    if (D <= 64 && a.max_len >= 1536) return n <= (int64_t)cus * (D == 64 ? 3 : 6) / 2;
+  } else {
+    if (D == 128) return a.max_len > 256 && n <= (int64_t)cus * (a.max_len >= 512 ? 2 : 1);
+    if (D <= 64 && a.max_len >= 1024) return n <= (int64_t)cus * (D == 64 ? 3 : 5) / 2;
+  }
   return n <= cus;
 }
 
-// fp32 at head dim 128: the tiles fill the LDS of a CU, so it holds one workgroup, and
-// that has 2 groups of 4 waves, but for short prompts: one group / two, 2048 tokens, 32 / 8
-// heads 233 / 207; 300 and 700 tokens 74 / 59; 16 prompts of 128 32 / 47.
-//
 // Short prompts take a wave each.  us, workgroups as above / waves: 512 of 16 tokens, 32 / 8
 // heads, D 128 253 / 54; 8 of 64 10.6 / 8.7; 256 of 64 154 / 108; 256 of 128 194 / 255; fp32, 12
 // heads, D 64, 512 of 16 115 / 26; 256 of 64 64 / 45.  fp32 heads of 128 and more need more of a
@@ -1152,7 +1156,7 @@ int launch_dim(const PromptArgs& a, int cus, hipStream_t stream) {
   } else if constexpr (D <= 64) {
     return split ? launch_one<T, D, 32, 4, 8>(a, stream) : launch_one<T, D, 64, 1, 4>(a, stream);
   } else if constexpr (D == 128) {
-    return a.max_len > 256 ? launch_one<T, D, 32, 2, 8>(a, stream) : launch_one<T, D, 32, 1, 4>(a, stream);
+    return split ? launch_one<T, D, 32, 2, 8>(a, stream) : launch_one<T, D, 32, 1, 4>(a, stream);
   } else {
     return launch_one<T, D, 32, 1, 4>(a, stream);
   }
