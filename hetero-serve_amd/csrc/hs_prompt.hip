@@ -130,6 +130,7 @@ __device__ inline void row_walk(const PromptArgs& a, int64_t row0, int i, int h)
 
 // ---- the matrix-core kernels ------------------------------------------------
 
+constexpr float kLeastScale = 1.2e-38f;   // no scale is taken as this one, fp32's least normal
 constexpr float kSlack = 8.0f;   // lazy raise of the running max, log2 units
 
 typedef short short4x __attribute__((ext_vector_type(4)));
@@ -579,8 +580,9 @@ __global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : D == 64 ? 3 : 2)
   // tiles on their way as well
 #pragma unroll
   for (int c = 0; c < kDC; ++c) asm volatile("" : "+v"(qf[c]));
-  // above 0, so that the -inf of a key behind the row stays one
-  const float qs = fmaxf(fabsf(a.qscale), 1e-30f);
+  // above 0, so that the -inf of a key behind the row stays one, and so small that no
+  // finite score counts
+  const float qs = fmaxf(fabsf(a.qscale), kLeastScale);
   State<kDB> st;
   st.clear();
   const int last_kt = min(first_row / kKeys, n_kt - 1);   // the only step with keys behind some row
@@ -820,7 +822,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_f32_kernel(Pr
       split8(x, y, sign, qf[c]);
     }
   }
-  const float qs = fmaxf(fabsf(a.qscale), 1e-30f);
+  const float qs = fmaxf(fabsf(a.qscale), kLeastScale);
 
   State<kDB> st;
   st.clear();
@@ -962,7 +964,7 @@ __global__ __launch_bounds__(64 * kWaves) void prompt_wave_kernel(PromptArgs a) 
   const uint8_t* vb = a.v + t.row0 * a.v_row + t.kvh * a.v_head;
   const int kl = swap23(j), vi = j & 15;
   const float sign = a.qscale < 0 ? -1.0f : 1.0f;
-  const float qs = fmaxf(fabsf(a.qscale), 1e-30f);
+  const float qs = fmaxf(fabsf(a.qscale), kLeastScale);
   const uint32_t to = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds[wave]);
   State<kDB> st;

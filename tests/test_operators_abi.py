@@ -109,6 +109,14 @@ def test_prompt_refusals(lib):
     assert _prompt(lib, T=0, q=None) == _prompt(lib, B=0, q=None) == _prompt(lib, longest=0, q=None) == 0
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
+def test_prompt_scales_that_are_none(lib, scale):
+    one = ctypes.c_void_p(0x1000)
+    rc = lib.hs_prompt_attention(one, one, one, 2, 256, 64, 128, 64, 128, 64, one, 1, 8, 8, 4, 2, 64,
+                                 scale, one, None)
+    _refused(lib, rc, -1, b"finite")
+
+
 def test_page_refusals(lib):
     _refused(lib, lib.hs_kv_copy(None, 1, 8, 1024, FAKE, FAKE, 3, None), -1, b"null")
     _refused(lib, lib.hs_kv_copy(FAKE, 1, 0, 1024, FAKE, FAKE, 3, None), -1, b"positive")

@@ -442,3 +442,19 @@ def test_short_prompts_replayed_and_laid_out_otherwise():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got[:90], want[:90])
+
+
+@pytest.mark.parametrize("lens", [[40, 20], [300, 5]])
+def test_no_scale_and_scores_of_any_size(lens):
+    """A scale of 0 makes every finite score 0, however large: the mean of the values."""
+    from heteroserve.model.prompt_attn import prompt_attention
+
+    for dtype in (F32, BF16):
+        q, k, v, cu = _rows(lens, 2, 1, 64, dtype, 3)
+        cu = torch.tensor(cu, device=DEV)
+        big = prompt_attention((q * 2.0 ** 50).to(dtype), (k * 2.0 ** 50).to(dtype), v, cu, max(lens), 0.0)
+        # scores of 0: other products, so only the rounding of the sums may differ
+        none = prompt_attention(torch.zeros_like(q), k, v, cu, max(lens), 0.0)
+        tol = 2 * max(lens) * 2.0 ** -24 * v.abs().max().item()
+        tol += 0 if dtype is F32 else 2 * torch.finfo(dtype).eps * v.abs().max().item()
+        assert (big.float() - none.float()).abs().max().item() <= tol
