@@ -652,7 +652,10 @@ def _head_rows(x, heads: int, D: int):
     s = x.stride()
     if s[2] == 1 and (s[1] == D or heads == 1) and s[0] >= heads * D:
         return x, s[0]
-    return _rows(x, heads, D)
+    x, row = _rows(x, heads, D)
+    if row < heads * D:      # rows that overlap, such as an expanded one's
+        return x.contiguous(), heads * D
+    return x, row
 
 
 def _contiguous_like(x, dtype):

@@ -298,3 +298,23 @@ def test_outputs_that_are_their_sources(dtype, D, pairs, interleaved, n):
         table.numel(), at.data_ptr(), seq.data_ptr(), stream))
     assert torch.equal(a, want[0]) and torch.equal(b, want[1])
     assert torch.equal(kc.view(-1, Hkv, D)[:n], want[1]) and torch.equal(vc.view(-1, Hkv, D)[:n], v)
+
+
+def test_expanded_and_overlapping_rows():
+    from heteroserve.kv import rotary
+
+    q, k, v = _inputs(1, 4, 2, 64, BF16, 5)
+    at, freq = torch.arange(6, dtype=torch.int32, device=DEV), _freq(32)
+    wide = [x.expand(6, -1, 64) for x in (q, k, v)]
+    want = rotary.rotate_qk(*[x.contiguous() for x in wide[:2]], at, freq)
+    got = rotary.rotate_qk(*wide[:2], at, freq)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    kc, vc = torch.zeros(2, 1, 16, 2, 64, dtype=BF16, device=DEV)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    got, none = rotary.rotate_append_kv(*wide, at, freq, kc, vc, table, at, torch.zeros_like(at))
+    assert torch.equal(got, want[0]) and none is None
+    assert torch.equal(kc[0, :6], want[1]) and torch.equal(vc[0, :6], v.expand(6, 2, 64))
+    flat = torch.randn(64 * 9, device=DEV).to(BF16)
+    slid = flat.as_strided((6, 2, 64), (64, 64, 1))
+    want = rotary.rotate_qk(slid.contiguous(), slid.contiguous(), at, freq)
+    assert torch.equal(rotary.rotate_qk(slid, slid, at, freq)[0], want[0])
