@@ -221,13 +221,12 @@ struct VPlace {
     else return c;
   }
 };
-constexpr int kThreads = 256;
 
 // The loads of K's or V's rows, kKeys at a time; rows past the sequence are read as
 // its last one (and masked), and behind the last tile it is read again.  A load of the
 // workgroup covers kStep rows; the swizzle repeats after kOff of them, so those many
 // offsets per lane serve all.
-template <int kC, int kKeys, typename Place>
+template <int kC, int kKeys, typename Place, int kThreads>
 struct TileLoads {
   static constexpr int kLoads = kKeys * kC / kThreads, kStep = kThreads / kC;
   static constexpr int kOff = Place::kPeriod > kStep ? Place::kPeriod / kStep : 1;
@@ -532,20 +531,20 @@ __device__ inline void landed() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLater) : "memory");
 }
 
-// 16-bit types.  KS groups of 4 / KS waves take KS neighbouring tiles of kBN keys each
+// 16-bit types.  KS groups of W / KS waves take KS neighbouring tiles of kBN keys each
 // step, for the same rows, and put their states together at the end: twice the
 // workgroups, each half as long, where there are few.
 //
 // A 32x32x16 product's accumulator register r of lane half h is row 8 (r / 4) + 4 h +
 // r % 4, its operand wants 8 h + r % 8 (+ 16 (r / 8)); lane j of K's operand reading key
 // swap23(j) turns the one into the other for the probabilities.
-template <typename T, int D, int kBN, int KS>
-__global__ __launch_bounds__(kThreads, KS > 1 || D == 256 ? 1 : D == 64 ? 3 : 2) void prompt_mma_kernel(
+template <typename T, int D, int kBN, int KS, int W>
+__global__ __launch_bounds__(64 * W, KS > 1 || D == 256 ? 1 : D == 64 && W == 4 ? 3 : 2) void prompt_mma_kernel(
     PromptArgs a) {
-  constexpr int R = 4 / KS, kC = D / 8, kKeys = KS * kBN, kRowBytes = 2 * D;
+  constexpr int R = W / KS, kC = D / 8, kKeys = KS * kBN, kRowBytes = 2 * D;
   constexpr int kKB = kBN / 32, kDC = D / 16, kDB = D / 32;
-  using KLoads = TileLoads<kC, kKeys, KPlace<kC>>;
-  using VLoads = TileLoads<kC, kKeys, VPlace<kC>>;
+  using KLoads = TileLoads<kC, kKeys, KPlace<kC>, 64 * W>;
+  using VLoads = TileLoads<kC, kKeys, VPlace<kC>, 64 * W>;
   __shared__ __align__(1024) uint8_t lds[2][2][kKeys * kRowBytes];   // [K, V][even, odd tiles]
 
   const int lane = threadIdx.x & 63, j = lane & 31, hh = lane >> 5;
@@ -1098,7 +1097,7 @@ int launch_one(PromptArgs a, hipStream_t stream) {
   if constexpr (sizeof(T) == 4)
     hipLaunchKernelGGL((prompt_f32_kernel<D, kBN, KS, W>), dim3((unsigned)grid), dim3(64 * W), 0, stream, a);
   else
-    hipLaunchKernelGGL((prompt_mma_kernel<T, D, kBN, KS>), dim3((unsigned)grid), dim3(64 * W), 0, stream, a);
+    hipLaunchKernelGGL((prompt_mma_kernel<T, D, kBN, KS, W>), dim3((unsigned)grid), dim3(64 * W), 0, stream, a);
   return HS_OK;
 }
 
@@ -1146,6 +1145,15 @@ bool few(const PromptArgs& a, int cus) {
 // heads, D 64, 512 of 16 115 / 26; 256 of 64 64 / 45.  fp32 heads of 128 and more need more of a
 // wave than it can hide: 32 / 8 heads, D 128, 512 of 16 359 / 139, 16 of 24 13.5 / 12.2, 1 of 24
 // 9.5 / 12.2, 256 of 64 271 / 277.
+//
+// 16-bit prompts of up to 768 tokens and different lengths (four fifths of the longest on
+// average, or less) take workgroups of 2 waves, 64 rows, and steps of 32 keys: fewer rows
+// past an end, and four workgroups a CU where two fitted, whose set-ups overlap.  us, 4 waves
+// / 2, evenly spread lengths: 1 to 200, 32 / 8 heads, D 128, 64 prompts 57 / 45, 300 276 / 227;
+// 1 to 400, 32 prompts 56 / 50; 200 to 400, 40 prompts 103 / 93; 1 to 700, 32 prompts 106 / 95;
+// 1 to 1000, 64 prompts 370 / 370; 1 to 2000, 32 prompts 485 / 502; all of one length: 128 of 256
+// tokens 221 / 228, 256 of 128, 12 heads, D 64 39 / 49; 1 to 200, 64 prompts, 32 / 8 heads, D 32
+// 22.9 / 17.3, 8 / 4 heads, D 256 43 / 37.
 template <typename T, int D>
 int launch_dim(const PromptArgs& a, int cus, hipStream_t stream) {
   constexpr bool kLarge = sizeof(T) == 4 && D >= 128;
@@ -1154,6 +1162,8 @@ int launch_dim(const PromptArgs& a, int cus, hipStream_t stream) {
   const bool split = few<T, D>(a, cus);
   if constexpr (sizeof(T) == 2) {
     constexpr int kBN = D >= 256 ? 32 : 64;
+    if (!split && a.max_len <= 768 && 5 * a.T <= 4 * sat_mul(a.B, a.max_len))
+      return launch_one<T, D, 32, 1, 2>(a, stream);
     return split ? launch_one<T, D, kBN, 2, 4>(a, stream) : launch_one<T, D, kBN, 1, 4>(a, stream);
   } else if constexpr (D <= 64) {
     return split ? launch_one<T, D, 32, 4, 8>(a, stream) : launch_one<T, D, 64, 1, 4>(a, stream);

@@ -458,3 +458,46 @@ def test_no_scale_and_scores_of_any_size(lens):
         tol = 2 * max(lens) * 2.0 ** -24 * v.abs().max().item()
         tol += 0 if dtype is F32 else 2 * torch.finfo(dtype).eps * v.abs().max().item()
         assert (big.float() - none.float()).abs().max().item() <= tol
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D,H,Hkv", [(32, 16, 8), (64, 12, 4), (128, 16, 2), (256, 8, 8)])
+def test_lengths_that_differ_and_are_many(dtype, D, H, Hkv):
+    """Many prompts of up to some hundred tokens, most far shorter than the longest, and
+    the same with rows behind them; lengths around 64 and none.  Tolerance as of
+    test_long."""
+    from heteroserve.model.prompt_attn import prompt_attention
+
+    gen = np.random.default_rng(D)
+    for lens in ([int(x) for x in gen.integers(0, 150, 60)], [63, 64, 65, 127, 128, 129, 1, 0, 400] * 4,
+                 [int(x) for x in gen.integers(1, 640, 9)] + [768] + [3] * 20):
+        q, k, v, cu = _rows(lens, H, Hkv, D, dtype, D + H, extra=5)
+        out = torch.full((sum(lens) + 5, H, D), 9.0, dtype=dtype, device=DEV)
+        got = prompt_attention(q, k, v, torch.tensor(cu, device=DEV), max(lens), D ** -0.5, out=out)
+        assert (got[-5:] == 9.0).all()
+        want = _dense_each(q, k, v, cu, D ** -0.5)[:-5]
+        rel = ((got[:-5].double() - want).norm(dim=-1) / want.norm(dim=-1)).max().item()
+        assert rel <= 64 * 2.0 ** -24 + 2 * torch.finfo(dtype).eps / 2
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_bad_values_among_lengths_that_differ(bad):
+    from heteroserve.model.prompt_attn import prompt_attention
+
+    lens = [200, 30, 90, 10, 150] * 8
+    q, k, v, cu = _rows(lens, 16, 16, 64, BF16, 11)
+    q, k, v = q.clone(), k.clone(), v.clone()
+    cu_d = torch.tensor(cu, device=DEV)
+    clean = prompt_attention(q, k, v, cu_d, 200, 0.125)
+    for dirty in (k, v):
+        kept, dirty[150, 3, 5] = dirty[150, 3, 5].clone(), bad
+        got = prompt_attention(q, k, v, cu_d, 200, 0.125)
+        same = torch.ones_like(got, dtype=torch.bool)
+        same[150:200, 3] = False
+        same[:150, 3] = False          # computed again by another order of sums, if in its tile
+        assert torch.equal(got[same], clean[same])
+        tol = 4 * torch.finfo(BF16).eps * clean[:150, 3].float().abs().max()
+        assert ((got[:150, 3] - clean[:150, 3]).float().abs() <= tol).all()
+        want = _dense(q[:200], k[:200], v[:200], [0, 200], 0.125)[150:, 3]
+        assert torch.equal(torch.isnan(want), torch.isnan(got[150:200, 3]))
+        dirty[150, 3, 5] = kept
