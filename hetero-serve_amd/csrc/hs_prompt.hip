@@ -11,16 +11,18 @@
 // side of such a load is linear (fp32 tiles pass through registers, see Split3).
 // S^T = K Q^T and O^T = V^T P^T: a lane holds one query's scores, so its maximum and sum
 // need one exchange of the two lane halves, and the probabilities are the second
-// product's operand where they stand.  Short prompts take a wave each instead.  Rows
-// are 128 and not 256 a workgroup because two workgroups then share a CU: one's
+// product's operand where they stand.  Short prompts take a wave each, and batches of
+// different short lengths 64 rows a workgroup (see few and launch_dim).  Rows are
+// otherwise 128 and not 256 a workgroup because two workgroups then share a CU: one's
 // set-up and barriers pass beside the other's products.  us at 256 / 128 rows, bf16:
 // one prompt of 2048 tokens, 32 / 8 heads, D 128 55 / 49, 32 of 128 tokens 50 / 27, one
 // of 8192 493 / 496.
 //
 // What bounds it: the matrix cores' power.  One prompt of 8192 tokens, 32 / 8 heads,
 // D 128, bf16: 491 us, 1120 TFLOP/s of useful products at 1.9 GHz (2.5 PFLOP/s
-// nominal at 2.4; the library's product of two 8192 x 8192 matrices reaches 1226).  The same loop without softmax and without LDS reads reached
-// 1534, without softmax 1347, without barriers and loads 1129.
+// nominal at 2.4; the library's product of two 8192 x 8192 matrices reaches 1226).  The
+// same loop without softmax and without LDS reads reached 1534, without softmax 1347,
+// without barriers and loads 1129.
 //
 // Numerics.  16-bit inputs are multiplied in their own type, the probabilities
 // rounded to it (relative to a maximum that is at most 2^8 too low, so none

@@ -870,7 +870,7 @@ def kv_fork(pool, block_tables, context_lens, ref_counts, parents, children, fre
         raise RuntimeError("context_lens must have one entry per table row, ref_counts one per block")
     if children.numel() != n or fresh.numel() != n:
         raise RuntimeError("parents, children and fresh must have the same length")
-    forked = ref_counts.new_empty(n)
+    forked = torch.empty_like(parents)
     with _DeviceGuard(index):
         check(L.hs_kv_fork(pool.data_ptr(), *_pages(pool), pool.shape[3], block_tables.data_ptr(), B, MB,
                            context_lens.data_ptr(), ref_counts.data_ptr(), parents.data_ptr(),
