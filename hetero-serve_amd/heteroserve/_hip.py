@@ -837,12 +837,12 @@ def kv_copy(pool, src_dev, dst_dev) -> None:
 
 
 def kv_copy_host_ids(pool, src, dst) -> None:
-    """kv_copy with at most HOST_IDS / 2 pairs in contiguous int64 numpy arrays."""
+    """kv_copy with at most HOST_IDS / 2 pairs in array("q")s."""
     L = lib("KV copy HIP kernel")
     index = pool.get_device()
     with _DeviceGuard(index):
-        check(L.hs_kv_copy_host_ids(pool.data_ptr(), *_pages(pool), src.ctypes.data, dst.ctypes.data,
-                                    src.size, _stream_at(index)))
+        check(L.hs_kv_copy_host_ids(pool.data_ptr(), *_pages(pool), src.buffer_info()[0],
+                                    dst.buffer_info()[0], len(src), _stream_at(index)))
 
 
 def kv_find_free(ref_counts, n: int):

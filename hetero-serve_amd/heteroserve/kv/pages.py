@@ -26,32 +26,47 @@ do.
 
 from __future__ import annotations
 
+from array import array
+
 from .. import _hip
-from .pack import _check_pool, _ids_array, _ids_tensor, _normalise_ids
+from .pack import _check_pool, _ids_tensor, _normalise_ids
+
+
+def _host_ids(block_ids, num_blocks: int):
+    """Block ids as an array("q"), wrapped and refused as _normalise_ids does.  A list of
+    ids that need no wrapping, the usual case, takes no numpy call (16 ids: 1.5 us
+    instead of 13)."""
+    if type(block_ids) is list and block_ids:
+        try:
+            ids = array("q", block_ids)
+            if 0 <= min(ids) and max(ids) < num_blocks:
+                return ids
+        except (TypeError, ValueError, OverflowError):
+            pass
+    return array("q", _normalise_ids(block_ids, num_blocks).tolist())
 
 
 def copy_blocks(pool, src_ids, dst_ids) -> None:
     """pool[:, :, dst_ids[i]] = pool[:, :, src_ids[i]], bit for bit.  Ids follow
     torch indexing; a destination may not repeat nor be a source."""
-    import numpy as np
-
     _hip.lib("KV copy HIP kernel")
     _check_pool(pool)
-    src = _normalise_ids(src_ids, pool.shape[2])
-    dst = _normalise_ids(dst_ids, pool.shape[2])
+    src = _host_ids(src_ids, pool.shape[2])
+    dst = _host_ids(dst_ids, pool.shape[2])
     n = len(src)
     if len(dst) != n:
         raise RuntimeError(f"{n} source blocks for {len(dst)} destinations")
     if n == 0:
         return
-    if _repeats(dst):
+    to = set(dst)
+    if len(to) != n:
         raise RuntimeError("a destination block repeats")
-    if not set(dst.tolist()).isdisjoint(src.tolist()):
+    if not to.isdisjoint(src):
         raise RuntimeError("a block is both source and destination")
     if 2 * n <= _hip.HOST_IDS:
-        _hip.kv_copy_host_ids(pool, _ids_array(src), _ids_array(dst))
+        _hip.kv_copy_host_ids(pool, src, dst)
     else:
-        both = _ids_tensor(np.concatenate([src, dst]), pool.device)
+        both = _ids_tensor(src + dst, pool.device)
         _hip.kv_copy(pool, both[:n], both[n:])
 
 

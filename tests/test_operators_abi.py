@@ -234,3 +234,17 @@ def test_refusals_under_asan_and_ubsan():
     out = r.stdout + r.stderr
     assert r.returncode == 0, out[-4000:]
     assert "runtime error" not in out and "AddressSanitizer" not in out, out[-4000:]
+
+
+def test_host_ids():
+    """Lists, arrays, tensors and the odd element: as torch indexing takes them."""
+    np, torch = pytest.importorskip("numpy"), pytest.importorskip("torch")
+    from heteroserve.kv import pages
+
+    for ids, want in (([3, 0, 9], [3, 0, 9]), ([-1, 2], [9, 2]), ([], []), ((4, 5), [4, 5]), ([True], [1]),
+                      (np.array([1, -10]), [1, 0]), (torch.tensor([[7], [8]]), [7, 8]), ([np.int32(6)], [6]),
+                      ([2.0], [2])):
+        assert pages._host_ids(ids, 10).tolist() == want
+    for ids in ([10], [0, -11], [2 ** 70], np.array([10])):
+        with pytest.raises(IndexError, match="out of bounds"):
+            pages._host_ids(ids, 10)
