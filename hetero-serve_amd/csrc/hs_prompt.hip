@@ -1148,24 +1148,26 @@ bool few(const PromptArgs& a, int cus) {
 // wave than it can hide: 32 / 8 heads, D 128, 512 of 16 359 / 139, 16 of 24 13.5 / 12.2, 1 of 24
 // 9.5 / 12.2, 256 of 64 271 / 277.
 //
-// 16-bit prompts of up to 768 tokens and different lengths (four fifths of the longest on
-// average, or less) take workgroups of 2 waves, 64 rows, and steps of 32 keys: fewer rows
+// Prompts of up to 768 tokens and different lengths (four fifths of the longest on average,
+// or less) take, in 16-bit types or at head dims 32 and 64, workgroups of 2 waves, 64 rows, and steps of 32 keys: fewer rows
 // past an end, and four workgroups a CU where two fitted, whose set-ups overlap.  us, 4 waves
 // / 2, evenly spread lengths: 1 to 200, 32 / 8 heads, D 128, 64 prompts 57 / 45, 300 276 / 227;
 // 1 to 400, 32 prompts 56 / 50; 200 to 400, 40 prompts 103 / 93; 1 to 700, 32 prompts 106 / 95;
 // 1 to 1000, 64 prompts 370 / 370; 1 to 2000, 32 prompts 485 / 502; all of one length: 128 of 256
 // tokens 221 / 228, 256 of 128, 12 heads, D 64 39 / 49; 1 to 200, 64 prompts, 32 / 8 heads, D 32
-// 22.9 / 17.3, 8 / 4 heads, D 256 43 / 37.
+// 22.9 / 17.3, 8 / 4 heads, D 256 43 / 37; fp32, 12 heads, D 64 44 / 37, 32 / 8 heads, D 32
+// 45 / 32, D 128 155 / 179, which splits each key's numbers for half the rows.
 template <typename T, int D>
 int launch_dim(const PromptArgs& a, int cus, hipStream_t stream) {
   constexpr bool kLarge = sizeof(T) == 4 && D >= 128;
   if (a.max_len <= (kLarge ? 32 : 64) && (!kLarge || sat_mul(a.B, a.H) >= 2 * cus))
     return launch_waves<T, D>(a, stream);
   const bool split = few<T, D>(a, cus);
-  if constexpr (sizeof(T) == 2) {
-    constexpr int kBN = D >= 256 ? 32 : 64;
+  if constexpr (!kLarge)
     if (!split && a.max_len <= 768 && 5 * a.T <= 4 * sat_mul(a.B, a.max_len))
       return launch_one<T, D, 32, 1, 2>(a, stream);
+  if constexpr (sizeof(T) == 2) {
+    constexpr int kBN = D >= 256 ? 32 : 64;
     return split ? launch_one<T, D, kBN, 2, 4>(a, stream) : launch_one<T, D, kBN, 1, 4>(a, stream);
   } else if constexpr (D <= 64) {
     return split ? launch_one<T, D, 32, 4, 8>(a, stream) : launch_one<T, D, 64, 1, 4>(a, stream);

@@ -460,7 +460,7 @@ def test_no_scale_and_scores_of_any_size(lens):
         assert (big.float() - none.float()).abs().max().item() <= tol
 
 
-@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("D,H,Hkv", [(32, 16, 8), (64, 12, 4), (128, 16, 2), (256, 8, 8)])
 def test_lengths_that_differ_and_are_many(dtype, D, H, Hkv):
     """Many prompts of up to some hundred tokens, most far shorter than the longest, and
@@ -477,15 +477,16 @@ def test_lengths_that_differ_and_are_many(dtype, D, H, Hkv):
         assert (got[-5:] == 9.0).all()
         want = _dense_each(q, k, v, cu, D ** -0.5)[:-5]
         rel = ((got[:-5].double() - want).norm(dim=-1) / want.norm(dim=-1)).max().item()
-        assert rel <= 64 * 2.0 ** -24 + 2 * torch.finfo(dtype).eps / 2
+        assert rel <= 64 * 2.0 ** -24 + (0 if dtype is F32 else 2 * torch.finfo(dtype).eps / 2)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
-def test_bad_values_among_lengths_that_differ(bad):
+def test_bad_values_among_lengths_that_differ(dtype, bad):
     from heteroserve.model.prompt_attn import prompt_attention
 
     lens = [200, 30, 90, 10, 150] * 8
-    q, k, v, cu = _rows(lens, 16, 16, 64, BF16, 11)
+    q, k, v, cu = _rows(lens, 16, 16, 64, dtype, 11)
     q, k, v = q.clone(), k.clone(), v.clone()
     cu_d = torch.tensor(cu, device=DEV)
     clean = prompt_attention(q, k, v, cu_d, 200, 0.125)
@@ -496,7 +497,7 @@ def test_bad_values_among_lengths_that_differ(bad):
         same[150:200, 3] = False
         same[:150, 3] = False          # computed again by another order of sums, if in its tile
         assert torch.equal(got[same], clean[same])
-        tol = 4 * torch.finfo(BF16).eps * clean[:150, 3].float().abs().max()
+        tol = (2.0 ** -16 if dtype is F32 else 4 * torch.finfo(dtype).eps) * clean[:150, 3].float().abs().max()
         assert ((got[:150, 3] - clean[:150, 3]).float().abs() <= tol).all()
         want = _dense(q[:200], k[:200], v[:200], [0, 200], 0.125)[150:, 3]
         assert torch.equal(torch.isnan(want), torch.isnan(got[150:200, 3]))
