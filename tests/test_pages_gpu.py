@@ -299,3 +299,37 @@ def test_no_fresh_block_from_the_host_is_no_block():
         pages.fork_blocks(pool, t, c, r, [0], [4], [-2])
     with pytest.raises(RuntimeError, match="2\\^31"):
         pages.find_free_blocks(r, 2 ** 31)
+
+
+def test_copies_replayed_in_a_graph():
+    """Block ids of a captured copy are the graph's own: replays copy what the pool then
+    holds."""
+    from heteroserve.kv import pages
+
+    pool = _pool(2, 9, 16, 2, 64)
+    src, dst = [0, 1, 1], [6, 7, 8]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pages.copy_blocks(pool, src, dst)
+    src[:], dst[:] = [5, 5, 5], [2, 3, 4]
+    for i in range(3):
+        pool.copy_(_pool(2, 9, 16, 2, 64, seed=i))
+        want = pool.clone()
+        want[:, :, 6:] = want[:, :, [0, 1, 1]]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(pool, want)
+
+
+def test_copies_of_pages_that_are_no_multiples_of_16_bytes_and_of_bytes():
+    from heteroserve.kv import pages
+
+    for shape, dtype in (((2, 2, 6, 3, 1, 5), torch.float16), ((1, 2, 6, 16, 1, 8), torch.uint8),
+                         ((1, 2, 6, 5, 1, 3), torch.uint8)):
+        pool = torch.randint(0, 120, shape, device=DEV).to(dtype)
+        want = pool.clone()
+        want[:, :, [4, 0]] = want[:, :, [2, 5]]
+        pages.copy_blocks(pool, [2, 5], [4, 0])
+        assert torch.equal(pool, want)
