@@ -34,7 +34,8 @@
 // Masked keys.  A score that a row does not see is -inf and its probability 0, but 0
 // times an infinite or NaN value is NaN in a product.  A row whose result is not
 // finite is therefore computed again by a walk that never touches the keys behind
-// it (row_walk); rows that hold such values by right pay for it too.
+// it (row_walk).  Rows that hold such values by right pay for it too: those of a key only
+// up to it, those of a value for all of the row's keys, many times the products' price.
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
 
@@ -109,6 +110,8 @@ __device__ inline void row_walk(const PromptArgs& a, int64_t row0, int i, int h)
 #pragma unroll
       for (int e = 0; e < kVec; ++e) acc[e] = ok ? fmaf(p, f[e], acc[e] * keep) : acc[e];
     }
+    // a score that is none, or infinite: so is the sum, and every element of the row
+    if (__builtin_amdgcn_ballot_w64(l != l) != 0) break;
   }
 #pragma unroll
   for (int off = kLpt; off < 64; off <<= 1) {
