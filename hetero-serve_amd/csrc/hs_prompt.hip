@@ -19,7 +19,7 @@
 // of 8192 493 / 496.
 //
 // What bounds it: the matrix cores' power.  One prompt of 8192 tokens, 32 / 8 heads,
-// D 128, bf16: 491 us, 1120 TFLOP/s of useful products at 1.9 GHz (2.5 PFLOP/s
+// D 128, bf16: 485 us, 1135 TFLOP/s of useful products at 1.9 GHz (2.5 PFLOP/s
 // nominal at 2.4; the library's product of two 8192 x 8192 matrices reaches 1226).  The
 // same loop without softmax and without LDS reads reached 1534, without softmax 1347,
 // without barriers and loads 1129.
