@@ -197,15 +197,17 @@ struct ForkArgs {
 };
 
 // A child's plan, the same in every workgroup that works for it: the parent's
-// full blocks, the tokens of its last one and where they lie.  False: no fork.
+// full blocks, the tokens of its last one and where they lie.  False: no fork, and
+// without `rows` (a row that is none, or its own parent) no row to empty either.
 struct ForkPlan {
+  bool rows;
   int parent, child, full, rem, last, fresh, ctx;
 };
 __device__ inline bool fork_plan(const ForkArgs& a, int i, ForkPlan& p) {
   p.parent = a.parents[i];
   p.child = a.children[i];
-  if (p.parent < 0 || p.parent >= a.B || p.child < 0 || p.child >= a.B || p.parent == p.child)
-    return false;
+  p.rows = p.parent >= 0 && p.parent < a.B && p.child >= 0 && p.child < a.B && p.parent != p.child;
+  if (!p.rows) return false;
   p.ctx = (int)max((int64_t)0, min((int64_t)a.ctx[p.parent], (int64_t)a.MB * a.BS));
   p.full = p.ctx / a.BS;
   p.rem = p.ctx - p.full * a.BS;
@@ -236,7 +238,7 @@ __global__ __launch_bounds__(kCopyThreads) void fork_kernel(ForkArgs a) {
     return;
   }
   if (threadIdx.x == 0) a.forked[i] = ok;
-  if (p.child < 0 || p.child >= a.B || p.child == p.parent) return;
+  if (!p.rows) return;
   int32_t* row = a.bt + (int64_t)p.child * a.MB;
   const int32_t* from = a.bt + (int64_t)p.parent * a.MB;   // read only where ok
   for (int j = threadIdx.x; j < a.MB; j += kCopyThreads) {
