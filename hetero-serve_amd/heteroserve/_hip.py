@@ -247,6 +247,23 @@ def _int32_on(t, device):
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 
+def _whole_on(what: str, t, device):
+    """_int32_on of integers only.  One that 32 bits do not hold becomes the nearest that
+    they do, so what named no row or block still names none."""
+    if not torch.is_tensor(t):
+        t = torch.as_tensor(t)
+    dt = t.dtype
+    if dt is not _INT32 and t.numel():
+        if dt.is_floating_point or dt.is_complex or dt is torch.bool:
+            raise RuntimeError(f"{what} must be integers, got {dt}")
+        if dt is torch.int64 or dt is torch.uint32 or dt is torch.uint64:
+            t = t.to(device=device, dtype=torch.int64)
+            if dt is torch.uint64:
+                t = t.masked_fill(t < 0, 0x7fffffff)
+            t = t.clamp(-0x80000000, 0x7fffffff)
+    return _int32_on(t, device)
+
+
 def _check_device(q, k_cache, v_cache) -> int:
     """The device index that all three tensors are on."""
     index = q.get_device()

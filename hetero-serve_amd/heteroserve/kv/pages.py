@@ -17,10 +17,10 @@ copy to the host, so a step that forks or frees can be captured in a graph:
     ref_counts     [num_blocks]: how many table rows (or other holders, such as a
                    prefix cache) keep a block; a block is free at 0
 
-Row indexes and fresh blocks come as device tensors, which are not read back (one
-that names no row or block is skipped), or from the host, where they follow torch
+Row indexes and fresh blocks come as device tensors of integers, which are not read back
+(one that names no row or block is skipped), or from the host, where they follow torch
 indexing (but a fresh block of -1 is none, as from find_free_blocks) and mistakes
-raise before anything is launched.  copy_blocks reads its ids back, as the pack calls
+raise before anything is launched.  A mask is no list of rows, on either side.  copy_blocks reads its ids back, as the pack calls
 do.
 """
 
@@ -88,7 +88,7 @@ def _indexes(values, size: int, what: str, device, none: bool = False):
     import torch
 
     if torch.is_tensor(values) and values.is_cuda:
-        return _hip._int32_on(values if values.dim() == 1 else values.reshape(-1), device), None
+        return _hip._whole_on(what, values if values.dim() == 1 else values.reshape(-1), device), None
     import numpy as np
 
     host = np.asarray(values.tolist() if torch.is_tensor(values) else values).reshape(-1)

@@ -65,3 +65,61 @@ def test_fork_of_a_row_that_is_none_leaves_the_child(parent):
     got = pages.fork_blocks(*state, _dev(parents), _dev(children), _dev(fresh))
     assert got.tolist() == done.tolist()
     assert s.same(state, want)
+
+
+@pytest.mark.parametrize("bad", [torch.tensor([True, False, True, True, False, False, True, True]),
+                                 torch.tensor([1.0, 2.9]), torch.tensor([3.0], dtype=torch.float16)])
+def test_rows_on_the_device_must_be_integers_too(bad):
+    """As from the host: a mask or a number with a fraction is no list of rows."""
+    from heteroserve.kv import pages
+
+    s = _State()
+    state, want = s.on_device(), s.host()
+    for rows in (bad, bad.to(DEV)):
+        with pytest.raises(RuntimeError, match="row must be integers"):
+            pages.free_blocks(*state[1:], rows)
+        for given in ([rows, [6] * len(rows), [0] * len(rows)], [[0], rows, [1]], [[0], [6], rows]):
+            with pytest.raises(RuntimeError, match="must be integers"):
+                pages.fork_blocks(*state, *given)
+    assert s.same(state, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint32, torch.uint64])
+def test_rows_on_the_device_past_32_bits_are_none(dtype):
+    """They are skipped, and are not the rows and blocks of their lower 32 bits."""
+    from heteroserve.kv import pages
+
+    s = _State()
+    state, want = s.on_device(), s.host()
+    far = [2 ** 32 - 1] if dtype is torch.uint32 else [2 ** 32, 2 ** 32 + 1, 2 ** 33 + 2, 2 ** 63 - 1]
+    if dtype is torch.int64:
+        far += [-2 ** 32 + 3, -2 ** 63 + 4]
+    if dtype is torch.uint64:
+        far += [2 ** 64 - 1, 2 ** 63 + 5]
+    wide = torch.tensor(far, dtype=dtype, device=DEV)
+    n = len(far)
+    pages.free_blocks(*state[1:], wide)
+    assert s.same(state, want)
+    child, fresh = _dev([6] + [-1] * (n - 1)), _dev(ops.find_free(s.refs, n))
+    assert not pages.fork_blocks(*state, wide, child, fresh).any()
+    assert not pages.fork_blocks(*state, _dev([0] * n), wide, fresh).any()
+    assert s.same(state, want)
+    want[1][6], want[2][6] = -1, 0
+    assert not pages.fork_blocks(*state, _dev([0] + [-1] * (n - 1)), child, wide).any()
+    assert s.same(state, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64,
+                                   torch.uint16, torch.uint32, torch.uint64])
+def test_rows_of_every_integer_type(dtype):
+    from heteroserve.kv import pages
+
+    s = _State()
+    state, want = s.on_device(), s.host()
+    fresh = ops.find_free(s.refs, 2)
+    done = ops.fork(*want, [0, 3], [6, 7], fresh)
+    rows = [torch.tensor(x, device=DEV).to(dtype) for x in ([0, 3], [6, 7], fresh)]
+    assert pages.fork_blocks(*state, *rows).tolist() == done.tolist() == [1, 1]
+    ops.free(*want[1:], [7, 0])
+    pages.free_blocks(*state[1:], torch.tensor([7, 0], device=DEV).to(dtype))
+    assert s.same(state, want)
