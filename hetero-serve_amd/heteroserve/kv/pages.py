@@ -91,14 +91,18 @@ def _indexes(values, size: int, what: str, device, none: bool = False):
         return _hip._whole_on(what, values if values.dim() == 1 else values.reshape(-1), device), None
     import numpy as np
 
-    host = np.asarray(values.tolist() if torch.is_tensor(values) else values).reshape(-1)
+    if torch.is_tensor(values):
+        values = values.numpy() if values.dtype is torch.uint64 else values.tolist()
+    host = np.asarray(values).reshape(-1)
     if host.size and host.dtype.kind not in "iu":
         raise RuntimeError(f"{what} must be integers, got {host.dtype}")
-    host = host.astype(np.int64)
-    bad = (host < (-1 if none else -size)) | (host >= size)
+    bad = host >= size        # in the values' own type: past 2^63 is not below 0
+    if host.dtype.kind == "i":
+        bad |= host < (-1 if none else -size)
     if bad.any():
         i = int(host[int(np.argmax(bad))])
         raise IndexError(f"{what} index {i} is out of bounds for size {size}")
+    host = host.astype(np.int64)
     if not none:
         host = np.where(host < 0, host + size, host)
     return torch.from_numpy(host.astype(np.int32)).to(device), host
