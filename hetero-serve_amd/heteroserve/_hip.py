@@ -692,17 +692,17 @@ def _rotary_head(q, k, positions, inv_freq, axes, interleaved):
     if k_rows != n or k_dim != D or k.dtype is not q.dtype:
         raise RuntimeError("k must have the rows, the head_dim and the dtype of q")
     dev = q.device
-    pos = _int32_on(positions, dev)
+    pos = _whole_on("positions", positions, dev)
     n_axes = 1 if pos.dim() <= 1 else pos.shape[0]
     if pos.dim() > 2 or pos.numel() != n_axes * n:
-        raise RuntimeError(f"positions must be [axes, {n}] or [{n}], got {tuple(positions.shape)}")
+        raise RuntimeError(f"positions must be [axes, {n}] or [{n}], got {tuple(pos.shape)}")
     freq = inv_freq
     if freq.dtype is not torch.float32 or freq.get_device() != index or not freq.is_contiguous():
         freq = freq.to(device=dev, dtype=torch.float32).contiguous()
     pairs = freq.numel()
     if not 0 < pairs <= D // 2:
         raise RuntimeError(f"inv_freq must have 1 to head_dim / 2 = {D // 2} entries, got {pairs}")
-    pa = None if axes is None else _int32_on(axes, dev)
+    pa = None if axes is None else _whole_on("axes", axes, dev)
     if pa is not None and pa.numel() != pairs:
         raise RuntimeError(f"{pa.numel()} axes for {pairs} rotary pairs")
     q, q_row = _head_rows(q, H, D)
@@ -743,9 +743,9 @@ def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, block_tables, 
         raise RuntimeError("k and v rows must have the same count and dtype")
     v, v_row = _head_rows(v, Hkv, D) if v.shape == k.shape else _rows(v, Hkv, D)
     dev = q.device
-    bt = _int32_on(block_tables, dev)
-    at = _int32_on(cache_positions, dev)
-    sid = None if seq_ids is None else _int32_on(seq_ids, dev)
+    bt = _whole_on("block_tables", block_tables, dev)
+    at = _whole_on("cache_positions", cache_positions, dev)
+    sid = None if seq_ids is None else _whole_on("seq_ids", seq_ids, dev)
     if bt.dim() != 2:
         raise RuntimeError("block_tables must be [B, max_blocks]")
     B, MB = bt.shape
@@ -808,7 +808,7 @@ def prompt_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float, out=Non
     if k.dtype is not dtype or v.dtype is not dtype:
         raise RuntimeError("q, k and v must have the same dtype")
     code = dtype_code(dtype)
-    cu = _int32_on(cu_seqlens, q.device)
+    cu = _whole_on("cu_seqlens", cu_seqlens, q.device)
     B = cu.numel() - 1
     if cu.dim() != 1 or B < 0:
         raise RuntimeError("cu_seqlens must be [B + 1]")

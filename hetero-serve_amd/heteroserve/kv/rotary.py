@@ -20,6 +20,9 @@ No reference counterpart (its models learn their positions); append_kv
     interleaved pairs are elements (2 i, 2 i + 1) instead of (i, pairs + i)
     out_dtype   of the returned q and k (default: the dtype they came in;
                 paged_attention takes float32 queries)
+
+Positions, axes, tables and numbers of other integer types are converted, the far ones
+to the nearest that 32 bits hold; others are refused (a position of 1.5 is not 1).
 """
 
 from __future__ import annotations
