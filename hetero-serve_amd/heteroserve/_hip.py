@@ -665,9 +665,9 @@ def block_tables(packed_dev, B: int, width: int, out) -> None:
 
 
 def _head_rows(x, heads: int, D: int):
-    """_rows of a tensor whose last two dims are known to be (heads, D)."""
+    """_rows of [n, heads, D] or [n, heads * D], a copy of rows that overlap."""
     s = x.stride()
-    if s[2] == 1 and (s[1] == D or heads == 1) and s[0] >= heads * D:
+    if len(s) == 3 and s[2] == 1 and (s[1] == D or heads == 1) and s[0] >= heads * D:
         return x, s[0]
     x, row = _rows(x, heads, D)
     if row < heads * D:      # rows that overlap, such as an expanded one's
@@ -741,7 +741,9 @@ def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, block_tables, 
         raise RuntimeError(f"K/V rows must be [n, {cache_heads}, {cache_dim}], got {tuple(k.shape)}")
     if v.dtype is not k.dtype or v.shape[0] != n:
         raise RuntimeError("k and v rows must have the same count and dtype")
-    v, v_row = _head_rows(v, Hkv, D) if v.shape == k.shape else _rows(v, Hkv, D)
+    if v.dim() == 3 and v.shape != k.shape:
+        raise RuntimeError(f"K/V rows must be [n, {Hkv}, {D}], got {tuple(v.shape)}")
+    v, v_row = _head_rows(v, Hkv, D)
     dev = q.device
     bt = _whole_on("block_tables", block_tables, dev)
     at = _whole_on("cache_positions", cache_positions, dev)
