@@ -198,11 +198,11 @@ __device__ inline float both_sum(float x) {
 
 // 16 bytes from base + every lane's offset to LDS, at the wave's byte offset `to` + 16 lane;
 // counted by vmcnt.  As a builtin, the compiler waits for all such loads before every
-// transposing read.  No output register is in flight, and nothing else here uses m0.
+// transposing read.  No output register is in flight.
 __device__ inline void load_to_lds(const uint8_t* base, uint32_t offset, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to),
                "v"(offset), "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
 
 // Where the 16-byte chunk c of row r lies in its LDS row of kC chunks, so that each
