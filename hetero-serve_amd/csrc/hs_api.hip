@@ -1010,7 +1010,8 @@ int hs_prompt_attention(const void* q, const void* k, const void* v, int dtype, 
   if (total > 0x7fffffffLL || std::min(total, (int64_t)max_seqlen) > (1 << 30))
     return fail(HS_EUNSUPPORTED, "too many rows for 32-bit offsets");
   if (H > 65535) return fail(HS_EUNSUPPORTED, "too many heads for one launch");
-  if (!(scale - scale == 0.0f)) return fail(HS_EINVAL, "scale must be finite");
+  const float powers = scale * kLog2e;   // what the kernels work with
+  if (!(powers - powers == 0.0f)) return fail(HS_EINVAL, "scale must be finite, times log2(e) as well");
   const int64_t sizes[6] = {q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride,
                             v_head_stride};
   const int64_t unit = dtype == HS_DTYPE_F32 ? 4 : 8;   // elements of 16 bytes

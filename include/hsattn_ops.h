@@ -73,7 +73,8 @@ int hs_rotary_append(const void* q, const void* k, const void* v, int src_dtype,
  *               16-byte aligned
  *   out         [total, H, D] of dtype, contiguous, 16-byte aligned; must not
  *               overlap the inputs
- *   D           32, 64, 128 or 256;  H % Hkv == 0;  scale finite
+ *   D           32, 64, 128 or 256;  H % Hkv == 0;  scale finite, and times
+ *               log2(e) as well (below 2.35e38)
  */
 int hs_prompt_attention(const void* q, const void* k, const void* v, int dtype,
                         int64_t q_row_stride, int64_t q_head_stride, int64_t k_row_stride,
