@@ -135,7 +135,8 @@ __device__ inline void row_walk(const PromptArgs& a, int64_t row0, int i, int h)
 
 // ---- the matrix-core kernels ------------------------------------------------
 
-constexpr float kLeastScale = 1.2e-38f;   // no scale is taken as this one, fp32's least normal
+// No scale is taken as this one, fp32's least number: all finite scores are below 5e-7 then.
+constexpr float kLeastScale = 0x1p-149f;
 constexpr float kSlack = 8.0f;   // lazy raise of the running max, log2 units
 
 typedef short short4x __attribute__((ext_vector_type(4)));

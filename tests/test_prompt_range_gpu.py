@@ -1,0 +1,68 @@
+"""Whole prompts at the ends of the number range: the largest values, scales and scores,
+and probabilities far below the largest one.  The helpers' tolerances are those of
+test_prompt_gpu.py; what differs is derived at each test."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+U = 2.0 ** -24
+
+
+def _batches():
+    """(lens, H, Hkv) that take a wave each, split keys, 64-row and 128-row workgroups."""
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    many = -(-cus // 16)
+    return [([1, 40, 64, 3], 2, 1), ([300, 7], 2, 2), ([130, 20, 70] * many, 16, 2),
+            ([200] * (2 * many), 16, 2)]
+
+
+def _call(q, k, v, cu, lens, scale):
+    from heteroserve.model.prompt_attn import prompt_attention
+
+    return prompt_attention(q, k, v, torch.tensor(cu, device=DEV), max(lens), scale)
+
+
+def _cu(lens):
+    return np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [0.0, 1e-40, -3e-39, 2e-38])
+@pytest.mark.parametrize("which", range(4))
+def test_least_scales_and_largest_scores(dtype, scale, which):
+    """q . k of up to 1e38 under a scale of 0 or of fp32's subnormals.  Tolerance of
+    test_prompt_gpu.py with the sums |q k| themselves, and what a step of subnormals (of
+    scale times log2(e), or in the place of 0) makes of a score: 2^-149 S powers of 2."""
+    lens, H, Hkv = _batches()[which]
+    cu, n, D = _cu(lens), sum(lens), 64
+    gen = torch.Generator(device=DEV).manual_seed(which)
+    big = 2.0 ** 60
+    q = (torch.randn(n, H, D, generator=gen, device=DEV).clamp(-3, 3) * big).to(dtype)
+    k = (torch.randn(n, Hkv, D, generator=gen, device=DEV).clamp(-3, 3) * big).to(dtype)
+    v = torch.randn(n, Hkv, D, generator=gen, device=DEV).to(dtype)
+    got = _call(q, k, v, cu, lens, scale).double()
+    held = float(np.float32(scale))
+    half = 0.0 if dtype is F32 else torch.finfo(dtype).eps / 2
+    worst = 0.0
+    for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
+        later = torch.ones(b - a, b - a, dtype=torch.bool, device=DEV).triu(1)
+        for h in range(H):
+            x, y = q[a:b, h].double(), k[a:b, h // (H // Hkv)].double()
+            z = v[a:b, h // (H // Hkv)].double()
+            s = torch.mm(x, y.t().contiguous()) * held
+            S = torch.mm(x.abs(), y.abs().t().contiguous()).max().item()
+            assert torch.mm(x, y.t().contiguous()).abs().max().item() < 3.4e38 and S * abs(held) < 60
+            p = torch.softmax(s.masked_fill(later, -np.inf), -1)
+            want, spread = torch.mm(p, z), torch.mm(p, z.abs())
+            rel = 2 * (2 * (D + 4) * U * S * abs(held) + 4 * U + (b - a) * U + 2.0 ** -149 * S)
+            tol = rel * spread + half * spread * (1 + rel)
+            tol = tol + half * (want.abs() + tol)
+            worst = max(worst, ((got[a:b, h] - want).abs() - tol).max().item())
+    assert worst <= 0.0
