@@ -45,6 +45,9 @@ namespace hs {
 
 namespace {
 
+// Where running maxima start: no finite score lies below, so a row of one is never empty.
+constexpr float kLowest = -0x1.fffffep127f;
+
 struct PromptArgs {
   const uint8_t *q, *k, *v;
   uint8_t* out;               // [T, H, D]
@@ -79,7 +82,7 @@ __device__ inline void row_walk(const PromptArgs& a, int64_t row0, int i, int h)
   const int kvh = h / (a.H / a.Hkv);
   const uint8_t* kp = a.k + row0 * a.k_row + kvh * a.k_head + c * 16;
   const uint8_t* vp = a.v + row0 * a.v_row + kvh * a.v_head + c * 16;
-  float q[kVec], acc[kVec], m = kNegBig, l = 0.0f;
+  float q[kVec], acc[kVec], m = kLowest, l = 0.0f;
   Elem<T>::to_f32(load16(a.q + (row0 + i) * a.q_row + h * a.q_head + c * 16), q);
 #pragma unroll
   for (int e = 0; e < kVec; ++e) {
@@ -430,7 +433,7 @@ struct State {
   float16x o[kDB];
 
   __device__ void clear() {
-    m = kNegBig;
+    m = kLowest;
     l = 0.0f;
 #pragma unroll
     for (int d = 0; d < kDB; ++d)

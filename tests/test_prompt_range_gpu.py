@@ -66,3 +66,29 @@ def test_least_scales_and_largest_scores(dtype, scale, which):
             tol = tol + half * (want.abs() + tol)
             worst = max(worst, ((got[a:b, h] - want).abs() - tol).max().item())
     assert worst <= 0.0
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("which", range(4))
+def test_lowest_scores(dtype, which):
+    """Every score is the same and near fp32's lowest number, in powers of 2: a row's mean.
+    (One product a score, and no rounding in the rest: a power of 2 as key.)"""
+    lens, H, Hkv = _batches()[which]
+    cu, n, D = _cu(lens), sum(lens), 64
+    gen = torch.Generator(device=DEV).manual_seed(which)
+    at = 1.5 * 2.0 ** 6 if dtype is F16 else 1.5 * 2.0 ** 62
+    q, k = (torch.zeros(n, h, D, dtype=dtype, device=DEV) for h in (H, Hkv))
+    q[..., 3], k[..., 3] = -at, at
+    v = torch.randn(n, Hkv, D, generator=gen, device=DEV).to(dtype)
+    scale = 3.2e38 / 1.4426950408889634 / (at * at)
+    got = _call(q, k, v, cu, lens, scale).double()
+    assert torch.isfinite(got).all()
+    half = 0.0 if dtype is F32 else torch.finfo(dtype).eps / 2
+    rel = 2 * (max(lens) + 4) * U
+    for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
+        count = torch.arange(1, b - a + 1, device=DEV, dtype=torch.float64)[:, None, None]
+        want = (v[a:b].double().cumsum(0) / count).repeat_interleave(H // Hkv, 1)
+        spread = (v[a:b].double().abs().cumsum(0) / count).repeat_interleave(H // Hkv, 1)
+        tol = rel * spread + half * spread
+        tol = tol + half * (want.abs() + tol) + (2.0 ** -25 if dtype is F16 else 0.0)
+        assert ((got[a:b] - want).abs() <= tol).all()
