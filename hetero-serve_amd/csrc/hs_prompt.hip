@@ -27,7 +27,9 @@
 // Numerics.  16-bit inputs are multiplied in their own type, the probabilities
 // rounded to it (relative to a maximum that is at most 2^8 too low, so none
 // overflows), and the sum adds the rounded ones, so that the rounding cancels where
-// one key dominates; scores, maxima, sums and O are fp32.  fp32 inputs are split into
+// one key dominates; scores, maxima, sums and O are fp32.  fp16 probabilities are held
+// 2^7 times larger (kLift), which 2^15 still fits: those far below 1, of which a long row
+// may have thousands for each one near it, keep steps of 2^-31 of it instead of 2^-24.  fp32 inputs are split into
 // three bf16 terms, which keeps fp32's accuracy (see Split3).  Scores are scaled in fp32
 // behind the product, not in the query's type before it.
 //
@@ -152,9 +154,10 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 template <typename T>
-struct Half;
+struct Half;   // kLift: powers of 2 that probabilities are held above themselves
 template <>
 struct Half<Bf16> {
+  static constexpr float kLift = 0.0f;
   // acc + both halves' values, in fp32
   __device__ static float sum2(uint32_t w, float acc) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w),
@@ -170,6 +173,7 @@ struct Half<Bf16> {
 };
 template <>
 struct Half<_Float16> {
+  static constexpr float kLift = 7.0f;
   __device__ static float sum2(uint32_t w, float acc) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3c003c00u),
                                   acc, false);
@@ -440,10 +444,10 @@ struct State {
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
   }
-  // The maximum of this lane's new scores, times qs; the running one is only raised
-  // where some row's lies more than kSlack above it.
-  __device__ void raise(float mx, float qs) {
-    mx = both_max(mx) * qs;
+  // The maximum of this lane's new scores, times qs; the running one, m + lift, is only
+  // raised where some row's lies more than kSlack above it.
+  __device__ void raise(float mx, float qs, float lift) {
+    mx = both_max(mx) * qs - lift;
     if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
       const float m_new = fmaxf(m, mx), keep = fast_exp2(m - m_new);
       m = m_new;
@@ -653,7 +657,7 @@ __global__ __launch_bounds__(64 * W, KS > 1 || D == 256 ? 1 : D == 64 && W == 4 
   // from gathering them).
   float mx = 0.0f;
   auto step = [&](int odd, int kt, float16x (&sc)[kKB], float16x (&sn)[kKB]) {
-    st.raise(mx, qs);
+    st.raise(mx, qs, Half<T>::kLift);
     arrive(odd);
     short8x kf[kQk], vf[kPv];
 #pragma unroll
@@ -686,7 +690,7 @@ __global__ __launch_bounds__(64 * W, KS > 1 || D == 256 ? 1 : D == 64 && W == 4 
     }
   };
   auto finish = [&](int odd, float16x (&sc)[kKB]) {
-    st.raise(mx, qs);
+    st.raise(mx, qs, Half<T>::kLift);
     arrive(odd);
 #pragma unroll
     for (int e = 0; e < kPairs; ++e) prob(sc, e);
@@ -876,7 +880,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_f32_kernel(Pr
     for (int kb = 0; kb < kKB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
-    st.raise(mx, qs);
+    st.raise(mx, qs, 0.0f);
     short8x pf[kKB * 2][3];
 #pragma unroll
     for (int g = 0; g < kKB * 2; ++g) {
@@ -1026,7 +1030,8 @@ __global__ __launch_bounds__(64 * kWaves) void prompt_wave_kernel(PromptArgs a) 
     float mx = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    st.raise(mx, qs);
+    if constexpr (kF32) st.raise(mx, qs, 0.0f);
+    else st.raise(mx, qs, Half<T>::kLift);
     if constexpr (kF32) {
       float p[16];
 #pragma unroll

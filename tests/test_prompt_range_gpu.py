@@ -92,3 +92,34 @@ def test_lowest_scores(dtype, which):
         tol = rel * spread + half * spread
         tol = tol + half * (want.abs() + tol) + (2.0 ** -25 if dtype is F16 else 0.0)
         assert ((got[a:b] - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lens,H,Hkv", [([60, 33], 2, 1), ([4097, 200], 2, 1), ([40, 700, 1] * 8, 64, 64),
+                                        ([2000] * 3, 16, 16)])
+@pytest.mark.parametrize("below", [20.0, 24.0, 26.0, 28.0])
+def test_many_keys_far_below_one(dtype, lens, H, Hkv, below):
+    """One key takes nearly all of a row but has no value; what the row gets is the sum of
+    many probabilities of 2^-below.  In fp16 they are held to 2^-32 of the largest one each
+    (2^7 times below the type's smallest step), the rest is relative to what they add up to."""
+    cu, n, D = _cu(lens), sum(lens), 64
+    q, k = (torch.zeros(n, h, D, dtype=dtype, device=DEV) for h in (H, Hkv))
+    v = torch.ones(n, Hkv, D, dtype=dtype, device=DEV)
+    q[..., 0] = 1
+    first = torch.tensor(cu[:-1].astype(np.int64), device=DEV)
+    k[first, :, 0] = 16.0
+    v[first] = 0
+    scale = below / 16 * 0.6931471805599453
+    got = _call(q, k, v, cu, lens, scale).double()
+    p = 2.0 ** -below
+    half = 0.0 if dtype is F32 else torch.finfo(dtype).eps / 2
+    for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
+        i = torch.arange(b - a, device=DEV, dtype=torch.float64)[:, None, None]
+        want = (i * p / (1 + i * p)).expand(b - a, H, D)
+        # scores of up to 28 times fp32's u, twice, and the scale's own rounding
+        rel = 2 * (4 * U * 28 + 4 * U + (b - a) * U)
+        tol = (rel + half) * want
+        tol = tol + half * (want + tol)
+        if dtype is F16:
+            tol = tol + i * 2.0 ** -32 + 2.0 ** -25
+        assert ((got[a:b] - want).abs() <= tol).all(), (a, (got[a:b] - want).abs().max())
