@@ -33,6 +33,10 @@
 // three bf16 terms, which keeps fp32's accuracy (see Split3).  Scores are scaled in fp32
 // behind the product, not in the query's type before it.
 //
+// O is a sum that is divided at its end, so values above fp32's largest over 2^8 times the
+// number of keys can overflow it where their mean would not: such a row is not finite, and
+// computed again with values scaled down (row_walk).
+//
 // Masked keys.  A score that a row does not see is -inf and its probability 0, but 0
 // times an infinite or NaN value is NaN in a product.  A row whose result is not
 // finite is therefore computed again by a walk that never touches the keys behind
@@ -75,7 +79,9 @@ __device__ inline void seq_rows(const PromptArgs& a, int b, int64_t& row0, int& 
 // head row is spread over kLpt lanes and a load of the wave covers kTpl keys;
 // each such group of lanes runs an online softmax of its own, and the states are
 // merged at the end.  Keys behind the row are not added, not even times 0, so what
-// they hold cannot reach it.
+// they hold cannot reach it.  Values are added times a power of 2 that keeps the sum of
+// i + 1 of them in range, and a mean of finite ones that rounds past the largest number is
+// that number.
 template <typename T, int D>
 __device__ inline void row_walk(const PromptArgs& a, int64_t row0, int i, int h) {
   constexpr int kVec = Elem<T>::kVec, kLpt = D / kVec, kTpl = 64 / kLpt;
@@ -85,6 +91,7 @@ __device__ inline void row_walk(const PromptArgs& a, int64_t row0, int i, int h)
   const uint8_t* kp = a.k + row0 * a.k_row + kvh * a.k_head + c * 16;
   const uint8_t* vp = a.v + row0 * a.v_row + kvh * a.v_head + c * 16;
   float q[kVec], acc[kVec], m = kLowest, l = 0.0f;
+  const float up = ldexpf(1.0f, 33 - __clz(i + 1)), down = 1.0f / up;   // up > 2 (i + 1)
   Elem<T>::to_f32(load16(a.q + (row0 + i) * a.q_row + h * a.q_head + c * 16), q);
 #pragma unroll
   for (int e = 0; e < kVec; ++e) {
@@ -113,7 +120,7 @@ __device__ inline void row_walk(const PromptArgs& a, int64_t row0, int i, int h)
       l = l * keep + p;
       Elem<T>::to_f32(vr[u], f);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) acc[e] = ok ? fmaf(p, f[e], acc[e] * keep) : acc[e];
+      for (int e = 0; e < kVec; ++e) acc[e] = ok ? fmaf(p, f[e] * down, acc[e] * keep) : acc[e];
     }
     // a score that is none, or infinite: so is the sum, and every element of the row
     if (__builtin_amdgcn_ballot_w64(l != l) != 0) break;
@@ -128,9 +135,12 @@ __device__ inline void row_walk(const PromptArgs& a, int64_t row0, int i, int h)
     m = mm;
   }
   if (slot != 0) return;
-  const float inv = 1.0f / l;
+  const float inv = up / l;
 #pragma unroll
-  for (int e = 0; e < kVec; ++e) acc[e] *= inv;
+  for (int e = 0; e < kVec; ++e) {
+    const float mean = acc[e] * inv;
+    acc[e] = fabsf(acc[e]) < INFINITY && fabsf(mean) == INFINITY ? copysignf(-kLowest, mean) : mean;
+  }
   uint8_t* dst = a.out + (((row0 + i) * a.H + h) * (int64_t)D) * (int)sizeof(T) + c * 16;
   if constexpr (sizeof(T) == 4)
     *reinterpret_cast<float4*>(dst) = make_float4(acc[0], acc[1], acc[2], acc[3]);

@@ -123,3 +123,28 @@ def test_many_keys_far_below_one(dtype, lens, H, Hkv, below):
         if dtype is F16:
             tol = tol + i * 2.0 ** -32 + 2.0 ** -25
         assert ((got[a:b] - want).abs() <= tol).all(), (a, (got[a:b] - want).abs().max())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("which", range(4))
+def test_values_up_to_the_types_largest(dtype, D, which):
+    """The mean of finite values is finite, whatever their sum.  Queries of 0: every
+    probability is 1 / n, a mean of n values; weights and sums in fp32 are each off by a
+    relative (n + 4) u, a 16-bit type's by half a step more, and so is the output."""
+    lens, H, Hkv = _batches()[which]
+    cu, n, top = _cu(lens), sum(lens), torch.finfo(dtype).max
+    gen = torch.Generator(device=DEV).manual_seed(D)
+    q = torch.zeros(n, H, D, dtype=dtype, device=DEV)
+    k = torch.randn(n, Hkv, D, generator=gen, device=DEV).to(dtype)
+    v = (torch.rand(n, Hkv, D, generator=gen, device=DEV, dtype=torch.float64) / 2 + 0.5) * top
+    v = v.to(dtype)
+    v[:, :, 1], v[:, :, 2] = top, -top
+    got = _call(q, k, v, cu, lens, D ** -0.5).double()
+    assert torch.isfinite(got).all()
+    half = 0.0 if dtype is F32 else torch.finfo(dtype).eps / 2
+    rel = 2 * (max(lens) + 4) * U + 2 * half + half * half
+    for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
+        count = torch.arange(1, b - a + 1, device=DEV, dtype=torch.float64)[:, None, None]
+        want = (v[a:b].double().cumsum(0) / count).repeat_interleave(H // Hkv, 1)
+        assert ((got[a:b] - want).abs() <= rel * want.abs()).all()
