@@ -253,7 +253,10 @@ def _whole_on(what: str, t, device):
     if not torch.is_tensor(t):
         t = torch.as_tensor(t)
     dt = t.dtype
-    if dt is not _INT32 and t.numel():
+    if dt is _INT32:
+        if t.get_device() == device.index and t.is_contiguous():
+            return t
+    elif t.numel():
         if dt.is_floating_point or dt.is_complex or dt is torch.bool:
             raise RuntimeError(f"{what} must be integers, got {dt}")
         if dt is torch.int64 or dt is torch.uint32 or dt is torch.uint64:
