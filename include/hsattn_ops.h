@@ -65,7 +65,9 @@ int hs_rotary_append(const void* q, const void* k, const void* v, int src_dtype,
  * over the rows j <= i of row i's own sequence; sequence b owns the rows
  * [cu_seqlens[b], cu_seqlens[b+1]) of [0, total).  Rows of no sequence, and
  * rows of a sequence from max_seqlen on, are left as they were.  What k and v
- * hold behind a row never reaches it, infinities and NaN included.
+ * hold behind a row never reaches it, infinities and NaN included; rows that see
+ * such a value are right and slow (a walk of their keys one by one).  Finite
+ * values under finite scores give finite rows, up to the type's largest.
  * No reference counterpart (its engine prefills through the cache).
  *   q, k, v     [total, H, D], [total, Hkv, D] twice, of dtype; rows and
  *               heads are the given strides apart (elements, at most 2^22;
