@@ -45,7 +45,8 @@ def _normalise_ids(block_ids, num_blocks: int):
     ids = None
     try:
         if torch.is_tensor(block_ids):
-            if not block_ids.is_floating_point() and not block_ids.is_complex():
+            if (not block_ids.is_floating_point() and not block_ids.is_complex()
+                    and block_ids.dtype is not torch.uint64):
                 ids = block_ids.detach().to("cpu").reshape(-1).to(torch.int64).numpy()
         else:
             arr = np.asarray(block_ids).reshape(-1)

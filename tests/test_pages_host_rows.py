@@ -34,3 +34,14 @@ def test_unsigned_values_past_64_bits_signed_are_no_negative_ones(value, none):
 def test_what_is_no_integer(values):
     with pytest.raises(RuntimeError, match="row must be integers"):
         _indexes(values)
+
+
+def test_block_ids_past_64_bits_signed_are_no_negative_ones():
+    """Of copies, and of the pack calls, which take them the same way."""
+    from heteroserve.kv import pack, pages
+
+    for read in (pages._host_ids, pack._normalise_ids):
+        assert read(torch.tensor([1, 6], dtype=torch.uint64), 8).tolist() == [1, 6]
+        for values in (np.array([2 ** 64 - 1], np.uint64), torch.tensor([0, 2 ** 64 - 1], dtype=torch.uint64)):
+            with pytest.raises(IndexError, match=f"index {2 ** 64 - 1} is out of bounds"):
+                read(values, 8)
