@@ -219,12 +219,17 @@ __device__ inline float both_sum(float x) {
 
 // 16 bytes from base + every lane's offset to LDS, at the wave's byte offset `to` + 16 lane;
 // counted by vmcnt.  As a builtin, the compiler waits for all such loads before every
-// transposing read.  No output register is in flight.
+// transposing read.  No output register is in flight.  m0 is reserved: the compiler keeps no
+// value there, and warns of it among the clobbers, where it says that one which the compiler
+// sets for an instruction of its own is lost (of this file's none needs it).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ inline void load_to_lds(const uint8_t* base, uint32_t offset, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to),
                "v"(offset), "s"(base)
                : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // Where the 16-byte chunk c of row r lies in its LDS row of kC chunks, so that each
 // reading pattern covers all 64 banks: K rows are read 16 at a time at one chunk, V
