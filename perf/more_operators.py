@@ -1,0 +1,402 @@
+"""What decoding over long contexts needs beside the 16-bit cache, as cases that can be timed.
+
+A case is a dict of plain values; its "kind" says which entry points it calls:
+
+  write     append_kv_q4 and read_kv_q4: new rows of keys and values quantised to 4
+            bits as they are written into the paged cache, and the values that
+            they stand for read back (a decode step's single tokens, whole prompts)
+  read      read_kv_q4: the cached prefixes of sequences, for a prefill that goes on
+            behind them
+  attend    paged_attention_q4: one query token per sequence over the 4-bit cache,
+            all of its keys or a window of the last ones and the first few (sinks)
+  window    paged_attention_window: the same window over a cache of the ordinary types
+
+With `own` false, `run` computes the same with elementary torch operations.
+Lengths are evenly spread over a case's range and dealt to the sequences in an
+order that the seed gives, so a case's work is the same for every seed.
+
+The 4-bit cache is a uint8 tensor [blocks, block, kv_heads, 5 D / 8].  Every 32
+elements of a head share a step s and a lowest value lo, both fp16:
+
+    lo = min x,   s = (max x - lo) / 15,   n = (x - lo) / s to the nearest of 0 .. 15
+
+and x is held as n s + lo.  A record is D / 2 bytes of n, 8 elements in a 32-bit
+word, element e in bits 4 e .., then the steps and then the lowest values.  With
+G = D / 32 groups, word w of a value's record holds elements 8 w .., word w of a
+key's elements 32 (w % G) + 8 (w // G) .. .
+"""
+
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+DEV = "cuda:0"
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+BYTES = {"f32": 4, "f16": 2, "bf16": 2}
+
+# (query heads, KV heads, head dim): GPT-2 small, the multi-head benchmark
+# batches, Llama-3-8B's grouped heads, and wider groups and head dims.
+GEOMETRIES = [(12, 12, 64), (32, 32, 128), (32, 8, 128), (32, 8, 64), (32, 4, 128), (16, 16, 64),
+              (16, 1, 128), (8, 8, 32), (8, 4, 256)]
+
+
+def listed():
+    return [
+        # One decode step of a small batch: eight new tokens, a few microseconds.
+        rows("write_step", "write", 8, 128, "bf16", "bf16", 8, 1, 1),
+        # Whole prompts as the projection left them.
+        rows("write_prompts", "write", 8, 128, "bf16", "bf16", 8, 256, 1792),
+        # fp32 projections of GPT-2 small, short blocks, odd sizes.
+        rows("write_odd", "write", 12, 64, "f32", "f32", 3, 101, 427, block=8),
+        # Prefixes of a batch of conversations, read for the next turn's prefill.
+        rows("read_prefixes", "read", 8, 128, "bf16", "bf16", 16, 1000, 4100),
+        # A short prefix of narrow heads.
+        rows("read_short", "read", 8, 32, "f16", "f16", 1, 300, 300),
+        # A small batch of GPT-2 small, contexts up to 512: launches count.
+        attend("attend_step", "attend", 12, 12, 64, "q4", 8, 1, 512, 0, 0),
+        # The ragged benchmark batch at Llama-3-8B's geometry.
+        attend("attend_batch", "attend", 32, 8, 128, "q4", 64, 16, 4096, 0, 0),
+        # Long documents: the cache is what a step reads.
+        attend("attend_long", "attend", 32, 8, 128, "q4", 16, 8192, 32768, 0, 0),
+        # Multi-head attention, odd lengths.
+        attend("attend_heads", "attend", 32, 32, 128, "q4", 17, 77, 2501, 0, 0),
+        # Long contexts of wide groups seen through a window.
+        attend("attend_window", "attend", 32, 4, 128, "q4", 64, 2000, 12000, 4096, 4),
+        # The same of an ordinary cache, the benchmark's grouped heads.
+        attend("window_batch", "window", 32, 8, 128, "bf16", 64, 500, 8500, 1024, 4),
+        # fp32 cache of GPT-2 small, contexts on both sides of the window.
+        attend("window_f32", "window", 12, 12, 64, "f32", 16, 1, 1024, 256, 1),
+    ]
+
+
+# --- case constructors -------------------------------------------------------
+
+
+def rows(name, kind, kv_heads, dim, src, out, batch, lo, hi, block=16):
+    return {"name": name, "kind": kind, "kv_heads": kv_heads, "dim": dim, "src": src, "out": out,
+            "batch": batch, "lo": lo, "hi": hi, "block": block}
+
+
+def attend(name, kind, heads, kv_heads, dim, dtype, batch, lo, hi, window, sinks, block=16):
+    """window 0: all keys are seen."""
+    return {"name": name, "kind": kind, "heads": heads, "kv_heads": kv_heads, "dim": dim,
+            "dtype": dtype, "batch": batch, "lo": lo, "hi": hi, "window": window, "sinks": sinks,
+            "block": block}
+
+
+# --- drawn cases -------------------------------------------------------------
+
+
+def _log(rng, lo, hi):
+    """A whole number of [lo, hi], spread over its logarithm."""
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 0.5)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["write", "read", "attend", "attend", "attend", "window", "window"])
+    while True:
+        heads, kv_heads, dim = rng.choice(GEOMETRIES)
+        block = rng.choice([16, 16, 16, 8, 32])
+        if kind in ("write", "read"):
+            hi = _log(rng, 1, 4096)
+            c = rows("", kind, kv_heads, dim, rng.choice(["f32", "f16", "bf16", "bf16"]),
+                     rng.choice(["f32", "f16", "bf16"]), _log(rng, 1, 64),
+                     max(1, hi // rng.choice([1, 3, 8])), hi, block)
+        else:
+            hi = _log(rng, 1, 32768)
+            windowed = kind == "window" or rng.random() < 0.4
+            c = attend("", kind, heads, kv_heads, dim,
+                       "q4" if kind == "attend" else rng.choice(["f32", "f16", "bf16", "bf16"]),
+                       _log(rng, 1, 128), max(1, hi // rng.choice([1, 4, 16])), hi,
+                       _log(rng, 1, 8192) if windowed else 0,
+                       rng.choice([0, 1, 4, 4, 16, 64]) if windowed else 0, block)
+        del c["name"]
+        if _affordable(c):
+            return c
+
+
+def _affordable(c):
+    """No dearer than the largest listed cases, with pools that fit three times over."""
+    most = 4.2e8 if c["kind"] == "attend" else 3e8
+    return work(c)["bytes"] <= most and int(_lengths(c).sum()) * 2 * _row(c) <= 3e9
+
+
+# --- sizes -------------------------------------------------------------------
+
+
+def _spread(lo, hi, n):
+    """n whole numbers spread evenly over [lo, hi]."""
+    return np.rint(lo + (hi - lo) * (np.arange(n) + 0.5) / n).astype(np.int64)
+
+
+def _lengths(c):
+    return _spread(c["lo"], c["hi"], c["batch"])
+
+
+def _record(dim):
+    """Bytes of one token's head in the 4-bit cache."""
+    return dim // 2 + dim // 32 * 4
+
+
+def _row(c):
+    """Bytes of one token of K (or V) in the cache."""
+    dtype = c.get("dtype", "q4")
+    return c["kv_heads"] * (_record(c["dim"]) if dtype == "q4" else c["dim"] * BYTES[dtype])
+
+
+def _seen(c):
+    """Keys that each sequence's query sees."""
+    s = _lengths(c)
+    return np.minimum(s, c["window"] + c["sinks"]) if c["window"] else s
+
+
+def work(case):
+    c = case
+    if c["kind"] in ("write", "read"):
+        n, e = int(_lengths(c).sum()), c["kv_heads"] * c["dim"]
+        nbytes = _row(c) + e * BYTES[c["out"]]
+        if c["kind"] == "write":
+            nbytes += e * BYTES[c["src"]] + _row(c)
+        return {"bytes": 2 * n * nbytes, "flops": 2 * n * e * (8 if c["kind"] == "write" else 2)}
+    seen = int(_seen(c).sum())
+    return {"bytes": seen * 2 * _row(c) + 2 * 4 * c["batch"] * c["heads"] * c["dim"],
+            "flops": 4 * c["heads"] * c["dim"] * seen}
+
+
+# --- the 4-bit records, in torch -----------------------------------------------
+
+
+def _words(dim, keys):
+    """The word that holds elements 8 w .. of a head, for every w."""
+    w = np.arange(dim // 8)
+    return w % 4 * (dim // 32) + w // 4 if keys else w
+
+
+def _quantise(x):
+    """(n, s, lo) of x [..., D]: n [..., D / 32, 32] whole numbers in x's type, s and lo
+    fp16 [..., D / 32]."""
+    g = x.clamp(-65504.0, 65504.0).unflatten(-1, (-1, 32))
+    lo = g.amin(-1).to(torch.float16)
+    s = ((g.amax(-1) - lo.to(x.dtype)) / 15).to(torch.float32).to(torch.float16)
+    step = s.to(x.dtype)[..., None]
+    n = ((g - lo.to(x.dtype)[..., None]) / torch.where(step == 0, 1.0, step)).round().clamp(0, 15)
+    return torch.where(step == 0, 0.0, n), s, lo
+
+
+def _pack(x, keys):
+    """The records of x [..., D] as bytes."""
+    n, s, lo = _quantise(x)
+    w = n.flatten(-2).to(torch.uint8).unflatten(-1, (-1, 4, 2))
+    w = w[..., 0] | (w[..., 1] << 4)                   # [..., D / 8, 4] bytes
+    at = torch.from_numpy(np.argsort(_words(x.shape[-1], keys))).to(x.device)
+    return torch.cat([w[..., at, :].flatten(-2), s.view(torch.uint8), lo.view(torch.uint8)], -1)
+
+
+def _unpack(r, dim, keys):
+    """The values, fp32, of records r [..., 5 D / 8]."""
+    g = dim // 32
+    at = torch.from_numpy(_words(dim, keys)).to(r.device)
+    w = r[..., :dim // 2].unflatten(-1, (-1, 4))[..., at, :].flatten(-2)
+    n = torch.stack([w & 15, w >> 4], -1).flatten(-2).float().unflatten(-1, (g, 32))
+    s, lo = (r[..., dim // 2 + 2 * g * i:dim // 2 + 2 * g * (i + 1)].contiguous().view(torch.float16)
+             .float()[..., None] for i in (0, 1))
+    return (n * s + lo).flatten(-2)
+
+
+# --- states ------------------------------------------------------------------
+
+
+def _int32(a):
+    return torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(DEV)
+
+
+def _tables(rng, held, blocks):
+    """Block tables, -1 padded: `held` blocks for each sequence, in no order."""
+    ids = rng.permutation(blocks)[:int(held.sum())]
+    bt = np.full((len(held), int(held.max())), -1, dtype=np.int32)
+    for i, r in enumerate(np.split(ids, np.cumsum(held)[:-1])):
+        bt[i, :len(r)] = r
+    return bt
+
+
+def _source(gen, shape, keys):
+    """fp32 rows: N(0, 1), and for keys a mean of their own for every channel, as
+    projections have them."""
+    x = torch.randn(shape, generator=gen, device=DEV)
+    if keys:
+        x += 1.5 * torch.randn(shape[-2:], generator=gen, device=DEV)
+    return x
+
+
+def _cache(gen, c, blocks, keys):
+    """[blocks, block, kv_heads, ...]: the whole cache filled, in slabs."""
+    dtype = c.get("dtype", "q4")
+    shape = (blocks, c["block"], c["kv_heads"], _record(c["dim"]) if dtype == "q4" else c["dim"])
+    cache = torch.empty(shape, dtype=torch.uint8 if dtype == "q4" else DTYPES[dtype], device=DEV)
+    slab = max(1, (1 << 26) // (c["block"] * c["kv_heads"] * c["dim"]))
+    for i in range(0, blocks, slab):
+        x = _source(gen, (min(slab, blocks - i),) + shape[1:3] + (c["dim"],), keys)
+        cache[i:i + slab] = _pack(x, keys) if dtype == "q4" else x.to(cache.dtype)
+    return cache
+
+
+def prepare(case, seed):
+    c = case
+    rng = np.random.default_rng(seed)
+    gen = torch.Generator(device=DEV).manual_seed(int(seed))
+    lengths = rng.permutation(_lengths(c))
+    # new rows lie behind what is cached already
+    before = rng.integers(0, 20 * c["block"], c["batch"]) if c["kind"] == "write" else 0 * lengths
+    held = -(-(before + lengths) // c["block"])
+    # as many blocks for every seed
+    most = -(-(_lengths(c) + (20 * c["block"] if c["kind"] == "write" else 0)) // c["block"])
+    blocks = int(most.sum()) + 8
+    pool = [_cache(gen, c, blocks, keys) for keys in (True, False)]
+    s = {"case": c, "k_cache": pool[0], "v_cache": pool[1], "lengths": [int(x) for x in lengths],
+         "tables": _int32(_tables(rng, held, blocks))}
+    if c["kind"] in ("write", "read"):
+        s.update(seq=_int32(np.repeat(np.arange(c["batch"]), lengths)),
+                 at=_int32(np.concatenate([b + np.arange(m) for b, m in zip(before, lengths)])))
+        if c["kind"] == "write":
+            n, e = int(lengths.sum()), c["kv_heads"] * c["dim"]
+            fused = torch.empty((n, 2 * e), dtype=DTYPES[c["src"]], device=DEV)
+            for i, name in enumerate("kv"):
+                part = fused[:, i * e:(i + 1) * e]
+                part.copy_(_source(gen, (n, c["kv_heads"], c["dim"]), name == "k").view(n, e))
+                s[name] = part.view(n, c["kv_heads"], c["dim"])
+    else:
+        s.update(q=torch.randn((c["batch"], c["heads"], c["dim"]), generator=gen, device=DEV),
+                 ctx=_int32(lengths), scale=1.0 / math.sqrt(c["dim"]))
+    return s
+
+
+# --- one pass ----------------------------------------------------------------
+
+_entries = None
+
+
+def run(state):
+    return (_run_own if own else _run_plain)(state)
+
+
+def _own_entries():
+    global _entries
+    if _entries is None:
+        if os.path.abspath("hetero-serve_amd") not in sys.path:
+            sys.path.insert(1, os.path.abspath("hetero-serve_amd"))
+        from heteroserve.kv import quant
+        from heteroserve.model.paged_attn_q4 import paged_attention_q4
+        from heteroserve.model.paged_attn_window import paged_attention_window
+
+        _entries = quant, paged_attention_q4, paged_attention_window
+    return _entries
+
+
+def _run_own(state):
+    s, c = state, state["case"]
+    quant, paged_attention_q4, paged_attention_window = _own_entries()
+    if c["kind"] in ("write", "read"):
+        if c["kind"] == "write":
+            quant.append_kv_q4(s["k_cache"], s["v_cache"], s["tables"], s["at"], s["k"], s["v"],
+                               seq_ids=s["seq"])
+        k, v = quant.read_kv_q4(s["k_cache"], s["v_cache"], s["tables"], s["at"], seq_ids=s["seq"],
+                                dtype=DTYPES[c["out"]])
+        return {"k": k, "v": v}
+    call = paged_attention_q4 if c["kind"] == "attend" else paged_attention_window
+    return call(s["q"], s["k_cache"], s["v_cache"], s["tables"], s["ctx"], s["scale"],
+                window=c["window"], sinks=c["sinks"])
+
+
+def _run_plain(state):
+    s, c = state, state["case"]
+    if c["kind"] in ("write", "read"):
+        seq, at = s["seq"].long(), s["at"].long()
+        slots = s["tables"][seq, at // c["block"]].long() * c["block"] + at % c["block"]
+        out = {}
+        for name in "kv":
+            flat = s[name + "_cache"].flatten(0, 1)
+            if c["kind"] == "write":           # 64 bits: values lie next to the borders of steps
+                flat[slots] = _pack(s[name].double(), name == "k")
+            out[name] = _unpack(flat[slots], c["dim"], name == "k").to(DTYPES[c["out"]])
+        return out
+    out = torch.empty_like(s["q"])
+    g = c["heads"] // c["kv_heads"]
+    for b, n in enumerate(s["lengths"]):
+        at = torch.arange(n, device=DEV)
+        if c["window"]:
+            at = at[(at < c["sinks"]) | (at >= n - c["window"])]
+        block = s["tables"][b][at // c["block"]].long()
+        k, v = (x[block, at % c["block"]] for x in (s["k_cache"], s["v_cache"]))
+        if c["dtype"] == "q4":
+            k, v = _unpack(k, c["dim"], True), _unpack(v, c["dim"], False)
+        k, v = k.float().permute(1, 2, 0).contiguous(), v.float().permute(1, 0, 2).contiguous()
+        p = torch.bmm(s["q"][b].view(-1, g, c["dim"]), k).mul_(s["scale"])
+        p = p.sub_(p.amax(-1, keepdim=True)).exp_()
+        p = p.div_(p.sum(-1, keepdim=True))
+        out[b] = torch.bmm(p, v).view(c["heads"], c["dim"])
+    return out
+
+
+# --- the same in 64 bits, from the definitions --------------------------------
+
+
+def _stands_for(x):
+    """What rows x [..., D] are held as, in 64 bits."""
+    x = x.double().reshape(*x.shape[:-1], -1, 32)
+    low = x.min(-1, keepdim=True).values.half().double()
+    step = ((x.max(-1, keepdim=True).values - low) / 15).float().half().double()
+    n = torch.clamp(torch.round((x - low) / step.clamp(min=1e-300)), 0, 15)
+    return (torch.where(step > 0, n, torch.zeros_like(n)) * step + low).flatten(-2)
+
+
+def _held(cache, rows_at, dim, keys):
+    """Values in 64 bits of the records at [(block, offset)] of a 4-bit cache, one head at a time."""
+    r = cache[rows_at[0], rows_at[1]].long()                          # [n, heads, bytes]
+    groups, out = dim // 32, torch.empty((*r.shape[:2], dim), dtype=torch.float64, device=r.device)
+    half = r[..., dim // 2:].to(torch.uint8).contiguous().view(torch.float16).double()
+    for x in range(dim):
+        word = x // 8 if not keys else (x % 32 // 8) * groups + x // 32
+        byte = r[..., 4 * word + x % 8 // 2]
+        n = (byte >> (4 * (x % 2))) & 15
+        out[..., x] = n.double() * half[..., x // 32] + half[..., groups + x // 32]
+    return out
+
+
+def exact(case, seed):
+    c = case
+    s = prepare(c, seed)
+    tables = s["tables"].cpu().numpy()
+
+    def places(b, at):
+        block = torch.from_numpy(tables[b, at // c["block"]].astype(np.int64)).to(DEV)
+        return block, torch.from_numpy((at % c["block"]).astype(np.int64)).to(DEV)
+
+    if c["kind"] == "write":
+        return {"k": _stands_for(s["k"]), "v": _stands_for(s["v"])}
+    if c["kind"] == "read":
+        seq, at = s["seq"].cpu().numpy(), s["at"].cpu().numpy()
+        where = places(seq, at)
+        return {"k": _held(s["k_cache"], where, c["dim"], True),
+                "v": _held(s["v_cache"], where, c["dim"], False)}
+    out = torch.empty(s["q"].shape, dtype=torch.float64, device=DEV)
+    group = c["heads"] // c["kv_heads"]
+    for b, n in enumerate(s["lengths"]):
+        at = np.arange(n)
+        if c["window"]:
+            at = np.concatenate([at[:min(c["sinks"], max(0, n - c["window"]))],
+                                 at[max(0, n - c["window"]):]])
+        where = places(b, at)
+        if c["dtype"] == "q4":
+            k, v = (_held(x, where, c["dim"], keys) for x, keys in
+                    ((s["k_cache"], True), (s["v_cache"], False)))
+        else:
+            k, v = s["k_cache"][where].double(), s["v_cache"][where].double()
+        for h in range(c["heads"]):
+            z = torch.mv(k[:, h // group].contiguous(), s["q"][b, h].double()) * s["scale"]
+            out[b, h] = torch.mv(v[:, h // group].t().contiguous(), torch.exp(z - torch.logsumexp(z, 0)))
+    return out
