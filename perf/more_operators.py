@@ -18,7 +18,7 @@ order that the seed gives, so a case's work is the same for every seed.
 The 4-bit cache is a uint8 tensor [blocks, block, kv_heads, 5 D / 8].  Every 32
 elements of a head share a step s and a lowest value lo, both fp16:
 
-    lo = min x,   s = (max x - lo) / 15,   n = (x - lo) / s to the nearest of 0 .. 15
+    lo = min x,   s = (max x - lo) / 15 (or 0),   n = (x - lo) / s to the nearest of 0 .. 15
 
 and x is held as n s + lo.  A record is D / 2 bytes of n, 8 elements in a 32-bit
 word, element e in bits 4 e .., then the steps and then the lowest values.  With
@@ -182,7 +182,7 @@ def _quantise(x):
     fp16 [..., D / 32]."""
     g = x.clamp(-65504.0, 65504.0).unflatten(-1, (-1, 32))
     lo = g.amin(-1).to(torch.float16)
-    s = ((g.amax(-1) - lo.to(x.dtype)) / 15).to(torch.float32).to(torch.float16)
+    s = ((g.amax(-1) - lo.to(x.dtype)) / 15).clamp(min=0).to(torch.float32).to(torch.float16)
     step = s.to(x.dtype)[..., None]
     n = ((g - lo.to(x.dtype)[..., None]) / torch.where(step == 0, 1.0, step)).round().clamp(0, 15)
     return torch.where(step == 0, 0.0, n), s, lo
