@@ -12,7 +12,10 @@
 
 #include "../../include/hsattn_ops.h"
 #include "hs_kernels.h"
+#include "hs_kvrows.h"
 #include "hs_private.h"
+#include "hs_q4.h"
+#include "hs_span.h"
 
 namespace hs {
 
@@ -1028,6 +1031,162 @@ int hs_prompt_attention(const void* q, const void* k, const void* v, int dtype, 
                         v_row_stride, v_head_stride, cu_seqlens, B, total,
                         (int)std::min(total, (int64_t)max_seqlen), H, Hkv, D, scale, out},
                        current_cus(), static_cast<hipStream_t>(stream));
+}
+
+// What the 4-bit cache's row calls have in common.
+static int check_q4_rows(const Q4Rows& w, const void* k, const void* v) {
+  if (w.n < 0 || w.Hkv <= 0 || w.D <= 0) return fail(HS_EINVAL, "KV row sizes must be positive");
+  if (w.NB <= 0 || w.BS <= 0 || w.B <= 0 || w.MB <= 0)
+    return fail(HS_EINVAL, "cache and table sizes must be positive");
+  if (!valid_dtype(w.dtype)) return fail(HS_EINVAL, "unsupported dtype code");
+  if (!valid_row_head_dim(w.D))
+    return fail(HS_EUNSUPPORTED, "unsupported head_dim " + std::to_string(w.D));
+  if (w.n == 0) return HS_OK;
+  if (!w.k_cache || !w.v_cache || !w.bt || !w.positions || !k || !v)
+    return fail(HS_EINVAL, "null pointer");
+  const uintptr_t unit = std::min(16, w.D / 8) - 1;
+  if ((reinterpret_cast<uintptr_t>(w.k_cache) | reinterpret_cast<uintptr_t>(w.v_cache)) & unit)
+    return fail(HS_EINVAL, "4-bit caches must be aligned to head_dim / 8 bytes, at most 16");
+  return HS_OK;
+}
+
+int hs_q4_append(void* k_cache, void* v_cache, int NB, int BS, int Hkv, int D,
+                 const int32_t* block_tables, int B, int MB, const int32_t* positions,
+                 const int32_t* seq_ids, int64_t n, const void* k_src, const void* v_src, int src_dtype,
+                 int64_t k_row_stride, int64_t v_row_stride, void* stream) {
+  Q4Rows w{k_cache, v_cache, NB, BS, Hkv, D, block_tables, B, MB, positions, seq_ids, n, src_dtype,
+           k_src, v_src, k_row_stride, v_row_stride, nullptr, nullptr};
+  const int rc = check_q4_rows(w, k_src, v_src);
+  if (rc != HS_OK) return rc;
+  if (k_row_stride < (int64_t)Hkv * D || v_row_stride < (int64_t)Hkv * D)
+    return fail(HS_EINVAL, "source row stride is smaller than Hkv * D");
+  if (n == 0) return HS_OK;
+  return launch_q4_append(w, static_cast<hipStream_t>(stream));
+}
+
+int hs_q4_read(const void* k_cache, const void* v_cache, int NB, int BS, int Hkv, int D,
+               const int32_t* block_tables, int B, int MB, const int32_t* positions,
+               const int32_t* seq_ids, int64_t n, void* k_out, void* v_out, int out_dtype, void* stream) {
+  Q4Rows w{const_cast<void*>(k_cache), const_cast<void*>(v_cache), NB, BS, Hkv, D, block_tables, B, MB,
+           positions, seq_ids, n, out_dtype, nullptr, nullptr, 0, 0, k_out, v_out};
+  const int rc = check_q4_rows(w, k_out, v_out);
+  if (rc != HS_OK || n == 0) return rc;
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(HS_EINVAL, "outputs must be 16-byte aligned");
+  return launch_q4_read(w, static_cast<hipStream_t>(stream));
+}
+
+// Sizes that the span decodes take (kv_dtype -1: the 4-bit cache).
+static int check_span_sizes(int kv_dtype, int B, int H, int Hkv, int D, int BS, int MB, int window,
+                            int sinks) {
+  if (kv_dtype != -1 && !valid_dtype(kv_dtype))
+    return fail(HS_EINVAL, "unknown kv dtype code " + std::to_string(kv_dtype));
+  if (B < 0 || H <= 0 || Hkv <= 0 || D <= 0 || BS <= 0 || MB <= 0)
+    return fail(HS_EINVAL, "sizes must be positive");
+  if (H % Hkv != 0) return fail(HS_EINVAL, "n_head must be divisible by n_kv_head");
+  if (!valid_row_head_dim(D))
+    return fail(HS_EUNSUPPORTED, "unsupported head_dim " + std::to_string(D));
+  if (window < 0 || sinks < 0) return fail(HS_EINVAL, "window and sinks must not be negative");
+  if (sat_mul(MB, BS) > 0x7fffffffLL)
+    return fail(HS_EUNSUPPORTED, "block table too wide: at most 2^31 - 1 tokens");
+  return HS_OK;
+}
+
+// Parts, and the bytes of their states (INT64_MAX when too large).
+static int64_t plan_span(SpanArgs& a, int kv_dtype, int D, int64_t* ml) {
+  const int64_t most = span_most(a.MB, a.BS, a.window, a.sinks);
+  a.part = span_part(kv_dtype, a.B, a.H, a.Hkv, D, most, current_cus());
+  a.P = (int)ceil_div(most, a.part);
+  return span_state_bytes(a.B, a.H, D, a.P, ml);
+}
+
+static size_t span_workspace(int kv_dtype, int B, int H, int Hkv, int D, int BS, int MB, int window,
+                             int sinks) {
+  if (check_span_sizes(kv_dtype, B, H, Hkv, D, BS, MB, window, sinks) != HS_OK || B == 0) return 0;
+  SpanArgs a{};
+  a.B = B;
+  a.H = H;
+  a.Hkv = Hkv;
+  a.BS = BS;
+  a.MB = MB;
+  a.window = window;
+  a.sinks = sinks;
+  const int64_t need = plan_span(a, kv_dtype, D, nullptr);
+  if (need == kTooLarge) return (size_t)fail(0, "decode part states too large for these sizes");
+  return (size_t)need;
+}
+
+static int span_decode(const float* q, const void* k_cache, const void* v_cache, int kv_dtype, int NB,
+                       const int32_t* bt, const int32_t* ctx, float* out, int B, int H, int Hkv, int D,
+                       int BS, int MB, float scale, int window, int sinks, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  const int rc = check_span_sizes(kv_dtype, B, H, Hkv, D, BS, MB, window, sinks);
+  if (rc != HS_OK) return rc;
+  if (NB <= 0) return fail(HS_EINVAL, "sizes must be positive");
+  if (sat_mul(NB, BS) > 0x7fffffffLL)
+    return fail(HS_EUNSUPPORTED, "cache too long: at most 2^31 - 1 tokens");
+  const float powers = scale * kLog2e;
+  if (!(powers - powers == 0.0f)) return fail(HS_EINVAL, "scale must be finite, times log2(e) as well");
+  if (B == 0) return HS_OK;
+  if (!q || !k_cache || !v_cache || !bt || !ctx || !out) return fail(HS_EINVAL, "null tensor pointer");
+  const uintptr_t unit = kv_dtype == -1 ? std::min(16, D / 8) - 1 : 15;
+  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & unit)
+    return fail(HS_EINVAL, "caches must be aligned to " + std::to_string(unit + 1) + " bytes");
+  if (!aligned16(q) || !aligned16(out)) return fail(HS_EINVAL, "q and out must be 16-byte aligned");
+  SpanArgs a{};
+  a.q = q;
+  a.k = static_cast<const uint8_t*>(k_cache);
+  a.v = static_cast<const uint8_t*>(v_cache);
+  a.bt = bt;
+  a.ctx = ctx;
+  a.out = out;
+  a.B = B;
+  a.H = H;
+  a.Hkv = Hkv;
+  a.BS = BS;
+  a.MB = MB;
+  a.NB = NB;
+  a.bs_shift = (BS & (BS - 1)) == 0 ? __builtin_ctz(BS) : -1;
+  a.window = window;
+  a.sinks = sinks;
+  a.qscale = powers;
+  int64_t ml = 0;
+  const int64_t need = plan_span(a, kv_dtype, D, &ml);
+  if (need == kTooLarge) return fail(HS_EUNSUPPORTED, "decode part states too large for these sizes");
+  if (need > 0 && (!workspace || workspace_bytes < (size_t)need))
+    return fail(HS_EWORKSPACE, "decode needs " + std::to_string(need) + " workspace bytes, got " +
+                                   std::to_string(workspace ? workspace_bytes : 0));
+  if (need > 0 && !aligned16(workspace)) return fail(HS_EINVAL, "workspace must be 16-byte aligned");
+  a.part_acc = static_cast<float*>(workspace);
+  a.part_ml = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) + ml) : nullptr;
+  return launch_span(a, kv_dtype, D, static_cast<hipStream_t>(stream));
+}
+
+size_t hs_q4_decode_workspace_bytes(int B, int H, int Hkv, int D, int BS, int MB, int window, int sinks) {
+  return span_workspace(-1, B, H, Hkv, D, BS, MB, window, sinks);
+}
+
+int hs_q4_decode(const float* q, const void* k_cache, const void* v_cache, int num_blocks,
+                 const int32_t* block_tables, const int32_t* context_lens, float* out, int B, int H,
+                 int Hkv, int D, int BS, int MB, float scale, int window, int sinks, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+  return span_decode(q, k_cache, v_cache, -1, num_blocks, block_tables, context_lens, out, B, H, Hkv, D,
+                     BS, MB, scale, window, sinks, workspace, workspace_bytes, stream);
+}
+
+size_t hs_window_decode_workspace_bytes(int kv_dtype, int B, int H, int Hkv, int D, int BS, int MB,
+                                        int window, int sinks) {
+  if (kv_dtype == -1) return (size_t)fail(0, "unknown kv dtype code -1");
+  return span_workspace(kv_dtype, B, H, Hkv, D, BS, MB, window, sinks);
+}
+
+int hs_window_decode(const float* q, const void* k_cache, const void* v_cache, int kv_dtype,
+                     int num_blocks, const int32_t* block_tables, const int32_t* context_lens, float* out,
+                     int B, int H, int Hkv, int D, int BS, int MB, float scale, int window, int sinks,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(kv_dtype))
+    return fail(HS_EINVAL, "unknown kv dtype code " + std::to_string(kv_dtype));
+  return span_decode(q, k_cache, v_cache, kv_dtype, num_blocks, block_tables, context_lens, out, B, H, Hkv,
+                     D, BS, MB, scale, window, sinks, workspace, workspace_bytes, stream);
 }
 
 static int copy_blocks(void* pool, int L, int NB, int64_t page_bytes, const int64_t* src,

@@ -225,6 +225,29 @@ struct Prompt {
 };
 int launch_prompt(const Prompt& w, int cus, hipStream_t stream);
 
+// Rows of the 4-bit cache (hs_q4_rows.hip): written from sources whose rows are
+// k_row and v_row elements apart, or read into rows without gaps.
+struct Q4Rows {
+  void *k_cache, *v_cache;
+  int NB, BS, Hkv, D;
+  const int32_t* bt;
+  int B, MB;
+  const int32_t *positions, *seq_ids;
+  int64_t n;
+  int dtype;                      // of the sources or outputs
+  const void *k_src, *v_src;
+  int64_t k_row, v_row;
+  void *k_out, *v_out;
+};
+int launch_q4_append(const Q4Rows& w, hipStream_t stream);
+int launch_q4_read(const Q4Rows& w, hipStream_t stream);
+
+// Decode over spans (hs_span.h, hs_span_decode.hip): keys of a part, and the launch.
+// kv_dtype -1 is the 4-bit cache.
+struct SpanArgs;
+int span_part(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, int cus);
+int launch_span(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream);
+
 // Pages inside one pool [L, 2, NB, page] (hs_pages.hip).
 int launch_copy_blocks(void* pool, int L, int NB, int64_t page, const int64_t* src,
                        const int64_t* dst, int n, hipStream_t stream);

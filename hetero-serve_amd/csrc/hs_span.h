@@ -1,0 +1,82 @@
+// Decode over spans: the keys that a sequence's new token sees when it sees the first
+// few of its context (sinks) and a window of the last ones, or all of them.
+//
+// The kernels number the visible keys 0 .. n - 1 and look every key's slot up in the block
+// table by itself, so neither a window's start nor a sink's end has to lie at a page's
+// border, and no key that is not seen is ever read.  Ranges of these numbers are the
+// parts that waves take; parts of one row are merged by span_merge_kernel.
+#pragma once
+
+#include "hs_common.h"
+
+#include <algorithm>
+
+namespace hs {
+
+struct SpanArgs {
+  const float* q;             // [B, H, D]
+  const uint8_t *k, *v;       // [NB, BS, Hkv, row of one head]
+  const int32_t* bt;          // [B, MB]
+  const int32_t* ctx;         // [B]
+  float* out;                 // [B, H, D]
+  float* part_acc;            // [B, H, P, D]   un-normalised outputs of parts
+  float* part_ml;             // [B, H, P, 2]   (max, sum), base-2 domain
+  int B, H, Hkv, BS, MB, NB;
+  int bs_shift;               // log2(BS), or -1
+  int window, sinks;          // window 0: all keys
+  int part, P;                // keys of a part, parts of the longest row
+  float qscale;               // scale * log2(e)
+};
+
+// The visible keys of one sequence.
+struct Span {
+  int n, sinks, skip;   // position of key i: i below sinks, i + skip from there on
+
+  __device__ Span(const SpanArgs& a, int b) {
+    const int64_t cap = (int64_t)a.MB * a.BS;
+    const int len = (int)max((int64_t)0, min((int64_t)a.ctx[b], cap));
+    const int first = a.window && len > a.window ? len - a.window : 0;   // of the window
+    sinks = min(a.sinks, first);
+    n = sinks + len - first;
+    skip = first - sinks;
+  }
+  // Keys [lo, hi) of part p; nparts parts in all.
+  __device__ bool part(const SpanArgs& a, int p, int& lo, int& hi, int& nparts) const {
+    nparts = (int)(((int64_t)n + a.part - 1) / a.part);
+    if (p >= nparts) return false;
+    lo = p * a.part;
+    hi = min((int64_t)lo + a.part, (int64_t)n);
+    return true;
+  }
+  // The slot of key i < n, as a row of the cache seen as [NB * BS] rows (below 2^31).
+  __device__ uint32_t slot(const SpanArgs& a, const int32_t* bt, int i) const {
+    const uint32_t pos = (uint32_t)(i < sinks ? i : i + skip);
+    uint32_t page, off;
+    if (a.bs_shift >= 0) {   // uniform
+      page = pos >> a.bs_shift;
+      off = pos & (uint32_t)(a.BS - 1);
+    } else {
+      page = pos / (uint32_t)a.BS;
+      off = pos - page * (uint32_t)a.BS;
+    }
+    return (uint32_t)safe_block(bt[page], a.NB) * (uint32_t)a.BS + off;
+  }
+};
+
+// Keys that the longest row of these sizes can see.
+inline int64_t span_most(int64_t MB, int64_t BS, int window, int sinks) {
+  const int64_t cap = sat_mul(MB, BS);
+  return window ? std::min(cap, (int64_t)window + sinks) : cap;
+}
+
+// Bytes of P parts' states, and where the (max, sum) pairs begin; INT64_MAX when too large.
+inline int64_t span_state_bytes(int B, int H, int D, int64_t P, int64_t* ml) {
+  if (P <= 1) return 0;
+  const int64_t rows = sat_mul(B, H, P), acc = sat_mul(rows, D * 4);
+  if (ml) *ml = acc;
+  return sat_add(acc, sat_mul(rows, 8));
+}
+
+void launch_span_merge(const SpanArgs& a, int D, hipStream_t stream);
+
+}  // namespace hs

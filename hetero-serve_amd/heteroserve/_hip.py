@@ -20,6 +20,7 @@ on ``torch.cuda.current_stream(device)`` of the input's device.
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 import threading
 from pathlib import Path
@@ -100,6 +101,16 @@ _OPERATORS = {
     "hs_kv_compact_workspace_bytes": (_c_size, [_c_int]),
     "hs_kv_compact": (_c_int, [_c_vp, _c_int, _c_int, _c_i64, _c_vp, _c_int, _c_int, _c_vp, _c_vp,
                                _c_vp, _c_vp, _c_size, _c_vp]),
+    "hs_q4_append": (_c_int, [_c_vp, _c_vp] + [_c_int] * 4 + [_c_vp, _c_int, _c_int, _c_vp, _c_vp, _c_i64,
+                              _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_vp]),
+    "hs_q4_read": (_c_int, [_c_vp, _c_vp] + [_c_int] * 4 + [_c_vp, _c_int, _c_int, _c_vp, _c_vp, _c_i64,
+                            _c_vp, _c_vp, _c_int, _c_vp]),
+    "hs_q4_decode_workspace_bytes": (_c_size, [_c_int] * 8),
+    "hs_q4_decode": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp] + [_c_int] * 6
+                     + [_c_float, _c_int, _c_int, _c_vp, _c_size, _c_vp]),
+    "hs_window_decode_workspace_bytes": (_c_size, [_c_int] * 9),
+    "hs_window_decode": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_vp, _c_vp, _c_vp] + [_c_int] * 6
+                         + [_c_float, _c_int, _c_int, _c_vp, _c_size, _c_vp]),
 }
 
 OPERATOR_SYMBOLS = tuple(_OPERATORS)
@@ -932,3 +943,147 @@ def kv_compact(pool, block_tables, ref_counts):
                               *block_tables.shape, ref_counts.data_ptr(), moved_to.data_ptr(),
                               live.data_ptr(), ws.data_ptr(), need, _stream_at(index)))
     return moved_to, live
+
+# ---------------------------------------------------------------------------
+# the 4-bit cache, and decode through a window
+# ---------------------------------------------------------------------------
+
+_Q4_DIMS = {20: 32, 40: 64, 80: 128, 160: 256}   # record bytes -> head_dim
+
+
+def _q4_shape(k_cache, v_cache):
+    """(NB, BS, Hkv, D) of a pair of 4-bit caches, and their device index."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise RuntimeError("k_cache and v_cache must be [NB, BS, Hkv, record_bytes(D)]")
+    if k_cache.dtype is not torch.uint8 or v_cache.dtype is not torch.uint8:
+        raise RuntimeError("a 4-bit cache must be uint8")
+    D = _Q4_DIMS.get(shape[3])
+    if D is None:
+        raise RuntimeError(f"a 4-bit cache has records of {sorted(_Q4_DIMS)} bytes, got {shape[3]}")
+    index = k_cache.get_device()
+    if index < 0 or v_cache.get_device() != index:
+        raise RuntimeError("kv cache must be on CUDA, on one device")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise RuntimeError("a 4-bit cache must be contiguous")
+    return (shape[0], shape[1], shape[2], D), index
+
+
+def _q4_rows(block_tables, positions, seq_ids, n, device):
+    """(tables, positions, sequence ids or None) of n rows, int32 on the device."""
+    bt = _whole_on("block_tables", block_tables, device)
+    at = _whole_on("positions", positions, device)
+    sid = None if seq_ids is None else _whole_on("seq_ids", seq_ids, device)
+    if bt.dim() != 2:
+        raise RuntimeError("block_tables must be [B, max_blocks]")
+    if n is None:
+        n = at.numel()
+    if at.numel() != n:
+        raise RuntimeError(f"{at.numel()} positions for {n} rows")
+    if sid is not None and sid.numel() != n:
+        raise RuntimeError(f"{sid.numel()} sequence ids for {n} rows")
+    if sid is None and n > bt.shape[0]:
+        raise RuntimeError("without seq_ids, row i uses table row i: more rows than tables")
+    return bt, at, sid
+
+
+def q4_append(k_cache, v_cache, block_tables, positions, k, v, seq_ids) -> None:
+    """Rows of k and v into a 4-bit cache via hs_q4_append."""
+    L = lib("4-bit KV append HIP kernel")
+    (NB, BS, Hkv, D), index = _q4_shape(k_cache, v_cache)
+    if k.get_device() != index or v.get_device() != index:
+        raise RuntimeError("kv cache and new rows must be on the same device")
+    code = dtype_code(k.dtype)
+    for x in (k, v):
+        if x.dim() == 3 and x.shape[1:] != (Hkv, D):
+            raise RuntimeError(f"K/V rows must be [n, {Hkv}, {D}], got {tuple(x.shape)}")
+    k, k_row = _head_rows(k, Hkv, D)
+    v, v_row = _head_rows(v, Hkv, D)
+    n = k.shape[0]
+    if v.shape[0] != n or v.dtype is not k.dtype:
+        raise RuntimeError("k and v rows must have the same count and dtype")
+    bt, at, sid = _q4_rows(block_tables, positions, seq_ids, n, k_cache.device)
+    with _DeviceGuard(index):
+        check(L.hs_q4_append(k_cache.data_ptr(), v_cache.data_ptr(), NB, BS, Hkv, D, bt.data_ptr(),
+                             bt.shape[0], bt.shape[1], at.data_ptr(),
+                             None if sid is None else sid.data_ptr(), n, k.data_ptr(), v.data_ptr(),
+                             code, k_row, v_row, _stream_at(index)))
+
+
+def q4_read(k_cache, v_cache, block_tables, positions, seq_ids, dtype):
+    """(k, v) [n, Hkv, D] out of a 4-bit cache via hs_q4_read."""
+    L = lib("4-bit KV read HIP kernel")
+    (NB, BS, Hkv, D), index = _q4_shape(k_cache, v_cache)
+    dtype = dtype or torch.float16
+    code = dtype_code(dtype)
+    dev = k_cache.device
+    bt, at, sid = _q4_rows(block_tables, positions, seq_ids, None, dev)
+    n = at.numel()
+    k = torch.empty((n, Hkv, D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    with _DeviceGuard(index):
+        check(L.hs_q4_read(k_cache.data_ptr(), v_cache.data_ptr(), NB, BS, Hkv, D, bt.data_ptr(),
+                           bt.shape[0], bt.shape[1], at.data_ptr(),
+                           None if sid is None else sid.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
+                           _stream_at(index)))
+    return k, v
+
+
+def _whole_number(what: str, x) -> int:
+    """A size that the library takes as 32 bits: sizes past that see no more than those."""
+    x = operator.index(x)
+    if x < 0:
+        raise RuntimeError(f"{what} must not be negative, got {x}")
+    return min(x, 0x7fffffff)
+
+
+def _span_decode(L, query, call, head, q, k_cache, v_cache, NB, BS, Hkv, block_tables, context_lens,
+                 scale, window, sinks, index):
+    """hs_q4_decode or hs_window_decode; head: what the query takes first."""
+    B, H, D = q.shape
+    dev = q.device
+    bt = _whole_on("block_tables", block_tables, dev)
+    ctx = _whole_on("context_lens", context_lens, dev)
+    if bt.dim() != 2 or bt.shape[0] != B:
+        raise RuntimeError("block_tables must be [B, max_blocks]")
+    if ctx.numel() != B:
+        raise RuntimeError("context_lens must have one entry per sequence")
+    window, sinks = _whole_number("window", window), _whole_number("sinks", sinks)
+    if q.data_ptr() & 15:
+        q = q.clone()
+    out = q.new_empty(q.shape)
+    if B == 0:
+        return out
+    MB = bt.shape[1]
+    with _DeviceGuard(index):
+        ws_bytes = _decode_workspace(query, index, *head, B, H, Hkv, D, BS, max(MB, 1), window, sinks)
+        ws = q.new_empty((ws_bytes + 3) // 4) if ws_bytes else None
+        check(call(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *head, NB, bt.data_ptr(),
+                   ctx.data_ptr(), out.data_ptr(), B, H, Hkv, D, BS, MB, float(scale), window, sinks,
+                   None if ws is None else ws.data_ptr(), ws_bytes, _stream_at(index)))
+    return out
+
+
+def q4_decode(q, k_cache, v_cache, block_tables, context_lens, scale: float, window: int, sinks: int):
+    """out[B, H, D] fp32: decode over a 4-bit cache via hs_q4_decode."""
+    L = lib("4-bit attention HIP kernel")
+    (NB, BS, Hkv, D), index = _q4_shape(k_cache, v_cache)
+    if q.dim() != 3 or q.shape[2] != D:
+        raise RuntimeError(f"q must be [B, H, {D}], got {tuple(q.shape)}")
+    if q.get_device() != index:
+        raise RuntimeError("q and the kv cache must be on the same device")
+    return _span_decode(L, L.hs_q4_decode_workspace_bytes, L.hs_q4_decode, (), _check_q(q), k_cache,
+                        v_cache, NB, BS, Hkv, block_tables, context_lens, scale, window, sinks, index)
+
+
+def window_decode(q, k_cache, v_cache, block_tables, context_lens, scale: float, window: int, sinks: int):
+    """out[B, H, D] fp32: decode through a window via hs_window_decode."""
+    L = lib("window attention HIP kernel")
+    index = _check_device(q, k_cache, v_cache)
+    if q.dim() != 3:
+        raise RuntimeError("q must be [B, H, D]")
+    q = _check_q(q)
+    k_cache, v_cache, (NB, BS, Hkv, _) = _check_kv(k_cache, v_cache, q.shape[2])
+    return _span_decode(L, L.hs_window_decode_workspace_bytes, L.hs_window_decode,
+                        (dtype_code(k_cache.dtype),), q, k_cache, v_cache, NB, BS, Hkv, block_tables,
+                        context_lens, scale, window, sinks, index)

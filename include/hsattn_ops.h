@@ -1,7 +1,8 @@
 /*
  * hsattn_ops.h -- what a prompt and its sequences need around the paged
  * attention of hsattn.h: rotary positions and the cache write, attention over
- * whole prompts, and the cache's pages while their sequences live.  The
+ * whole prompts, the cache's pages while their sequences live, a cache held in 4
+ * bits, and decode through a window.  The
  * conventions (pointers, streams, status codes, dtype codes, block tables) are
  * hsattn.h's.  Nothing here replaces a function of the reference.
  */
@@ -146,6 +147,72 @@ size_t hs_kv_compact_workspace_bytes(int NB);
 int hs_kv_compact(void* pool, int L, int NB, int64_t page_bytes, int32_t* block_tables, int B,
                   int MB, int32_t* ref_counts, int32_t* moved_to, int32_t* live, void* workspace,
                   size_t workspace_bytes, void* stream);
+
+/*
+ * A cache held in 4 bits.  A cache is [NB, BS, Hkv, HS_Q4_RECORD_BYTES(D)] bytes,
+ * one record for each token and KV head, so its pages are copied, forked, packed
+ * and moved as the bytes of any other.  Every 32 elements of a head share a step s
+ * and a lowest value lo, both fp16:
+ *   lo = min x,  s = max(0, (max x - lo) / 15)
+ *   n  = (x - lo) / s to the nearest of 0 .. 15, ties to even (0 where s is 0)
+ * and x is held as n s + lo.  Values beyond fp16's largest count as that; a group
+ * that holds a NaN is NaN as a whole.  lo, s (through fp32) and n are rounded from
+ * the exact quotients.  A record is D / 8 32-bit words of 8 elements n (element e in
+ * bits 4 e .. 4 e + 3), then D / 32 steps, then D / 32 lowest values.  Word w holds
+ * elements 8 w .. of a value's head, and elements 32 (w % G) + 8 (w / G) .. of a
+ * key's, G = D / 32.  D is 32, 64, 128 or 256.  Caches are aligned to D / 8 bytes, at
+ * most 16.  No reference counterpart.
+ */
+#define HS_Q4_RECORD_BYTES(D) ((D) / 2 + (D) / 8)
+
+/*
+ * hs_kv_append into a 4-bit cache: row i of k_src and v_src (n rows of Hkv * D
+ * elements of src_dtype, rows the given strides of elements apart) goes to position
+ * positions[i] of sequence seq_ids[i] (row i of the tables when seq_ids is NULL,
+ * which needs n <= B).  Rows that hs_kv_append would skip are not written; rows must
+ * not share a slot.
+ */
+int hs_q4_append(void* k_cache, void* v_cache, int NB, int BS, int Hkv, int D,
+                 const int32_t* block_tables, int B, int MB, const int32_t* positions,
+                 const int32_t* seq_ids, int64_t n, const void* k_src, const void* v_src,
+                 int src_dtype, int64_t k_row_stride, int64_t v_row_stride, void* stream);
+
+/*
+ * The way back: row i of k_out and v_out [n, Hkv, D] of out_dtype (16-byte aligned,
+ * no part of the caches) is what the cache holds at position positions[i] of
+ * sequence seq_ids[i], n s + lo rounded once, or zeros where hs_q4_append would skip.
+ * Rows may share a slot.
+ */
+int hs_q4_read(const void* k_cache, const void* v_cache, int NB, int BS, int Hkv, int D,
+               const int32_t* block_tables, int B, int MB, const int32_t* positions,
+               const int32_t* seq_ids, int64_t n, void* k_out, void* v_out, int out_dtype,
+               void* stream);
+
+/*
+ * hs_decode over what a sequence's new token sees through a window: of the ctx_b
+ * cached tokens (the new one among them) the last `window` and the first `sinks`.
+ * window 0: all of them.  What other tokens' slots hold never reaches a row,
+ * infinities and NaN included.  hs_q4_decode reads a 4-bit cache, hs_window_decode
+ * one of kv_dtype; scores, softmax and sums are fp32, products as near as fp32's.
+ * A row that sees an infinity or a NaN may be NaN in the elements that it reaches.
+ *   q, out      [B, H, D] float32, 16-byte aligned
+ *   D           32, 64, 128 or 256;  H % Hkv == 0;  MB * BS and num_blocks * BS
+ *               below 2^31;  scale finite, and times log2(e) as well
+ *   workspace   device scratch of the query's size for the same arguments, with the
+ *               launch device current (may be NULL when that is 0), 16-byte aligned
+ */
+size_t hs_q4_decode_workspace_bytes(int B, int H, int Hkv, int D, int BS, int MB, int window,
+                                    int sinks);
+int hs_q4_decode(const float* q, const void* k_cache, const void* v_cache, int num_blocks,
+                 const int32_t* block_tables, const int32_t* context_lens, float* out, int B,
+                 int H, int Hkv, int D, int BS, int MB, float scale, int window, int sinks,
+                 void* workspace, size_t workspace_bytes, void* stream);
+size_t hs_window_decode_workspace_bytes(int kv_dtype, int B, int H, int Hkv, int D, int BS, int MB,
+                                        int window, int sinks);
+int hs_window_decode(const float* q, const void* k_cache, const void* v_cache, int kv_dtype,
+                     int num_blocks, const int32_t* block_tables, const int32_t* context_lens,
+                     float* out, int B, int H, int Hkv, int D, int BS, int MB, float scale,
+                     int window, int sinks, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

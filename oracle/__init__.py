@@ -26,4 +26,5 @@ builder, which this image does not have.
     splits        choose_num_splits
     operators     rotary positions, whole prompts, pages (no reference
                   counterpart: from their definitions, in 64 bits)
+    long_context  the 4-bit cache, decode through a window (the same)
 """
