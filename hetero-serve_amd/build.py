@@ -70,6 +70,7 @@ PER_FILE_FLAGS = {
     "hs_prefill_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "hs_decode_splitmm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "hs_prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+    "hs_q4_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
 }
 
 

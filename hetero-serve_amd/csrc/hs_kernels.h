@@ -247,6 +247,7 @@ int launch_q4_read(const Q4Rows& w, hipStream_t stream);
 struct SpanArgs;
 int span_part(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, int cus);
 int launch_span(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream);
+int launch_q4_decode(const SpanArgs& a, int D, hipStream_t stream);   // hs_q4_decode.hip
 
 // Pages inside one pool [L, 2, NB, page] (hs_pages.hip).
 int launch_copy_blocks(void* pool, int L, int NB, int64_t page, const int64_t* src,

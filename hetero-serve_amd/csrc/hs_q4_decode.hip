@@ -1,0 +1,536 @@
+// Decode over a 4-bit cache (hs_q4.h) on the matrix cores, through spans (hs_span.h).
+//
+// With k = n - 8 and mid = lo + 8 s, a group's middle, an element is k s + mid, and
+//   score_t = sum_d (k_td s_tg + mid_tg) q_d = sum_g s_tg (sum_{d in g} k_td q_d) + sum_g mid_tg Q_g
+//   out_d   = sum_t p_t (k_td s_tg + mid_tg) = sum_t (p_t s_tg) k_td + sum_t p_t mid_tg
+// where g = d / 32 is the element's group and Q_g the sum of the query over it.  So whole
+// numbers go to the products, and s and mid are applied to fp32 sums (keys) or to the fp32
+// probabilities (values); the elements themselves are never made.  With n and lo in the
+// place of k and mid, the two sums are several times larger than what they add up to, and
+// so was the error: 8e-6 of the row where it is 4e-7, at 4096 keys.
+//
+// Numerics.  A nibble in the low bits of 1024's mantissa is 1024 + n, or 1024 + 16 n four bits
+// further up; less 1032 or 1152 they are k and 16 k, exactly, and the 16 is taken out of the
+// other operand.  (As masked, without the 1024, they are the subnormals n 2^-24, which the
+// matrix cores take, but they align sums by the operands' exponents: an accuracy of 2^-16 was
+// left.)  mid has two fp16 terms.  Query and probabilities are fp32 and go in as two fp16 terms, hi + lo with 22 bits: each head's query
+// times the power of two that brings its largest element to [2^14, 2^15), probabilities as
+// 2^7 p, at most 2^15 under the lazy raise of the maximum, and p_t s_tg times a power of two
+// R that follows the largest step (see kStepRoom).  Products of such terms are exact in the
+// fp32 accumulators.
+//
+// A wave serves up to 16 query heads of one KV head over one part of a row's visible keys,
+// 64 keys (a chunk) at a time:
+//   S^T = K Q^T      16x16x32, A: 16 keys x 32 dims, a group a product, so that its sums can
+//                    be scaled by the group's steps.  The record's order puts what a lane
+//                    wants of all groups side by side: D / 8 bytes, one load for 16 keys.
+//   O^T += V^T P^T   16x16x32, A: 16 dims x 32 keys, values transposed on their way out of LDS
+//                    by ds_read_b64_tr_b4, which gives a lane 16 keys of one dim.
+// Which key is which row of the first product is free; taking key 16 (j / 4) + 4 r + j % 4 for
+// row j of product r leaves each lane with the 16 probabilities of the keys that the
+// transposing read gives it.  They never leave the registers.
+// Steps and lowest values are loaded one key a lane, and go through LDS as s and mid.  Waves share
+// nothing, so there are no barriers.  Keys past the part's end are read as its last one and
+// count nothing: their scores are -inf, their s and mid 0.
+#include "hs_kernels.h"
+#include "hs_q4.h"
+#include "hs_span.h"
+
+#include <algorithm>
+
+// Contraction would take (float)(_Float16)x for x and leave a split's second term 0.
+#pragma clang fp contract(off)
+
+namespace hs {
+
+namespace {
+
+typedef _Float16 half2x __attribute__((ext_vector_type(2)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float float4x __attribute__((ext_vector_type(4)));
+typedef int int2x __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4;          // of a workgroup
+constexpr int kChunk = 64;         // keys of a step
+constexpr int kSlots = 16;         // query heads of a wave
+constexpr float kSlack = 8.0f;     // lazy raise of the running max, log2 units
+constexpr float kLift = 7.0f;      // probabilities are held 2^kLift times larger
+// Where running maxima start: no finite score lies below, so a row of one is never empty.
+constexpr float kLowest = -0x1.fffffep127f;
+// R is chosen so that the largest step so far times R lies in [2^-3, 2^-2), and again when
+// one times R passes 1 = 2^(kStepRoom - 2 + ...): p s R is at most 2^15 then.
+constexpr int kStepRoom = 2;
+
+// What a wave keeps in LDS of its chunk.  Rows of values are D / 2 + 8 bytes apart: the 16
+// rows of two transposing reads' 8 bytes cover all 64 banks once at every D.  Steps
+// lie by group, so that a lane's 16 keys are two 16-byte reads.
+template <int D>
+struct Chunk {
+  static constexpr int G = D / kQ4Group, kPar = kChunk + 8;
+  alignas(16) uint8_t v[kChunk][D / 2 + 8];
+  alignas(16) _Float16 ks[G][kPar];
+  alignas(16) _Float16 vs[G][kPar];
+  alignas(16) _Float16 vmid[2 * G][kPar];       // both terms, keys in unpack8's order
+  alignas(16) _Float16 kmid[kChunk][2][G];
+};
+
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+
+template <int N>
+__device__ inline Words<N> load_words(const uint8_t* p) {
+  Words<N> x;
+  if constexpr (N == 1) {
+    x.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 t = *reinterpret_cast<const uint2*>(p);
+    x.w[0] = t.x, x.w[1] = t.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 t = load16(p + 4 * i);
+      x.w[i] = t.x, x.w[i + 1] = t.y, x.w[i + 2] = t.z, x.w[i + 3] = t.w;
+    }
+  }
+  return x;
+}
+
+// The k of a word's 8 numbers as operand halves, of elements 0 4 1 5 2 6 3 7, those of the second
+// and fourth pair 16 times larger.  The masks are held in registers that the compiler does not
+// see through, so that an and and an or are one instruction (as literals they are two).
+struct Unpack {
+  uint32_t low = 0x000f000fu, high = 0x00f000f0u, k1024 = 0x64006400u;
+
+  __device__ Unpack() {
+    asm("" : "+s"(low), "+s"(high));
+    asm("" : "+v"(k1024));
+  }
+  __device__ half8 operator()(uint32_t x) const {
+    const uint32_t y = x >> 8;
+    constexpr _Float16 a = 1024.0f + 8.0f, b = 1024.0f + 128.0f;
+    return __builtin_bit_cast(half8, make_uint4((x & low) | k1024, (x & high) | k1024, (y & low) | k1024,
+                                                (y & high) | k1024)) -
+           half8{a, a, b, b, a, a, b, b};
+  }
+};
+// The element of a word that half e of unpack8 is, and its place.
+__device__ constexpr int half_element(int e) { return (e >> 1) + 4 * (e & 1); }
+__device__ inline int half_place(int i) { return 2 * (i & 3) + (i >> 2 & 1); }
+
+__device__ inline float4x mma(half8 a, half8 b, float4x c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+__device__ inline float max_across_groups(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ inline float sum_across_groups(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Two fp16 terms hi + lo of two numbers, 22 bits of them.  The first ones pass through a
+// register that the compiler does not see through: it may round one product to fp16 in two
+// ways, with and without a stop at fp32, and the second term has to be the rest of the first
+// as it is used.
+struct Terms {
+  uint32_t hi, lo;
+};
+
+__device__ inline Terms split(float x, float y) {
+  Terms t;
+  t.hi = __builtin_bit_cast(uint32_t, half2x{(_Float16)x, (_Float16)y});
+  asm("" : "+v"(t.hi));
+  const half2x h = __builtin_bit_cast(half2x, t.hi);
+  t.lo = __builtin_bit_cast(uint32_t, half2x{(_Float16)(x - (float)h[0]), (_Float16)(y - (float)h[1])});
+  return t;
+}
+
+// The terms of keys 16 g + 8 t ..: their probabilities times R (over 16 where the key is odd),
+// x of the first four and y of the others, times their steps.  An instruction for each
+// term, where the compiler takes five for two of them.  One that writes half a register is
+// not followed by one that reads it: a wait is needed between those.
+__device__ inline void split_steps(const float4x& x, const float4x& y, const uint4& steps, half8& hi,
+                                   half8& lo) {
+  uint32_t h0, h1, h2, h3, l0, l1, l2, l3;
+  asm("v_fma_mixlo_f16 %0, %8, %16, 0 op_sel_hi:[0,1,0]\n\t"
+      "v_fma_mixlo_f16 %1, %9, %16, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
+      "v_fma_mixlo_f16 %2, %10, %17, 0 op_sel_hi:[0,1,0]\n\t"
+      "v_fma_mixlo_f16 %3, %11, %17, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
+      "v_fma_mixhi_f16 %0, %12, %18, 0 op_sel_hi:[0,1,0]\n\t"
+      "v_fma_mixhi_f16 %1, %13, %18, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
+      "v_fma_mixhi_f16 %2, %14, %19, 0 op_sel_hi:[0,1,0]\n\t"
+      "v_fma_mixhi_f16 %3, %15, %19, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
+      "v_fma_mixlo_f16 %4, %8, %16, -%0 op_sel_hi:[0,1,1]\n\t"
+      "v_fma_mixlo_f16 %5, %9, %16, -%1 op_sel:[0,1,0] op_sel_hi:[0,1,1]\n\t"
+      "v_fma_mixlo_f16 %6, %10, %17, -%2 op_sel_hi:[0,1,1]\n\t"
+      "v_fma_mixlo_f16 %7, %11, %17, -%3 op_sel:[0,1,0] op_sel_hi:[0,1,1]\n\t"
+      "v_fma_mixhi_f16 %4, %12, %18, -%0 op_sel:[0,0,1] op_sel_hi:[0,1,1]\n\t"
+      "v_fma_mixhi_f16 %5, %13, %18, -%1 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
+      "v_fma_mixhi_f16 %6, %14, %19, -%2 op_sel:[0,0,1] op_sel_hi:[0,1,1]\n\t"
+      "v_fma_mixhi_f16 %7, %15, %19, -%3 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
+      "s_nop 1"
+      : "=&v"(h0), "=&v"(h1), "=&v"(h2), "=&v"(h3), "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3)
+      : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(y[0]), "v"(y[1]), "v"(y[2]), "v"(y[3]),
+        "v"(steps.x), "v"(steps.y), "v"(steps.z), "v"(steps.w));
+  hi = __builtin_bit_cast(half8, make_uint4(h0, h1, h2, h3));
+  lo = __builtin_bit_cast(half8, make_uint4(l0, l1, l2, l3));
+}
+
+// Half i of packed halves.
+template <int N>
+__device__ inline _Float16 half_of(const Words<N>& x, int i) {
+  return __builtin_bit_cast(_Float16, (uint16_t)(x.w[i / 2] >> (16 * (i & 1))));
+}
+
+// One wave's LDS traffic is in order; this keeps the compiler's in order too.
+__device__ inline void lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// kByGroup: the 16 columns of the products are heads times groups, column j head j / G's sums
+// over group j % G alone: 16 / G heads a wave.  Otherwise they are 16 heads.  By group, a lane
+// scales its scores by one group's steps and adds the groups' up with its neighbours', and
+// makes the second product's operand for one group instead of all: 580 vector instructions a
+// chunk instead of 720 at D 128, but for a quarter of the heads.
+template <int D, bool kByGroup>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void q4_decode_kernel(SpanArgs a) {
+  constexpr int G = D / kQ4Group, kPiece = D / 8, kT = D / 16;
+  constexpr int kHeads = kByGroup ? kSlots / G : kSlots;     // of a wave
+  constexpr int kMid = G == 8 ? 8 : 4;   // groups that a lane has of the product of the mids
+  __shared__ Chunk<D> chunks[kWaves];
+  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Chunk<D>& w = chunks[wv];
+  const int group = a.H / a.Hkv, n_hc = (group + kHeads - 1) / kHeads, units = a.Hkv * n_hc;
+  const uint32_t id = blockIdx.x * kWaves + wv;
+  if (id >= (uint64_t)a.B * a.P * units) return;
+  const uint32_t rp = id / units;
+  const int unit = id - rp * units, b = rp / a.P, p = rp - b * a.P;
+  const int kvh = unit / n_hc, hc = unit - kvh * n_hc;
+  const int h0 = kvh * group + hc * kHeads, gc = min(kHeads, group - hc * kHeads);
+  const int jh = kByGroup ? j / G : j, jg = kByGroup ? j % G : 0;   // this column's head, group
+  const Span span(a, b);
+  const int64_t row0 = (int64_t)b * a.H + h0;
+  int lo, hi, nparts;
+  if (!span.part(a, p, lo, hi, nparts)) {
+    if (span.n == 0 && p == 0)       // nothing to attend to: zero rows
+      for (int d = lane; d < gc * D; d += 64) a.out[row0 * D + d] = 0.0f;
+    return;
+  }
+  const int32_t* bt = a.bt + (int64_t)b * a.MB;
+  const uint32_t tok = (uint32_t)a.Hkv * q4_record_bytes(D);
+  const uint8_t* kbase = a.k + kvh * q4_record_bytes(D);
+  const uint8_t* vbase = a.v + kvh * q4_record_bytes(D);
+
+  struct Loads {
+    Words<G> k[4], v[4], kp, vp;
+  } r;
+  auto slot_of = [&](int c0) { return (int)span.slot(a, bt, min(c0 + lane, hi - 1)); };
+  auto at = [&](const uint8_t* base, int slot) { return base + (uint64_t)(uint32_t)slot * tok; };
+  auto load = [&](int slot) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r.k[i] = load_words<G>(at(kbase, __shfl(slot, 16 * (j >> 2) + 4 * i + (j & 3))) + g * kPiece);
+    r.kp = load_words<G>(at(kbase, slot) + D / 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r.v[i] = load_words<G>(at(vbase, __shfl(slot, 16 * i + (lane >> 2))) + (lane & 3) * kPiece);
+    r.vp = load_words<G>(at(vbase, slot) + D / 2);
+  };
+  load(slot_of(lo));
+  int next = slot_of(min(lo + kChunk, hi - 1));
+
+  // The query in two terms, in the order of the keys' halves, and its sums by group.
+  const Unpack unpack;
+  half8 qf[G][2];
+  _Float16 qsum[kMid];
+  float back;     // what scores are to be multiplied by
+  {
+    const float* qp = a.q + (row0 + min(jh, gc - 1)) * D + 8 * g;
+    const float sc = jh < gc ? a.qscale : 0.0f;
+    float x[G][8], most = 0.0f;
+#pragma unroll
+    for (int st = 0; st < G; ++st)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[st][e] = qp[32 * st + e] * sc;
+        most = fmaxf(most, fabsf(x[st][e]));
+      }
+    most = max_across_groups(most);
+    int up = 0;
+    if (most > 0.0f && most < INFINITY) up = min(9 - __builtin_amdgcn_frexp_expf(most), 120);
+    back = ldexpf(1.0f, -up);
+    float sums[G];
+#pragma unroll
+    for (int st = 0; st < G; ++st) {
+      sums[st] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[st][e] = ldexpf(x[st][e], up);
+        sums[st] += x[st][e];
+      }
+      sums[st] = sum_across_groups(sums[st]);
+      const bool mine = !kByGroup || st == jg;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = mine ? x[st][half_element(e)] * (e & 2 ? 0x1p-4f : 1.0f) : 0.0f;
+        qf[st][0][e] = (_Float16)y;
+        qf[st][1][e] = (_Float16)(y - (float)qf[st][0][e]);
+      }
+    }
+    // term g % 2 of the sums, against term g / 2 of the mids
+#pragma unroll
+    for (int e = 0; e < kMid; ++e) {
+      const float y = e < G && (!kByGroup || e == jg) ? sums[e % G] : 0.0f;
+      const _Float16 h = (_Float16)y;
+      qsum[e] = g & 1 ? (_Float16)(y - (float)h) : h;
+    }
+  }
+
+  float4x o[kT], oz = {0.0f, 0.0f, 0.0f, 0.0f}, ones = oz;
+#pragma unroll
+  for (int d = 0; d < kT; ++d) o[d] = float4x{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = kLowest, room = 0.0f, R = 1.0f;   // steps up to `room` fit R
+
+  for (int c0 = lo; c0 < hi; c0 += kChunk) {
+    const bool last = c0 + kChunk > hi;   // uniform
+    lds_order();
+    {
+      const bool ok = c0 + lane < hi;
+      float step = 0.0f;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        r.kp.w[i] = ok ? r.kp.w[i] : 0u;
+        r.vp.w[i] = ok ? r.vp.w[i] : 0u;
+      }
+      const int place = (lane & ~7) | half_place(lane & 7);
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        w.ks[i][lane] = half_of(r.kp, i);
+        w.vs[i][lane] = half_of(r.vp, i);
+        const float km = fmaf((float)half_of(r.kp, i), 8.0f, (float)half_of(r.kp, G + i));
+        const float vm = fmaf((float)half_of(r.vp, i), 8.0f, (float)half_of(r.vp, G + i));
+        const Terms t = split(km, vm);
+        w.kmid[lane][0][i] = half_of(Words<1>{t.hi}, 0);
+        w.kmid[lane][1][i] = half_of(Words<1>{t.lo}, 0);
+        w.vmid[i][place] = half_of(Words<1>{t.hi}, 1);
+        w.vmid[G + i][place] = half_of(Words<1>{t.lo}, 1);
+        step = fmaxf(step, (float)half_of(r.vp, i));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int u = 0; u < G; ++u)
+          *reinterpret_cast<uint32_t*>(&w.v[16 * i + (lane >> 2)][(lane & 3) * kPiece + 4 * u]) =
+              r.v[i].w[u];
+      if (__builtin_amdgcn_ballot_w64(step > room) != 0) {
+        step = fmaxf(step, __shfl_xor(step, 1));
+        step = fmaxf(step, __shfl_xor(step, 2));
+        step = fmaxf(step, __shfl_xor(step, 4));
+        step = fmaxf(step, __shfl_xor(step, 8));
+        const int e = __builtin_amdgcn_frexp_expf(max_across_groups(step)) + kStepRoom;
+        const float R_new = ldexpf(1.0f, -e), keep = R_new / R;
+        room = ldexpf(1.0f, e);
+        R = R_new;
+#pragma unroll
+        for (int d = 0; d < kT; ++d) o[d] *= keep;
+      }
+    }
+    lds_order();
+
+    // scores of keys 16 g + 4 i + e, for column j: the mids' part, then the steps'
+    float4x s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const _Float16* km = w.kmid[16 * (j >> 2) + 4 * i + (j & 3)][g >> 1];
+      const float4x none = {0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (G == 8) {
+        half8 q;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = qsum[e];
+        s[i] = mma(*reinterpret_cast<const half8*>(km), q, none);
+      } else {
+        half4 x = {(_Float16)0.0f, (_Float16)0.0f, (_Float16)0.0f, (_Float16)0.0f}, q;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (e < G) x[e] = km[e % G];
+          q[e] = qsum[e];
+        }
+        s[i] = __builtin_amdgcn_mfma_f32_16x16x16f16(x, q, none, 0, 0, 0);
+      }
+    }
+    if constexpr (kByGroup) {
+      float4x x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = float4x{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int st = 0; st < G; ++st)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const half8 kf = unpack(r.k[i].w[st]);
+          x[i] = mma(kf, qf[st][0], x[i]);
+          x[i] = mma(kf, qf[st][1], x[i]);
+        }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const half8 ks = *reinterpret_cast<const half8*>(&w.ks[jg][16 * g + 8 * t]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int i = 2 * t + e / 4;
+          s[i][e % 4] = group_sum<G>(fmaf((float)ks[e], x[i][e % 4], s[i][e % 4]));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int st = 0; st < G; ++st) {
+        const half8 k0 = *reinterpret_cast<const half8*>(&w.ks[st][16 * g]);
+        const half8 k1 = *reinterpret_cast<const half8*>(&w.ks[st][16 * g + 8]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const half8 kf = unpack(r.k[i].w[st]);
+          float4x x = mma(kf, qf[st][0], float4x{0.0f, 0.0f, 0.0f, 0.0f});
+          x = mma(kf, qf[st][1], x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][e] = fmaf((float)(i < 2 ? k0 : k1)[4 * (i & 1) + e], x[e], s[i][e]);
+        }
+      }
+    }
+    if (c0 + kChunk < hi) {
+      load(next);
+      next = slot_of(min(c0 + 2 * kChunk, hi - 1));
+    }
+    if (last) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c0 + 16 * g + 4 * i + e >= hi) s[i][e] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[i][e]);
+    mx *= back;
+    if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+      const float m_new = fmaxf(m, max_across_groups(mx)), keep = fast_exp2(m - m_new);
+      m = m_new;
+      oz *= keep;
+      ones *= keep;
+#pragma unroll
+      for (int d = 0; d < kT; ++d) o[d] *= keep;
+    }
+    // 2^kLift p; its terms against the mids, and against ones (the sum)
+    const float mb = m - kLift;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] = fast_exp2(fmaf(s[i][e], back, -mb));
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const Terms x = split(s[2 * t][e], s[2 * t + 1][e]);
+        h[e] = x.hi;
+        l[e] = x.lo;
+      }
+      const half8 ph = __builtin_bit_cast(half8, make_uint4(h[0], h[1], h[2], h[3]));
+      const half8 pl = __builtin_bit_cast(half8, make_uint4(l[0], l[1], l[2], l[3]));
+      const half8 one = (_Float16)1.0f;
+      half8 mid = one;
+      if (j < 2 * G) mid = *reinterpret_cast<const half8*>(&w.vmid[j & (2 * G - 1)][16 * g + 8 * t]);
+      oz = mma(mid, ph, oz);
+      oz = mma(mid, pl, oz);
+      if constexpr (G == 8) {      // no row is left
+        ones = mma(one, ph, ones);
+        ones = mma(one, pl, ones);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] *= e & 1 ? R * 0x1p-4f : R;
+    half8 ph[2], pl[2];
+#pragma unroll
+    for (int d = 0; d < kT; ++d) {
+      if (d == 0 || (!kByGroup && d % 2 == 0)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          split_steps(s[2 * t], s[2 * t + 1],
+                      *reinterpret_cast<const uint4*>(&w.vs[kByGroup ? jg : d / 2][16 * g + 8 * t]), ph[t],
+                      pl[t]);
+      }
+      typedef __attribute__((address_space(3))) int2x lds_int2x;
+      const int2x x = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_int2x*)(&w.v[16 * g + j][8 * d]));
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const half8 vf = unpack((uint32_t)x[t]);
+        o[d] = mma(vf, ph[t], o[d]);
+        o[d] = mma(vf, pl[t], o[d]);
+      }
+    }
+  }
+
+  // rows 0 .. G - 1 and G .. 2 G - 1 of oz are the groups' sums of p and the mids' terms,
+  // further ones the sum of p
+  const float l = G == 8 ? ones[0] : __shfl(oz[0], 48 + j);
+  const bool whole = nparts == 1;
+  const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+  const float out_scale = 1.0f / R;
+  const int64_t pi = (row0 + jh) * a.P + p;
+  float* to = whole ? a.out + (row0 + jh) * D : a.part_acc + pi * D;
+#pragma unroll
+  for (int d = 0; d < kT; ++d) {
+    const int first = d / 2, second = G + d / 2;
+    const float mid = __shfl(oz[first % 4], 16 * (first / 4) + j) +
+                      __shfl(oz[second % 4], 16 * (second / 4) + j);
+    if (jh < gc && (!kByGroup || jg == d / 2))
+      *reinterpret_cast<float4*>(to + 16 * d + 4 * g) =
+          make_float4(fmaf(o[d][0], out_scale, mid) * inv, fmaf(o[d][1], out_scale, mid) * inv,
+                      fmaf(o[d][2], out_scale, mid) * inv, fmaf(o[d][3], out_scale, mid) * inv);
+  }
+  if (!whole && jh < gc && jg == 0 && g == 0) reinterpret_cast<float2*>(a.part_ml)[pi] = make_float2(m - kLift, l);
+}
+
+template <int D, bool kByGroup>
+void launch_one(const SpanArgs& a, hipStream_t stream) {
+  const int heads = kByGroup ? kSlots * kQ4Group / D : kSlots;
+  const int units = a.Hkv * (int)ceil_div(a.H / a.Hkv, heads);
+  const int64_t wgs = ceil_div(sat_mul(a.B, a.P, units), kWaves);
+  hipLaunchKernelGGL((q4_decode_kernel<D, kByGroup>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, stream, a);
+}
+
+template <int D>
+void launch_dim(const SpanArgs& a, hipStream_t stream) {
+  if constexpr (D == kQ4Group) return launch_one<D, true>(a, stream);   // the same thing
+  else if (a.H / a.Hkv <= kSlots * kQ4Group / D) launch_one<D, true>(a, stream);
+  else launch_one<D, false>(a, stream);
+}
+
+}  // namespace
+
+// The parts' states or rows; the caller has checked the grid and merges.
+int launch_q4_decode(const SpanArgs& a, int D, hipStream_t stream) {
+  switch (D) {
+    case 32: launch_dim<32>(a, stream); break;
+    case 64: launch_dim<64>(a, stream); break;
+    case 128: launch_dim<128>(a, stream); break;
+    case 256: launch_dim<256>(a, stream); break;
+    default: return fail(HS_EUNSUPPORTED, "unsupported head_dim " + std::to_string(D));
+  }
+  return HS_OK;
+}
+
+}  // namespace hs

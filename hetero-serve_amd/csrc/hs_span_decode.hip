@@ -270,7 +270,7 @@ int launch_span(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream) {
     return fail(HS_EUNSUPPORTED, "grid too large: sequences * parts * heads = " + std::to_string(waves));
   int rc;
   profile_begin(stream);
-  if (kv_dtype < 0) rc = launch_walk_dim<FourBits>(a, D, stream);
+  if (kv_dtype < 0) rc = launch_q4_decode(a, D, stream);
   else if (kv_dtype == HS_DTYPE_F32) rc = launch_walk_dim<float>(a, D, stream);
   else if (kv_dtype == HS_DTYPE_F16) rc = launch_walk_dim<_Float16>(a, D, stream);
   else rc = launch_walk_dim<Bf16>(a, D, stream);

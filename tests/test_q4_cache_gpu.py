@@ -179,6 +179,7 @@ def _attend(lens, H, Hkv, D, BS, window, sinks, seed, scale=None, junk=True, wid
     rec = np.full(shape, 0xff, np.uint8) if junk else np.zeros(shape, np.uint8)   # fp16 NaN
     q = rng.normal(size=(len(lens), H, D)).astype(np.float32) * q_size
     want, tol = np.zeros((2, len(lens), H, D))
+    _attend.spread = np.zeros_like(want)
     for b, n in enumerate(lens):
         at = lc.visible(n, window, sinks)
         page, off = bt[b, at // BS], at % BS
@@ -189,7 +190,7 @@ def _attend(lens, H, Hkv, D, BS, window, sinks, seed, scale=None, junk=True, wid
             rec[i, page, off] = kv[-1]
         out, spread, weight = lc.decode(q[b], lc.values(kv[0], True), lc.values(kv[1], False), scale,
                                         lc.sizes(kv[0], True), lc.sizes(kv[1], False))
-        want[b] = out
+        want[b], _attend.spread[b] = out, spread
         tol[b] = (D + 64) * 2.0 ** -23 * weight + (len(at) + 64) * 2.0 ** -23 * spread
     cache = torch.tensor(rec, device=DEV)
     got = paged_attention_q4(torch.tensor(q, device=DEV), cache[0], cache[1], torch.tensor(bt),
@@ -210,6 +211,19 @@ def _check(*args, **how):
 def test_attention(H, Hkv, D, BS):
     """Lengths of zero, one, around tiles and parts; groups of every size."""
     _check([0, 1, 2, 15, 16, 17, 63, 64, 65, 127, 130, 200], H, Hkv, D, BS, 0, 0, H + D)
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(8, 2, 128), (4, 4, 64), (16, 1, 32), (2, 1, 256), (16, 2, 128),
+                                     (12, 1, 64), (4, 1, 256)])
+def test_rounding_errors_average_out(H, Hkv, D):
+    """The bounds above are of the worst case, which lost second terms would pass.  For 300
+    keys with errors that do not depend on one another: probabilities off by up to 2^-20 (a
+    score of up to 16 is rounded) and products by 2^-22 leave 2^-24 of the sum of their sizes,
+    sums of 10 chunks' products rounded to 2^-24 about 2^-23; a second term that is missing
+    (2^-12 of each product) leaves 2^-17, one that is wrong once in a thousand 2^-21."""
+    got, want, _ = _attend([300] * 24, H, Hkv, D, 16, 0, 0, D)
+    spread = _attend.spread
+    assert np.sqrt(np.mean((got - want) ** 2)) <= 2.0 ** -22 * np.sqrt(np.mean(spread ** 2))
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (63, 1), (64, 0), (65, 64), (100, 7),
