@@ -1086,15 +1086,15 @@ static int check_span_sizes(int kv_dtype, int B, int H, int Hkv, int D, int BS, 
   if (!valid_row_head_dim(D))
     return fail(HS_EUNSUPPORTED, "unsupported head_dim " + std::to_string(D));
   if (window < 0 || sinks < 0) return fail(HS_EINVAL, "window and sinks must not be negative");
-  if (sat_mul(MB, BS) > 0x7fffffffLL)
-    return fail(HS_EUNSUPPORTED, "block table too wide: at most 2^31 - 1 tokens");
+  if (sat_mul(MB, BS) > (1 << 30))
+    return fail(HS_EUNSUPPORTED, "block table too wide: at most 2^30 tokens");
   return HS_OK;
 }
 
 // Parts, and the bytes of their states (INT64_MAX when too large).
 static int64_t plan_span(SpanArgs& a, int kv_dtype, int D, int64_t* ml) {
   const int64_t most = span_most(a.MB, a.BS, a.window, a.sinks);
-  a.part = span_part(kv_dtype, a.B, a.H, a.Hkv, D, most, current_cus());
+  span_plan(kv_dtype, a.B, a.H, a.Hkv, D, most, current_cus(), &a.part, &a.heads);
   a.P = (int)ceil_div(most, a.part);
   return span_state_bytes(a.B, a.H, D, a.P, ml);
 }

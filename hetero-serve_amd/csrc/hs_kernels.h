@@ -242,12 +242,14 @@ struct Q4Rows {
 int launch_q4_append(const Q4Rows& w, hipStream_t stream);
 int launch_q4_read(const Q4Rows& w, hipStream_t stream);
 
-// Decode over spans (hs_span.h, hs_span_decode.hip): keys of a part, and the launch.
-// kv_dtype -1 is the 4-bit cache.
+// Decode over spans (hs_span.h, hs_span_decode.hip): keys of a part (and KV heads of a
+// workgroup) for rows of at most `most` keys, and the launch.  kv_dtype -1 is the 4-bit cache.
 struct SpanArgs;
-int span_part(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, int cus);
+void span_plan(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, int cus, int* part, int* heads);
 int launch_span(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream);
-int launch_q4_decode(const SpanArgs& a, int D, hipStream_t stream);   // hs_q4_decode.hip
+// The 4-bit cache's part of both (hs_q4_decode.hip).
+void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, int cus, int* part, int* heads);
+int launch_q4_decode(const SpanArgs& a, int D, hipStream_t stream);
 
 // Pages inside one pool [L, 2, NB, page] (hs_pages.hip).
 int launch_copy_blocks(void* pool, int L, int NB, int64_t page, const int64_t* src,

@@ -33,6 +33,7 @@
 // nothing, so there are no barriers.  Keys past the part's end are read as its last one and
 // count nothing: their scores are -inf, their s and mid 0.
 #include "hs_kernels.h"
+#include "hs_kvrows.h"
 #include "hs_q4.h"
 #include "hs_span.h"
 
@@ -51,7 +52,6 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float4x __attribute__((ext_vector_type(4)));
 typedef int int2x __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4;          // of a workgroup
 constexpr int kChunk = 64;         // keys of a step
 constexpr int kSlots = 16;         // query heads of a wave
 constexpr float kSlack = 8.0f;     // lazy raise of the running max, log2 units
@@ -62,18 +62,21 @@ constexpr float kLowest = -0x1.fffffep127f;
 // one times R passes 1 = 2^(kStepRoom - 2 + ...): p s R is at most 2^15 then.
 constexpr int kStepRoom = 2;
 
-// What a wave keeps in LDS of its chunk.  Rows of values are D / 2 + 8 bytes apart: the 16
-// rows of two transposing reads' 8 bytes cover all 64 banks once at every D.  Steps
-// lie by group, so that a lane's 16 keys are two 16-byte reads.
+// What a wave keeps in LDS: its chunk's records as they were loaded, and of its values' steps
+// and middles what lies by key there by group, so that a lane's 16 keys are two 16-byte
+// reads.  (Rows of records are 20 dwords apart at D 128: the keys' 16-byte reads of 16 rows
+// cover all banks, the values' transposing ones half of them.)
 template <int D>
 struct Chunk {
   static constexpr int G = D / kQ4Group, kPar = kChunk + 8;
-  alignas(16) uint8_t v[kChunk][D / 2 + 8];
+  alignas(16) uint8_t k[kChunk][q4_record_bytes(D)];
+  alignas(16) uint8_t v[kChunk][(q4_record_bytes(D) + 7) / 8 * 8];   // (8-byte reads)
   alignas(16) _Float16 ks[G][kPar];
   alignas(16) _Float16 vs[G][kPar];
   alignas(16) _Float16 vmid[2 * G][kPar];       // both terms, keys in unpack8's order
-  alignas(16) _Float16 kmid[kChunk][2][G];
 };
+
+constexpr int kWaves = 4;   // of a workgroup
 
 template <int N>
 struct Words {
@@ -186,6 +189,16 @@ __device__ inline void split_steps(const float4x& x, const float4x& y, const uin
   lo = __builtin_bit_cast(half8, make_uint4(l0, l1, l2, l3));
 }
 
+template <int N>
+__device__ inline void store_words(uint8_t* p, const Words<N>& x) {
+  if constexpr (N == 1) *reinterpret_cast<uint32_t*>(p) = x.w[0];
+  else if constexpr (N == 2) *reinterpret_cast<uint2*>(p) = make_uint2(x.w[0], x.w[1]);
+  else
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<uint4*>(p + 4 * i) = make_uint4(x.w[i], x.w[i + 1], x.w[i + 2], x.w[i + 3]);
+}
+
 // Half i of packed halves.
 template <int N>
 __device__ inline _Float16 half_of(const Words<N>& x, int i) {
@@ -198,58 +211,69 @@ __device__ inline void lds_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// One workgroup: one part of one row, for hw KV heads side by side.  Its waves are these heads
+// times np phases, which take neighbouring chunks of a step of 64 np keys in turn and put
+// their states together at the end.
+//
 // kByGroup: the 16 columns of the products are heads times groups, column j head j / G's sums
 // over group j % G alone: 16 / G heads a wave.  Otherwise they are 16 heads.  By group, a lane
 // scales its scores by one group's steps and adds the groups' up with its neighbours', and
 // makes the second product's operand for one group instead of all: 580 vector instructions a
 // chunk instead of 720 at D 128, but for a quarter of the heads.
 template <int D, bool kByGroup>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void q4_decode_kernel(SpanArgs a) {
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void q4_decode_kernel(SpanArgs a) {
   constexpr int G = D / kQ4Group, kPiece = D / 8, kT = D / 16;
+  constexpr int kRecord = q4_record_bytes(D), kLoads = kRecord / kPiece;   // 5 pieces a record
   constexpr int kHeads = kByGroup ? kSlots / G : kSlots;     // of a wave
   constexpr int kMid = G == 8 ? 8 : 4;   // groups that a lane has of the product of the mids
   __shared__ Chunk<D> chunks[kWaves];
+  __shared__ float2 states[kWaves][kSlots];
+  static_assert(kHeads * (D + 4) * 4 <= (int)sizeof(Chunk<D>), "a wave's outputs fit");
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Chunk<D>& w = chunks[wv];
-  const int group = a.H / a.Hkv, n_hc = (group + kHeads - 1) / kHeads, units = a.Hkv * n_hc;
-  const uint32_t id = blockIdx.x * kWaves + wv;
-  if (id >= (uint64_t)a.B * a.P * units) return;
-  const uint32_t rp = id / units;
-  const int unit = id - rp * units, b = rp / a.P, p = rp - b * a.P;
-  const int kvh = unit / n_hc, hc = unit - kvh * n_hc;
+  const int hw = a.heads, np = kWaves / hw, hsub = wv % hw, ph = wv / hw;
+  const int group = a.H / a.Hkv, n_hc = (group + kHeads - 1) / kHeads, units = a.Hkv / hw * n_hc;
+  const uint32_t rp = blockIdx.x / (uint32_t)units;
+  const int unit = blockIdx.x - rp * units, b = rp / a.P, p = rp - b * a.P;
+  const int hg = unit / n_hc, hc = unit - hg * n_hc, kvh = hg * hw + hsub;
   const int h0 = kvh * group + hc * kHeads, gc = min(kHeads, group - hc * kHeads);
   const int jh = kByGroup ? j / G : j, jg = kByGroup ? j % G : 0;   // this column's head, group
   const Span span(a, b);
   const int64_t row0 = (int64_t)b * a.H + h0;
   int lo, hi, nparts;
-  if (!span.part(a, p, lo, hi, nparts)) {
-    if (span.n == 0 && p == 0)       // nothing to attend to: zero rows
+  if (!span.part(a, p, lo, hi, nparts)) {   // all of the workgroup
+    if (span.n == 0 && p == 0 && ph == 0)   // nothing to attend to: zero rows
       for (int d = lane; d < gc * D; d += 64) a.out[row0 * D + d] = 0.0f;
     return;
   }
   const int32_t* bt = a.bt + (int64_t)b * a.MB;
-  const uint32_t tok = (uint32_t)a.Hkv * q4_record_bytes(D);
-  const uint8_t* kbase = a.k + kvh * q4_record_bytes(D);
-  const uint8_t* vbase = a.v + kvh * q4_record_bytes(D);
+  const uint32_t tok = (uint32_t)a.Hkv * kRecord;
+  const uint8_t* kbase = a.k + kvh * kRecord;
+  const uint8_t* vbase = a.v + kvh * kRecord;
 
-  struct Loads {
-    Words<G> k[4], v[4], kp, vp;
-  } r;
-  auto slot_of = [&](int c0) { return (int)span.slot(a, bt, min(c0 + lane, hi - 1)); };
-  auto at = [&](const uint8_t* base, int slot) { return base + (uint64_t)(uint32_t)slot * tok; };
+  // A chunk's records come in pieces of D / 8 bytes, 64 lanes neighbouring pieces, and go to
+  // LDS through registers: a chunk's loads are on their way while the one before is computed,
+  // its slots' table entries while the one before that is.
+  // (Operands straight from memory, the numbers and then the steps: 3.6 TB/s for the loads
+  // alone; whole records 4.2.)
+  Words<G> kr[kLoads], vr[kLoads];
   auto load = [&](int slot) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r.k[i] = load_words<G>(at(kbase, __shfl(slot, 16 * (j >> 2) + 4 * i + (j & 3))) + g * kPiece);
-    r.kp = load_words<G>(at(kbase, slot) + D / 2);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r.v[i] = load_words<G>(at(vbase, __shfl(slot, 16 * i + (lane >> 2))) + (lane & 3) * kPiece);
-    r.vp = load_words<G>(at(vbase, slot) + D / 2);
+    for (int i = 0; i < kLoads; ++i) {
+      const int c = lane + 64 * i, key = c / kLoads;
+      const uint64_t at = (uint64_t)(uint32_t)__shfl(slot, key) * tok + (c - key * kLoads) * kPiece;
+      kr[i] = load_words<G>(kbase + at);
+      vr[i] = load_words<G>(vbase + at);
+    }
   };
-  load(slot_of(lo));
-  int next = slot_of(min(lo + kChunk, hi - 1));
+  const int step = kChunk * np, first = lo + kChunk * ph;
+  auto place_of = [&](int c0) { return span.place(a, bt, min(c0 + lane, hi - 1)); };
+  Span::Place ahead{};
+  if (first < hi) {
+    ahead = place_of(first + step);
+    load(Span::slot(a, place_of(first)));
+  }
 
   // The query in two terms, in the order of the keys' halves, and its sums by group.
   const Unpack unpack;
@@ -269,7 +293,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void q4_decode_kerne
       }
     most = max_across_groups(most);
     int up = 0;
-    if (most > 0.0f && most < INFINITY) up = min(9 - __builtin_amdgcn_frexp_expf(most), 120);
+    if (most > 0.0f && most < INFINITY) up = min(7 - __builtin_amdgcn_frexp_expf(most), 120);
     back = ldexpf(1.0f, -up);
     float sums[G];
 #pragma unroll
@@ -289,10 +313,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void q4_decode_kerne
         qf[st][1][e] = (_Float16)(y - (float)qf[st][0][e]);
       }
     }
-    // term g % 2 of the sums, against term g / 2 of the mids
+    // term g % 2 of the sums, against the lowest values, and of 8 of them, against the steps
 #pragma unroll
     for (int e = 0; e < kMid; ++e) {
-      const float y = e < G && (!kByGroup || e == jg) ? sums[e % G] : 0.0f;
+      const float y = e < G && (!kByGroup || e == jg) ? sums[e % G] * (g < 2 ? 1.0f : 8.0f) : 0.0f;
       const _Float16 h = (_Float16)y;
       qsum[e] = g & 1 ? (_Float16)(y - (float)h) : h;
     }
@@ -303,43 +327,41 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void q4_decode_kerne
   for (int d = 0; d < kT; ++d) o[d] = float4x{0.0f, 0.0f, 0.0f, 0.0f};
   float m = kLowest, room = 0.0f, R = 1.0f;   // steps up to `room` fit R
 
-  for (int c0 = lo; c0 < hi; c0 += kChunk) {
-    const bool last = c0 + kChunk > hi;   // uniform
+  for (int c0 = first; c0 < hi; c0 += step) {
+    const bool last = hi - c0 < kChunk;   // uniform
+    lds_order();
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      store_words(w.k[0] + (lane + 64 * i) * kPiece, kr[i]);
+      const int c = lane + 64 * i;
+      store_words(w.v[0] + c * kPiece + (D == 32 ? c / kLoads * ((int)sizeof(w.v[0]) - kRecord) : 0), vr[i]);
+    }
+    if (c0 + step < hi) {
+      const int slot = Span::slot(a, ahead);
+      ahead = place_of(c0 + 2 * step);
+      load(slot);
+    }
     lds_order();
     {
-      const bool ok = c0 + lane < hi;
-      float step = 0.0f;
-#pragma unroll
-      for (int i = 0; i < G; ++i) {
-        r.kp.w[i] = ok ? r.kp.w[i] : 0u;
-        r.vp.w[i] = ok ? r.vp.w[i] : 0u;
-      }
+      const Words<G> kp = load_words<G>(w.k[lane] + D / 2), vp = load_words<G>(w.v[lane] + D / 2);
       const int place = (lane & ~7) | half_place(lane & 7);
+      float most = 0.0f;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        w.ks[i][lane] = half_of(r.kp, i);
-        w.vs[i][lane] = half_of(r.vp, i);
-        const float km = fmaf((float)half_of(r.kp, i), 8.0f, (float)half_of(r.kp, G + i));
-        const float vm = fmaf((float)half_of(r.vp, i), 8.0f, (float)half_of(r.vp, G + i));
-        const Terms t = split(km, vm);
-        w.kmid[lane][0][i] = half_of(Words<1>{t.hi}, 0);
-        w.kmid[lane][1][i] = half_of(Words<1>{t.lo}, 0);
-        w.vmid[i][place] = half_of(Words<1>{t.hi}, 1);
-        w.vmid[G + i][place] = half_of(Words<1>{t.lo}, 1);
-        step = fmaxf(step, (float)half_of(r.vp, i));
+        const float x = (float)half_of(vp, i);
+        const Terms t = split(fmaf(x, 8.0f, (float)half_of(vp, G + i)), 0.0f);
+        w.ks[i][lane] = half_of(kp, i);
+        w.vs[i][lane] = half_of(vp, i);
+        w.vmid[i][place] = half_of(Words<1>{t.hi}, 0);
+        w.vmid[G + i][place] = half_of(Words<1>{t.lo}, 0);
+        most = fmaxf(most, x);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int u = 0; u < G; ++u)
-          *reinterpret_cast<uint32_t*>(&w.v[16 * i + (lane >> 2)][(lane & 3) * kPiece + 4 * u]) =
-              r.v[i].w[u];
-      if (__builtin_amdgcn_ballot_w64(step > room) != 0) {
-        step = fmaxf(step, __shfl_xor(step, 1));
-        step = fmaxf(step, __shfl_xor(step, 2));
-        step = fmaxf(step, __shfl_xor(step, 4));
-        step = fmaxf(step, __shfl_xor(step, 8));
-        const int e = __builtin_amdgcn_frexp_expf(max_across_groups(step)) + kStepRoom;
+      if (__builtin_amdgcn_ballot_w64(most > room) != 0) {
+        most = fmaxf(most, __shfl_xor(most, 1));
+        most = fmaxf(most, __shfl_xor(most, 2));
+        most = fmaxf(most, __shfl_xor(most, 4));
+        most = fmaxf(most, __shfl_xor(most, 8));
+        const int e = __builtin_amdgcn_frexp_expf(max_across_groups(most)) + kStepRoom;
         const float R_new = ldexpf(1.0f, -e), keep = R_new / R;
         room = ldexpf(1.0f, e);
         R = R_new;
@@ -349,11 +371,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void q4_decode_kerne
     }
     lds_order();
 
+    Words<G> kw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kw[i] = load_words<G>(w.k[16 * (j >> 2) + 4 * i + (j & 3)] + g * kPiece);
     // scores of keys 16 g + 4 i + e, for column j: the mids' part, then the steps'
     float4x s[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const _Float16* km = w.kmid[16 * (j >> 2) + 4 * i + (j & 3)][g >> 1];
+      // lowest values (lane groups 0 and 1) and steps of a key
+      const _Float16* km = reinterpret_cast<const _Float16*>(w.k[16 * (j >> 2) + 4 * i + (j & 3)] + D / 2) +
+                           (g < 2 ? G : 0);
       const float4x none = {0.0f, 0.0f, 0.0f, 0.0f};
       if constexpr (G == 8) {
         half8 q;
@@ -378,7 +405,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void q4_decode_kerne
       for (int st = 0; st < G; ++st)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const half8 kf = unpack(r.k[i].w[st]);
+          const half8 kf = unpack(kw[i].w[st]);
           x[i] = mma(kf, qf[st][0], x[i]);
           x[i] = mma(kf, qf[st][1], x[i]);
         }
@@ -398,7 +425,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void q4_decode_kerne
         const half8 k1 = *reinterpret_cast<const half8*>(&w.ks[st][16 * g + 8]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const half8 kf = unpack(r.k[i].w[st]);
+          const half8 kf = unpack(kw[i].w[st]);
           float4x x = mma(kf, qf[st][0], float4x{0.0f, 0.0f, 0.0f, 0.0f});
           x = mma(kf, qf[st][1], x);
 #pragma unroll
@@ -406,16 +433,12 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void q4_decode_kerne
         }
       }
     }
-    if (c0 + kChunk < hi) {
-      load(next);
-      next = slot_of(min(c0 + 2 * kChunk, hi - 1));
-    }
     if (last) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (c0 + 16 * g + 4 * i + e >= hi) s[i][e] = -INFINITY;
+          if (16 * g + 4 * i + e >= hi - c0) s[i][e] = -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
@@ -446,70 +469,109 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void q4_decode_kerne
         h[e] = x.hi;
         l[e] = x.lo;
       }
-      const half8 ph = __builtin_bit_cast(half8, make_uint4(h[0], h[1], h[2], h[3]));
-      const half8 pl = __builtin_bit_cast(half8, make_uint4(l[0], l[1], l[2], l[3]));
+      const half8 p1 = __builtin_bit_cast(half8, make_uint4(h[0], h[1], h[2], h[3]));
+      const half8 p2 = __builtin_bit_cast(half8, make_uint4(l[0], l[1], l[2], l[3]));
       const half8 one = (_Float16)1.0f;
       half8 mid = one;
       if (j < 2 * G) mid = *reinterpret_cast<const half8*>(&w.vmid[j & (2 * G - 1)][16 * g + 8 * t]);
-      oz = mma(mid, ph, oz);
-      oz = mma(mid, pl, oz);
+      oz = mma(mid, p1, oz);
+      oz = mma(mid, p2, oz);
       if constexpr (G == 8) {      // no row is left
-        ones = mma(one, ph, ones);
-        ones = mma(one, pl, ones);
+        ones = mma(one, p1, ones);
+        ones = mma(one, p2, ones);
       }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[i][e] *= e & 1 ? R * 0x1p-4f : R;
-    half8 ph[2], pl[2];
+    half8 hi2[2], lo2[2];
 #pragma unroll
     for (int d = 0; d < kT; ++d) {
       if (d == 0 || (!kByGroup && d % 2 == 0)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
           split_steps(s[2 * t], s[2 * t + 1],
-                      *reinterpret_cast<const uint4*>(&w.vs[kByGroup ? jg : d / 2][16 * g + 8 * t]), ph[t],
-                      pl[t]);
+                      *reinterpret_cast<const uint4*>(&w.vs[kByGroup ? jg : d / 2][16 * g + 8 * t]), hi2[t],
+                      lo2[t]);
       }
       typedef __attribute__((address_space(3))) int2x lds_int2x;
-      const int2x x = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_int2x*)(&w.v[16 * g + j][8 * d]));
+      const int2x x = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_int2x*)(w.v[lane] + 8 * d));
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const half8 vf = unpack((uint32_t)x[t]);
-        o[d] = mma(vf, ph[t], o[d]);
-        o[d] = mma(vf, pl[t], o[d]);
+        o[d] = mma(vf, hi2[t], o[d]);
+        o[d] = mma(vf, lo2[t], o[d]);
       }
     }
   }
 
   // rows 0 .. G - 1 and G .. 2 G - 1 of oz are the groups' sums of p and the mids' terms,
   // further ones the sum of p
-  const float l = G == 8 ? ones[0] : __shfl(oz[0], 48 + j);
-  const bool whole = nparts == 1;
-  const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+  float l = G == 8 ? ones[0] : __shfl(oz[0], 48 + j);
+  m -= kLift;
   const float out_scale = 1.0f / R;
-  const int64_t pi = (row0 + jh) * a.P + p;
-  float* to = whole ? a.out + (row0 + jh) * D : a.part_acc + pi * D;
 #pragma unroll
   for (int d = 0; d < kT; ++d) {
     const int first = d / 2, second = G + d / 2;
     const float mid = __shfl(oz[first % 4], 16 * (first / 4) + j) +
                       __shfl(oz[second % 4], 16 * (second / 4) + j);
-    if (jh < gc && (!kByGroup || jg == d / 2))
-      *reinterpret_cast<float4*>(to + 16 * d + 4 * g) =
-          make_float4(fmaf(o[d][0], out_scale, mid) * inv, fmaf(o[d][1], out_scale, mid) * inv,
-                      fmaf(o[d][2], out_scale, mid) * inv, fmaf(o[d][3], out_scale, mid) * inv);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[d][e] = fmaf(o[d][e], out_scale, mid);
   }
-  if (!whole && jh < gc && jg == 0 && g == 0) reinterpret_cast<float2*>(a.part_ml)[pi] = make_float2(m - kLift, l);
+  const bool whole = nparts == 1;
+  const int64_t pi = (row0 + jh) * a.P + p;
+  if (np == 1) {
+    const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    float* to = whole ? a.out + (row0 + jh) * D : a.part_acc + pi * D;
+#pragma unroll
+    for (int d = 0; d < kT; ++d)
+      if (jh < gc && (!kByGroup || jg == d / 2)) *reinterpret_cast<float4x*>(to + 16 * d + 4 * g) = o[d] * inv;
+    if (!whole && jh < gc && jg == 0 && g == 0) reinterpret_cast<float2*>(a.part_ml)[pi] = make_float2(m, l);
+    return;
+  }
+  // the phases' states put together
+  lds_order();
+  if (jg == 0 && g == 0) states[wv][jh] = make_float2(m, l);
+  __syncthreads();
+  float mm = m;
+  for (int i = 0; i < np; ++i) mm = fmaxf(mm, states[hsub + hw * i][jh].x);
+  l = 0.0f;
+  for (int i = 0; i < np; ++i) {
+    const float2 x = states[hsub + hw * i][jh];
+    l = fmaf(x.y, fast_exp2(x.x - mm), l);
+  }
+  const float keep = fast_exp2(m - mm) * (!whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l);
+#pragma unroll
+  for (int d = 0; d < kT; ++d)
+    if (!kByGroup || jg == d / 2)
+      *reinterpret_cast<float4x*>(reinterpret_cast<float*>(&w) + jh * (D + 4) + 16 * d + 4 * g) = o[d] * keep;
+  if (!whole && ph == 0 && jh < gc && jg == 0 && g == 0)
+    reinterpret_cast<float2*>(a.part_ml)[pi] = make_float2(mm, l);
+  __syncthreads();
+  for (int x = ph * 64 + lane; x < gc * (D / 4); x += np * 64) {
+    const int h = x / (D / 4), d = x % (D / 4) * 4;
+    float4x sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < np; ++i)
+      sum += *reinterpret_cast<const float4x*>(reinterpret_cast<const float*>(&chunks[hsub + hw * i]) +
+                                               h * (D + 4) + d);
+    float* to = whole ? a.out + (row0 + h) * D : a.part_acc + ((row0 + h) * a.P + p) * D;
+    *reinterpret_cast<float4x*>(to + d) = sum;
+  }
+}
+
+// Query heads of a wave.
+int heads_per_wave(int H, int Hkv, int D) {
+  const int by_group = kSlots * kQ4Group / D;
+  return H / Hkv <= by_group ? by_group : kSlots;
 }
 
 template <int D, bool kByGroup>
 void launch_one(const SpanArgs& a, hipStream_t stream) {
-  const int heads = kByGroup ? kSlots * kQ4Group / D : kSlots;
-  const int units = a.Hkv * (int)ceil_div(a.H / a.Hkv, heads);
-  const int64_t wgs = ceil_div(sat_mul(a.B, a.P, units), kWaves);
-  hipLaunchKernelGGL((q4_decode_kernel<D, kByGroup>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, stream, a);
+  const int64_t n_hc = ceil_div(a.H / a.Hkv, heads_per_wave(a.H, a.Hkv, D));
+  const int64_t wgs = sat_mul(a.B, a.P, a.Hkv / a.heads * n_hc);
+  hipLaunchKernelGGL((q4_decode_kernel<D, kByGroup>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, stream,
+                     a);
 }
 
 template <int D>
@@ -521,8 +583,43 @@ void launch_dim(const SpanArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// The parts' states or rows; the caller has checked the grid and merges.
+// Short rows are whole: as many KV heads side by side as leave a workgroup for each CU, where
+// their steps are at most eight, or one head and four phases where there are too few for
+// that and they take two steps.  Longer rows are cut into parts of 512 keys, shorter ones (of
+// two steps) and fewer heads side by side while the parts are fewer than the CUs.  us, D 128,
+// 32 / 8 heads, heads side by side x keys of a part: 64 rows of 64..512 keys 4 x 512 24, 2 x 512
+// 17.9, 1 x 512 19.8; 1 of 512 1 x 512 10.2, 4 x 64 10.5; 8 of 1024..2048 4 x 128 15.9, 2 x 256
+// 16.7, 1 x 512 17.5; 64 of 16..4096 4 x 1024 71, 4 x 512 74, 2 x 1024 76; 16 of 8k..32k 4 x 512 121,
+// 4 x 1024 136, 1 x 1024 172; 1 of 4096 1 x 256 13.0, 4 x 64 15.2.
+void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, int cus, int* part, int* heads) {
+  const int64_t n_hc = ceil_div(H / Hkv, heads_per_wave(H, Hkv, D));
+  int side = kWaves;
+  while (Hkv % side) side /= 2;
+  auto workgroups = [&](int hw, int64_t len) { return sat_mul(B, Hkv / hw * n_hc, ceil_div(most, len)); };
+  for (int hw = side; hw >= 1; hw /= 2) {
+    const int64_t step = kChunk * kWaves / hw, steps = ceil_div(most, step);
+    if (steps <= 8 && (workgroups(hw, most) >= cus || (hw == 1 && steps <= 2))) {
+      *part = (int)(steps * step);
+      *heads = hw;
+      return;
+    }
+  }
+  for (int hw = side; hw >= 1; hw /= 2)
+    for (int len = 512; len >= 2 * kChunk * kWaves / hw; len /= 2)
+      if (workgroups(hw, len) >= cus) {
+        *part = len;
+        *heads = hw;
+        return;
+      }
+  *part = kChunk * kWaves;
+  *heads = 1;
+}
+
+// The parts' states or rows; the caller merges.
 int launch_q4_decode(const SpanArgs& a, int D, hipStream_t stream) {
+  const int64_t n_hc = ceil_div(a.H / a.Hkv, heads_per_wave(a.H, a.Hkv, D));
+  if (!grid_fits(sat_mul(a.B, a.P, a.Hkv / a.heads * n_hc), 64 * kWaves))
+    return fail(HS_EUNSUPPORTED, "grid too large: sequences * parts * KV heads");
   switch (D) {
     case 32: launch_dim<32>(a, stream); break;
     case 64: launch_dim<64>(a, stream); break;

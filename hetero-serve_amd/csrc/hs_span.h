@@ -25,6 +25,7 @@ struct SpanArgs {
   int bs_shift;               // log2(BS), or -1
   int window, sinks;          // window 0: all keys
   int part, P;                // keys of a part, parts of the longest row
+  int heads;                  // 4-bit cache: KV heads of a workgroup
   float qscale;               // scale * log2(e)
 };
 
@@ -48,18 +49,24 @@ struct Span {
     hi = min((int64_t)lo + a.part, (int64_t)n);
     return true;
   }
-  // The slot of key i < n, as a row of the cache seen as [NB * BS] rows (below 2^31).
-  __device__ uint32_t slot(const SpanArgs& a, const int32_t* bt, int i) const {
+  // Where key i < n lies: its page's table entry and its place in the page.
+  struct Place {
+    int32_t block;
+    uint32_t off;
+  };
+  __device__ Place place(const SpanArgs& a, const int32_t* bt, int i) const {
     const uint32_t pos = (uint32_t)(i < sinks ? i : i + skip);
-    uint32_t page, off;
-    if (a.bs_shift >= 0) {   // uniform
-      page = pos >> a.bs_shift;
-      off = pos & (uint32_t)(a.BS - 1);
-    } else {
-      page = pos / (uint32_t)a.BS;
-      off = pos - page * (uint32_t)a.BS;
-    }
-    return (uint32_t)safe_block(bt[page], a.NB) * (uint32_t)a.BS + off;
+    if (a.bs_shift >= 0)   // uniform
+      return {bt[pos >> a.bs_shift], pos & (uint32_t)(a.BS - 1)};
+    const uint32_t page = pos / (uint32_t)a.BS;
+    return {bt[page], pos - page * (uint32_t)a.BS};
+  }
+  // As a row of the cache seen as [NB * BS] rows (below 2^31).
+  __device__ static uint32_t slot(const SpanArgs& a, const Place& x) {
+    return (uint32_t)safe_block(x.block, a.NB) * (uint32_t)a.BS + x.off;
+  }
+  __device__ uint32_t slot(const SpanArgs& a, const int32_t* bt, int i) const {
+    return slot(a, place(a, bt, i));
   }
 };
 

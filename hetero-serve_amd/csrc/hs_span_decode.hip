@@ -170,24 +170,26 @@ __global__ __launch_bounds__(64 * kWaves) void span_walk_kernel(SpanArgs a) {
   }
 }
 
-// The rows whose keys are several parts': one wave per (row, head), lanes over D.
+// The rows whose keys are several parts': one workgroup per (row, head), lanes over D, a
+// quarter of the parts each wave.
 template <int D>
-__global__ __launch_bounds__(256) void span_merge_kernel(SpanArgs a) {
+__global__ __launch_bounds__(64 * kWaves) void span_merge_kernel(SpanArgs a) {
   constexpr int kPer = (D + 63) / 64, kBatch = 8;
-  const int lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= (int64_t)a.B * a.H) return;
+  __shared__ float sums[kWaves][kPer * 64], most[kWaves], totals[kWaves];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int64_t w = blockIdx.x;
   const Span span(a, (int)(w / a.H));
   int lo, hi, n;
   if (!span.part(a, 0, lo, hi, n) || n == 1) return;   // written already
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + w * a.P;
+  const int each = (n + kWaves - 1) / kWaves, first = min(n, wv * each), end = min(n, first + each);
   float mm = kLowest;
-  for (int p = lane; p < n; p += 64) mm = fmaxf(mm, ml[p].x);
+  for (int p = first + lane; p < end; p += 64) mm = fmaxf(mm, ml[p].x);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) mm = fmaxf(mm, __shfl_xor(mm, off));
   float acc[kPer] = {}, l = 0.0f;
-  for (int p0 = 0; p0 < n; p0 += 64) {
-    const int here = min(64, n - p0);
+  for (int p0 = first; p0 < end; p0 += 64) {
+    const int here = min(64, end - p0);
     const float2 st = lane < here ? ml[p0 + lane] : make_float2(kLowest, 0.0f);
     const float wt = lane < here ? fast_exp2(st.x - mm) : 0.0f;
     l = fmaf(st.y, wt, l);
@@ -210,11 +212,30 @@ __global__ __launch_bounds__(256) void span_merge_kernel(SpanArgs a) {
     }
   }
   l = group_sum<64>(l);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) sums[wv][lane + 64 * i] = acc[i];
+  if (lane == 0) {
+    most[wv] = mm;
+    totals[wv] = l;
+  }
+  __syncthreads();
+  if (wv != 0) return;
+  mm = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+  l = 0.0f;
+  float keep[kWaves];
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    keep[i] = fast_exp2(most[i] - mm);
+    l = fmaf(totals[i], keep[i], l);
+  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int d = lane + 64 * i;
-    if (d < D) a.out[w * D + d] = acc[i] * inv;
+    float x = 0.0f;
+#pragma unroll
+    for (int u = 0; u < kWaves; ++u) x = fmaf(sums[u][d], keep[u], x);
+    if (d < D) a.out[w * D + d] = x * inv;
   }
 }
 
@@ -245,7 +266,7 @@ int launch_walk_dim(const SpanArgs& a, int D, hipStream_t stream) {
 }  // namespace
 
 void launch_span_merge(const SpanArgs& a, int D, hipStream_t stream) {
-  const dim3 grid((unsigned)ceil_div((int64_t)a.B * a.H, 4)), block(256);
+  const dim3 grid((unsigned)((int64_t)a.B * a.H)), block(64 * kWaves);
   switch (D) {
     case 32: hipLaunchKernelGGL((span_merge_kernel<32>), grid, block, 0, stream, a); break;
     case 64: hipLaunchKernelGGL((span_merge_kernel<64>), grid, block, 0, stream, a); break;
@@ -256,17 +277,18 @@ void launch_span_merge(const SpanArgs& a, int D, hipStream_t stream) {
 
 // Keys of a part: 512, cut down to 64 while the waves of the longest rows would be fewer
 // than eight for each CU.
-int span_part(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, int cus) {
-  int part = 512;
+void span_plan(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, int cus, int* part, int* heads) {
+  if (kv_dtype < 0) return q4_decode_plan(B, H, Hkv, D, most, cus, part, heads);
+  *part = 512;
+  *heads = 0;
   const int64_t waves = sat_mul(B, H / row_attn_heads_per_wave(H, Hkv));
-  while (part > 64 && sat_mul(waves, ceil_div(most, part)) < 8 * (int64_t)cus) part /= 2;
-  return part;
+  while (*part > 64 && sat_mul(waves, ceil_div(most, *part)) < 8 * (int64_t)cus) *part /= 2;
 }
 
 // The parts, and the merge of rows of several.  kv_dtype -1: the 4-bit cache.
 int launch_span(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream) {
-  const int64_t waves = sat_mul(a.B, a.P, a.H);
-  if (!grid_fits(ceil_div(waves, kWaves), 64 * kWaves))
+  const int64_t rows = sat_mul(a.B, a.H), waves = sat_mul(rows, a.P);
+  if (!grid_fits(rows, 64 * kWaves) || !grid_fits(ceil_div(waves, kWaves), 64 * kWaves))
     return fail(HS_EUNSUPPORTED, "grid too large: sequences * parts * heads = " + std::to_string(waves));
   int rc;
   profile_begin(stream);

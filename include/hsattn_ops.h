@@ -196,8 +196,8 @@ int hs_q4_read(const void* k_cache, const void* v_cache, int NB, int BS, int Hkv
  * one of kv_dtype; scores, softmax and sums are fp32, products as near as fp32's.
  * A row that sees an infinity or a NaN may be NaN in the elements that it reaches.
  *   q, out      [B, H, D] float32, 16-byte aligned
- *   D           32, 64, 128 or 256;  H % Hkv == 0;  MB * BS and num_blocks * BS
- *               below 2^31;  scale finite, and times log2(e) as well
+ *   D           32, 64, 128 or 256;  H % Hkv == 0;  MB * BS at most 2^30, num_blocks
+ *               * BS below 2^31;  scale finite, and times log2(e) as well
  *   workspace   device scratch of the query's size for the same arguments, with the
  *               launch device current (may be NULL when that is 0), 16-byte aligned
  */
