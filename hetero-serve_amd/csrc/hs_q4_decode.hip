@@ -77,6 +77,7 @@ struct Chunk {
 };
 
 constexpr int kWaves = 4;   // of a workgroup
+constexpr int kXcds = 8;    // workgroups are dealt to them in turn
 
 template <int N>
 struct Words {
@@ -234,8 +235,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
   Chunk<D>& w = chunks[wv];
   const int hw = a.heads, np = kWaves / hw, hsub = wv % hw, ph = wv / hw;
   const int group = a.H / a.Hkv, n_hc = (group + kHeads - 1) / kHeads, units = a.Hkv / hw * n_hc;
-  const uint32_t rp = blockIdx.x / (uint32_t)units;
-  const int unit = blockIdx.x - rp * units, b = rp / a.P, p = rp - b * a.P;
+  // The heads of one part run on one XCD, one behind the other: they share lines of 128 bytes.
+  const uint32_t turn = blockIdx.x / kXcds, rp = turn / (uint32_t)units * kXcds + blockIdx.x % kXcds;
+  if (rp >= (uint64_t)a.B * a.P) return;
+  const int unit = turn % (uint32_t)units, b = rp / a.P, p = rp - b * a.P;
   const int hg = unit / n_hc, hc = unit - hg * n_hc, kvh = hg * hw + hsub;
   const int h0 = kvh * group + hc * kHeads, gc = min(kHeads, group - hc * kHeads);
   const int jh = kByGroup ? j / G : j, jg = kByGroup ? j % G : 0;   // this column's head, group
@@ -569,7 +572,7 @@ int heads_per_wave(int H, int Hkv, int D) {
 template <int D, bool kByGroup>
 void launch_one(const SpanArgs& a, hipStream_t stream) {
   const int64_t n_hc = ceil_div(a.H / a.Hkv, heads_per_wave(a.H, a.Hkv, D));
-  const int64_t wgs = sat_mul(a.B, a.P, a.Hkv / a.heads * n_hc);
+  const int64_t wgs = ceil_div(sat_mul(a.B, a.P), kXcds) * kXcds * (a.Hkv / a.heads * n_hc);
   hipLaunchKernelGGL((q4_decode_kernel<D, kByGroup>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, stream,
                      a);
 }
@@ -618,7 +621,7 @@ void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, int cus, int* pa
 // The parts' states or rows; the caller merges.
 int launch_q4_decode(const SpanArgs& a, int D, hipStream_t stream) {
   const int64_t n_hc = ceil_div(a.H / a.Hkv, heads_per_wave(a.H, a.Hkv, D));
-  if (!grid_fits(sat_mul(a.B, a.P, a.Hkv / a.heads * n_hc), 64 * kWaves))
+  if (!grid_fits(sat_mul(sat_add(sat_mul(a.B, a.P), kXcds), a.Hkv / a.heads * n_hc), 64 * kWaves))
     return fail(HS_EUNSUPPORTED, "grid too large: sequences * parts * KV heads");
   switch (D) {
     case 32: launch_dim<32>(a, stream); break;
