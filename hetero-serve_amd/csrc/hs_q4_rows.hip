@@ -33,23 +33,42 @@ struct Q4Args {
   int64_t k_row, v_row;             // bytes between source rows
   int64_t n;
   int Hkv, D;
+  int row_shift, head_shift, bs_shift;   // log2 of a row's words, a head's, BS, or -1
   RowMap map;
 };
 
-// Row, head and word of the flat index i over rows of Hkv D / 8 words.
+// Row, record in the row and word in the record of the flat index i over rows of Hkv D / 8
+// words.  Shifts where the row's words are a power of 2: divisions are a third of these
+// kernels' instructions otherwise.
 __device__ inline void split_word(const Q4Args& a, int64_t i, int64_t& row, int& h, int& w) {
-  const uint32_t words = (uint32_t)a.D / 8, per = (uint32_t)a.Hkv * words;
   uint32_t in_row;
-  if (a.n * per <= 0xffffffffLL) {   // uniform
-    const uint32_t r = (uint32_t)i / per;
-    row = r;
-    in_row = (uint32_t)i - r * per;
+  if (a.row_shift >= 0) {   // uniform
+    row = i >> a.row_shift;
+    in_row = (uint32_t)i & ((1u << a.row_shift) - 1);
   } else {
-    row = i / per;
-    in_row = (uint32_t)(i - row * per);
+    const uint32_t per = (uint32_t)a.Hkv << a.head_shift;
+    if (a.n * per <= 0xffffffffLL) {   // uniform
+      const uint32_t r = (uint32_t)i / per;
+      row = r;
+      in_row = (uint32_t)i - r * per;
+    } else {
+      row = i / per;
+      in_row = (uint32_t)(i - row * per);
+    }
   }
-  h = (int)(in_row / words);
-  w = (int)(in_row - (uint32_t)h * words);
+  h = (int)(in_row >> a.head_shift);
+  w = (int)(in_row & ((1u << a.head_shift) - 1));
+}
+
+// RowMap's slot of row i, the page by a shift where BS is a power of 2.
+__device__ inline int64_t slot_of(const Q4Args& a, int64_t i) {
+  if (a.bs_shift < 0) return a.map.slot(i);   // uniform
+  const int64_t b = a.map.seq_ids ? a.map.seq_ids[i] : i;
+  const int pos = a.map.positions[i];
+  if (b < 0 || b >= a.map.B || pos < 0 || pos >> a.bs_shift >= a.map.MB) return -1;
+  const int blk = a.map.bt[b * a.map.MB + (pos >> a.bs_shift)];
+  if (blk < 0 || blk >= a.map.NB) return -1;
+  return ((int64_t)blk << a.bs_shift) + (pos & (a.map.BS - 1));
 }
 
 template <typename T, bool kVec>
@@ -78,14 +97,11 @@ __device__ inline _Float16 q4_step(float most, float lo) {
   return (_Float16)exact;
 }
 
-template <typename T, bool kVec, bool kKeys>
-__device__ inline void append_word(const Q4Args& a, int64_t row, int h, int w) {
-  const int64_t slot = a.map.slot(row);
-  if (slot < 0) return;              // all four threads of a group
+// One word of a record from its 8 elements; the three neighbouring threads have the rest of
+// the group.
+template <bool kKeys>
+__device__ inline void write_word(const Q4Args& a, uint8_t* rec, int w, const float* x) {
   const int G = a.D / kQ4Group;
-  float x[8];
-  load_elements<T, kVec>((kKeys ? a.k_src : a.v_src) + row * (kKeys ? a.k_row : a.v_row) +
-                             ((int64_t)h * a.D + 8 * w) * Codec<T>::kBytes, x);
   float hi = x[0], lo = x[0];
 #pragma unroll
   for (int e = 1; e < 8; ++e) {
@@ -101,19 +117,24 @@ __device__ inline void append_word(const Q4Args& a, int64_t row, int h, int w) {
   const _Float16 lo16 = (_Float16)fminf(fmaxf(lo, -kF16Most), kF16Most);
   const float base = (float)lo16;
   const _Float16 s16 = none ? (_Float16)0.0f : q4_step(hi, base);
-  const float s = (float)s16, inv = 1.0f / s;
-  // adding 1.5 2^23 rounds to a whole number and leaves it in the low bits
+  const float s = (float)s16, inv = __builtin_amdgcn_rcpf(s);
+  // Adding 1.5 2^23 rounds to a whole number and leaves it in the low bits, the rest of
+  // which are taken off at the end.
   constexpr float kWhole = 12582912.0f;
-  float t[8], r[8], far = 0.0f;
+  constexpr uint32_t kBits = 0x4b400000u * 0x11111111u;   // those of kWhole, every 4 bits
+  float t[8], near = 0.5f;           // to half way
   uint32_t word = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     t[e] = __builtin_amdgcn_fmed3f((x[e] - base) * inv, 0.0f, 15.0f);
-    r[e] = t[e] + kWhole;
-    far = fmaxf(far, fabsf(t[e] - (r[e] - kWhole)));
-    word += (__float_as_uint(r[e]) - __float_as_uint(kWhole)) << (4 * e);
+    word += __float_as_uint(t[e] + kWhole) << (4 * e);
   }
-  if (far > 0.5f - 0x1p-16f) {
+  word -= kBits;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2)
+    near = fminf(near, fminf(fabsf(__builtin_amdgcn_fractf(t[e]) - 0.5f),
+                             fabsf(__builtin_amdgcn_fractf(t[e + 1]) - 0.5f)));
+  if (near < 0x1p-16f) {
     word = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -122,8 +143,6 @@ __device__ inline void append_word(const Q4Args& a, int64_t row, int h, int w) {
     }
   }
   if (!(s > 0.0f)) word = 0;         // one value, or none
-  uint8_t* rec = (kKeys ? a.k_cache : a.v_cache) +
-                 (slot * a.Hkv + h) * (int64_t)q4_record_bytes(a.D);
   *reinterpret_cast<uint32_t*>(rec + 4 * q4_word<kKeys>(w, G)) = word;
   // the group's first thread stores the step, the second the lowest value
   const int part = w & 3, g = w >> 2;
@@ -135,7 +154,7 @@ __device__ inline void append_word(const Q4Args& a, int64_t row, int h, int w) {
   }
 }
 
-// grid.x covers the words, grid.y K and V.
+// A thread: one word of a key's record and the value's, whose slot is the same.
 template <typename T, bool kVec>
 __global__ __launch_bounds__(kThreads) void q4_append_kernel(Q4Args a) {
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -143,29 +162,30 @@ __global__ __launch_bounds__(kThreads) void q4_append_kernel(Q4Args a) {
   int64_t row;
   int h, w;
   split_word(a, i, row, h, w);
-  if (blockIdx.y == 0) append_word<T, kVec, true>(a, row, h, w);
-  else append_word<T, kVec, false>(a, row, h, w);
+  const int64_t e = ((int64_t)h * a.D + 8 * w) * Codec<T>::kBytes;
+  float k[8], v[8];                  // on their way while the slot is looked up
+  load_elements<T, kVec>(a.k_src + row * a.k_row + e, k);
+  load_elements<T, kVec>(a.v_src + row * a.v_row + e, v);
+  const int64_t slot = slot_of(a, row);
+  if (slot < 0) return;              // all four threads of a group
+  const int64_t rec = (slot * a.Hkv + h) * q4_record_bytes(a.D);
+  write_word<true>(a, a.k_cache + rec, w, k);
+  write_word<false>(a, a.v_cache + rec, w, v);
 }
 
-template <typename T, bool kKeys>
-__device__ inline void read_word(const Q4Args& a, int64_t row, int h, int w) {
-  const int G = a.D / kQ4Group;
-  const int64_t slot = a.map.slot(row);
-  float x[8];
-  if (slot < 0) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+// The values of 8 elements, not read again by this kernel or kept for it.
+template <typename T>
+__device__ inline void store8_stream(uint8_t* p, const float* x) {
+  if constexpr (sizeof(T) == 4) {
+    store16_stream(p, make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                                 __float_as_uint(x[3])));
+    store16_stream(p + 16, make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]),
+                                      __float_as_uint(x[7])));
   } else {
-    const uint8_t* rec = (kKeys ? a.k_cache : a.v_cache) +
-                         (slot * a.Hkv + h) * (int64_t)q4_record_bytes(a.D);
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(rec + 4 * q4_word<kKeys>(w, G));
-    const _Float16* par = reinterpret_cast<const _Float16*>(rec + a.D / 2) + (w >> 2);
-    const float s = (float)par[0], lo = (float)par[G];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((word >> (4 * e)) & 15u), s, lo);
+    uint4 w;
+    Codec<T>::store8(reinterpret_cast<uint8_t*>(&w), x);
+    store16_stream(p, w);
   }
-  Codec<T>::store8((kKeys ? a.k_out : a.v_out) +
-                       ((row * a.Hkv + h) * (int64_t)a.D + 8 * w) * Codec<T>::kBytes, x);
 }
 
 template <typename T>
@@ -175,8 +195,25 @@ __global__ __launch_bounds__(kThreads) void q4_read_kernel(Q4Args a) {
   int64_t row;
   int h, w;
   split_word(a, i, row, h, w);
-  if (blockIdx.y == 0) read_word<T, true>(a, row, h, w);
-  else read_word<T, false>(a, row, h, w);
+  const int G = a.D / kQ4Group;
+  const int64_t slot = slot_of(a, row);
+  float x[2][8] = {};
+  if (slot >= 0) {
+    const int64_t at = (slot * a.Hkv + h) * q4_record_bytes(a.D);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const uint8_t* rec = (c == 0 ? a.k_cache : a.v_cache) + at;
+      const int place = c == 0 ? q4_word<true>(w, G) : q4_word<false>(w, G);
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(rec + 4 * place);
+      const _Float16* par = reinterpret_cast<const _Float16*>(rec + a.D / 2) + (w >> 2);
+      const float s = (float)par[0], lo = (float)par[G];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[c][e] = fmaf((float)((word >> (4 * e)) & 15u), s, lo);
+    }
+  }
+  const int64_t to = ((row * a.Hkv + h) * (int64_t)a.D + 8 * w) * Codec<T>::kBytes;
+  store8_stream<T>(a.k_out + to, x[0]);
+  store8_stream<T>(a.v_out + to, x[1]);
 }
 
 template <typename T>
@@ -192,6 +229,10 @@ Q4Args rows_args(const Q4Rows& w) {
   a.n = w.n;
   a.Hkv = w.Hkv;
   a.D = w.D;
+  auto shift = [](int64_t x) { return x > 0 && (x & (x - 1)) == 0 && x < 1 << 30 ? __builtin_ctzll(x) : -1; };
+  a.head_shift = shift(w.D / 8);
+  a.row_shift = shift((int64_t)w.Hkv * (w.D / 8));
+  a.bs_shift = shift(w.BS);
   a.map.bt = w.bt;
   a.map.positions = w.positions;
   a.map.seq_ids = w.seq_ids;
@@ -210,7 +251,7 @@ bool rows_grid(const Q4Rows& w, int64_t row_bytes, dim3& grid) {
       sat_mul(w.n, row_bytes) == INT64_MAX ||
       sat_mul((int64_t)w.NB * w.BS, sat_mul(w.Hkv, q4_record_bytes(w.D))) == INT64_MAX)
     return false;
-  grid = dim3((unsigned)wgs, 2);
+  grid = dim3((unsigned)wgs);
   return true;
 }
 
