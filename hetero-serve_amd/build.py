@@ -71,6 +71,7 @@ PER_FILE_FLAGS = {
     "hs_decode_splitmm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "hs_prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "hs_q4_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+    "hs_window_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
 }
 
 

@@ -35,7 +35,7 @@
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
 #include "hs_q4.h"
-#include "hs_span.h"
+#include "hs_span_mma.h"
 
 #include <algorithm>
 
@@ -46,18 +46,15 @@ namespace hs {
 
 namespace {
 
+using namespace span_mma;
+
 typedef _Float16 half2x __attribute__((ext_vector_type(2)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef float float4x __attribute__((ext_vector_type(4)));
 typedef int int2x __attribute__((ext_vector_type(2)));
 
 constexpr int kChunk = 64;         // keys of a step
-constexpr int kSlots = 16;         // query heads of a wave
-constexpr float kSlack = 8.0f;     // lazy raise of the running max, log2 units
 constexpr float kLift = 7.0f;      // probabilities are held 2^kLift times larger
-// Where running maxima start: no finite score lies below, so a row of one is never empty.
-constexpr float kLowest = -0x1.fffffep127f;
 // R is chosen so that the largest step so far times R lies in [2^-3, 2^-2), and again when
 // one times R passes 1 = 2^(kStepRoom - 2 + ...): p s R is at most 2^15 then.
 constexpr int kStepRoom = 2;
@@ -75,9 +72,6 @@ struct Chunk {
   alignas(16) _Float16 vs[G][kPar];
   alignas(16) _Float16 vmid[2 * G][kPar];       // both terms, keys in unpack8's order
 };
-
-constexpr int kWaves = 4;   // of a workgroup
-constexpr int kXcds = 8;    // workgroups are dealt to them in turn
 
 template <int N>
 struct Words {
@@ -126,20 +120,6 @@ __device__ inline int half_place(int i) { return 2 * (i & 3) + (i >> 2 & 1); }
 
 __device__ inline float4x mma(half8 a, half8 b, float4x c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-__device__ inline float max_across_groups(float x) {
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-__device__ inline float sum_across_groups(float x) {
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // Two fp16 terms hi + lo of two numbers, 22 bits of them.  The first ones pass through a
@@ -206,16 +186,6 @@ __device__ inline _Float16 half_of(const Words<N>& x, int i) {
   return __builtin_bit_cast(_Float16, (uint16_t)(x.w[i / 2] >> (16 * (i & 1))));
 }
 
-// One wave's LDS traffic is in order; this keeps the compiler's in order too.
-__device__ inline void lds_order() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
-// One workgroup: one part of one row, for hw KV heads side by side.  Its waves are these heads
-// times np phases, which take neighbouring chunks of a step of 64 np keys in turn and put
-// their states together at the end.
-//
 // kByGroup: the 16 columns of the products are heads times groups, column j head j / G's sums
 // over group j % G alone: 16 / G heads a wave.  Otherwise they are 16 heads.  By group, a lane
 // scales its scores by one group's steps and adds the groups' up with its neighbours', and
@@ -231,29 +201,20 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
   __shared__ float2 states[kWaves][kSlots];
   static_assert(kHeads * (D + 4) * 4 <= (int)sizeof(Chunk<D>), "a wave's outputs fit");
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
-  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Chunk<D>& w = chunks[wv];
-  const int hw = a.heads, np = kWaves / hw, hsub = wv % hw, ph = wv / hw;
-  const int group = a.H / a.Hkv, n_hc = (group + kHeads - 1) / kHeads, units = a.Hkv / hw * n_hc;
-  // The heads of one part run on one XCD, one behind the other: they share lines of 128 bytes.
-  const uint32_t turn = blockIdx.x / kXcds, rp = turn / (uint32_t)units * kXcds + blockIdx.x % kXcds;
-  if (rp >= (uint64_t)a.B * a.P) return;
-  const int unit = turn % (uint32_t)units, b = rp / a.P, p = rp - b * a.P;
-  const int hg = unit / n_hc, hc = unit - hg * n_hc, kvh = hg * hw + hsub;
-  const int h0 = kvh * group + hc * kHeads, gc = min(kHeads, group - hc * kHeads);
+  Task t;
+  if (!t.find(a, kHeads)) return;
+  Chunk<D>& w = chunks[t.wv];
   const int jh = kByGroup ? j / G : j, jg = kByGroup ? j % G : 0;   // this column's head, group
-  const Span span(a, b);
-  const int64_t row0 = (int64_t)b * a.H + h0;
+  const Span span(a, t.b);
   int lo, hi, nparts;
-  if (!span.part(a, p, lo, hi, nparts)) {   // all of the workgroup
-    if (span.n == 0 && p == 0 && ph == 0)   // nothing to attend to: zero rows
-      for (int d = lane; d < gc * D; d += 64) a.out[row0 * D + d] = 0.0f;
+  if (!span.part(a, t.p, lo, hi, nparts)) {   // all of the workgroup
+    if (span.n == 0 && t.p == 0) zero_rows<D>(a, t);
     return;
   }
-  const int32_t* bt = a.bt + (int64_t)b * a.MB;
+  const int32_t* bt = a.bt + (int64_t)t.b * a.MB;
   const uint32_t tok = (uint32_t)a.Hkv * kRecord;
-  const uint8_t* kbase = a.k + kvh * kRecord;
-  const uint8_t* vbase = a.v + kvh * kRecord;
+  const uint8_t* kbase = a.k + t.kvh * kRecord;
+  const uint8_t* vbase = a.v + t.kvh * kRecord;
 
   // A chunk's records come in pieces of D / 8 bytes, 64 lanes neighbouring pieces, and go to
   // LDS through registers: a chunk's loads are on their way while the one before is computed,
@@ -270,7 +231,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
       vr[i] = load_words<G>(vbase + at);
     }
   };
-  const int step = kChunk * np, first = lo + kChunk * ph;
+  const int step = kChunk * t.np, first = lo + kChunk * t.ph;
   auto place_of = [&](int c0) { return span.place(a, bt, min(c0 + lane, hi - 1)); };
   Span::Place ahead{};
   if (first < hi) {
@@ -284,8 +245,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
   _Float16 qsum[kMid];
   float back;     // what scores are to be multiplied by
   {
-    const float* qp = a.q + (row0 + min(jh, gc - 1)) * D + 8 * g;
-    const float sc = jh < gc ? a.qscale : 0.0f;
+    const float* qp = a.q + (t.row0 + min(jh, t.gc - 1)) * D + 8 * g;
+    const float sc = jh < t.gc ? a.qscale : 0.0f;
     float x[G][8], most = 0.0f;
 #pragma unroll
     for (int st = 0; st < G; ++st)
@@ -352,11 +313,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         const float x = (float)half_of(vp, i);
-        const Terms t = split(fmaf(x, 8.0f, (float)half_of(vp, G + i)), 0.0f);
+        const Terms m2 = split(fmaf(x, 8.0f, (float)half_of(vp, G + i)), 0.0f);
         w.ks[i][lane] = half_of(kp, i);
         w.vs[i][lane] = half_of(vp, i);
-        w.vmid[i][place] = half_of(Words<1>{t.hi}, 0);
-        w.vmid[G + i][place] = half_of(Words<1>{t.lo}, 0);
+        w.vmid[i][place] = half_of(Words<1>{m2.hi}, 0);
+        w.vmid[G + i][place] = half_of(Words<1>{m2.lo}, 0);
         most = fmaxf(most, x);
       }
       if (__builtin_amdgcn_ballot_w64(most > room) != 0) {
@@ -464,7 +425,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[i][e] = fast_exp2(fmaf(s[i][e], back, -mb));
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < 2; ++t) {   // (keys 8 t .. of each lane's 16)
       uint32_t h[4], l[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -522,45 +483,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[d][e] = fmaf(o[d][e], out_scale, mid);
   }
-  const bool whole = nparts == 1;
-  const int64_t pi = (row0 + jh) * a.P + p;
-  if (np == 1) {
-    const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-    float* to = whole ? a.out + (row0 + jh) * D : a.part_acc + pi * D;
-#pragma unroll
-    for (int d = 0; d < kT; ++d)
-      if (jh < gc && (!kByGroup || jg == d / 2)) *reinterpret_cast<float4x*>(to + 16 * d + 4 * g) = o[d] * inv;
-    if (!whole && jh < gc && jg == 0 && g == 0) reinterpret_cast<float2*>(a.part_ml)[pi] = make_float2(m, l);
-    return;
-  }
-  // the phases' states put together
-  lds_order();
-  if (jg == 0 && g == 0) states[wv][jh] = make_float2(m, l);
-  __syncthreads();
-  float mm = m;
-  for (int i = 0; i < np; ++i) mm = fmaxf(mm, states[hsub + hw * i][jh].x);
-  l = 0.0f;
-  for (int i = 0; i < np; ++i) {
-    const float2 x = states[hsub + hw * i][jh];
-    l = fmaf(x.y, fast_exp2(x.x - mm), l);
-  }
-  const float keep = fast_exp2(m - mm) * (!whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l);
-#pragma unroll
-  for (int d = 0; d < kT; ++d)
-    if (!kByGroup || jg == d / 2)
-      *reinterpret_cast<float4x*>(reinterpret_cast<float*>(&w) + jh * (D + 4) + 16 * d + 4 * g) = o[d] * keep;
-  if (!whole && ph == 0 && jh < gc && jg == 0 && g == 0)
-    reinterpret_cast<float2*>(a.part_ml)[pi] = make_float2(mm, l);
-  __syncthreads();
-  for (int x = ph * 64 + lane; x < gc * (D / 4); x += np * 64) {
-    const int h = x / (D / 4), d = x % (D / 4) * 4;
-    float4x sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < np; ++i)
-      sum += *reinterpret_cast<const float4x*>(reinterpret_cast<const float*>(&chunks[hsub + hw * i]) +
-                                               h * (D + 4) + d);
-    float* to = whole ? a.out + (row0 + h) * D : a.part_acc + ((row0 + h) * a.P + p) * D;
-    *reinterpret_cast<float4x*>(to + d) = sum;
-  }
+  finish<D, kHeads>(
+      a, t, nparts == 1, o, m, l, jh, jg == 0 && g == 0, [&](int d) { return !kByGroup || jg == d / 2; },
+      [&](int wave) { return reinterpret_cast<float*>(&chunks[wave]); }, states);
 }
 
 // Query heads of a wave.
@@ -571,8 +496,7 @@ int heads_per_wave(int H, int Hkv, int D) {
 
 template <int D, bool kByGroup>
 void launch_one(const SpanArgs& a, hipStream_t stream) {
-  const int64_t n_hc = ceil_div(a.H / a.Hkv, heads_per_wave(a.H, a.Hkv, D));
-  const int64_t wgs = ceil_div(sat_mul(a.B, a.P), kXcds) * kXcds * (a.Hkv / a.heads * n_hc);
+  const int64_t wgs = workgroups(a, heads_per_wave(a.H, a.Hkv, D));
   hipLaunchKernelGGL((q4_decode_kernel<D, kByGroup>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, stream,
                      a);
 }
@@ -586,42 +510,17 @@ void launch_dim(const SpanArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// Short rows are whole: as many KV heads side by side as leave a workgroup for each CU, where
-// their steps are at most eight, or one head and four phases where there are too few for
-// that and they take two steps.  Longer rows are cut into parts of 512 keys, shorter ones (of
-// two steps) and fewer heads side by side while the parts are fewer than the CUs.  us, D 128,
-// 32 / 8 heads, heads side by side x keys of a part: 64 rows of 64..512 keys 4 x 512 24, 2 x 512
-// 17.9, 1 x 512 19.8; 1 of 512 1 x 512 10.2, 4 x 64 10.5; 8 of 1024..2048 4 x 128 15.9, 2 x 256
-// 16.7, 1 x 512 17.5; 64 of 16..4096 4 x 1024 71, 4 x 512 74, 2 x 1024 76; 16 of 8k..32k 4 x 512 121,
-// 4 x 1024 136, 1 x 1024 172; 1 of 4096 1 x 256 13.0, 4 x 64 15.2.
+// us, D 128, 32 / 8 heads, heads side by side x keys of a part: 64 rows of 64..512 keys 4 x 512
+// 24, 2 x 512 17.9, 1 x 512 19.8; 1 of 512 1 x 512 10.2, 4 x 64 10.5; 8 of 1024..2048 4 x 128 15.9,
+// 2 x 256 16.7, 1 x 512 17.5; 64 of 16..4096 4 x 1024 71, 4 x 512 74, 2 x 1024 76; 16 of 8k..32k
+// 4 x 512 121, 4 x 1024 136, 1 x 1024 172; 1 of 4096 1 x 256 13.0, 4 x 64 15.2.
 void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, int cus, int* part, int* heads) {
-  const int64_t n_hc = ceil_div(H / Hkv, heads_per_wave(H, Hkv, D));
-  int side = kWaves;
-  while (Hkv % side) side /= 2;
-  auto workgroups = [&](int hw, int64_t len) { return sat_mul(B, Hkv / hw * n_hc, ceil_div(most, len)); };
-  for (int hw = side; hw >= 1; hw /= 2) {
-    const int64_t step = kChunk * kWaves / hw, steps = ceil_div(most, step);
-    if (steps <= 8 && (workgroups(hw, most) >= cus || (hw == 1 && steps <= 2))) {
-      *part = (int)(steps * step);
-      *heads = hw;
-      return;
-    }
-  }
-  for (int hw = side; hw >= 1; hw /= 2)
-    for (int len = 512; len >= 2 * kChunk * kWaves / hw; len /= 2)
-      if (workgroups(hw, len) >= cus) {
-        *part = len;
-        *heads = hw;
-        return;
-      }
-  *part = kChunk * kWaves;
-  *heads = 1;
+  plan(B, H, Hkv, heads_per_wave(H, Hkv, D), kChunk, most, cus, part, heads);
 }
 
 // The parts' states or rows; the caller merges.
 int launch_q4_decode(const SpanArgs& a, int D, hipStream_t stream) {
-  const int64_t n_hc = ceil_div(a.H / a.Hkv, heads_per_wave(a.H, a.Hkv, D));
-  if (!grid_fits(sat_mul(sat_add(sat_mul(a.B, a.P), kXcds), a.Hkv / a.heads * n_hc), 64 * kWaves))
+  if (!grid_fits(workgroups(a, heads_per_wave(a.H, a.Hkv, D)), 64 * kWaves))
     return fail(HS_EUNSUPPORTED, "grid too large: sequences * parts * KV heads");
   switch (D) {
     case 32: launch_dim<32>(a, stream); break;

@@ -279,6 +279,7 @@ void launch_span_merge(const SpanArgs& a, int D, hipStream_t stream) {
 // than eight for each CU.
 void span_plan(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, int cus, int* part, int* heads) {
   if (kv_dtype < 0) return q4_decode_plan(B, H, Hkv, D, most, cus, part, heads);
+  if (window_decode_serves(kv_dtype, D)) return window_decode_plan(B, H, Hkv, most, cus, part, heads);
   *part = 512;
   *heads = 0;
   const int64_t waves = sat_mul(B, H / row_attn_heads_per_wave(H, Hkv));
@@ -293,6 +294,7 @@ int launch_span(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream) {
   int rc;
   profile_begin(stream);
   if (kv_dtype < 0) rc = launch_q4_decode(a, D, stream);
+  else if (window_decode_serves(kv_dtype, D)) rc = launch_window_decode(a, kv_dtype, D, stream);
   else if (kv_dtype == HS_DTYPE_F32) rc = launch_walk_dim<float>(a, D, stream);
   else if (kv_dtype == HS_DTYPE_F16) rc = launch_walk_dim<_Float16>(a, D, stream);
   else rc = launch_walk_dim<Bf16>(a, D, stream);
