@@ -1094,7 +1094,8 @@ static int check_span_sizes(int kv_dtype, int B, int H, int Hkv, int D, int BS, 
 // Parts, and the bytes of their states (INT64_MAX when too large).
 static int64_t plan_span(SpanArgs& a, int kv_dtype, int D, int64_t* ml) {
   const int64_t most = span_most(a.MB, a.BS, a.window, a.sinks);
-  span_plan(kv_dtype, a.B, a.H, a.Hkv, D, most, current_cus(), &a.part, &a.heads);
+  span_plan(kv_dtype, a.B, a.H, a.Hkv, D, most, most < (int64_t)a.MB * a.BS, current_cus(), &a.part,
+            &a.heads);
   a.P = (int)ceil_div(most, a.part);
   return span_state_bytes(a.B, a.H, D, a.P, ml);
 }

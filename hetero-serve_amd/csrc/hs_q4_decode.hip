@@ -515,7 +515,7 @@ void launch_dim(const SpanArgs& a, hipStream_t stream) {
 // 2 x 256 16.7, 1 x 512 17.5; 64 of 16..4096 4 x 1024 71, 4 x 512 74, 2 x 1024 76; 16 of 8k..32k
 // 4 x 512 121, 4 x 1024 136, 1 x 1024 172; 1 of 4096 1 x 256 13.0, 4 x 64 15.2.
 void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, int cus, int* part, int* heads) {
-  plan(B, H, Hkv, heads_per_wave(H, Hkv, D), kChunk, most, cus, part, heads);
+  plan(B, H, Hkv, heads_per_wave(H, Hkv, D), kChunk, most, 8, cus, part, heads);
 }
 
 // The parts' states or rows; the caller merges.

@@ -1,14 +1,17 @@
-// Decode over spans (hs_span.h) on the vector units: fp32, fp16 and bf16 caches, and the
-// 4-bit cache.
+// Decode over spans (hs_span.h) on the vector units: fp32 caches, and fp16 and bf16 ones of head
+// dim 256; and the merge of rows whose keys are several parts.
 //
-// A wave serves G query heads of one KV head for one part of a row's visible keys.  One
+// A workgroup serves G query heads of one KV head for one part of a row's visible keys; its
+// four waves take the part's steps in turn and put their states together through LDS.  One
 // key's head row is spread over kLpt lanes, kVec elements each, and a load of the wave
 // covers kTpl keys; each such group of lanes runs an online softmax over its keys, in base
 // 2 with scale * log2(e) folded into the query, and the groups' states are merged at the
-// end.  Scores, sums and outputs are fp32.
+// end.  Scores, sums and outputs are fp32.  A step's keys and values are on their way while
+// the one before is computed, its table entries while the one before that is.  Behind a window
+// of 1024, 64 fp32 rows of 12 heads of 64, 390 MB, take 80 us (4.9 TB/s; 130 with a wave
+// for a part and nothing ahead), of 32 / 8 heads of 128, 520 MB, 100 (5.2 TB/s; 170).
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
-#include "hs_q4.h"
 #include "hs_span.h"
 
 #include <algorithm>
@@ -22,68 +25,55 @@ constexpr float kSlack = 8.0f;    // lazy raise of the running max, log2 units
 // Where running maxima start: no finite score lies below, so a row of one is never empty.
 constexpr float kLowest = -0x1.fffffep127f;
 
-// What a lane holds of one key's or value's head row.
-template <typename T, int D>
-struct Plain {
-  static constexpr int kVec = Elem<T>::kVec;
-  static constexpr int kRow = D * 16 / Elem<T>::kVec;   // bytes of a head row
-  struct Piece {
-    uint4 w;
-  };
-  template <bool kKeys>
-  __device__ static Piece load(const uint8_t* row, int c) {
-    return {load16_stream(row + 16 * c)};
-  }
-  __device__ static void to_f32(const Piece& x, float* f) { Elem<T>::to_f32(x.w, f); }
-};
-
-struct FourBits {};
-template <int D>
-struct Plain<FourBits, D> {
-  static constexpr int kVec = 8;
-  static constexpr int kRow = q4_record_bytes(D);
-  struct Piece {
-    uint32_t w;
-    _Float16 s, lo;
-  };
-  template <bool kKeys>
-  __device__ static Piece load(const uint8_t* row, int c) {
-    constexpr int G = D / kQ4Group;
-    const _Float16* par = reinterpret_cast<const _Float16*>(row + D / 2) + (c >> 2);
-    return {*reinterpret_cast<const uint32_t*>(row + 4 * q4_word<kKeys>(c, G)), par[0], par[G]};
-  }
-  __device__ static void to_f32(const Piece& x, float* f) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = fmaf((float)((x.w >> (4 * e)) & 15u), (float)x.s, (float)x.lo);
-  }
-};
-
 template <typename T, int D, int G>
 __global__ __launch_bounds__(64 * kWaves) void span_walk_kernel(SpanArgs a) {
-  using C = Plain<T, D>;
-  constexpr int kVec = C::kVec, kLpt = D / kVec, kTpl = 64 / kLpt;
-  constexpr int kU = G >= 4 || D > 128 ? 2 : 4;      // loads in flight
+  constexpr int kVec = Elem<T>::kVec, kLpt = D / kVec, kTpl = 64 / kLpt;
+  constexpr int kU = G >= 4 || D > 128 ? 2 : 4;      // loads in flight, of keys and of values
+  constexpr int kStep = kTpl * kU;
+  __shared__ float s_m[kWaves][G], s_l[kWaves][G], s_acc[kWaves][G][D];
   const int lane = threadIdx.x & 63, slot = lane / kLpt, c = lane % kLpt;
-  const int n_hw = a.H / G;
-  const int64_t w = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (w >= (int64_t)a.B * a.P * n_hw) return;
-  const int h0 = (int)(w % n_hw) * G;
-  const int64_t rp = w / n_hw;
-  const int b = (int)(rp / a.P), p = (int)(rp % a.P);
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t n_hw = a.H / G, rp = blockIdx.x / n_hw;
+  const int h0 = (int)(blockIdx.x - rp * n_hw) * G;
+  const int b = (int)(rp / (uint32_t)a.P), p = (int)(rp % (uint32_t)a.P);
   const Span span(a, b);
   const int64_t o0 = ((int64_t)b * a.H + h0) * D;
   int lo, hi, nparts;
-  if (!span.part(a, p, lo, hi, nparts)) {
+  if (!span.part(a, p, lo, hi, nparts)) {   // all of the workgroup
     if (span.n == 0 && p == 0)       // nothing to attend to: zero rows
-      for (int d = lane; d < G * D; d += 64) a.out[o0 + d] = 0.0f;
+      for (int d = threadIdx.x; d < G * D; d += 64 * kWaves) a.out[o0 + d] = 0.0f;
     return;
   }
-  const int kvh = h0 / (a.H / a.Hkv);
-  const int64_t row = (int64_t)a.Hkv * C::kRow;
-  const uint8_t* kp = a.k + (int64_t)kvh * C::kRow;
-  const uint8_t* vp = a.v + (int64_t)kvh * C::kRow;
+  const int64_t row = (int64_t)a.Hkv * D * sizeof(T);
+  const uint8_t* kp = a.k + (h0 / (a.H / a.Hkv)) * D * (int)sizeof(T) + 16 * c;
+  const uint8_t* vp = a.v + (h0 / (a.H / a.Hkv)) * D * (int)sizeof(T) + 16 * c;
   const int32_t* bt = a.bt + (int64_t)b * a.MB;
 
+  Span::Place ahead[kU];
+  uint4 kr[kU], vr[kU];
+  auto look = [&](int t0) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) ahead[u] = span.place(a, bt, min(t0 + u * kTpl + slot, hi - 1));
+  };
+  auto load = [&](const int64_t (&at)[kU]) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      kr[u] = load16_stream(kp + at[u]);
+      vr[u] = load16_stream(vp + at[u]);
+    }
+  };
+  auto rows_of = [&](int64_t (&at)[kU]) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) at[u] = (int64_t)Span::slot(a, ahead[u]) * row;
+  };
+  const int first = lo + wv * kStep;
+  if (first < hi) {
+    int64_t at[kU];
+    look(first);
+    rows_of(at);
+    look(first + kWaves * kStep);
+    load(at);
+  }
   float q[G][kVec], acc[G][kVec], m[G], l[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
@@ -95,16 +85,18 @@ __global__ __launch_bounds__(64 * kWaves) void span_walk_kernel(SpanArgs a) {
     m[g] = kLowest;
     l[g] = 0.0f;
   }
-  for (int t0 = lo; t0 < hi; t0 += kTpl * kU) {
-    typename C::Piece kr[kU], vr[kU];
-    bool ok[kU];
+  for (int t0 = first; t0 < hi; t0 += kWaves * kStep) {
+    uint4 kc[kU], vc[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int t = t0 + u * kTpl + slot;
-      ok[u] = t < hi;
-      const int64_t at = span.slot(a, bt, min(t, hi - 1)) * row;
-      kr[u] = C::template load<true>(kp + at, c);
-      vr[u] = C::template load<false>(vp + at, c);
+      kc[u] = kr[u];
+      vc[u] = vr[u];
+    }
+    if (t0 + kWaves * kStep < hi) {   // uniform
+      int64_t at[kU];
+      rows_of(at);
+      look(t0 + 2 * kWaves * kStep);
+      load(at);
     }
     float pu[G][kU];
 #pragma unroll
@@ -113,11 +105,11 @@ __global__ __launch_bounds__(64 * kWaves) void span_walk_kernel(SpanArgs a) {
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
         float f[kVec], d = 0.0f;
-        C::to_f32(kr[u], f);
+        Elem<T>::to_f32(kc[u], f);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) d = fmaf(q[g][e], f[e], d);
         d = group_sum<kLpt>(d);
-        pu[g][u] = ok[u] ? d : -INFINITY;
+        pu[g][u] = t0 + u * kTpl + slot < hi ? d : -INFINITY;
         mx = fmaxf(mx, pu[g][u]);
       }
       if (__builtin_amdgcn_ballot_w64(mx > m[g] + kSlack) != 0) {
@@ -135,11 +127,12 @@ __global__ __launch_bounds__(64 * kWaves) void span_walk_kernel(SpanArgs a) {
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
+      const bool ok = t0 + u * kTpl + slot < hi;
       float f[kVec];
-      C::to_f32(vr[u], f);
+      Elem<T>::to_f32(vc[u], f);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        f[e] = ok[u] ? f[e] : 0.0f;   // read twice where the part ends, and not added, not even times 0
+        f[e] = ok ? f[e] : 0.0f;   // read twice where the part ends, and not added, not even times 0
 #pragma unroll
         for (int g = 0; g < G; ++g) acc[g][e] = fmaf(pu[g][u], f[e], acc[g][e]);
       }
@@ -158,15 +151,32 @@ __global__ __launch_bounds__(64 * kWaves) void span_walk_kernel(SpanArgs a) {
       m[g] = mm;
     }
     if (slot != 0) continue;
-    const bool whole = nparts == 1;
-    const float inv = !whole ? 1.0f : l[g] == 0.0f ? 0.0f : 1.0f / l[g];
-    const int64_t pi = ((int64_t)b * a.H + h0 + g) * a.P + p;
-    float* to = (whole ? a.out + o0 + g * D : a.part_acc + pi * D) + c * kVec;
 #pragma unroll
-    for (int e = 0; e < kVec; e += 4)
-      *reinterpret_cast<float4*>(to + e) = make_float4(acc[g][e] * inv, acc[g][e + 1] * inv,
-                                                       acc[g][e + 2] * inv, acc[g][e + 3] * inv);
-    if (!whole && c == 0) reinterpret_cast<float2*>(a.part_ml)[pi] = make_float2(m[g], l[g]);
+    for (int e = 0; e < kVec; ++e) s_acc[wv][g][c * kVec + e] = acc[g][e];
+    if (c == 0) {
+      s_m[wv][g] = m[g];
+      s_l[wv][g] = l[g];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < G * D; i += 64 * kWaves) {
+    const int g = i / D, d = i % D;
+    float mm = s_m[0][g], sum = 0.0f, x = 0.0f;
+#pragma unroll
+    for (int v = 1; v < kWaves; ++v) mm = fmaxf(mm, s_m[v][g]);
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const float w = fast_exp2(s_m[v][g] - mm);
+      sum = fmaf(s_l[v][g], w, sum);
+      x = fmaf(s_acc[v][g][d], w, x);
+    }
+    if (nparts == 1) {
+      a.out[o0 + i] = sum == 0.0f ? 0.0f : x * (1.0f / sum);
+    } else {
+      const int64_t pi = ((int64_t)b * a.H + h0 + g) * a.P + p;
+      a.part_acc[pi * D + d] = x;
+      if (d == 0) reinterpret_cast<float2*>(a.part_ml)[pi] = make_float2(mm, sum);
+    }
   }
 }
 
@@ -242,7 +252,7 @@ __global__ __launch_bounds__(64 * kWaves) void span_merge_kernel(SpanArgs a) {
 template <typename T, int D>
 void launch_walk(const SpanArgs& a, hipStream_t stream) {
   const int G = row_attn_heads_per_wave(a.H, a.Hkv);
-  const dim3 grid((unsigned)ceil_div(sat_mul(a.B, a.P, a.H / G), kWaves)), block(64 * kWaves);
+  const dim3 grid((unsigned)sat_mul(a.B, a.P, a.H / G)), block(64 * kWaves);
   switch (G) {
     case 8: hipLaunchKernelGGL((span_walk_kernel<T, D, 8>), grid, block, 0, stream, a); break;
     case 4: hipLaunchKernelGGL((span_walk_kernel<T, D, 4>), grid, block, 0, stream, a); break;
@@ -251,14 +261,21 @@ void launch_walk(const SpanArgs& a, hipStream_t stream) {
   }
 }
 
-template <typename T>
-int launch_walk_dim(const SpanArgs& a, int D, hipStream_t stream) {
-  switch (D) {
-    case 32: launch_walk<T, 32>(a, stream); break;
-    case 64: launch_walk<T, 64>(a, stream); break;
-    case 128: launch_walk<T, 128>(a, stream); break;
-    case 256: launch_walk<T, 256>(a, stream); break;
-    default: return fail(HS_EUNSUPPORTED, "unsupported head_dim " + std::to_string(D));
+// fp32 and head dim 256: the others have the matrix cores (hs_window_decode.hip).
+int launch_walk_type(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream) {
+  const int64_t wgs = sat_mul(a.B, a.P, a.H / row_attn_heads_per_wave(a.H, a.Hkv));
+  if (!grid_fits(wgs, 64 * kWaves))
+    return fail(HS_EUNSUPPORTED, "grid too large: sequences * parts * heads = " + std::to_string(wgs));
+  if (D == 256) {
+    if (kv_dtype == HS_DTYPE_F32) launch_walk<float, 256>(a, stream);
+    else if (kv_dtype == HS_DTYPE_F16) launch_walk<_Float16, 256>(a, stream);
+    else launch_walk<Bf16, 256>(a, stream);
+  } else if (D == 128) {
+    launch_walk<float, 128>(a, stream);
+  } else if (D == 64) {
+    launch_walk<float, 64>(a, stream);
+  } else {
+    launch_walk<float, 32>(a, stream);
   }
   return HS_OK;
 }
@@ -275,29 +292,30 @@ void launch_span_merge(const SpanArgs& a, int D, hipStream_t stream) {
   }
 }
 
-// Keys of a part: 512, cut down to 64 while the waves of the longest rows would be fewer
-// than eight for each CU.
-void span_plan(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, int cus, int* part, int* heads) {
+// Vector units: rows are whole where that makes a workgroup for each CU, or they are short;
+// otherwise parts of 2048 keys, cut down to 256 while the workgroups are fewer than two for
+// each CU.
+void span_plan(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
+               int* heads) {
   if (kv_dtype < 0) return q4_decode_plan(B, H, Hkv, D, most, cus, part, heads);
-  if (window_decode_serves(kv_dtype, D)) return window_decode_plan(B, H, Hkv, most, cus, part, heads);
-  *part = 512;
+  if (window_decode_serves(kv_dtype, D))
+    return window_decode_plan(B, H, Hkv, most, windowed, cus, part, heads);
   *heads = 0;
-  const int64_t waves = sat_mul(B, H / row_attn_heads_per_wave(H, Hkv));
-  while (*part > 64 && sat_mul(waves, ceil_div(most, *part)) < 8 * (int64_t)cus) *part /= 2;
+  const int64_t wgs = sat_mul(B, H / row_attn_heads_per_wave(H, Hkv));
+  int len = 2048;
+  while (len > 256 && sat_mul(wgs, ceil_div(most, len)) < 2 * (int64_t)cus) len /= 2;
+  *part = most <= 512 || (most <= 4096 && wgs >= cus) ? (int)most : len;
 }
 
 // The parts, and the merge of rows of several.  kv_dtype -1: the 4-bit cache.
 int launch_span(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream) {
-  const int64_t rows = sat_mul(a.B, a.H), waves = sat_mul(rows, a.P);
-  if (!grid_fits(rows, 64 * kWaves) || !grid_fits(ceil_div(waves, kWaves), 64 * kWaves))
-    return fail(HS_EUNSUPPORTED, "grid too large: sequences * parts * heads = " + std::to_string(waves));
+  if (!grid_fits(sat_mul(a.B, a.H), 64 * kWaves))
+    return fail(HS_EUNSUPPORTED, "grid too large: sequences * heads");
   int rc;
   profile_begin(stream);
   if (kv_dtype < 0) rc = launch_q4_decode(a, D, stream);
   else if (window_decode_serves(kv_dtype, D)) rc = launch_window_decode(a, kv_dtype, D, stream);
-  else if (kv_dtype == HS_DTYPE_F32) rc = launch_walk_dim<float>(a, D, stream);
-  else if (kv_dtype == HS_DTYPE_F16) rc = launch_walk_dim<_Float16>(a, D, stream);
-  else rc = launch_walk_dim<Bf16>(a, D, stream);
+  else rc = launch_walk_type(a, kv_dtype, D, stream);
   profile_end(stream);
   if (rc != HS_OK) return rc;
   if (a.P > 1) launch_span_merge(a, D, stream);

@@ -131,17 +131,18 @@ inline int64_t workgroups(const SpanArgs& a, int heads) {
 }
 
 // Short rows are whole: as many KV heads side by side as leave a workgroup for each CU, where
-// their steps are at most eight, or one head and four phases where there are too few for
+// their steps are at most most_steps, or one head and four phases where there are too few for
 // that and they take two steps.  Longer rows are cut into parts of eight chunks, shorter ones
 // (of two steps) and fewer heads side by side while the parts are fewer than the CUs.
-inline void plan(int B, int H, int Hkv, int heads, int chunk, int64_t most, int cus, int* part, int* side) {
+inline void plan(int B, int H, int Hkv, int heads, int chunk, int64_t most, int most_steps, int cus, int* part,
+                 int* side) {
   const int64_t n_hc = ceil_div(H / Hkv, heads);
   int wide = kWaves;
   while (Hkv % wide) wide /= 2;
   auto wgs = [&](int hw, int64_t len) { return sat_mul(B, Hkv / hw * n_hc, ceil_div(most, len)); };
   for (int hw = wide; hw >= 1; hw /= 2) {
     const int64_t step = chunk * kWaves / hw, steps = ceil_div(most, step);
-    if (steps <= 8 && (wgs(hw, most) >= cus || (hw == 1 && steps <= 2))) {
+    if (steps <= most_steps && (wgs(hw, most) >= cus || (hw == 1 && steps <= 2))) {
       *part = (int)(steps * step);
       *side = hw;
       return;
