@@ -59,8 +59,11 @@ struct Task {
     const uint32_t turn = blockIdx.x / kXcds, rp = turn / (uint32_t)units * kXcds + blockIdx.x % kXcds;
     if (rp >= (uint64_t)a.B * a.P) return false;
     const int unit = turn % (uint32_t)units;
-    b = rp / (uint32_t)a.P;
-    p = rp - b * a.P;
+    // First parts first, for rows of several lengths end at several parts; and a row's parts on
+    // every XCD in turn.
+    const uint32_t B = a.B;
+    p = rp / B;
+    b = (rp - p * B + (B % 2 == 0 ? p : 0)) % B;
     kvh = unit / n_hc * hw + hsub;
     const int hc = unit % n_hc;
     h0 = kvh * group + hc * heads;
