@@ -250,7 +250,8 @@ void span_plan(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, bool wi
                int* heads);
 int launch_span(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream);
 // The 4-bit cache's part of both (hs_q4_decode.hip).
-void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, int cus, int* part, int* heads);
+void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
+                    int* heads);
 int launch_q4_decode(const SpanArgs& a, int D, hipStream_t stream);
 // fp16 and bf16 caches on the matrix cores (hs_window_decode.hip).
 bool window_decode_serves(int kv_dtype, int D);

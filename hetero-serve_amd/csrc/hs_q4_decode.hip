@@ -13,11 +13,12 @@
 // further up; less 1032 or 1152 they are k and 16 k, exactly, and the 16 is taken out of the
 // other operand.  (As masked, without the 1024, they are the subnormals n 2^-24, which the
 // matrix cores take, but they align sums by the operands' exponents: an accuracy of 2^-16 was
-// left.)  mid has two fp16 terms.  Query and probabilities are fp32 and go in as two fp16 terms, hi + lo with 22 bits: each head's query
-// times the power of two that brings its largest element to [2^14, 2^15), probabilities as
-// 2^7 p, at most 2^15 under the lazy raise of the maximum, and p_t s_tg times a power of two
-// R that follows the largest step (see kStepRoom).  Products of such terms are exact in the
-// fp32 accumulators.
+// left.)  Query and probabilities are fp32 and go in as two fp16 terms, hi + lo with 22 bits: each
+// head's query times the power of two that brings its largest element to [2^6, 2^7), so that 8
+// times a group's sum is below 2^15; probabilities as 2^7 p, at most 2^15 under the lazy raise
+// of the maximum, and p_t s_tg times a power of two R that follows the largest step (see
+// kStepRoom).  A key's mid is not made: mid Q is lo Q + s 8 Q, of halves as they are stored.  A
+// value's has two fp16 terms.  Products of such terms are exact in the fp32 accumulators.
 //
 // A wave serves up to 16 query heads of one KV head over one part of a row's visible keys,
 // 64 keys (a chunk) at a time:
@@ -29,9 +30,12 @@
 // Which key is which row of the first product is free; taking key 16 (j / 4) + 4 r + j % 4 for
 // row j of product r leaves each lane with the 16 probabilities of the keys that the
 // transposing read gives it.  They never leave the registers.
-// Steps and lowest values are loaded one key a lane, and go through LDS as s and mid.  Waves share
-// nothing, so there are no barriers.  Keys past the part's end are read as its last one and
-// count nothing: their scores are -inf, their s and mid 0.
+// Waves share nothing before their states are put together, so the walk has no barriers.  Keys
+// past the part's end are read as its last one and count nothing: their scores are -inf.
+//
+// 64 rows of 16..4096 keys, D 128, 32 / 8 heads, 168 MB, take 66 us, of 2048 each 48 (3.5 TB/s; the
+// loads alone 4.2), 16 rows of 8k..32k, 419 MB, 119.  The vector units' work on unpacked
+// numbers, splits and exponentials is what the loads wait for.
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
 #include "hs_q4.h"
@@ -55,8 +59,8 @@ typedef int int2x __attribute__((ext_vector_type(2)));
 
 constexpr int kChunk = 64;         // keys of a step
 constexpr float kLift = 7.0f;      // probabilities are held 2^kLift times larger
-// R is chosen so that the largest step so far times R lies in [2^-3, 2^-2), and again when
-// one times R passes 1 = 2^(kStepRoom - 2 + ...): p s R is at most 2^15 then.
+// R is chosen so that the largest step so far times R lies in [2^-3, 2^-2), and chosen again when a
+// step times R passes 1, for p s R is at most 2^15 up to there.
 constexpr int kStepRoom = 2;
 
 // What a wave keeps in LDS: its chunk's records as they were loaded, and of its values' steps
@@ -70,7 +74,7 @@ struct Chunk {
   alignas(16) uint8_t v[kChunk][(q4_record_bytes(D) + 7) / 8 * 8];   // (8-byte reads)
   alignas(16) _Float16 ks[G][kPar];
   alignas(16) _Float16 vs[G][kPar];
-  alignas(16) _Float16 vmid[2 * G][kPar];       // both terms, keys in unpack8's order
+  alignas(16) _Float16 vmid[2 * G][kPar];       // both terms, keys in Unpack's order
 };
 
 template <int N>
@@ -114,7 +118,7 @@ struct Unpack {
            half8{a, a, b, b, a, a, b, b};
   }
 };
-// The element of a word that half e of unpack8 is, and its place.
+// The element of a word that half e of Unpack's is, and its place.
 __device__ constexpr int half_element(int e) { return (e >> 1) + 4 * (e & 1); }
 __device__ inline int half_place(int i) { return 2 * (i & 3) + (i >> 2 & 1); }
 
@@ -189,8 +193,8 @@ __device__ inline _Float16 half_of(const Words<N>& x, int i) {
 // kByGroup: the 16 columns of the products are heads times groups, column j head j / G's sums
 // over group j % G alone: 16 / G heads a wave.  Otherwise they are 16 heads.  By group, a lane
 // scales its scores by one group's steps and adds the groups' up with its neighbours', and
-// makes the second product's operand for one group instead of all: 580 vector instructions a
-// chunk instead of 720 at D 128, but for a quarter of the heads.
+// makes the second product's operand for one group instead of all: 64 rows of 16..4096 keys, D 128,
+// 32 / 8 heads, took 91 us where 16 columns for 4 heads took 119.
 template <int D, bool kByGroup>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void q4_decode_kernel(SpanArgs a) {
   constexpr int G = D / kQ4Group, kPiece = D / 8, kT = D / 16;
@@ -512,10 +516,11 @@ void launch_dim(const SpanArgs& a, hipStream_t stream) {
 
 // us, D 128, 32 / 8 heads, heads side by side x keys of a part: 64 rows of 64..512 keys 4 x 512
 // 24, 2 x 512 17.9, 1 x 512 19.8; 1 of 512 1 x 512 10.2, 4 x 64 10.5; 8 of 1024..2048 4 x 128 15.9,
-// 2 x 256 16.7, 1 x 512 17.5; 64 of 16..4096 4 x 1024 71, 4 x 512 74, 2 x 1024 76; 16 of 8k..32k
-// 4 x 512 121, 4 x 1024 136, 1 x 1024 172; 1 of 4096 1 x 256 13.0, 4 x 64 15.2.
-void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, int cus, int* part, int* heads) {
-  plan(B, H, Hkv, heads_per_wave(H, Hkv, D), kChunk, most, 8, cus, part, heads);
+// 2 x 256 16.7, 1 x 512 17.5; 64 of 16..4096 2 x 512 63, 4 x 512 66, 1 x 1024 68; 16 of 8k..32k
+// 4 x 512 119, 2 x 1024 120, 4 x 1024 126; 1 of 4096 1 x 256 13.0, 4 x 64 15.2.
+void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
+                    int* heads) {
+  plan(B, H, Hkv, heads_per_wave(H, Hkv, D), kChunk, most, windowed, cus, part, heads);
 }
 
 // The parts' states or rows; the caller merges.

@@ -297,7 +297,7 @@ void launch_span_merge(const SpanArgs& a, int D, hipStream_t stream) {
 // each CU.
 void span_plan(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
                int* heads) {
-  if (kv_dtype < 0) return q4_decode_plan(B, H, Hkv, D, most, cus, part, heads);
+  if (kv_dtype < 0) return q4_decode_plan(B, H, Hkv, D, most, windowed, cus, part, heads);
   if (window_decode_serves(kv_dtype, D))
     return window_decode_plan(B, H, Hkv, most, windowed, cus, part, heads);
   *heads = 0;

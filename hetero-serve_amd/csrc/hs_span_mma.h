@@ -134,11 +134,15 @@ inline int64_t workgroups(const SpanArgs& a, int heads) {
 }
 
 // Short rows are whole: as many KV heads side by side as leave a workgroup for each CU, where
-// their steps are at most most_steps, or one head and four phases where there are too few for
+// their steps are at most eight, or one head and four phases where there are too few for
 // that and they take two steps.  Longer rows are cut into parts of eight chunks, shorter ones
 // (of two steps) and fewer heads side by side while the parts are fewer than the CUs.
-inline void plan(int B, int H, int Hkv, int heads, int chunk, int64_t most, int most_steps, int cus, int* part,
+// Rows behind a window are as long as each other, so more of them are whole.  us, parts / whole,
+// windows of 1024: over 64 rows of 32 / 8 heads, bf16, D 128 55 / 46, D 64 33 / 25, 4 bits, D 128
+// 30 / 28; 8 heads, bf16, D 32 23.5 / 19; 8 rows of 32 heads, bf16, D 128 35 / 27.5.
+inline void plan(int B, int H, int Hkv, int heads, int chunk, int64_t most, bool windowed, int cus, int* part,
                  int* side) {
+  const int most_steps = windowed ? 20 : 8;
   const int64_t n_hc = ceil_div(H / Hkv, heads);
   int wide = kWaves;
   while (Hkv % wide) wide /= 2;
