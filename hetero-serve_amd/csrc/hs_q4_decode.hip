@@ -217,8 +217,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
   }
   const int32_t* bt = a.bt + (int64_t)t.b * a.MB;
   const uint32_t tok = (uint32_t)a.Hkv * kRecord;
-  const uint8_t* kbase = a.k + t.kvh * kRecord;
-  const uint8_t* vbase = a.v + t.kvh * kRecord;
+  const uint8_t* kbase = a.k + (int64_t)t.kvh * kRecord;
+  const uint8_t* vbase = a.v + (int64_t)t.kvh * kRecord;
 
   // A chunk's records come in pieces of D / 8 bytes, 64 lanes neighbouring pieces, and go to
   // LDS through registers: a chunk's loads are on their way while the one before is computed,

@@ -45,8 +45,8 @@ __global__ __launch_bounds__(64 * kWaves) void span_walk_kernel(SpanArgs a) {
     return;
   }
   const int64_t row = (int64_t)a.Hkv * D * sizeof(T);
-  const uint8_t* kp = a.k + (h0 / (a.H / a.Hkv)) * D * (int)sizeof(T) + 16 * c;
-  const uint8_t* vp = a.v + (h0 / (a.H / a.Hkv)) * D * (int)sizeof(T) + 16 * c;
+  const uint8_t* kp = a.k + h0 / (a.H / a.Hkv) * (int64_t)(D * sizeof(T)) + 16 * c;
+  const uint8_t* vp = a.v + h0 / (a.H / a.Hkv) * (int64_t)(D * sizeof(T)) + 16 * c;
   const int32_t* bt = a.bt + (int64_t)b * a.MB;
 
   Span::Place ahead[kU];

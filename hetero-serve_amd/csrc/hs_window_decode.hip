@@ -125,8 +125,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_decode_kernel(SpanArgs 
   }
   const int32_t* bt = a.bt + (int64_t)t.b * a.MB;
   const uint32_t tok = (uint32_t)a.Hkv * D * 2;
-  const uint8_t* kbase = a.k + (t.kvh * D + lane % kLanes * 8) * 2;
-  const uint8_t* vbase = a.v + (t.kvh * D + lane % kLanes * 8) * 2;
+  const uint8_t* kbase = a.k + ((int64_t)t.kvh * D + lane % kLanes * 8) * 2;
+  const uint8_t* vbase = a.v + ((int64_t)t.kvh * D + lane % kLanes * 8) * 2;
 
   uint4 kr[kLoads], vr[kLoads];
   auto load = [&](int slot) {
