@@ -33,9 +33,10 @@
 // Waves share nothing before their states are put together, so the walk has no barriers.  Keys
 // past the part's end are read as its last one and count nothing: their scores are -inf.
 //
-// 64 rows of 16..4096 keys, D 128, 32 / 8 heads, 168 MB, take 66 us, of 2048 each 48 (3.5 TB/s; the
-// loads alone 4.2), 16 rows of 8k..32k, 419 MB, 119.  The vector units' work on unpacked
-// numbers, splits and exponentials is what the loads wait for.
+// Times, D 128, 32 / 8 heads: 64 rows of 16..4096 keys, 168 MB, 66 us, of 2048 each 50, of 8192
+// each, 671 MB, 163 (4.1 TB/s): without the arithmetic 152, without the loads 118.  16 rows of
+// 8k..32k, 419 MB, 119.  Loads two chunks ahead, three waves a SIMD and waves' priorities
+// gained nothing.
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
 #include "hs_q4.h"

@@ -136,7 +136,9 @@ inline int64_t workgroups(const SpanArgs& a, int heads) {
 // Short rows are whole: as many KV heads side by side as leave a workgroup for each CU, where
 // their steps are at most eight, or one head and four phases where there are too few for
 // that and they take two steps.  Longer rows are cut into parts of eight chunks, shorter ones
-// (of two steps) and fewer heads side by side while the parts are fewer than the CUs.
+// (of two steps) and fewer heads side by side while the parts are fewer than the CUs; of
+// sixteen where all waves are phases of one head and two workgroups a CU are left (64 rows of
+// 16..8192 keys, 4 bits, 16 heads over 1: 31 us, 33.5 of eight; 512 rows of 8192 168, 196).
 // Rows behind a window are as long as each other, so more of them are whole.  us, parts / whole,
 // windows of 1024: over 64 rows of 32 / 8 heads, bf16, D 128 55 / 46, D 64 33 / 25, 4 bits, D 128
 // 30 / 28; 8 heads, bf16, D 32 23.5 / 19; 8 rows of 32 heads, bf16, D 128 35 / 27.5.
@@ -156,8 +158,8 @@ inline void plan(int B, int H, int Hkv, int heads, int chunk, int64_t most, bool
     }
   }
   for (int hw = wide; hw >= 1; hw /= 2)
-    for (int len = 8 * chunk; len >= 2 * chunk * kWaves / hw; len /= 2)
-      if (wgs(hw, len) >= cus) {
+    for (int len = (hw == 1 ? 16 : 8) * chunk; len >= 2 * chunk * kWaves / hw; len /= 2)
+      if (wgs(hw, len) >= (len > 8 * chunk ? 2 : 1) * (int64_t)cus) {
         *part = len;
         *side = hw;
         return;
