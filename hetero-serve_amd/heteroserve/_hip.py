@@ -1055,12 +1055,20 @@ def _span_decode(L, query, call, head, q, k_cache, v_cache, NB, BS, Hkv, block_t
     if B == 0:
         return out
     MB = bt.shape[1]
+    sizes = (*head, B, H, Hkv, D, BS, MB, window, sinks)
+    key = (query.__name__, index, sizes)
+    ws_bytes = known = _WS_SIZES.get(key)
     with _DeviceGuard(index):
-        ws_bytes = _decode_workspace(query, index, *head, B, H, Hkv, D, BS, max(MB, 1), window, sinks)
+        if known is None:
+            ws_bytes = query(*sizes)
         ws = q.new_empty((ws_bytes + 3) // 4) if ws_bytes else None
         check(call(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *head, NB, bt.data_ptr(),
                    ctx.data_ptr(), out.data_ptr(), B, H, Hkv, D, BS, MB, float(scale), window, sinks,
                    None if ws is None else ws.data_ptr(), ws_bytes, _stream_at(index)))
+    if known is None:   # a size of 0 too, now that the call has not refused it
+        if len(_WS_SIZES) >= _WS_SIZES_MAX:
+            _WS_SIZES.clear()
+        _WS_SIZES[key] = ws_bytes
     return out
 
 
