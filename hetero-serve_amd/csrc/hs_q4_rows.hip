@@ -6,15 +6,16 @@
 // values beyond fp16's largest count as that; a group that holds a NaN is NaN as a whole (lo
 // is NaN, s 0).
 // A thread takes 8 elements, one word of a record, and 4 neighbouring threads a group,
-// which find its ends with two exchanges inside the quad.  The quotients are fp32
-// products with 1 / s, less than 2^-18 off; the few that come within 2^-16 of half
-// way between two numbers, and the steps that lie as near to a border between two fp16
-// numbers, are computed again in fp64.  So what is written is the definition's, to the bit,
-// and does not depend on the order or precision of this code.
+// which find its ends with two exchanges inside the quad (two words a thread: 20 us
+// instead of 17 for 8192 rows).  The quotients are fp32 products with 1 / s; the few that
+// come near half way between two numbers, and the steps that lie near a border between two
+// fp16 numbers, are computed again in fp64.  So what is written is the definition's, to the
+// bit, and does not depend on the order or precision of this code.
 //
-// Both kernels move each byte once.  8192 rows of 8 heads of 128, bf16, are written in 17 us (44 MB,
-// 2.6 TB/s; bound by the arithmetic of steps and quotients) and read in 10.5 (4.2 TB/s); prefixes
-// of 219 MB as fp16 are read in 40 us (5.5 TB/s, HBM).  A decode step's rows are bound by the launch.
+// Both kernels move each byte once.  8192 rows of 8 heads of 128, bf16, are written in 15 us (44 MB,
+// 2.9 TB/s; the arithmetic of steps and quotients is active in 70 % of the cycles) and read in
+// 8.5 to 9.5 (4.9 TB/s); prefixes of 219 MB are read in 33.5 us (6.5 TB/s, HBM).  (17.5, 10.2 and 39.5
+// with places and addresses for each thread.)  A decode step's rows are bound by the launch.
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
 #include "hs_q4.h"
@@ -26,6 +27,7 @@ namespace hs {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kUnit = 8;           // elements of a thread, of keys and of values: a word
 
 struct Q4Args {
   uint8_t *k_cache, *v_cache;
@@ -38,11 +40,10 @@ struct Q4Args {
   RowMap map;
 };
 
-// Row, record in the row and word in the record of the flat index i over rows of Hkv D / 8
-// words.  Shifts where the row's words are a power of 2: divisions are a third of these
-// kernels' instructions otherwise.
-__device__ inline void split_word(const Q4Args& a, int64_t i, int64_t& row, int& h, int& w) {
-  uint32_t in_row;
+// Row and word in the row of the flat index i over rows of Hkv D / 8 words.  Shifts where the
+// row's words are a power of 2: divisions are a third of these kernels' instructions
+// otherwise.
+__device__ inline void split_word(const Q4Args& a, int64_t i, int64_t& row, uint32_t& in_row) {
   if (a.row_shift >= 0) {   // uniform
     row = i >> a.row_shift;
     in_row = (uint32_t)i & ((1u << a.row_shift) - 1);
@@ -57,9 +58,29 @@ __device__ inline void split_word(const Q4Args& a, int64_t i, int64_t& row, int&
       in_row = (uint32_t)(i - row * per);
     }
   }
-  h = (int)(in_row >> a.head_shift);
-  w = (int)(in_row & ((1u << a.head_shift) - 1));
 }
+
+// What a thread takes: row, record in the row, word in the record.  kWaveRow: a row has a
+// multiple of 64 words, so a wave's threads are in one, and its place, its slot and their
+// addresses are scalar.
+struct Unit {
+  int64_t row;
+  int h, w;
+
+  // False past the last row.
+  template <bool kWaveRow>
+  __device__ bool find(const Q4Args& a) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t i = (int64_t)blockIdx.x * kThreads + 64 * wave + (kWaveRow ? 0 : lane);
+    if (i >= a.n * ((int64_t)a.Hkv << a.head_shift)) return false;
+    uint32_t in_row;
+    split_word(a, i, row, in_row);
+    if constexpr (kWaveRow) in_row += lane;
+    h = (int)(in_row >> a.head_shift);
+    w = (int)(in_row & ((1u << a.head_shift) - 1));
+    return true;
+  }
+};
 
 // RowMap's slot of row i, the page by a shift where BS is a power of 2.
 __device__ inline int64_t slot_of(const Q4Args& a, int64_t i) {
@@ -78,7 +99,7 @@ __device__ inline void load_elements(const uint8_t* p, float* x) {
     Codec<T>::load8(p, x);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = Codec<T>::load1(p + e * Codec<T>::kBytes);
+    for (int e = 0; e < kUnit; ++e) x[e] = Codec<T>::load1(p + e * Codec<T>::kBytes);
   }
 }
 
@@ -105,7 +126,7 @@ __device__ inline void write_word(const Q4Args& a, uint8_t* rec, int w, const fl
   const int G = a.D / kQ4Group;
   float hi = x[0], lo = x[0];
 #pragma unroll
-  for (int e = 1; e < 8; ++e) {
+  for (int e = 1; e < kUnit; ++e) {
     hi = nan_max(hi, x[e]);
     lo = nan_min(lo, x[e]);
   }
@@ -114,31 +135,32 @@ __device__ inline void write_word(const Q4Args& a, uint8_t* rec, int w, const fl
   hi = nan_max(hi, dpp<kDppQuadXor2>(hi));
   lo = nan_min(lo, dpp<kDppQuadXor2>(lo));
   const bool none = hi != hi;
-  hi = fminf(fmaxf(hi, -kF16Most), kF16Most);
-  const _Float16 lo16 = (_Float16)fminf(fmaxf(lo, -kF16Most), kF16Most);
+  const float most = fminf(fmaxf(hi, -kF16Most), kF16Most), least = fminf(fmaxf(lo, -kF16Most), kF16Most);
+  const _Float16 lo16 = (_Float16)least;
   const float base = (float)lo16;
-  const _Float16 s16 = none ? (_Float16)0.0f : q4_step(hi, base);
+  const _Float16 s16 = none ? (_Float16)0.0f : q4_step(most, base);
   const float s = (float)s16, inv = __builtin_amdgcn_rcpf(s);
-  // Adding 1.5 2^23 rounds to a whole number and leaves it in the low bits, the rest of
-  // which are taken off at the end.
+  // The fp32 quotient is off by less than 2^-21 of it, so where both ends of twice that
+  // range round to one number, that is the one.  Adding 1.5 2^23 rounds to a whole number
+  // and leaves it in the low bits, the rest of which are taken off at the end.
   constexpr float kWhole = 12582912.0f;
   constexpr uint32_t kBits = 0x4b400000u * 0x11111111u;   // those of kWhole, every 4 bits
-  float t[8], near = 0.5f;           // to half way
-  uint32_t word = 0;
+  const float inv_a = inv * (1.0f + 0x1p-20f), inv_b = inv * (1.0f - 0x1p-20f);
+  uint32_t word = 0, other = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    t[e] = __builtin_amdgcn_fmed3f((x[e] - base) * inv, 0.0f, 15.0f);
-    word += __float_as_uint(t[e] + kWhole) << (4 * e);
+  for (int e = 0; e < kUnit; ++e) {
+    const float d = x[e] - base;
+    word += __float_as_uint(fmaf(d, inv_a, kWhole)) << (4 * e);
+    other += __float_as_uint(fmaf(d, inv_b, kWhole)) << (4 * e);
   }
+  // No quotient lies below -0.48 or above 15.3: lo is near its fp16 number, the step far enough
+  // above fp16's smallest (2^-24 apart) to have 6 bits, and no element counts as another.
+  const bool inside = hi == most && lo == least && 2.1f * (base - lo) < s && s >= 0x1p-19f;
   word -= kBits;
-#pragma unroll
-  for (int e = 0; e < 8; e += 2)
-    near = fminf(near, fminf(fabsf(__builtin_amdgcn_fractf(t[e]) - 0.5f),
-                             fabsf(__builtin_amdgcn_fractf(t[e + 1]) - 0.5f)));
-  if (near < 0x1p-16f) {
+  if (s > 0.0f && !(inside && word + kBits == other)) {
     word = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < kUnit; ++e) {
       const double q = rint(((double)x[e] - (double)base) / (double)s);
       word |= (uint32_t)(q < 0.0 ? 0.0 : q > 15.0 ? 15.0 : q) << (4 * e);
     }
@@ -156,22 +178,20 @@ __device__ inline void write_word(const Q4Args& a, uint8_t* rec, int w, const fl
 }
 
 // A thread: one word of a key's record and the value's, whose slot is the same.
-template <typename T, bool kVec>
+template <typename T, bool kVec, bool kWaveRow>
 __global__ __launch_bounds__(kThreads) void q4_append_kernel(Q4Args a) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= a.n * ((int64_t)a.Hkv * (a.D / 8))) return;
-  int64_t row;
-  int h, w;
-  split_word(a, i, row, h, w);
-  const int64_t e = ((int64_t)h * a.D + 8 * w) * Codec<T>::kBytes;
-  float k[8], v[8];                  // on their way while the slot is looked up
-  load_elements<T, kVec>(a.k_src + row * a.k_row + e, k);
-  load_elements<T, kVec>(a.v_src + row * a.v_row + e, v);
-  const int64_t slot = slot_of(a, row);
+  Unit u;
+  if (!u.find<kWaveRow>(a)) return;
+  const uint32_t e = ((uint32_t)u.h * a.D + kUnit * u.w) * Codec<T>::kBytes;
+  float k[kUnit], v[kUnit];          // on their way while the slot is looked up
+  load_elements<T, kVec>(a.k_src + u.row * a.k_row + e, k);
+  load_elements<T, kVec>(a.v_src + u.row * a.v_row + e, v);
+  const int64_t slot = slot_of(a, u.row);
   if (slot < 0) return;              // all four threads of a group
-  const int64_t rec = (slot * a.Hkv + h) * q4_record_bytes(a.D);
-  write_word<true>(a, a.k_cache + rec, w, k);
-  write_word<false>(a, a.v_cache + rec, w, v);
+  const uint32_t R = q4_record_bytes(a.D), rec = u.h * R;
+  const int64_t at = slot * (a.Hkv * R);
+  write_word<true>(a, a.k_cache + at + rec, u.w, k);
+  write_word<false>(a, a.v_cache + at + rec, u.w, v);
 }
 
 // The values of 8 elements, not read again by this kernel or kept for it.
@@ -189,38 +209,48 @@ __device__ inline void store8_stream(uint8_t* p, const float* x) {
   }
 }
 
-template <typename T>
+template <typename T, bool kWaveRow>
 __global__ __launch_bounds__(kThreads) void q4_read_kernel(Q4Args a) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= a.n * ((int64_t)a.Hkv * (a.D / 8))) return;
-  int64_t row;
-  int h, w;
-  split_word(a, i, row, h, w);
+  Unit u;
+  if (!u.find<kWaveRow>(a)) return;
   const int G = a.D / kQ4Group;
-  const int64_t slot = slot_of(a, row);
+  const int64_t slot = slot_of(a, u.row);
   float x[2][8] = {};
   if (slot >= 0) {
-    const int64_t at = (slot * a.Hkv + h) * q4_record_bytes(a.D);
+    const uint32_t R = q4_record_bytes(a.D), in_row = u.h * R;
+    const int64_t at = slot * (a.Hkv * R);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const uint8_t* rec = (c == 0 ? a.k_cache : a.v_cache) + at;
-      const int place = c == 0 ? q4_word<true>(w, G) : q4_word<false>(w, G);
+      const uint8_t* rec = (c == 0 ? a.k_cache : a.v_cache) + at + in_row;
+      const int place = c == 0 ? q4_word<true>(u.w, G) : q4_word<false>(u.w, G);
       const uint32_t word = *reinterpret_cast<const uint32_t*>(rec + 4 * place);
-      const _Float16* par = reinterpret_cast<const _Float16*>(rec + a.D / 2) + (w >> 2);
+      const _Float16* par = reinterpret_cast<const _Float16*>(rec + a.D / 2) + (u.w >> 2);
       const float s = (float)par[0], lo = (float)par[G];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[c][e] = fmaf((float)((word >> (4 * e)) & 15u), s, lo);
     }
   }
-  const int64_t to = ((row * a.Hkv + h) * (int64_t)a.D + 8 * w) * Codec<T>::kBytes;
-  store8_stream<T>(a.k_out + to, x[0]);
-  store8_stream<T>(a.v_out + to, x[1]);
+  const int64_t to = u.row * ((int64_t)a.Hkv * a.D * Codec<T>::kBytes);
+  const uint32_t e = ((uint32_t)u.h * a.D + kUnit * u.w) * Codec<T>::kBytes;
+  store8_stream<T>(a.k_out + to + e, x[0]);
+  store8_stream<T>(a.v_out + to + e, x[1]);
 }
+
+bool wave_rows(const Q4Args& a) { return ((int64_t)a.Hkv << a.head_shift) % 64 == 0; }
 
 template <typename T>
 void launch_append_type(const Q4Args& a, dim3 grid, bool vec, hipStream_t stream) {
-  if (vec) hipLaunchKernelGGL((q4_append_kernel<T, true>), grid, dim3(kThreads), 0, stream, a);
-  else hipLaunchKernelGGL((q4_append_kernel<T, false>), grid, dim3(kThreads), 0, stream, a);
+  const dim3 block(kThreads);
+  if (!vec) hipLaunchKernelGGL((q4_append_kernel<T, false, false>), grid, block, 0, stream, a);
+  else if (wave_rows(a)) hipLaunchKernelGGL((q4_append_kernel<T, true, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((q4_append_kernel<T, true, false>), grid, block, 0, stream, a);
+}
+
+template <typename T>
+void launch_read_type(const Q4Args& a, dim3 grid, hipStream_t stream) {
+  const dim3 block(kThreads);
+  if (wave_rows(a)) hipLaunchKernelGGL((q4_read_kernel<T, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((q4_read_kernel<T, false>), grid, block, 0, stream, a);
 }
 
 Q4Args rows_args(const Q4Rows& w) {
@@ -231,8 +261,8 @@ Q4Args rows_args(const Q4Rows& w) {
   a.Hkv = w.Hkv;
   a.D = w.D;
   auto shift = [](int64_t x) { return x > 0 && (x & (x - 1)) == 0 && x < 1 << 30 ? __builtin_ctzll(x) : -1; };
-  a.head_shift = shift(w.D / 8);
-  a.row_shift = shift((int64_t)w.Hkv * (w.D / 8));
+  a.head_shift = shift(w.D / kUnit);
+  a.row_shift = shift((int64_t)w.Hkv * (w.D / kUnit));
   a.bs_shift = shift(w.BS);
   a.map.bt = w.bt;
   a.map.positions = w.positions;
@@ -247,8 +277,8 @@ Q4Args rows_args(const Q4Rows& w) {
 
 // The grid over n rows' words, or false where no launch or offset holds it.
 bool rows_grid(const Q4Rows& w, int64_t row_bytes, dim3& grid) {
-  const int64_t words = sat_mul(w.n, sat_mul(w.Hkv, w.D / 8)), wgs = ceil_div(words, kThreads);
-  if (sat_mul(w.Hkv, w.D) > 0x7fffffffLL || !grid_fits(wgs, kThreads) || wgs > 0x7fffffffLL ||
+  const int64_t words = sat_mul(w.n, sat_mul(w.Hkv, w.D / kUnit)), wgs = ceil_div(words, kThreads);
+  if (sat_mul(w.Hkv, w.D) > 1 << 29 || !grid_fits(wgs, kThreads) || wgs > 0x7fffffffLL ||
       sat_mul(w.n, row_bytes) == INT64_MAX ||
       sat_mul((int64_t)w.NB * w.BS, sat_mul(w.Hkv, q4_record_bytes(w.D))) == INT64_MAX)
     return false;
@@ -287,12 +317,9 @@ int launch_q4_read(const Q4Rows& w, hipStream_t stream) {
   if (!rows_grid(w, sat_mul(w.Hkv, w.D, dtype_bytes(w.dtype)), grid))
     return fail(HS_EUNSUPPORTED, "4-bit read too large for one launch");
   profile_begin(stream);
-  if (w.dtype == HS_DTYPE_F32)
-    hipLaunchKernelGGL((q4_read_kernel<float>), grid, dim3(kThreads), 0, stream, a);
-  else if (w.dtype == HS_DTYPE_F16)
-    hipLaunchKernelGGL((q4_read_kernel<_Float16>), grid, dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((q4_read_kernel<Bf16>), grid, dim3(kThreads), 0, stream, a);
+  if (w.dtype == HS_DTYPE_F32) launch_read_type<float>(a, grid, stream);
+  else if (w.dtype == HS_DTYPE_F16) launch_read_type<_Float16>(a, grid, stream);
+  else launch_read_type<Bf16>(a, grid, stream);
   profile_end(stream);
   return check_launch("4-bit KV read");
 }

@@ -376,6 +376,35 @@ def test_small_and_odd_arguments():
             call(q, *args, bt[:, :0], ctx, 0.1, 7, 2)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,D", [(16, 32), (8, 64), (12, 128), (6, 256), (3, 128), (5, 64)])
+def test_rows_of_whole_waves_and_others(dtype, heads, D):
+    """Rows of 64 and 192 words, whose place is a wave's, and of 48 and 40, to the byte; some
+    of them name no slot."""
+    from heteroserve.kv import quant
+
+    gen = torch.Generator(DEV).manual_seed(D)
+    n, NB, page = 75, 7, 13
+    k, v = (torch.randn(n, heads, D, generator=gen, device=DEV).to(dtype) for _ in range(2))
+    bt = torch.tensor([[3, 0, 6], [5, 2, -1]], dtype=torch.int32)
+    seq, at = np.arange(n) % 2, np.arange(n) // 2
+    seq[10], at[20] = 7, 3 * page
+    pool = quant.empty_pool_q4(1, NB, page, heads, D, device=DEV).fill_(0x5a)
+    want = pool.cpu().numpy()
+    quant.append_kv_q4(pool[0, 0], pool[0, 1], bt, torch.tensor(at), k, v, seq_ids=torch.tensor(seq))
+    named = np.array([s < 2 and p < 3 * page and bt[s, p // page] >= 0 for s, p in zip(seq, at)])
+    assert 2 < (~named).sum() < n // 2
+    for i, x in enumerate((k, v)):
+        rec = lc.records(*lc.quantise(_np(x)), keys=i == 0)
+        want[0, i][bt.numpy()[seq[named], at[named] // page], at[named] % page] = rec[named]
+    assert np.array_equal(pool.cpu().numpy(), want)
+    got = quant.read_kv_q4(pool[0, 0], pool[0, 1], bt, torch.tensor(at), seq_ids=torch.tensor(seq), dtype=dtype)
+    for i, x in enumerate(got):
+        held = np.zeros((n, heads, D))
+        held[named] = lc.values(want[0, i][bt.numpy()[seq[named], at[named] // page], at[named] % page], i == 0)
+        assert torch.equal(x.cpu(), torch.tensor(held).to(F32).to(dtype))
+
+
 @pytest.mark.parametrize("B", [1, 2, 3, 8, 9, 16, 24, 30])
 def test_batches_of_every_count(B):
     """Rows and parts are dealt to the chip in an order that depends on their number."""
