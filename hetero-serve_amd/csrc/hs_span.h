@@ -41,12 +41,18 @@ struct Span {
     n = sinks + len - first;
     skip = first - sinks;
   }
-  // Keys [lo, hi) of part p; nparts parts in all.
-  __device__ bool part(const SpanArgs& a, int p, int& lo, int& hi, int& nparts) const {
-    nparts = (int)(((int64_t)n + a.part - 1) / a.part);
-    if (p >= nparts) return false;
+  __device__ int parts(const SpanArgs& a) const {
+    return (int)(((uint32_t)n + (uint32_t)a.part - 1) / (uint32_t)a.part);
+  }
+  // Keys [lo, hi) of part p, nparts parts in all; p is counted so that every row's last part is
+  // P - 1, and becomes its number in the row.  Work that begins with the lowest p begins with
+  // whole parts and ends with the rows' last ones, which are shorter.
+  __device__ bool part(const SpanArgs& a, int& p, int& lo, int& hi, int& nparts) const {
+    nparts = parts(a);
+    p -= a.P - nparts;
+    if (p < 0) return false;
     lo = p * a.part;
-    hi = min((int64_t)lo + a.part, (int64_t)n);
+    hi = min(lo + a.part, n);
     return true;
   }
   // Where key i < n lies: its page's table entry and its place in the page.

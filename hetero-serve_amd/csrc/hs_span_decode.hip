@@ -35,12 +35,13 @@ __global__ __launch_bounds__(64 * kWaves) void span_walk_kernel(SpanArgs a) {
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t n_hw = a.H / G, rp = blockIdx.x / n_hw;
   const int h0 = (int)(blockIdx.x - rp * n_hw) * G;
-  const int b = (int)(rp / (uint32_t)a.P), p = (int)(rp % (uint32_t)a.P);
+  const int b = (int)(rp / (uint32_t)a.P);
+  int p = (int)(rp % (uint32_t)a.P);
   const Span span(a, b);
   const int64_t o0 = ((int64_t)b * a.H + h0) * D;
   int lo, hi, nparts;
   if (!span.part(a, p, lo, hi, nparts)) {   // all of the workgroup
-    if (span.n == 0 && p == 0)       // nothing to attend to: zero rows
+    if (span.n == 0 && p == -a.P)    // nothing to attend to: zero rows
       for (int d = threadIdx.x; d < G * D; d += 64 * kWaves) a.out[o0 + d] = 0.0f;
     return;
   }
@@ -189,8 +190,8 @@ __global__ __launch_bounds__(64 * kWaves) void span_merge_kernel(SpanArgs a) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int64_t w = blockIdx.x;
   const Span span(a, (int)(w / a.H));
-  int lo, hi, n;
-  if (!span.part(a, 0, lo, hi, n) || n == 1) return;   // written already
+  const int n = span.parts(a);
+  if (n <= 1) return;   // written already
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + w * a.P;
   const int each = (n + kWaves - 1) / kWaves, first = min(n, wv * each), end = min(n, first + each);
   float mm = kLowest;

@@ -59,8 +59,7 @@ struct Task {
     const uint32_t turn = blockIdx.x / kXcds, rp = turn / (uint32_t)units * kXcds + blockIdx.x % kXcds;
     if (rp >= (uint64_t)a.B * a.P) return false;
     const int unit = turn % (uint32_t)units;
-    // First parts first, for rows of several lengths end at several parts; and a row's parts on
-    // every XCD in turn.
+    // Parts of all rows next to each other, and a row's parts on every XCD in turn.
     const uint32_t B = a.B;
     p = rp / B;
     b = (rp - p * B + (B % 2 == 0 ? p : 0)) % B;

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_decode_kernel(SpanArgs 
   const Span span(a, t.b);
   int lo, hi, nparts;
   if (!span.part(a, t.p, lo, hi, nparts)) {   // all of the workgroup
-    if (span.n == 0 && t.p == 0) zero_rows<D>(a, t);
+    if (span.n == 0 && t.p == -a.P) zero_rows<D>(a, t);
     return;
   }
   const int32_t* bt = a.bt + (int64_t)t.b * a.MB;
