@@ -1095,8 +1095,9 @@ static int check_span_sizes(int kv_dtype, int B, int H, int Hkv, int D, int BS, 
 static int64_t plan_span(SpanArgs& a, int kv_dtype, int D, int64_t* ml) {
   const int64_t most = span_most(a.MB, a.BS, a.window, a.sinks);
   span_plan(kv_dtype, a.B, a.H, a.Hkv, D, most, most < (int64_t)a.MB * a.BS, current_cus(), &a.part,
-            &a.heads);
+            &a.heads, &a.room);
   a.P = (int)ceil_div(most, a.part);
+  if (a.B > kSpanDealt || sat_mul(a.B, a.P) <= a.room) a.room = 0;   // nothing to fit
   return span_state_bytes(a.B, a.H, D, a.P, ml);
 }
 
@@ -1159,6 +1160,7 @@ static int span_decode(const float* q, const void* k_cache, const void* v_cache,
   if (need > 0 && !aligned16(workspace)) return fail(HS_EINVAL, "workspace must be 16-byte aligned");
   a.part_acc = static_cast<float*>(workspace);
   a.part_ml = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) + ml) : nullptr;
+  a.fitted = need ? reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + need - 16) : nullptr;
   return launch_span(a, kv_dtype, D, static_cast<hipStream_t>(stream));
 }
 

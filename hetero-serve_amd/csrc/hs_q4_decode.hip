@@ -33,10 +33,10 @@
 // Waves share nothing before their states are put together, so the walk has no barriers.  Keys
 // past the part's end are read as its last one and count nothing: their scores are -inf.
 //
-// Times, D 128, 32 / 8 heads: 64 rows of 16..4096 keys, 168 MB, 66 us, of 2048 each 50, of 8192
-// each, 671 MB, 163 (4.1 TB/s): without the arithmetic 152, without the loads 118.  16 rows of
-// 8k..32k, 419 MB, 119.  Loads two chunks ahead, three waves a SIMD and waves' priorities
-// gained nothing.
+// Times, D 128, 32 / 8 heads: 64 rows of 16..4096 keys, 168 MB, 56 us, of 2048 each 49, of 8192
+// each, 671 MB, 157 (4.3 TB/s; with parts of 512 keys 163, 152 of it without the arithmetic, 118
+// without the loads).  16 rows of 8k..32k, 419 MB, 103.  Loads two chunks ahead, three waves
+// a SIMD and waves' priorities gained nothing.
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
 #include "hs_q4.h"
@@ -207,12 +207,12 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
   static_assert(kHeads * (D + 4) * 4 <= (int)sizeof(Chunk<D>), "a wave's outputs fit");
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   Task t;
-  if (!t.find(a, kHeads)) return;
+  if (!t.find(a, kHeads, kChunk)) return;
   Chunk<D>& w = chunks[t.wv];
   const int jh = kByGroup ? j / G : j, jg = kByGroup ? j % G : 0;   // this column's head, group
   const Span span(a, t.b);
   int lo, hi, nparts;
-  if (!span.part(a, t.p, lo, hi, nparts)) {   // all of the workgroup
+  if (!span.part(a, t.part, t.p, lo, hi, nparts)) {   // all of the workgroup
     if (span.n == 0 && t.p == -a.P) zero_rows<D>(a, t);
     return;
   }
@@ -423,7 +423,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
 #pragma unroll
       for (int d = 0; d < kT; ++d) o[d] *= keep;
     }
-    // 2^kLift p; its terms against the mids, and against ones (the sum)
+    // 2^kLift p; its terms against the mids, and against ones (the sum).  Chunks are added by the
+    // vector units, which round to the nearest: the matrix cores cut off, which adds up in
+    // sums of one sign (parts of 128 chunks: 8e-6 of the row instead of 2e-6).
+    float4x z = {0.0f, 0.0f, 0.0f, 0.0f}, zl = z;
     const float mb = m - kLift;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -443,13 +446,15 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
       const half8 one = (_Float16)1.0f;
       half8 mid = one;
       if (j < 2 * G) mid = *reinterpret_cast<const half8*>(&w.vmid[j & (2 * G - 1)][16 * g + 8 * t]);
-      oz = mma(mid, p1, oz);
-      oz = mma(mid, p2, oz);
+      z = mma(mid, p1, z);
+      z = mma(mid, p2, z);
       if constexpr (G == 8) {      // no row is left
-        ones = mma(one, p1, ones);
-        ones = mma(one, p2, ones);
+        zl = mma(one, p1, zl);
+        zl = mma(one, p2, zl);
       }
     }
+    oz += z;
+    ones += zl;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -515,13 +520,16 @@ void launch_dim(const SpanArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// us, D 128, 32 / 8 heads, heads side by side x keys of a part: 64 rows of 64..512 keys 4 x 512
+// us, D 128, 32 / 8 heads, heads side by side x keys of a part (as planned, before they are
+// fitted): 64 rows of 64..512 keys 4 x 512
 // 24, 2 x 512 17.9, 1 x 512 19.8; 1 of 512 1 x 512 10.2, 4 x 64 10.5; 8 of 1024..2048 4 x 128 15.9,
 // 2 x 256 16.7, 1 x 512 17.5; 64 of 16..4096 2 x 512 63, 4 x 512 66, 1 x 1024 68; 16 of 8k..32k
 // 4 x 512 119, 2 x 1024 120, 4 x 1024 126; 1 of 4096 1 x 256 13.0, 4 x 64 15.2.
 void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
-                    int* heads) {
-  plan(B, H, Hkv, heads_per_wave(H, Hkv, D), kChunk, most, windowed, cus, part, heads);
+                    int* heads, int* room) {
+  const int hpw = heads_per_wave(H, Hkv, D);
+  plan(B, H, Hkv, hpw, kChunk, most, windowed, cus, part, heads);
+  *room = parts_on_chip(B, H, Hkv, hpw, *heads, cus * (D == 256 ? 1 : D == 128 ? 2 : 3));
 }
 
 // The parts' states or rows; the caller merges.

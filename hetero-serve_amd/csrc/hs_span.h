@@ -13,6 +13,8 @@
 
 namespace hs {
 
+constexpr int kSpanDealt = 256;   // rows at most whose parts are fitted and dealt by their number
+
 struct SpanArgs {
   const float* q;             // [B, H, D]
   const uint8_t *k, *v;       // [NB, BS, Hkv, row of one head]
@@ -24,7 +26,9 @@ struct SpanArgs {
   int B, H, Hkv, BS, MB, NB;
   int bs_shift;               // log2(BS), or -1
   int window, sinks;          // window 0: all keys
-  int part, P;                // keys of a part, parts of the longest row
+  int part, P;                // keys of a part at least, parts of the longest row at most
+  int room;                   // parts in all that their length is fitted to, or 0
+  int32_t* fitted;            // the parts' keys then
   int heads;                  // 4-bit cache: KV heads of a workgroup
   float qscale;               // scale * log2(e)
 };
@@ -41,18 +45,18 @@ struct Span {
     n = sinks + len - first;
     skip = first - sinks;
   }
-  __device__ int parts(const SpanArgs& a) const {
-    return (int)(((uint32_t)n + (uint32_t)a.part - 1) / (uint32_t)a.part);
+  __device__ int parts(int part) const {
+    return (int)(((uint32_t)n + (uint32_t)part - 1) / (uint32_t)part);
   }
   // Keys [lo, hi) of part p, nparts parts in all; p is counted so that every row's last part is
   // P - 1, and becomes its number in the row.  Work that begins with the lowest p begins with
   // whole parts and ends with the rows' last ones, which are shorter.
-  __device__ bool part(const SpanArgs& a, int& p, int& lo, int& hi, int& nparts) const {
-    nparts = parts(a);
+  __device__ bool part(const SpanArgs& a, int part, int& p, int& lo, int& hi, int& nparts) const {
+    nparts = parts(part);
     p -= a.P - nparts;
     if (p < 0) return false;
-    lo = p * a.part;
-    hi = min(lo + a.part, n);
+    lo = p * part;
+    hi = n - lo < part ? n : lo + part;
     return true;
   }
   // Where key i < n lies: its page's table entry and its place in the page.
@@ -82,12 +86,13 @@ inline int64_t span_most(int64_t MB, int64_t BS, int window, int sinks) {
   return window ? std::min(cap, (int64_t)window + sinks) : cap;
 }
 
-// Bytes of P parts' states, and where the (max, sum) pairs begin; INT64_MAX when too large.
+// Bytes of P parts' states, and where the (max, sum) pairs begin (16 bytes for the fitted length
+// lie last); INT64_MAX when too large.
 inline int64_t span_state_bytes(int B, int H, int D, int64_t P, int64_t* ml) {
   if (P <= 1) return 0;
   const int64_t rows = sat_mul(B, H, P), acc = sat_mul(rows, D * 4);
   if (ml) *ml = acc;
-  return sat_add(acc, sat_mul(rows, 8));
+  return sat_add(sat_add(acc, sat_mul(rows, 8)), 16);
 }
 
 void launch_span_merge(const SpanArgs& a, int D, hipStream_t stream);

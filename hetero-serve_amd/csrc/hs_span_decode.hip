@@ -40,7 +40,7 @@ __global__ __launch_bounds__(64 * kWaves) void span_walk_kernel(SpanArgs a) {
   const Span span(a, b);
   const int64_t o0 = ((int64_t)b * a.H + h0) * D;
   int lo, hi, nparts;
-  if (!span.part(a, p, lo, hi, nparts)) {   // all of the workgroup
+  if (!span.part(a, a.part, p, lo, hi, nparts)) {   // all of the workgroup
     if (span.n == 0 && p == -a.P)    // nothing to attend to: zero rows
       for (int d = threadIdx.x; d < G * D; d += 64 * kWaves) a.out[o0 + d] = 0.0f;
     return;
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(64 * kWaves) void span_merge_kernel(SpanArgs a) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int64_t w = blockIdx.x;
   const Span span(a, (int)(w / a.H));
-  const int n = span.parts(a);
+  const int n = span.parts(a.room ? *a.fitted : a.part);
   if (n <= 1) return;   // written already
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + w * a.P;
   const int each = (n + kWaves - 1) / kWaves, first = min(n, wv * each), end = min(n, first + each);
@@ -297,11 +297,11 @@ void launch_span_merge(const SpanArgs& a, int D, hipStream_t stream) {
 // otherwise parts of 2048 keys, cut down to 256 while the workgroups are fewer than two for
 // each CU.
 void span_plan(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
-               int* heads) {
-  if (kv_dtype < 0) return q4_decode_plan(B, H, Hkv, D, most, windowed, cus, part, heads);
+               int* heads, int* room) {
+  if (kv_dtype < 0) return q4_decode_plan(B, H, Hkv, D, most, windowed, cus, part, heads, room);
   if (window_decode_serves(kv_dtype, D))
-    return window_decode_plan(B, H, Hkv, most, windowed, cus, part, heads);
-  *heads = 0;
+    return window_decode_plan(B, H, Hkv, D, most, windowed, cus, part, heads, room);
+  *heads = *room = 0;
   const int64_t wgs = sat_mul(B, H / row_attn_heads_per_wave(H, Hkv));
   int len = 2048;
   while (len > 256 && sat_mul(wgs, ceil_div(most, len)) < 2 * (int64_t)cus) len /= 2;

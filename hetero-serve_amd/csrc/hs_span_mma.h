@@ -16,6 +16,8 @@ typedef float float4x __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;          // of a workgroup
 constexpr int kXcds = 8;           // workgroups are dealt to them in turn
 constexpr int kSlots = 16;         // columns of the products
+constexpr int kDealt = kSpanDealt / 64;   // rows of a lane
+constexpr int kLongest = 32;       // steps of a fitted part: what the matrix cores cut off adds up
 constexpr float kSlack = 8.0f;     // lazy raise of the running max, log2 units
 // Where running maxima start: no finite score lies below, so a row of one is never empty.
 constexpr float kLowest = -0x1.fffffep127f;
@@ -41,14 +43,100 @@ __device__ inline void lds_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// The sum of x over lanes up to this one.
+__device__ inline int sum_up_to(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // from 1, 2, 4, 8 lanes below
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // lane 15 of a row to the next row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // lane 31 to rows 2 and 3
+  return x;
+}
+
 // A wave's task.  `heads` query heads of a KV head a wave.
 struct Task {
   int wv, hw, np, hsub, ph;   // wave; heads side by side, phases; this wave's
-  int b, p, kvh, h0, gc;      // row, part; KV head, first query head, how many
+  int part, b, p, kvh, h0, gc;   // keys of a part; row, part; KV head, first query head, how many
   int64_t row0;               // head h0 of row b, of [B, H]
 
-  // False: nothing there, for all of the workgroup.
-  __device__ bool find(const SpanArgs& a, int heads) {
+  // Part x of a call whose parts are fitted to the chip: they have the fewest steps, and those of
+  // a.part at least, with which they are a.room at most, or kLongest.  Whole parts come first, then the
+  // rows' last ones that are not whole, then the rows without keys: XCDs, to which
+  // workgroups go in turn, have as many as each other, and long parts do not begin late.
+  // Every wave finds all this by itself, in less than 1 us (which batches whose parts are few
+  // anyway do not pay).  us, parts of 512 keys / fitted, D 128, 32 / 8 heads, 4 bits: 64 rows of
+  // 16..4096 keys 62 / 56, of 16..8192 97 / 88, of 8192 each 163 / 157, 16 of 8k..32k 117 / 103; 64 of
+  // 500..4000, D 256, 85 / 61; over bf16, 64 of 64..4096 110 / 101.
+  __device__ bool fit(const SpanArgs& a, uint32_t x, int step) {
+    const int lane = threadIdx.x & 63;
+    int n[kDealt];                   // keys of row 64 r + lane; none behind the last row
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kDealt; ++r) {
+      n[r] = -1;
+      if (64 * r >= a.B) continue;   // uniform
+      n[r] = Span(a, min(64 * r + lane, a.B - 1)).n;
+      if (64 * r + lane >= a.B) n[r] = -1;
+      sum += (float)max(n[r], 0);
+    }
+    auto parts_of = [&](int keys) {
+      int count = 0;
+#pragma unroll
+      for (int r = 0; r < kDealt; ++r)
+        if (64 * r < a.B) count += ((uint32_t)max(n[r], 0) + (uint32_t)keys - 1) / (uint32_t)keys;
+      return __builtin_amdgcn_readlane(sum_up_to(count), 63);
+    };
+    part = a.part;
+    if (parts_of(part) > a.room) {
+      sum = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(group_sum<64>(sum))));
+      int steps = max(part / step, (int)(sum / ((float)step * (float)a.room)));
+      for (;;) {
+        steps = min(steps, kLongest);
+        part = steps * step;
+        if (steps == kLongest || parts_of(part) <= a.room) break;
+        steps += max(1, steps / 16);
+      }
+    }
+    if (x == 0 && threadIdx.x == 0) *a.fitted = part;
+
+    int whole[kDealt], left = x;
+#pragma unroll
+    for (int r = 0; r < kDealt; ++r) {
+      whole[r] = 0;
+      if (64 * r >= a.B) continue;
+      whole[r] = (uint32_t)max(n[r], 0) / (uint32_t)part;
+      const int up_to = sum_up_to(whole[r]), all = __builtin_amdgcn_readlane(up_to, 63);
+      if (left < all) {              // uniform
+        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(up_to > left));
+        const int mine = __builtin_amdgcn_readlane(whole[r], l), keys = __builtin_amdgcn_readlane(n[r], l);
+        b = 64 * r + l;
+        p = left - (__builtin_amdgcn_readlane(up_to, l) - mine) + a.P - mine - (keys > mine * part);
+        return true;
+      }
+      left -= all;
+    }
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind)
+#pragma unroll
+      for (int r = 0; r < kDealt; ++r) {
+        const bool is = kind == 0 ? n[r] > whole[r] * part : n[r] == 0;
+        const uint64_t rows = __builtin_amdgcn_ballot_w64(is);
+        const int all = __builtin_popcountll(rows);
+        if (left < all) {
+          const int below = __builtin_amdgcn_mbcnt_hi(rows >> 32, __builtin_amdgcn_mbcnt_lo((uint32_t)rows, 0));
+          const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(is && below == left));
+          b = 64 * r + l;
+          p = kind == 0 ? a.P - 1 : 0;
+          return true;
+        }
+        left -= all;
+      }
+    return false;
+  }
+
+  // False: nothing there, for all of the workgroup.  p as Span::part counts.
+  __device__ bool find(const SpanArgs& a, int heads, int chunk) {
     wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     hw = a.heads;
     np = kWaves / hw;
@@ -59,10 +147,15 @@ struct Task {
     const uint32_t turn = blockIdx.x / kXcds, rp = turn / (uint32_t)units * kXcds + blockIdx.x % kXcds;
     if (rp >= (uint64_t)a.B * a.P) return false;
     const int unit = turn % (uint32_t)units;
-    // Parts of all rows next to each other, and a row's parts on every XCD in turn.
-    const uint32_t B = a.B;
-    p = rp / B;
-    b = (rp - p * B + (B % 2 == 0 ? p : 0)) % B;
+    part = a.part;
+    if (a.room) {                    // uniform
+      if (!fit(a, rp, chunk * np)) return false;
+    } else {
+      // Parts of all rows next to each other, and a row's parts on every XCD in turn.
+      const uint32_t B = a.B;
+      p = rp / B;
+      b = (rp - p * B + (B % 2 == 0 ? p : 0)) % B;
+    }
     kvh = unit / n_hc * hw + hsub;
     const int hc = unit % n_hc;
     h0 = kvh * group + hc * heads;
@@ -130,6 +223,14 @@ __device__ inline void finish(const SpanArgs& a, const Task& t, bool whole, floa
 inline int64_t workgroups(const SpanArgs& a, int heads) {
   const int64_t units = a.Hkv / a.heads * ceil_div(a.H / a.Hkv, heads);
   return sat_mul(ceil_div(sat_mul(a.B, a.P), kXcds), kXcds, units);
+}
+
+// Parts that are on the chip at a time, which holds `slots` workgroups, each XCD as many; where
+// that is fewer than two a row, of as many rounds as give two.
+inline int parts_on_chip(int B, int H, int Hkv, int heads, int side, int slots) {
+  const int64_t units = Hkv / side * ceil_div(H / Hkv, heads);
+  const int64_t round = std::max<int64_t>(slots / kXcds / units, 1) * kXcds;
+  return (int)std::min<int64_t>(ceil_div(2 * (int64_t)B, round) * round, 0x7fffffff);
 }
 
 // Short rows are whole: as many KV heads side by side as leave a workgroup for each CU, where

@@ -115,11 +115,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_decode_kernel(SpanArgs 
   static_assert(kSlots * (D + 4) * 4 <= (int)sizeof(Chunk<D>), "a wave's outputs fit");
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   Task t;
-  if (!t.find(a, kSlots)) return;
+  if (!t.find(a, kSlots, kChunk)) return;
   Chunk<D>& w = chunks[t.wv];
   const Span span(a, t.b);
   int lo, hi, nparts;
-  if (!span.part(a, t.p, lo, hi, nparts)) {   // all of the workgroup
+  if (!span.part(a, t.part, t.p, lo, hi, nparts)) {   // all of the workgroup
     if (span.n == 0 && t.p == -a.P) zero_rows<D>(a, t);
     return;
   }
@@ -265,8 +265,10 @@ bool window_decode_serves(int kv_dtype, int D) {
   return (kv_dtype == HS_DTYPE_F16 || kv_dtype == HS_DTYPE_BF16) && D <= 128;
 }
 
-void window_decode_plan(int B, int H, int Hkv, int64_t most, bool windowed, int cus, int* part, int* heads) {
+void window_decode_plan(int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
+                        int* heads, int* room) {
   plan(B, H, Hkv, kSlots, kChunk, most, windowed, cus, part, heads);
+  *room = parts_on_chip(B, H, Hkv, kSlots, *heads, cus * (D == 128 ? 2 : D == 64 ? 3 : 5));
 }
 
 int launch_window_decode(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream) {

@@ -414,3 +414,38 @@ def test_batches_of_every_count(B):
         q = s.rows(B)[0]
         s.check(0, q, s.attend(0, q))
         s.check(0, q, s.attend(0, q, 2100, 1), 2100, 1)
+
+
+@pytest.mark.parametrize("B", [63, 64, 65, 128, 129, 200, 256, 257])
+@pytest.mark.parametrize("q4", [True, False])
+def test_large_ragged_batches(q4, B):
+    """Whole parts, parts that are not, and empty rows in every order, on both sides of the
+    counts where parts are dealt otherwise; pages are shared, so that they stay few."""
+    from heteroserve.kv import quant
+    from heteroserve.model.paged_attn_q4 import paged_attention_q4
+    from heteroserve.model.paged_attn_window import paged_attention_window
+
+    rng = np.random.default_rng(B)
+    D, pages, MB = 64, 300, 280
+    gen = torch.Generator(DEV).manual_seed(B)
+    k, v = (torch.randn(pages * BS, HKV, D, generator=gen, device=DEV) for _ in range(2))
+    lens = rng.choice([0, 1, 255, 256, 257, 512, 513, 1024, 2048, 3333, MB * BS], B)
+    lens[B // 2] = MB * BS                   # a row of the table's width
+    bt = rng.integers(0, pages, (B, MB)).astype(np.int32)
+    q = torch.randn(B, H, D, generator=gen, device=DEV)
+    args = (_dev(bt), _dev(lens), D ** -0.5)
+    if q4:
+        pool = quant.empty_pool_q4(1, pages, BS, HKV, D, device=DEV)
+        at = torch.arange(pages * BS)
+        quant.append_kv_q4(pool[0, 0], pool[0, 1], torch.arange(pages)[None], at, k, v,
+                           seq_ids=torch.zeros_like(at))
+        got = paged_attention_q4(q, pool[0, 0], pool[0, 1], *args)
+        k, v = (lc.values(pool[0, i].cpu().numpy().reshape(-1, HKV, 5 * D // 8), i == 0) for i in (0, 1))
+    else:
+        got = paged_attention_window(q, k.half().view(pages, BS, HKV, D), v.half().view(pages, BS, HKV, D),
+                                     *args, 0)
+        k, v = _np(k.half()), _np(v.half())
+    for b in range(B):
+        pos = np.arange(lens[b])
+        rows = bt[b, pos // BS] * BS + pos % BS
+        _check(q[b], got[b], k[rows], v[rows], D)
