@@ -191,16 +191,17 @@ __device__ inline _Float16 half_of(const Words<N>& x, int i) {
   return __builtin_bit_cast(_Float16, (uint16_t)(x.w[i / 2] >> (16 * (i & 1))));
 }
 
-// kByGroup: the 16 columns of the products are heads times groups, column j head j / G's sums
-// over group j % G alone: 16 / G heads a wave.  Otherwise they are 16 heads.  By group, a lane
-// scales its scores by one group's steps and adds the groups' up with its neighbours', and
-// makes the second product's operand for one group instead of all: 64 rows of 16..4096 keys, D 128,
-// 32 / 8 heads, took 91 us where 16 columns for 4 heads took 119.
-template <int D, bool kByGroup>
+// The 16 columns of the products are 16 / S heads times S shares of the groups: column j has head
+// j / S's sums over groups j % S * G / S .. alone.  So a lane scales its scores by G / S groups'
+// steps, adds the shares up with its neighbours, and makes the second product's operand
+// for these groups instead of all: 64 rows of 16..4096 keys, D 128, 32 / 8 heads, took 91 us with
+// S = 4 where they took 119 with 1; behind a window of 4096, 32 / 4 heads, 48 with S = 2, 54 with 1.
+template <int D, int S>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void q4_decode_kernel(SpanArgs a) {
   constexpr int G = D / kQ4Group, kPiece = D / 8, kT = D / 16;
   constexpr int kRecord = q4_record_bytes(D), kLoads = kRecord / kPiece;   // 5 pieces a record
-  constexpr int kHeads = kByGroup ? kSlots / G : kSlots;     // of a wave
+  constexpr int kHeads = kSlots / S;     // of a wave
+  constexpr int kShare = G / S;          // groups of a column
   constexpr int kMid = G == 8 ? 8 : 4;   // groups that a lane has of the product of the mids
   __shared__ Chunk<D> chunks[kWaves];
   __shared__ float2 states[kWaves][kSlots];
@@ -209,7 +210,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
   Task t;
   if (!t.find(a, kHeads, kChunk)) return;
   Chunk<D>& w = chunks[t.wv];
-  const int jh = kByGroup ? j / G : j, jg = kByGroup ? j % G : 0;   // this column's head, group
+  const int jh = j / S, js = j % S;      // this column's head, share
   const Span span(a, t.b);
   int lo, hi, nparts;
   if (!span.part(a, t.part, t.p, lo, hi, nparts)) {   // all of the workgroup
@@ -274,7 +275,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
         sums[st] += x[st][e];
       }
       sums[st] = sum_across_groups(sums[st]);
-      const bool mine = !kByGroup || st == jg;
+      const bool mine = st / kShare == js;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float y = mine ? x[st][half_element(e)] * (e & 2 ? 0x1p-4f : 1.0f) : 0.0f;
@@ -285,7 +286,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
     // term g % 2 of the sums, against the lowest values, and of 8 of them, against the steps
 #pragma unroll
     for (int e = 0; e < kMid; ++e) {
-      const float y = e < G && (!kByGroup || e == jg) ? sums[e % G] * (g < 2 ? 1.0f : 8.0f) : 0.0f;
+      const float y = e < G && e / kShare == js ? sums[e % G] * (g < 2 ? 1.0f : 8.0f) : 0.0f;
       const _Float16 h = (_Float16)y;
       qsum[e] = g & 1 ? (_Float16)(y - (float)h) : h;
     }
@@ -366,41 +367,34 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
         s[i] = __builtin_amdgcn_mfma_f32_16x16x16f16(x, q, none, 0, 0, 0);
       }
     }
-    if constexpr (kByGroup) {
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) {   // group i of every share
       float4x x[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = float4x{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int r = 0; r < 4; ++r) x[r] = float4x{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int st = 0; st < G; ++st)
+      for (int st = i; st < G; st += kShare)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const half8 kf = unpack(kw[i].w[st]);
-          x[i] = mma(kf, qf[st][0], x[i]);
-          x[i] = mma(kf, qf[st][1], x[i]);
+        for (int r = 0; r < 4; ++r) {
+          const half8 kf = unpack(kw[r].w[st]);
+          x[r] = mma(kf, qf[st][0], x[r]);
+          x[r] = mma(kf, qf[st][1], x[r]);
         }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const half8 ks = *reinterpret_cast<const half8*>(&w.ks[jg][16 * g + 8 * t]);
+        const half8 ks = *reinterpret_cast<const half8*>(&w.ks[js * kShare + i][16 * g + 8 * t]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int i = 2 * t + e / 4;
-          s[i][e % 4] = group_sum<G>(fmaf((float)ks[e], x[i][e % 4], s[i][e % 4]));
+          const int r = 2 * t + e / 4;
+          s[r][e % 4] = fmaf((float)ks[e], x[r][e % 4], s[r][e % 4]);
         }
       }
-    } else {
+    }
+    if constexpr (S > 1) {
 #pragma unroll
-      for (int st = 0; st < G; ++st) {
-        const half8 k0 = *reinterpret_cast<const half8*>(&w.ks[st][16 * g]);
-        const half8 k1 = *reinterpret_cast<const half8*>(&w.ks[st][16 * g + 8]);
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const half8 kf = unpack(kw[i].w[st]);
-          float4x x = mma(kf, qf[st][0], float4x{0.0f, 0.0f, 0.0f, 0.0f});
-          x = mma(kf, qf[st][1], x);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] = fmaf((float)(i < 2 ? k0 : k1)[4 * (i & 1) + e], x[e], s[i][e]);
-        }
-      }
+        for (int e = 0; e < 4; ++e) s[r][e] = group_sum<S>(s[r][e]);
     }
     if (last) {
 #pragma unroll
@@ -459,23 +453,23 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[i][e] *= e & 1 ? R * 0x1p-4f : R;
-    half8 hi2[2], lo2[2];
 #pragma unroll
-    for (int d = 0; d < kT; ++d) {
-      if (d == 0 || (!kByGroup && d % 2 == 0)) {
+    for (int i = 0; i < kShare; ++i) {
+      half8 hi2[2], lo2[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          split_steps(s[2 * t], s[2 * t + 1],
-                      *reinterpret_cast<const uint4*>(&w.vs[kByGroup ? jg : d / 2][16 * g + 8 * t]), hi2[t],
-                      lo2[t]);
-      }
-      typedef __attribute__((address_space(3))) int2x lds_int2x;
-      const int2x x = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_int2x*)(w.v[lane] + 8 * d));
+      for (int t = 0; t < 2; ++t)
+        split_steps(s[2 * t], s[2 * t + 1],
+                    *reinterpret_cast<const uint4*>(&w.vs[js * kShare + i][16 * g + 8 * t]), hi2[t], lo2[t]);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const half8 vf = unpack((uint32_t)x[t]);
-        o[d] = mma(vf, hi2[t], o[d]);
-        o[d] = mma(vf, lo2[t], o[d]);
+      for (int d = 2 * i; d < kT; d += d % 2 ? 2 * kShare - 1 : 1) {
+        typedef __attribute__((address_space(3))) int2x lds_int2x;
+        const int2x x = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_int2x*)(w.v[lane] + 8 * d));
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const half8 vf = unpack((uint32_t)x[t]);
+          o[d] = mma(vf, hi2[t], o[d]);
+          o[d] = mma(vf, lo2[t], o[d]);
+        }
       }
     }
   }
@@ -494,28 +488,28 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
     for (int e = 0; e < 4; ++e) o[d][e] = fmaf(o[d][e], out_scale, mid);
   }
   finish<D, kHeads>(
-      a, t, nparts == 1, o, m, l, jh, jg == 0 && g == 0, [&](int d) { return !kByGroup || jg == d / 2; },
+      a, t, nparts == 1, o, m, l, jh, js == 0 && g == 0, [&](int d) { return js == d / 2 / kShare; },
       [&](int wave) { return reinterpret_cast<float*>(&chunks[wave]); }, states);
 }
 
-// Query heads of a wave.
-int heads_per_wave(int H, int Hkv, int D) {
-  const int by_group = kSlots * kQ4Group / D;
-  return H / Hkv <= by_group ? by_group : kSlots;
+// Columns of a head: as many as leave a wave the KV head's query heads, the groups at most.
+int shares(int H, int Hkv, int D) {
+  int s = D / kQ4Group;
+  while (s > 1 && H / Hkv * s > kSlots) s /= 2;
+  return s;
 }
 
-template <int D, bool kByGroup>
+template <int D, int S>
 void launch_one(const SpanArgs& a, hipStream_t stream) {
-  const int64_t wgs = workgroups(a, heads_per_wave(a.H, a.Hkv, D));
-  hipLaunchKernelGGL((q4_decode_kernel<D, kByGroup>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, stream,
-                     a);
+  const int64_t wgs = workgroups(a, kSlots / S);
+  hipLaunchKernelGGL((q4_decode_kernel<D, S>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, stream, a);
 }
 
-template <int D>
+template <int D, int S = D / kQ4Group>
 void launch_dim(const SpanArgs& a, hipStream_t stream) {
-  if constexpr (D == kQ4Group) return launch_one<D, true>(a, stream);   // the same thing
-  else if (a.H / a.Hkv <= kSlots * kQ4Group / D) launch_one<D, true>(a, stream);
-  else launch_one<D, false>(a, stream);
+  if constexpr (S > 1)
+    if (shares(a.H, a.Hkv, D) < S) return launch_dim<D, S / 2>(a, stream);
+  launch_one<D, S>(a, stream);
 }
 
 }  // namespace
@@ -527,14 +521,14 @@ void launch_dim(const SpanArgs& a, hipStream_t stream) {
 // 4 x 512 119, 2 x 1024 120, 4 x 1024 126; 1 of 4096 1 x 256 13.0, 4 x 64 15.2.
 void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
                     int* heads, int* room) {
-  const int hpw = heads_per_wave(H, Hkv, D);
+  const int hpw = kSlots / shares(H, Hkv, D);
   plan(B, H, Hkv, hpw, kChunk, most, windowed, cus, part, heads);
   *room = parts_on_chip(B, H, Hkv, hpw, *heads, cus * (D == 256 ? 1 : D == 128 ? 2 : 3));
 }
 
 // The parts' states or rows; the caller merges.
 int launch_q4_decode(const SpanArgs& a, int D, hipStream_t stream) {
-  if (!grid_fits(workgroups(a, heads_per_wave(a.H, a.Hkv, D)), 64 * kWaves))
+  if (!grid_fits(workgroups(a, kSlots / shares(a.H, a.Hkv, D)), 64 * kWaves))
     return fail(HS_EUNSUPPORTED, "grid too large: sequences * parts * KV heads");
   switch (D) {
     case 32: launch_dim<32>(a, stream); break;

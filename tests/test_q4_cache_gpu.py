@@ -213,6 +213,14 @@ def test_attention(H, Hkv, D, BS):
     _check([0, 1, 2, 15, 16, 17, 63, 64, 65, 127, 130, 200], H, Hkv, D, BS, 0, 0, H + D)
 
 
+@pytest.mark.parametrize("H,Hkv,D", [(5, 1, 128), (14, 2, 128), (9, 1, 128), (9, 1, 256), (20, 1, 256),
+                                     (7, 1, 256), (6, 2, 256), (5, 1, 64), (10, 5, 64), (33, 1, 128)])
+def test_groups_of_every_size(H, Hkv, D):
+    """Columns of the products by heads and groups in every split, not all of them used."""
+    _check([0, 3, 64, 100, 333], H, Hkv, D, 16, 0, 0, H + D)
+    _check([0, 3, 64, 100, 333], H, Hkv, D, 16, 90, 2, H + D)
+
+
 @pytest.mark.parametrize("H,Hkv,D", [(8, 2, 128), (4, 4, 64), (16, 1, 32), (2, 1, 256), (16, 2, 128),
                                      (12, 1, 64), (4, 1, 256)])
 def test_rounding_errors_average_out(H, Hkv, D):
