@@ -312,14 +312,23 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
       load(slot);
     }
     lds_order();
+    // What middles and the ones beside them are multiplied by: less than 1 in chunks of records that
+    // no append writes, with middles beyond fp16.
+    float unit;
     {
       const Words<G> kp = load_words<G>(w.k[lane] + D / 2), vp = load_words<G>(w.v[lane] + D / 2);
       const int place = (lane & ~7) | half_place(lane & 7);
-      float most = 0.0f;
+      float most = 0.0f, mids[G], far = 0.0f;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        mids[i] = fmaf((float)half_of(vp, i), 8.0f, (float)half_of(vp, G + i));
+        far = fmaxf(far, fabsf(mids[i]));
+      }
+      unit = __builtin_amdgcn_ballot_w64(far > kF16Most) != 0 ? 0x1p-4f : 1.0f;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         const float x = (float)half_of(vp, i);
-        const Terms m2 = split(fmaf(x, 8.0f, (float)half_of(vp, G + i)), 0.0f);
+        const Terms m2 = split(mids[i] * unit, 0.0f);
         w.ks[i][lane] = half_of(kp, i);
         w.vs[i][lane] = half_of(vp, i);
         w.vmid[i][place] = half_of(Words<1>{m2.hi}, 0);
@@ -437,7 +446,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
       }
       const half8 p1 = __builtin_bit_cast(half8, make_uint4(h[0], h[1], h[2], h[3]));
       const half8 p2 = __builtin_bit_cast(half8, make_uint4(l[0], l[1], l[2], l[3]));
-      const half8 one = (_Float16)1.0f;
+      const half8 one = (_Float16)unit;
       half8 mid = one;
       if (j < 2 * G) mid = *reinterpret_cast<const half8*>(&w.vmid[j & (2 * G - 1)][16 * g + 8 * t]);
       z = mma(mid, p1, z);
@@ -447,8 +456,12 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
         zl = mma(one, p2, zl);
       }
     }
-    oz += z;
-    ones += zl;
+    const float back_unit = unit == 1.0f ? 1.0f : 16.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      oz[e] = fmaf(z[e], back_unit, oz[e]);
+      ones[e] = fmaf(zl[e], back_unit, ones[e]);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll

@@ -193,7 +193,8 @@ int hs_q4_read(const void* k_cache, const void* v_cache, int NB, int BS, int Hkv
  * cached tokens (the new one among them) the last `window` and the first `sinks`.
  * window 0: all of them.  What other tokens' slots hold never reaches a row,
  * infinities and NaN included.  hs_q4_decode reads a 4-bit cache, hs_window_decode
- * one of kv_dtype; scores, softmax and sums are fp32, products as near as fp32's.
+ * one of kv_dtype; scores, softmax and sums are fp32, products as near as fp32's (of
+ * a 4-bit cache: relative to their group's range).
  * A row that sees an infinity or a NaN may be NaN in the elements that it reaches.
  *   q, out      [B, H, D] float32, 16-byte aligned
  *   D           32, 64, 128 or 256;  H % Hkv == 0;  MB * BS at most 2^30, num_blocks

@@ -449,3 +449,60 @@ def test_large_ragged_batches(q4, B):
         pos = np.arange(lens[b])
         rows = bt[b, pos // BS] * BS + pos % BS
         _check(q[b], got[b], k[rows], v[rows], D)
+
+
+@pytest.mark.parametrize("q4", [True, False])
+def test_a_captured_batch_with_other_lengths(q4):
+    """More parts than the chip holds at a time, whose length follows the rows': a graph of one
+    call, replayed over other lengths and tables with eager calls between, is the eager
+    call to the bit."""
+    from heteroserve.model.paged_attn_q4 import paged_attention_q4
+    from heteroserve.model.paged_attn_window import paged_attention_window
+
+    rng = np.random.default_rng(5)
+    B, heads, kv, D, pages, MB = 48, 16, 8, 128, 400, 300
+    gen = torch.Generator(DEV).manual_seed(5)
+    if q4:
+        cache = torch.randint(0, 120, (2, pages, BS, kv, 80), generator=gen, device=DEV, dtype=torch.uint8)
+        call = paged_attention_q4                # (bytes below 0x78: finite steps and lowest values)
+    else:
+        cache = torch.randn(2, pages, BS, kv, D, generator=gen, device=DEV).half()
+        call = paged_attention_window
+    tables = _dev(rng.integers(0, pages, (B, MB)))
+    ctx = _dev(np.full(B, MB * BS))
+    q = torch.randn(B, heads, D, generator=gen, device=DEV) * 1e-4
+
+    def run():
+        return call(q, cache[0], cache[1], tables, ctx, 0.1, 0, 0)
+
+    lengths = [rng.integers(0, MB * BS + 1, B), np.full(B, 3), np.where(np.arange(B) == 7, MB * BS, 0),
+               np.full(B, MB * BS), rng.integers(500, 600, B)]
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for lens in lengths:
+        ctx.copy_(_dev(lens))
+        tables.copy_(_dev(rng.integers(0, pages, (B, MB))))
+        want = run().clone()
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.isfinite(want).all()
+        assert not want[torch.tensor(lens == 0, device=DEV)].any()
+
+
+@pytest.mark.parametrize("q4,dtype,D", [(True, F16, 128), (True, F16, 256), (False, BF16, 64), (False, F16, 128),
+                                        (False, F32, 64), (False, BF16, 256)])
+@pytest.mark.parametrize("odd", [float("nan"), float("inf"), -float("inf")])
+def test_a_query_that_is_no_number(q4, dtype, D, odd):
+    """It takes its own head's row, and no other."""
+    s = _Chat([70, 300], 0, D, dtype, q4, seed=D)
+    q = s.rows(2)[0].float().contiguous()
+    want = s.attend(0, q, 100, 2)
+    q[1, 3, 17] = odd
+    got = s.attend(0, q, 100, 2)
+    assert torch.isfinite(want).all() and not torch.isfinite(got[1, 3]).any()
+    got[1, 3] = want[1, 3]
+    assert torch.equal(got, want)

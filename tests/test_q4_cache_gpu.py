@@ -439,3 +439,38 @@ def test_pages_of_the_pool_move_as_bytes():
     pack.write_blocks_device(other, [2, 0, 7], payload)
     for a, b in zip(want, attend(other, torch.tensor([[2, 0, 7]]), ctx[:1])):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(4, 4, 64), (8, 2, 128), (16, 2, 128), (6, 3, 256), (3, 1, 32)])
+def test_records_of_any_finite_numbers(H, Hkv, D):
+    """Steps and lowest values up to fp16's largest, which no append writes together: values
+    of up to 16 times that, in some chunks of a row and not in others.
+
+    The sizes that errors are relative to are those of what is added: n s + lo is (n - 8) s and
+    lo + 8 s, at most 8 s + |lo + 8 s|, of keys (n - 8) s, lo and 8 s, at most 16 s + |lo|, where the
+    tests above, whose elements' n differ from key to key, do with n s + |lo| (an element of 0 in a group
+    of large ones is off by 2^-22 of their step, half of which it may be off by itself)."""
+    from heteroserve.model.paged_attn_q4 import paged_attention_q4
+
+    rng = np.random.default_rng(D + H)
+    n, BS, G = 400, 16, D // 32
+    rec = rng.integers(0, 256, (2, 32, BS, Hkv, 5 * D // 8)).astype(np.uint8)
+    step = (rng.random((2, 32, BS, Hkv, G)) * 65504).astype(np.float16)
+    low = (rng.uniform(-1, 1, step.shape) * 65504).astype(np.float16)
+    for x in (step, low):                    # blocks of ordinary sizes between
+        x[:, 8:20] = (x[:, 8:20].astype(np.float64) * 1e-4).astype(np.float16)
+    rec[..., D // 2:] = np.concatenate([step, low], -1).view(np.uint8)
+    lens, bt = [n, 130, 17], np.stack([rng.permutation(32)[:25] for _ in range(3)])
+    q = (rng.normal(size=(3, H, D)) * 1e-6).astype(np.float32)
+    cache = torch.tensor(rec, device=DEV)
+    got = _np(paged_attention_q4(torch.tensor(q, device=DEV), cache[0], cache[1], torch.tensor(bt),
+                                 torch.tensor(lens), 0.1))
+    for b, m in enumerate(lens):
+        at = np.arange(m)
+        k, v = (rec[i][bt[b, at // BS], at % BS] for i in (0, 1))
+        (ks, kl), (vs, vl) = (np.split(np.repeat(np.ascontiguousarray(x[..., D // 2:]).view(np.float16)
+                                                 .astype(np.float64), 32, -1), 2, -1) for x in (k, v))
+        want, spread, weight = lc.decode(q[b], lc.values(k, True), lc.values(v, False), 0.1,
+                                         16 * ks + np.abs(kl), 8 * vs + np.abs(vl + 8 * vs))
+        tol = (D + 64) * 2.0 ** -23 * weight + (m + 64) * 2.0 ** -23 * spread
+        assert (np.abs(got[b] - want) <= tol).all(), (b, (np.abs(got[b] - want) / tol).max())
