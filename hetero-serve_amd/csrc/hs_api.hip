@@ -1094,10 +1094,14 @@ static int check_span_sizes(int kv_dtype, int B, int H, int Hkv, int D, int BS, 
 // Parts, and the bytes of their states (INT64_MAX when too large).
 static int64_t plan_span(SpanArgs& a, int kv_dtype, int D, int64_t* ml) {
   const int64_t most = span_most(a.MB, a.BS, a.window, a.sinks);
+  int longest = 0;
   span_plan(kv_dtype, a.B, a.H, a.Hkv, D, most, most < (int64_t)a.MB * a.BS, current_cus(), &a.part,
-            &a.heads, &a.room);
+            &a.heads, &a.room, &longest);
   a.P = (int)ceil_div(most, a.part);
-  if (a.B > kSpanDealt || sat_mul(a.B, a.P) <= a.room) a.room = 0;   // nothing to fit
+  int64_t tasks = sat_mul(a.B, a.P);
+  if (a.room == 0 || a.B > kSpanDealt || tasks <= a.room) a.room = 0;   // nothing to fit
+  else tasks = std::min(tasks, std::max<int64_t>(a.room, a.B * ceil_div(most, longest)) + a.B);
+  a.tasks = (int)std::min<int64_t>(tasks, 0x7fffffff);
   return span_state_bytes(a.B, a.H, D, a.P, ml);
 }
 

@@ -244,20 +244,20 @@ int launch_q4_read(const Q4Rows& w, hipStream_t stream);
 
 // Decode over spans (hs_span.h, hs_span_decode.hip): keys of a part (and KV heads of a
 // workgroup) for rows of at most `most` keys, fewer than the tables hold if windowed, and how
-// many parts their length may be fitted to (0: it may not); and the
+// many parts their length may be fitted to (0: it may not), up to which length; and the
 // launch.  kv_dtype -1 is the 4-bit cache.
 struct SpanArgs;
 void span_plan(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
-               int* heads, int* room);
+               int* heads, int* room, int* longest);
 int launch_span(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream);
 // The 4-bit cache's part of both (hs_q4_decode.hip).
 void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
-                    int* heads, int* room);
+                    int* heads, int* room, int* longest);
 int launch_q4_decode(const SpanArgs& a, int D, hipStream_t stream);
 // fp16 and bf16 caches on the matrix cores (hs_window_decode.hip).
 bool window_decode_serves(int kv_dtype, int D);
 void window_decode_plan(int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
-                        int* heads, int* room);
+                        int* heads, int* room, int* longest);
 int launch_window_decode(const SpanArgs& a, int kv_dtype, int D, hipStream_t stream);
 
 // Pages inside one pool [L, 2, NB, page] (hs_pages.hip).

@@ -533,9 +533,10 @@ void launch_dim(const SpanArgs& a, hipStream_t stream) {
 // 2 x 256 16.7, 1 x 512 17.5; 64 of 16..4096 2 x 512 63, 4 x 512 66, 1 x 1024 68; 16 of 8k..32k
 // 4 x 512 119, 2 x 1024 120, 4 x 1024 126; 1 of 4096 1 x 256 13.0, 4 x 64 15.2.
 void q4_decode_plan(int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
-                    int* heads, int* room) {
+                    int* heads, int* room, int* longest) {
   const int hpw = kSlots / shares(H, Hkv, D);
   plan(B, H, Hkv, hpw, kChunk, most, windowed, cus, part, heads);
+  *longest = kLongest * kChunk * kWaves / *heads;
   *room = parts_on_chip(B, H, Hkv, hpw, *heads, cus * (D == 256 ? 1 : D == 128 ? 2 : 3));
 }
 

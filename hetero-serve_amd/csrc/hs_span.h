@@ -28,6 +28,7 @@ struct SpanArgs {
   int window, sinks;          // window 0: all keys
   int part, P;                // keys of a part at least, parts of the longest row at most
   int room;                   // parts in all that their length is fitted to, or 0
+  int tasks;                  // parts and empty rows at most, over all rows
   int32_t* fitted;            // the parts' keys then
   int heads;                  // 4-bit cache: KV heads of a workgroup
   float qscale;               // scale * log2(e)

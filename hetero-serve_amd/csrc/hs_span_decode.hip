@@ -297,11 +297,11 @@ void launch_span_merge(const SpanArgs& a, int D, hipStream_t stream) {
 // otherwise parts of 2048 keys, cut down to 256 while the workgroups are fewer than two for
 // each CU.
 void span_plan(int kv_dtype, int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
-               int* heads, int* room) {
-  if (kv_dtype < 0) return q4_decode_plan(B, H, Hkv, D, most, windowed, cus, part, heads, room);
+               int* heads, int* room, int* longest) {
+  if (kv_dtype < 0) return q4_decode_plan(B, H, Hkv, D, most, windowed, cus, part, heads, room, longest);
   if (window_decode_serves(kv_dtype, D))
-    return window_decode_plan(B, H, Hkv, D, most, windowed, cus, part, heads, room);
-  *heads = *room = 0;
+    return window_decode_plan(B, H, Hkv, D, most, windowed, cus, part, heads, room, longest);
+  *heads = *room = *longest = 0;
   const int64_t wgs = sat_mul(B, H / row_attn_heads_per_wave(H, Hkv));
   int len = 2048;
   while (len > 256 && sat_mul(wgs, ceil_div(most, len)) < 2 * (int64_t)cus) len /= 2;

@@ -65,7 +65,8 @@ struct Task {
   // rows' last ones that are not whole, then the rows without keys: XCDs, to which
   // workgroups go in turn, have as many as each other, and long parts do not begin late.
   // Every wave finds all this by itself, in less than 1 us (which batches whose parts are few
-  // anyway do not pay).  us, parts of 512 keys / fitted, D 128, 32 / 8 heads, 4 bits: 64 rows of
+  // anyway do not pay), and the grid holds a.tasks: 64 rows of 16..4096 keys in tables of 32768 take
+  // 55 us (79 with a workgroup for every part of the table), of 131072 69 (187).  us, parts of 512 keys / fitted, D 128, 32 / 8 heads, 4 bits: 64 rows of
   // 16..4096 keys 62 / 56, of 16..8192 97 / 88, of 8192 each 163 / 157, 16 of 8k..32k 117 / 103; 64 of
   // 500..4000, D 256, 85 / 61; over bf16, 64 of 64..4096 110 / 101.
   __device__ bool fit(const SpanArgs& a, uint32_t x, int step) {
@@ -88,17 +89,20 @@ struct Task {
       return __builtin_amdgcn_readlane(sum_up_to(count), 63);
     };
     part = a.part;
-    if (parts_of(part) > a.room) {
+    int parts = parts_of(part);
+    if (parts > a.room) {
       sum = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(group_sum<64>(sum))));
       int steps = max(part / step, (int)(sum / ((float)step * (float)a.room)));
       for (;;) {
         steps = min(steps, kLongest);
         part = steps * step;
-        if (steps == kLongest || parts_of(part) <= a.room) break;
+        parts = parts_of(part);
+        if (steps == kLongest || parts <= a.room) break;
         steps += max(1, steps / 16);
       }
     }
     if (x == 0 && threadIdx.x == 0) *a.fitted = part;
+    if (x >= (uint32_t)parts + a.B) return false;
 
     int whole[kDealt], left = x;
 #pragma unroll
@@ -145,7 +149,7 @@ struct Task {
     const int group = a.H / a.Hkv, n_hc = (group + heads - 1) / heads, units = a.Hkv / hw * n_hc;
     // The heads of one part run on one XCD, one behind the other: they share lines of 128 bytes.
     const uint32_t turn = blockIdx.x / kXcds, rp = turn / (uint32_t)units * kXcds + blockIdx.x % kXcds;
-    if (rp >= (uint64_t)a.B * a.P) return false;
+    if (rp >= (uint32_t)a.tasks) return false;
     const int unit = turn % (uint32_t)units;
     part = a.part;
     if (a.room) {                    // uniform
@@ -222,7 +226,7 @@ __device__ inline void finish(const SpanArgs& a, const Task& t, bool whole, floa
 // Workgroups of `heads` query heads a wave; INT64_MAX when too many.
 inline int64_t workgroups(const SpanArgs& a, int heads) {
   const int64_t units = a.Hkv / a.heads * ceil_div(a.H / a.Hkv, heads);
-  return sat_mul(ceil_div(sat_mul(a.B, a.P), kXcds), kXcds, units);
+  return sat_mul(ceil_div(a.tasks, kXcds), kXcds, units);
 }
 
 // Parts that are on the chip at a time, which holds `slots` workgroups, each XCD as many; where

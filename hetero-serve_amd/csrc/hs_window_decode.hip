@@ -266,8 +266,9 @@ bool window_decode_serves(int kv_dtype, int D) {
 }
 
 void window_decode_plan(int B, int H, int Hkv, int D, int64_t most, bool windowed, int cus, int* part,
-                        int* heads, int* room) {
+                        int* heads, int* room, int* longest) {
   plan(B, H, Hkv, kSlots, kChunk, most, windowed, cus, part, heads);
+  *longest = kLongest * kChunk * kWaves / *heads;
   *room = parts_on_chip(B, H, Hkv, kSlots, *heads, cus * (D == 128 ? 2 : D == 64 ? 3 : 5));
 }
 

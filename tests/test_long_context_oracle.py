@@ -162,6 +162,22 @@ def test_workspace_queries(lib):
         assert lib.hs_window_decode_workspace_bytes(kv, 2, 4, 2, 64, 16, 2 ** 12, 0, 0) == 0
 
 
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("window", [0, 1, 256, 5000])
+def test_workspace_queries_of_every_kind(lib, D, window):
+    """One row to many, tables narrow and wide, every type: sizes that grow with the rows, and 0
+    where a row is one part whatever it holds."""
+    for MB in (1, 32, 2048, 2 ** 16):
+        sizes = []
+        for B in (1, 3, 64, 256, 257, 5000):
+            kinds = [lib.hs_window_decode_workspace_bytes(kv, B, 12, 6, D, 16, MB, window, 4) for kv in range(3)]
+            sizes.append([*kinds, lib.hs_q4_decode_workspace_bytes(B, 12, 6, D, 16, MB, window, 4)])
+        if MB == 1 or window == 1:
+            assert not np.any(sizes)
+        if MB >= 2048 and not window:
+            assert np.all(sizes) and all(np.all(np.diff(x[2:5]) > 0) for x in zip(*sizes))
+
+
 def test_the_unknown_kv_type_is_refused(lib):
     for kv in (-1, 3):
         _refused(lib, _decode(lib, kv=kv), -1, b"dtype")

@@ -506,3 +506,42 @@ def test_a_query_that_is_no_number(q4, dtype, D, odd):
     assert torch.isfinite(want).all() and not torch.isfinite(got[1, 3]).any()
     got[1, 3] = want[1, 3]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("q4", [True, False])
+@pytest.mark.parametrize("long", [0, 1, 20])
+def test_tables_wider_than_most_rows(q4, long):
+    """A table of 32768 tokens, of which `long` rows hold all and the others few or none; the
+    workgroups are counted for the longest."""
+    from heteroserve.kv import quant
+    from heteroserve.model.paged_attn_q4 import paged_attention_q4
+    from heteroserve.model.paged_attn_window import paged_attention_window
+
+    rng = np.random.default_rng(long)
+    B, D, pages, MB = 40, 32, 200, 2048
+    gen = torch.Generator(DEV).manual_seed(long)
+    k, v = (torch.randn(pages * BS, HKV, D, generator=gen, device=DEV).half() for _ in range(2))
+    lens = rng.integers(0, 700, B)
+    lens[rng.permutation(B)[:long]] = MB * BS
+    lens[:3] = 0
+    bt = rng.integers(0, pages, (B, MB)).astype(np.int32)
+    q = torch.randn(B, H, D, generator=gen, device=DEV)
+    args = (_dev(bt), _dev(lens), D ** -0.5)
+    if q4:
+        pool = quant.empty_pool_q4(1, pages, BS, HKV, D, device=DEV)
+        at = torch.arange(pages * BS)
+        quant.append_kv_q4(pool[0, 0], pool[0, 1], torch.arange(pages)[None], at, k, v,
+                           seq_ids=torch.zeros_like(at))
+        got = paged_attention_q4(q, pool[0, 0], pool[0, 1], *args)
+        k, v = (lc.values(pool[0, i].cpu().numpy().reshape(-1, HKV, 5 * D // 8), i == 0) for i in (0, 1))
+    else:
+        got = paged_attention_window(q, k.view(pages, BS, HKV, D), v.view(pages, BS, HKV, D), *args, 0)
+        k, v = _np(k), _np(v)
+    seen = 0
+    for b in range(B):
+        pos = np.arange(lens[b])
+        rows = bt[b, pos // BS] * BS + pos % BS
+        if lens[b] < MB * BS or seen < 4:
+            _check(q[b], got[b], k[rows], v[rows], D)
+        seen += lens[b] == MB * BS
+    assert torch.isfinite(got).all()
