@@ -196,6 +196,8 @@ int hs_q4_read(const void* k_cache, const void* v_cache, int NB, int BS, int Hkv
  * one of kv_dtype; scores, softmax and sums are fp32, products as near as fp32's (of
  * a 4-bit cache: relative to their group's range).
  * A row that sees an infinity or a NaN may be NaN in the elements that it reaches.
+ * A call repeated gives the same bits; how a row's sums are split, and so its last
+ * bits, depends on the sizes and on the lengths of all rows.
  *   q, out      [B, H, D] float32, 16-byte aligned
  *   D           32, 64, 128 or 256;  H % Hkv == 0;  MB * BS at most 2^30, num_blocks
  *               * BS below 2^31;  scale finite, and times log2(e) as well
