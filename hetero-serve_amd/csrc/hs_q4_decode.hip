@@ -4,21 +4,28 @@
 //   score_t = sum_d (k_td s_tg + mid_tg) q_d = sum_g s_tg (sum_{d in g} k_td q_d) + sum_g mid_tg Q_g
 //   out_d   = sum_t p_t (k_td s_tg + mid_tg) = sum_t (p_t s_tg) k_td + sum_t p_t mid_tg
 // where g = d / 32 is the element's group and Q_g the sum of the query over it.  So whole
-// numbers go to the products, and s and mid are applied to fp32 sums (keys) or to the fp32
+// numbers go to the products, and s is applied to fp32 sums (keys) or to the fp32
 // probabilities (values); the elements themselves are never made.  With n and lo in the
 // place of k and mid, the two sums are several times larger than what they add up to, and
-// so was the error: 8e-6 of the row where it is 4e-7, at 4096 keys.
+// so was the error: 8e-6 of the row where it is 4e-7, at 4096 keys.  The sums over the mids are
+// small: the keys' goes to the matrix cores, the values' and that of p are fp32 sums of the
+// vector units.
 //
 // Numerics.  A nibble in the low bits of 1024's mantissa is 1024 + n, or 1024 + 16 n four bits
 // further up; less 1032 or 1152 they are k and 16 k, exactly, and the 16 is taken out of the
 // other operand.  (As masked, without the 1024, they are the subnormals n 2^-24, which the
 // matrix cores take, but they align sums by the operands' exponents: an accuracy of 2^-16 was
-// left.)  Query and probabilities are fp32 and go in as two fp16 terms, hi + lo with 22 bits: each
-// head's query times the power of two that brings its largest element to [2^6, 2^7), so that 8
-// times a group's sum is below 2^15; probabilities as 2^7 p, at most 2^15 under the lazy raise
-// of the maximum, and p_t s_tg times a power of two R that follows the largest step (see
-// kStepRoom).  A key's mid is not made: mid Q is lo Q + s 8 Q, of halves as they are stored.  A
-// value's has two fp16 terms.  Products of such terms are exact in the fp32 accumulators.
+// left.)  The query is fp32 and goes in as two fp16 terms, hi + lo with 22 bits: each head's times
+// the power of two that brings its largest element to [2^6, 2^7), so that 8 times a group's sum is
+// below 2^15.  A key's mid is not made: mid Q is lo Q + s 8 Q, of halves as they are stored.
+//   p s goes in as two such terms too, times a power of two R for each head and group: two terms
+// have 22 bits down to 2^-3 and end at 2^-24, so R follows the largest p s that the wave has met,
+// which it brings to [2^12, 2^13), and is chosen again when one passes 2^15.  When the row's maximum
+// rises, and the sums so far count for less, R rises with it.  So numbers are cut off at 2^-32 of the
+// largest one's share of the output, as far as fp32 sums reach, however small p is next to the
+// row's largest (a first key that takes nearly all of the weight and has next to no values), and
+// whatever the steps of other groups and of keys that have no weight.  Products of such terms
+// are exact in the fp32 accumulators.
 //
 // A wave serves up to 16 query heads of one KV head over one part of a row's visible keys,
 // 64 keys (a chunk) at a time:
@@ -53,19 +60,17 @@ namespace {
 
 using namespace span_mma;
 
-typedef _Float16 half2x __attribute__((ext_vector_type(2)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef int int2x __attribute__((ext_vector_type(2)));
 
 constexpr int kChunk = 64;         // keys of a step
-constexpr float kLift = 7.0f;      // probabilities are held 2^kLift times larger
-// R is chosen so that the largest step so far times R lies in [2^-3, 2^-2), and chosen again when a
-// step times R passes 1, for p s R is at most 2^15 up to there.
-constexpr int kStepRoom = 2;
+// The largest p s so far times R is at most 2^kMost; when a larger one comes R is chosen so that
+// it lies below 2^kAim.  R is 2^kFree at most.
+constexpr int kMost = 15, kAim = 13, kFree = 127;
 
-// What a wave keeps in LDS: its chunk's records as they were loaded, and of its values' steps
-// and middles what lies by key there by group, so that a lane's 16 keys are two 16-byte
+// What a wave keeps in LDS: its chunk's records as they were loaded, and of its steps and its
+// values' middles what lies by key there by group, so that a lane's 16 keys are a few 16-byte
 // reads.  (Rows of records are 20 dwords apart at D 128: the keys' 16-byte reads of 16 rows
 // cover all banks, the values' transposing ones half of them.)
 template <int D>
@@ -75,7 +80,7 @@ struct Chunk {
   alignas(16) uint8_t v[kChunk][(q4_record_bytes(D) + 7) / 8 * 8];   // (8-byte reads)
   alignas(16) _Float16 ks[G][kPar];
   alignas(16) _Float16 vs[G][kPar];
-  alignas(16) _Float16 vmid[2 * G][kPar];       // both terms, keys in Unpack's order
+  alignas(16) float vmid[G][kPar];
 };
 
 template <int N>
@@ -119,58 +124,40 @@ struct Unpack {
            half8{a, a, b, b, a, a, b, b};
   }
 };
-// The element of a word that half e of Unpack's is, and its place.
+// The element of a word that half e of Unpack's is.
 __device__ constexpr int half_element(int e) { return (e >> 1) + 4 * (e & 1); }
-__device__ inline int half_place(int i) { return 2 * (i & 3) + (i >> 2 & 1); }
 
 __device__ inline float4x mma(half8 a, half8 b, float4x c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Two fp16 terms hi + lo of two numbers, 22 bits of them.  The first ones pass through a
-// register that the compiler does not see through: it may round one product to fp16 in two
-// ways, with and without a stop at fp32, and the second term has to be the rest of the first
-// as it is used.
-struct Terms {
-  uint32_t hi, lo;
-};
-
-__device__ inline Terms split(float x, float y) {
-  Terms t;
-  t.hi = __builtin_bit_cast(uint32_t, half2x{(_Float16)x, (_Float16)y});
-  asm("" : "+v"(t.hi));
-  const half2x h = __builtin_bit_cast(half2x, t.hi);
-  t.lo = __builtin_bit_cast(uint32_t, half2x{(_Float16)(x - (float)h[0]), (_Float16)(y - (float)h[1])});
-  return t;
-}
-
-// The terms of keys 16 g + 8 t ..: their probabilities times R (over 16 where the key is odd),
-// x of the first four and y of the others, times their steps.  An instruction for each
-// term, where the compiler takes five for two of them.  One that writes half a register is
-// not followed by one that reads it: a wait is needed between those.
-__device__ inline void split_steps(const float4x& x, const float4x& y, const uint4& steps, half8& hi,
+// The terms, hi + lo with 22 bits, of keys 16 g + 8 t ..: their p s in the order of Unpack's halves,
+// x of the first four and y of the others, times R (R / 16 where the key is odd).  An instruction
+// for each term, where the compiler takes several.  One that writes half a register is not
+// followed by one that reads it: a wait is needed between those.
+__device__ inline void split_terms(const float4x& x, const float4x& y, float even, float odd, half8& hi,
                                    half8& lo) {
   uint32_t h0, h1, h2, h3, l0, l1, l2, l3;
-  asm("v_fma_mixlo_f16 %0, %8, %16, 0 op_sel_hi:[0,1,0]\n\t"
-      "v_fma_mixlo_f16 %1, %9, %16, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
-      "v_fma_mixlo_f16 %2, %10, %17, 0 op_sel_hi:[0,1,0]\n\t"
-      "v_fma_mixlo_f16 %3, %11, %17, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
-      "v_fma_mixhi_f16 %0, %12, %18, 0 op_sel_hi:[0,1,0]\n\t"
-      "v_fma_mixhi_f16 %1, %13, %18, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
-      "v_fma_mixhi_f16 %2, %14, %19, 0 op_sel_hi:[0,1,0]\n\t"
-      "v_fma_mixhi_f16 %3, %15, %19, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
-      "v_fma_mixlo_f16 %4, %8, %16, -%0 op_sel_hi:[0,1,1]\n\t"
-      "v_fma_mixlo_f16 %5, %9, %16, -%1 op_sel:[0,1,0] op_sel_hi:[0,1,1]\n\t"
-      "v_fma_mixlo_f16 %6, %10, %17, -%2 op_sel_hi:[0,1,1]\n\t"
-      "v_fma_mixlo_f16 %7, %11, %17, -%3 op_sel:[0,1,0] op_sel_hi:[0,1,1]\n\t"
-      "v_fma_mixhi_f16 %4, %12, %18, -%0 op_sel:[0,0,1] op_sel_hi:[0,1,1]\n\t"
-      "v_fma_mixhi_f16 %5, %13, %18, -%1 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
-      "v_fma_mixhi_f16 %6, %14, %19, -%2 op_sel:[0,0,1] op_sel_hi:[0,1,1]\n\t"
-      "v_fma_mixhi_f16 %7, %15, %19, -%3 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
+  asm("v_fma_mixlo_f16 %0, %8, %16, 0\n\t"
+      "v_fma_mixlo_f16 %1, %9, %17, 0\n\t"
+      "v_fma_mixlo_f16 %2, %10, %16, 0\n\t"
+      "v_fma_mixlo_f16 %3, %11, %17, 0\n\t"
+      "v_fma_mixhi_f16 %0, %12, %16, 0\n\t"
+      "v_fma_mixhi_f16 %1, %13, %17, 0\n\t"
+      "v_fma_mixhi_f16 %2, %14, %16, 0\n\t"
+      "v_fma_mixhi_f16 %3, %15, %17, 0\n\t"
+      "v_fma_mixlo_f16 %4, %8, %16, -%0 op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixlo_f16 %5, %9, %17, -%1 op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixlo_f16 %6, %10, %16, -%2 op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixlo_f16 %7, %11, %17, -%3 op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixhi_f16 %4, %12, %16, -%0 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixhi_f16 %5, %13, %17, -%1 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixhi_f16 %6, %14, %16, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixhi_f16 %7, %15, %17, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
       "s_nop 1"
       : "=&v"(h0), "=&v"(h1), "=&v"(h2), "=&v"(h3), "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3)
-      : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(y[0]), "v"(y[1]), "v"(y[2]), "v"(y[3]),
-        "v"(steps.x), "v"(steps.y), "v"(steps.z), "v"(steps.w));
+      : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(y[0]), "v"(y[1]), "v"(y[2]), "v"(y[3]), "v"(even),
+        "v"(odd));
   hi = __builtin_bit_cast(half8, make_uint4(h0, h1, h2, h3));
   lo = __builtin_bit_cast(half8, make_uint4(l0, l1, l2, l3));
 }
@@ -292,10 +279,18 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
     }
   }
 
-  float4x o[kT], oz = {0.0f, 0.0f, 0.0f, 0.0f}, ones = oz;
+  // Over this lane's keys: the sum l of p, and of p mid for each group of the share.  The outputs
+  // are held times R, of the group's column.
+  float4x o[kT];
+  float om[kShare], R[kShare], l = 0.0f;
 #pragma unroll
   for (int d = 0; d < kT; ++d) o[d] = float4x{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = kLowest, room = 0.0f, R = 1.0f;   // steps up to `room` fit R
+#pragma unroll
+  for (int i = 0; i < kShare; ++i) {
+    om[i] = 0.0f;
+    R[i] = ldexpf(1.0f, kFree);
+  }
+  float m = kLowest;
 
   for (int c0 = first; c0 < hi; c0 += step) {
     const bool last = hi - c0 < kChunk;   // uniform
@@ -312,40 +307,13 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
       load(slot);
     }
     lds_order();
-    // What middles and the ones beside them are multiplied by: less than 1 in chunks of records that
-    // no append writes, with middles beyond fp16.
-    float unit;
     {
       const Words<G> kp = load_words<G>(w.k[lane] + D / 2), vp = load_words<G>(w.v[lane] + D / 2);
-      const int place = (lane & ~7) | half_place(lane & 7);
-      float most = 0.0f, mids[G], far = 0.0f;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        mids[i] = fmaf((float)half_of(vp, i), 8.0f, (float)half_of(vp, G + i));
-        far = fmaxf(far, fabsf(mids[i]));
-      }
-      unit = __builtin_amdgcn_ballot_w64(far > kF16Most) != 0 ? 0x1p-4f : 1.0f;
-#pragma unroll
-      for (int i = 0; i < G; ++i) {
-        const float x = (float)half_of(vp, i);
-        const Terms m2 = split(mids[i] * unit, 0.0f);
         w.ks[i][lane] = half_of(kp, i);
         w.vs[i][lane] = half_of(vp, i);
-        w.vmid[i][place] = half_of(Words<1>{m2.hi}, 0);
-        w.vmid[G + i][place] = half_of(Words<1>{m2.lo}, 0);
-        most = fmaxf(most, x);
-      }
-      if (__builtin_amdgcn_ballot_w64(most > room) != 0) {
-        most = fmaxf(most, __shfl_xor(most, 1));
-        most = fmaxf(most, __shfl_xor(most, 2));
-        most = fmaxf(most, __shfl_xor(most, 4));
-        most = fmaxf(most, __shfl_xor(most, 8));
-        const int e = __builtin_amdgcn_frexp_expf(max_across_groups(most)) + kStepRoom;
-        const float R_new = ldexpf(1.0f, -e), keep = R_new / R;
-        room = ldexpf(1.0f, e);
-        R = R_new;
-#pragma unroll
-        for (int d = 0; d < kT; ++d) o[d] *= keep;
+        w.vmid[i][lane] = fmaf((float)half_of(vp, i), 8.0f, (float)half_of(vp, G + i));
       }
     }
     lds_order();
@@ -419,60 +387,63 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
       for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[i][e]);
     mx *= back;
     if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
-      const float m_new = fmaxf(m, max_across_groups(mx)), keep = fast_exp2(m - m_new);
+      const float m_new = fmaxf(m, max_across_groups(mx)), by = m_new - m, keep = fast_exp2(-by);
       m = m_new;
-      oz *= keep;
-      ones *= keep;
+      l *= keep;
 #pragma unroll
-      for (int d = 0; d < kT; ++d) o[d] *= keep;
+      for (int i = 0; i < kShare; ++i) {
+        // R grows as what is there shrinks: what comes may be as small
+        const int more = min((int)fminf(by, 2.0f * kFree), kFree + 1 - __builtin_amdgcn_frexp_expf(R[i]));
+        R[i] = ldexpf(R[i], more);
+        om[i] *= keep;
+        const float times = ldexpf(keep, more);
+#pragma unroll
+        for (int d = 0; d < kT; ++d)
+          if (d / 2 % kShare == i) o[d] *= times;
+      }
     }
-    // 2^kLift p; its terms against the mids, and against ones (the sum).  Chunks are added by the
-    // vector units, which round to the nearest: the matrix cores cut off, which adds up in
-    // sums of one sign (parts of 128 chunks: 8e-6 of the row instead of 2e-6).
-    float4x z = {0.0f, 0.0f, 0.0f, 0.0f}, zl = z;
-    const float mb = m - kLift;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] = fast_exp2(fmaf(s[i][e], back, -mb));
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {   // (keys 8 t .. of each lane's 16)
-      uint32_t h[4], l[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const Terms x = split(s[2 * t][e], s[2 * t + 1][e]);
-        h[e] = x.hi;
-        l[e] = x.lo;
+        s[i][e] = fast_exp2(fmaf(s[i][e], back, -m));
+        l += s[i][e];
       }
-      const half8 p1 = __builtin_bit_cast(half8, make_uint4(h[0], h[1], h[2], h[3]));
-      const half8 p2 = __builtin_bit_cast(half8, make_uint4(l[0], l[1], l[2], l[3]));
-      const half8 one = (_Float16)unit;
-      half8 mid = one;
-      if (j < 2 * G) mid = *reinterpret_cast<const half8*>(&w.vmid[j & (2 * G - 1)][16 * g + 8 * t]);
-      z = mma(mid, p1, z);
-      z = mma(mid, p2, z);
-      if constexpr (G == 8) {      // no row is left
-        zl = mma(one, p1, zl);
-        zl = mma(one, p2, zl);
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) {   // group i of every share
+      float4x ps[4];
+      float most = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const half8 vs = *reinterpret_cast<const half8*>(&w.vs[js * kShare + i][16 * g + 8 * t]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int r = 2 * t + e / 4;
+          ps[r][e % 4] = fmaf(s[r][e % 4], (float)vs[e], 0.0f);   // (one instruction)
+          most = fmaxf(most, fabsf(ps[r][e % 4]));
+        }
       }
-    }
-    const float back_unit = unit == 1.0f ? 1.0f : 16.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      oz[e] = fmaf(z[e], back_unit, oz[e]);
-      ones[e] = fmaf(zl[e], back_unit, ones[e]);
-    }
+      for (int r = 0; r < 4; ++r) {
+        const float4x mid = *reinterpret_cast<const float4x*>(&w.vmid[js * kShare + i][16 * g + 4 * r]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int e = 0; e < 4; ++e) om[i] = fmaf(s[r][e], mid[e], om[i]);
+      }
+      if (__builtin_amdgcn_ballot_w64(most * R[i] > ldexpf(1.0f, kMost)) != 0) {
+        most = max_across_groups(most);
+        if (most * R[i] > ldexpf(1.0f, kMost) && most < INFINITY) {
+          const int less = kAim + 1 - __builtin_amdgcn_frexp_expf(most) - __builtin_amdgcn_frexp_expf(R[i]);
+          const float times = ldexpf(1.0f, less);
+          R[i] = ldexpf(R[i], less);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] *= e & 1 ? R * 0x1p-4f : R;
-#pragma unroll
-    for (int i = 0; i < kShare; ++i) {
+          for (int d = 0; d < kT; ++d)
+            if (d / 2 % kShare == i) o[d] *= times;
+        }
+      }
       half8 hi2[2], lo2[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        split_steps(s[2 * t], s[2 * t + 1],
-                    *reinterpret_cast<const uint4*>(&w.vs[js * kShare + i][16 * g + 8 * t]), hi2[t], lo2[t]);
+        split_terms(ps[2 * t], ps[2 * t + 1], R[i], R[i] * 0x1p-4f, hi2[t], lo2[t]);
 #pragma unroll
       for (int d = 2 * i; d < kT; d += d % 2 ? 2 * kShare - 1 : 1) {
         typedef __attribute__((address_space(3))) int2x lds_int2x;
@@ -487,21 +458,17 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
     }
   }
 
-  // rows 0 .. G - 1 and G .. 2 G - 1 of oz are the groups' sums of p and the mids' terms,
-  // further ones the sum of p
-  float l = G == 8 ? ones[0] : __shfl(oz[0], 48 + j);
-  m -= kLift;
-  const float out_scale = 1.0f / R;
 #pragma unroll
-  for (int d = 0; d < kT; ++d) {
-    const int first = d / 2, second = G + d / 2;
-    const float mid = __shfl(oz[first % 4], 16 * (first / 4) + j) +
-                      __shfl(oz[second % 4], 16 * (second / 4) + j);
+  for (int i = 0; i < kShare; ++i) {
+    const float mid = sum_across_groups(om[i]), over = 1.0f / R[i];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[d][e] = fmaf(o[d][e], out_scale, mid);
+    for (int d = 0; d < kT; ++d)
+      if (d / 2 % kShare == i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] = fmaf(o[d][e], over, mid);
   }
   finish<D, kHeads>(
-      a, t, nparts == 1, o, m, l, jh, js == 0 && g == 0, [&](int d) { return js == d / 2 / kShare; },
+      a, t, nparts == 1, o, m, sum_across_groups(l), jh, js == 0 && g == 0, [&](int d) { return js == d / 2 / kShare; },
       [&](int wave) { return reinterpret_cast<float*>(&chunks[wave]); }, states);
 }
 
