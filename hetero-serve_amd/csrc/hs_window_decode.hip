@@ -13,11 +13,14 @@
 // its last one, with scores of -inf.
 //
 // Numerics.  Keys and values are multiplied as they are stored.  Query and probabilities are
-// fp32 and go in as terms of the cache's type: three bf16 ones have fp32's 24 bits, two fp16
-// ones 22, where each head's query is first brought to [2^14, 2^15) by a power of two, taken
-// back out of its scores, and the probabilities are held 2^7 times larger (at most 2^15 under
-// the lazy raise of the maximum).  Products of such terms are exact in the fp32 accumulators.
-// (Two bf16 terms would have 16 bits, fp32 has 24.)
+// fp32 and go in as terms of the cache's type.  Three bf16 ones have fp32's 24 bits and range
+// (two would have 16).  Two fp16 ones have 22 bits down to 2^-3 and end at 2^-24.  So each head's
+// query is first brought to [2^14, 2^15) by a power of two, taken back out of its scores, and what
+// is lost of an element is at most 2^-39 of the largest.  The probabilities of a chunk are taken in
+// ranges of 2^18, one in nearly all chunks: the largest of each head is brought there likewise, those
+// down to 2^-3 go to the matrix cores, and the rest is taken in the same way until none is left, since
+// the values of the larger ones may be next to nothing (a first key that takes nearly all of the
+// weight).  Products of such terms are exact in the fp32 accumulators.
 //
 // Bound by HBM: behind a window of 1024, 64 rows of 32 / 8 heads, D 128, 265 MB, take 46 us (5.8
 // TB/s), 32 rows of 32 heads 86 (6.1 TB/s); small batches by their steps' latency.
@@ -45,11 +48,10 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int kChunk = 32;         // keys of a step
 
 template <typename T>
-struct Half;   // kTerms of its type a number; kLift: powers of 2 that probabilities are held above themselves
+struct Half;   // kTerms of its type a number
 template <>
 struct Half<Bf16> {
   static constexpr int kTerms = 3;
-  static constexpr float kLift = 0.0f;
   __device__ static float4x mma(short8x a, short8x b, float4x c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
                                                    c, 0, 0, 0);
@@ -65,7 +67,6 @@ struct Half<Bf16> {
 template <>
 struct Half<_Float16> {
   static constexpr int kTerms = 2;
-  static constexpr float kLift = 7.0f;
   __device__ static float4x mma(short8x a, short8x b, float4x c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c,
                                                   0, 0, 0);
@@ -224,30 +225,66 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_decode_kernel(SpanArgs 
 #pragma unroll
       for (int d = 0; d < kT; ++d) o[d] *= keep;
     }
-    const float mb = m - H::kLift;
     float p[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      p[e] = fast_exp2(fmaf(s[e / 4][e % 4], back, -mb));
+      p[e] = fast_exp2(fmaf(s[e / 4][e % 4], back, -m));
       l += p[e];
     }
-    short8x pf[kTerms];
-    split8<T>(p, pf);
-
     // V[16 (e / 4) + 4 g + e % 4][16 d + j], e = 0 .. 7: lane i of 16 supplies 8 bytes of row i / 4
-#pragma unroll
-    for (int d = 0; d < kT; ++d) {
+    auto values = [&](int d) {
       typedef __attribute__((address_space(3))) short4x lds_short4x;
       const uint16_t* at = &w.v[4 * g + (j >> 2)][16 * d + 4 * (j & 3)];
-      const short8x vf = __builtin_shufflevector(
+      return __builtin_shufflevector(
           __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4x*)at),
           __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4x*)(at + 16 * (D + 16))), 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    short8x pf[kTerms];
+    if constexpr (kTerms == 3) {
+      split8<T>(p, pf);
 #pragma unroll
-      for (int n = 0; n < kTerms; ++n) o[d] = H::mma(vf, pf[n], o[d]);
+      for (int d = 0; d < kT; ++d) {
+        const short8x vf = values(d);
+#pragma unroll
+        for (int n = 0; n < kTerms; ++n) o[d] = H::mma(vf, pf[n], o[d]);
+      }
+    } else {
+      bool more;
+      do {
+        float most = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, p[e]);
+        const int up = min(15 - __builtin_amdgcn_frexp_expf(max_across_groups(most)), 127);
+        const float over = ldexpf(1.0f, -up), least = up < 127 ? 0.125f : 0.0f;
+        float x[8], lowest = INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = ldexpf(p[e], up);
+          lowest = fminf(lowest, x[e]);
+        }
+        more = false;
+        if (__builtin_amdgcn_ballot_w64(lowest < least) != 0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const bool later = x[e] < least;  // (a NaN is not)
+            x[e] = later ? 0.0f : x[e];
+            p[e] = later ? p[e] : 0.0f;
+            more |= p[e] > 0.0f;
+          }
+        }
+        split8<T>(x, pf);
+#pragma unroll
+        for (int d = 0; d < kT; ++d) {
+          const short8x vf = values(d);
+          const float4x sum = H::mma(vf, pf[1], H::mma(vf, pf[0], float4x{0.0f, 0.0f, 0.0f, 0.0f}));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][e] = fmaf(sum[e], over, o[d][e]);
+        }
+      } while (__builtin_amdgcn_ballot_w64(more) != 0);
     }
   }
   finish<D, kSlots>(
-      a, t, nparts == 1, o, m - H::kLift, sum_across_groups(l), j, g == 0, [](int) { return true; },
+      a, t, nparts == 1, o, m, sum_across_groups(l), j, g == 0, [](int) { return true; },
       [&](int wave) { return reinterpret_cast<float*>(&chunks[wave]); }, states);
 }
 

@@ -130,3 +130,31 @@ def test_maxima_that_rise_over_4_bits(H, Hkv, D):
     small ones: what came before counts less and less."""
     for size in (0.0, 2.0 ** -8):
         _case("q4", 700, H, Hkv, D, [5, 130, 131, 400], 40, size, 2, 0, 0, D)
+
+
+TYPES = [F16, BF16, F32]
+
+
+@pytest.mark.parametrize("gap", [8, 14, 20, 30, 60, 110])
+@pytest.mark.parametrize("size", [0.0, 2.0 ** -10, 1.0])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D", GEOMETRIES)
+def test_a_sink_of_an_ordinary_cache(H, Hkv, D, dtype, size, gap):
+    for n, rows, window, sinks in ((300, 2, 0, 0), (2500, 2, 0, 0), (3000, 128, 1020, 4)):
+        _case(dtype, n, H, Hkv, D, [0], gap, size, rows, window, sinks, gap + D)
+
+
+@pytest.mark.parametrize("where", [0, 150, 299])
+@pytest.mark.parametrize("gap", [-14, -22, -30, -40, -60, -110])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D", GEOMETRIES)
+def test_huge_values_that_count_for_nothing_in_an_ordinary_cache(H, Hkv, D, dtype, gap, where):
+    for size in (2.0 ** 10, 2.0 ** 15):
+        _case(dtype, 300, H, Hkv, D, [where], gap, size, 2, 0, 0, D - gap)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D", GEOMETRIES)
+def test_maxima_that_rise_in_an_ordinary_cache(H, Hkv, D, dtype):
+    for size in (0.0, 2.0 ** -8):
+        _case(dtype, 700, H, Hkv, D, [5, 130, 131, 400], 40, size, 2, 0, 0, D)
