@@ -15,17 +15,18 @@
 // further up; less 1032 or 1152 they are k and 16 k, exactly, and the 16 is taken out of the
 // other operand.  (As masked, without the 1024, they are the subnormals n 2^-24, which the
 // matrix cores take, but they align sums by the operands' exponents: an accuracy of 2^-16 was
-// left.)  The query is fp32 and goes in as two fp16 terms, hi + lo with 22 bits: each head's times
-// the power of two that brings its largest element to [2^6, 2^7), so that 8 times a group's sum is
-// below 2^15.  A key's mid is not made: mid Q is lo Q + s 8 Q, of halves as they are stored.
-//   p s goes in as two such terms too, times a power of two R for each head and group: two terms
-// have 22 bits down to 2^-3 and end at 2^-24, so R follows the largest p s that the wave has met,
-// which it brings to [2^12, 2^13), and is chosen again when one passes 2^15.  When the row's maximum
-// rises, and the sums so far count for less, R rises with it.  So numbers are cut off at 2^-32 of the
-// largest one's share of the output, as far as fp32 sums reach, however small p is next to the
-// row's largest (a first key that takes nearly all of the weight and has next to no values), and
-// whatever the steps of other groups and of keys that have no weight.  Products of such terms
-// are exact in the fp32 accumulators.
+// left.)  Query and probabilities are fp32 and go in as two fp16 terms, hi + lo, which have 22 bits
+// down to 2^-3 and end at 2^-24.  A query's are times the power of two that brings its head's largest
+// element to [2^14, 2^15), its sums times one that is 2^kQueryUp less, so that 8 times a sum is below
+// 2^15: what is lost of an element is at most 2^-35 of the largest, of a sum 2^-31.  A key's mid is
+// not made: mid Q is lo Q + s 8 Q, of halves as they are stored.
+//   p s has a power of two R for each head and group, which follows the largest p s that the wave
+// has met: it brings that to [2^12, 2^13), and is chosen again when one passes 2^15.  When the row's
+// maximum rises, and the sums so far count for less, R rises with it.  So what is lost is 2^-32 of
+// the largest one, as far as fp32 sums reach, however small p is next to the row's largest (a first
+// key that takes nearly all of the weight and has next to no values), and whatever the steps of
+// other groups and of keys without weight.  Products of such terms are exact in the fp32
+// accumulators.
 //
 // A wave serves up to 16 query heads of one KV head over one part of a row's visible keys,
 // 64 keys (a chunk) at a time:
@@ -68,6 +69,7 @@ constexpr int kChunk = 64;         // keys of a step
 // The largest p s so far times R is at most 2^kMost; when a larger one comes R is chosen so that
 // it lies below 2^kAim.  R is 2^kFree at most.
 constexpr int kMost = 15, kAim = 13, kFree = 127;
+constexpr int kQueryUp = 8;        // powers of 2 that the query is held above its sums
 
 // What a wave keeps in LDS: its chunk's records as they were loaded, and of its steps and its
 // values' middles what lies by key there by group, so that a lane's 16 keys are a few 16-byte
@@ -251,7 +253,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
     most = max_across_groups(most);
     int up = 0;
     if (most > 0.0f && most < INFINITY) up = min(7 - __builtin_amdgcn_frexp_expf(most), 120);
-    back = ldexpf(1.0f, -up);
+    back = ldexpf(1.0f, -up - kQueryUp);
     float sums[G];
 #pragma unroll
     for (int st = 0; st < G; ++st) {
@@ -265,7 +267,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
       const bool mine = st / kShare == js;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float y = mine ? x[st][half_element(e)] * (e & 2 ? 0x1p-4f : 1.0f) : 0.0f;
+        const float y = mine ? x[st][half_element(e)] * (float)(1 << (e & 2 ? kQueryUp - 4 : kQueryUp)) : 0.0f;
         qf[st][0][e] = (_Float16)y;
         qf[st][1][e] = (_Float16)(y - (float)qf[st][0][e]);
       }
@@ -343,6 +345,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
         }
         s[i] = __builtin_amdgcn_mfma_f32_16x16x16f16(x, q, none, 0, 0, 0);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] *= (float)(1 << kQueryUp);
     }
 #pragma unroll
     for (int i = 0; i < kShare; ++i) {   // group i of every share

@@ -158,3 +158,41 @@ def test_huge_values_that_count_for_nothing_in_an_ordinary_cache(H, Hkv, D, dtyp
 def test_maxima_that_rise_in_an_ordinary_cache(H, Hkv, D, dtype):
     for size in (0.0, 2.0 ** -8):
         _case(dtype, 700, H, Hkv, D, [5, 130, 131, 400], 40, size, 2, 0, 0, D)
+
+
+@pytest.mark.parametrize("H,Hkv,D", [x for x in GEOMETRIES if x[2] > 32])
+@pytest.mark.parametrize("kind", ["q4", F16, BF16, F32])
+@pytest.mark.parametrize("n", [3, 300])
+def test_one_large_element_of_a_query(H, Hkv, D, kind, n):
+    """2^14 times the others, where the keys are next to nothing: 2^-20, in a group of their own.
+    Products are off by 2^-22 and what they add up to by as much, so scores by less than 2^-21 of
+    their terms' sizes.  Two fp16 terms that end at 2^-27 of the largest element leave 2^-19."""
+    from heteroserve.model.paged_attn_q4 import paged_attention_q4
+    from heteroserve.model.paged_attn_window import paged_attention_window
+
+    rng = np.random.default_rng(D + H)
+    G = D // 32
+    num, vals = rng.integers(0, 16, (n, Hkv, G, 32)), _values(rng, n, Hkv, D, [], 0)
+    s = np.full((n, Hkv, G), 2.0 ** -4)
+    s[..., 1] = 2.0 ** -20
+    keys = num, s, -8 * s
+    q = rng.normal(size=(2, H, D)).astype(np.float32)
+    q[:, np.arange(H), 32 + rng.integers(0, 32, H)] = 2.0 ** 14
+    pages = -(-n // BS)
+    flat = np.zeros((2, pages * BS, Hkv, 5 * D // 8 if kind == "q4" else D))
+    if kind == "q4":
+        held = [lc.records(*x, keys=i == 0) for i, x in enumerate((keys, vals))]
+        k, v = (lc.values(x, i == 0) for i, x in enumerate(held))
+        sizes, call, kept = [lc.sizes(x, i == 0) for i, x in enumerate(held)], paged_attention_q4, torch.uint8
+    else:
+        held = [_held(x, kind).double().numpy() for x in (keys, vals)]
+        k, v = held
+        sizes, call, kept = [np.abs(k), np.abs(v)], paged_attention_window, kind
+    flat[:, :n] = held
+    cache = torch.tensor(flat).to(kept).view(2, pages, BS, Hkv, -1).to(DEV)
+    got = call(torch.tensor(q, device=DEV), cache[0], cache[1], torch.arange(pages).expand(2, pages),
+               torch.full((2,), n), 0.25, window=0).double().cpu().numpy()
+    for b in range(2):
+        want, spread, weight = lc.decode(q[b], k, v, 0.25, *sizes)
+        err, most = (np.sqrt((x ** 2).reshape(H, -1, 32).mean(-1)) for x in (got[b] - want, spread + weight))
+        assert (err <= 2.0 ** -21 * most).all(), (b, (err / most * 2.0 ** 21).max(-1))
