@@ -21,6 +21,7 @@
 #include "hs_q4.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace hs {
 
@@ -227,7 +228,11 @@ __global__ __launch_bounds__(kThreads) void q4_read_kernel(Q4Args a) {
       const _Float16* par = reinterpret_cast<const _Float16*>(rec + a.D / 2) + (u.w >> 2);
       const float s = (float)par[0], lo = (float)par[G];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[c][e] = fmaf((float)((word >> (4 * e)) & 15u), s, lo);
+      for (int e = 0; e < 8; ++e) {
+        x[c][e] = fmaf((float)((word >> (4 * e)) & 15u), s, lo);
+        // s is rounded, so 15 s + lo may lie beyond what was written, and round to an infinity
+        if constexpr (std::is_same<T, _Float16>::value) x[c][e] = nan_min(nan_max(x[c][e], -kF16Most), kF16Most);
+      }
     }
   }
   const int64_t to = u.row * ((int64_t)a.Hkv * a.D * Codec<T>::kBytes);

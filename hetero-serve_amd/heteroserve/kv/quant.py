@@ -63,5 +63,7 @@ def append_kv_q4(k_cache, v_cache, block_tables, positions, k, v, seq_ids=None) 
 
 def read_kv_q4(k_cache, v_cache, block_tables, positions, seq_ids=None, dtype=None):
     """(k, v) [n, Hkv, D] of dtype (float32, float16 or bfloat16; float16 when None): the
-    tokens at positions[i] of sequences seq_ids[i], n s + lo rounded once."""
+    tokens at positions[i] of sequences seq_ids[i], n s + lo rounded to fp32 and then to
+    dtype.  In float16 values beyond its largest count as that (lo + 15 s may be: s is
+    rounded)."""
     return _hip.q4_read(k_cache, v_cache, block_tables, positions, seq_ids, dtype)

@@ -180,8 +180,9 @@ int hs_q4_append(void* k_cache, void* v_cache, int NB, int BS, int Hkv, int D,
 /*
  * The way back: row i of k_out and v_out [n, Hkv, D] of out_dtype (16-byte aligned,
  * no part of the caches) is what the cache holds at position positions[i] of
- * sequence seq_ids[i], n s + lo rounded once, or zeros where hs_q4_append would skip.
- * Rows may share a slot.
+ * sequence seq_ids[i], n s + lo rounded to fp32 and then to out_dtype, or zeros where
+ * hs_q4_append would skip.  In fp16 values beyond its largest count as that here too (15 s +
+ * lo may be: s is rounded).  Rows may share a slot.
  */
 int hs_q4_read(const void* k_cache, const void* v_cache, int NB, int BS, int Hkv, int D,
                const int32_t* block_tables, int B, int MB, const int32_t* positions,
