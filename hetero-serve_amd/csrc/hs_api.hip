@@ -1091,18 +1091,29 @@ static int check_span_sizes(int kv_dtype, int B, int H, int Hkv, int D, int BS, 
   return HS_OK;
 }
 
-// Parts, and the bytes of their states (INT64_MAX when too large).
-static int64_t plan_span(SpanArgs& a, int kv_dtype, int D, int64_t* ml) {
+// Parts of more rows than are fitted are longer where their states would take more than this: 512 rows
+// of 16..4096 keys of 4 bits, 32 / 8 heads, D 128, in tables of 32768 take 414 us and 136 MB, 486 us and
+// 545 MB with parts of 512.
+constexpr int64_t kSpanRoomBytes = 1 << 28;
+
+// Parts, and where their states lie.
+static SpanLayout plan_span(SpanArgs& a, int kv_dtype, int D) {
   const int64_t most = span_most(a.MB, a.BS, a.window, a.sinks);
   int longest = 0;
   span_plan(kv_dtype, a.B, a.H, a.Hkv, D, most, most < (int64_t)a.MB * a.BS, current_cus(), &a.part,
             &a.heads, &a.room, &longest);
+  auto states = [&] { return sat_mul(a.B, ceil_div(most, a.part), a.H); };
+  if (a.B > kSpanDealt)   // not fitted
+    while (a.part < longest && sat_mul(states(), D * 4 + 8) > kSpanRoomBytes) a.part = std::min(2 * a.part, longest);
   a.P = (int)ceil_div(most, a.part);
   int64_t tasks = sat_mul(a.B, a.P);
   if (a.room == 0 || a.B > kSpanDealt || tasks <= a.room) a.room = 0;   // nothing to fit
-  else tasks = std::min(tasks, std::max<int64_t>(a.room, a.B * ceil_div(most, longest)) + a.B);
+  else {
+    a.states = std::min(tasks, std::max<int64_t>(a.room, a.B * ceil_div(most, longest)));
+    tasks = std::min(tasks, a.states + a.B);
+  }
   a.tasks = (int)std::min<int64_t>(tasks, 0x7fffffff);
-  return span_state_bytes(a.B, a.H, D, a.P, ml);
+  return SpanLayout(a, D);
 }
 
 static size_t span_workspace(int kv_dtype, int B, int H, int Hkv, int D, int BS, int MB, int window,
@@ -1116,7 +1127,7 @@ static size_t span_workspace(int kv_dtype, int B, int H, int Hkv, int D, int BS,
   a.MB = MB;
   a.window = window;
   a.sinks = sinks;
-  const int64_t need = plan_span(a, kv_dtype, D, nullptr);
+  const int64_t need = plan_span(a, kv_dtype, D).end;
   if (need == kTooLarge) return (size_t)fail(0, "decode part states too large for these sizes");
   return (size_t)need;
 }
@@ -1155,16 +1166,20 @@ static int span_decode(const float* q, const void* k_cache, const void* v_cache,
   a.window = window;
   a.sinks = sinks;
   a.qscale = powers;
-  int64_t ml = 0;
-  const int64_t need = plan_span(a, kv_dtype, D, &ml);
+  const SpanLayout layout = plan_span(a, kv_dtype, D);
+  const int64_t need = layout.end;
   if (need == kTooLarge) return fail(HS_EUNSUPPORTED, "decode part states too large for these sizes");
   if (need > 0 && (!workspace || workspace_bytes < (size_t)need))
     return fail(HS_EWORKSPACE, "decode needs " + std::to_string(need) + " workspace bytes, got " +
                                    std::to_string(workspace ? workspace_bytes : 0));
   if (need > 0 && !aligned16(workspace)) return fail(HS_EINVAL, "workspace must be 16-byte aligned");
-  a.part_acc = static_cast<float*>(workspace);
-  a.part_ml = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) + ml) : nullptr;
-  a.fitted = need ? reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + need - 16) : nullptr;
+  if (need > 0) {
+    char* ws = static_cast<char*>(workspace);
+    a.part_acc = reinterpret_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float*>(ws + layout.ml);
+    a.fitted = reinterpret_cast<int32_t*>(ws + layout.fitted);
+    a.numbers = reinterpret_cast<int32_t*>(ws + layout.numbers);
+  }
   return launch_span(a, kv_dtype, D, static_cast<hipStream_t>(stream));
 }
 

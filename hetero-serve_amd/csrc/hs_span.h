@@ -21,15 +21,18 @@ struct SpanArgs {
   const int32_t* bt;          // [B, MB]
   const int32_t* ctx;         // [B]
   float* out;                 // [B, H, D]
-  float* part_acc;            // [B, H, P, D]   un-normalised outputs of parts
-  float* part_ml;             // [B, H, P, 2]   (max, sum), base-2 domain
+  // States of parts: [B, H, P] of them, or [states, H] where parts are fitted, by their number.
+  float* part_acc;            // [.., D]        un-normalised outputs
+  float* part_ml;             // [.., 2]        (max, sum), base-2 domain
   int B, H, Hkv, BS, MB, NB;
   int bs_shift;               // log2(BS), or -1
   int window, sinks;          // window 0: all keys
   int part, P;                // keys of a part at least, parts of the longest row at most
   int room;                   // parts in all that their length is fitted to, or 0
   int tasks;                  // parts and empty rows at most, over all rows
-  int32_t* fitted;            // the parts' keys then
+  int64_t states;             // parts at most then
+  int32_t* fitted;            // their keys
+  int32_t* numbers;           // [B, 2]         of a row's first part, which the next ones follow, and of its last
   int heads;                  // 4-bit cache: KV heads of a workgroup
   float qscale;               // scale * log2(e)
 };
@@ -87,14 +90,20 @@ inline int64_t span_most(int64_t MB, int64_t BS, int window, int sinks) {
   return window ? std::min(cap, (int64_t)window + sinks) : cap;
 }
 
-// Bytes of P parts' states, and where the (max, sum) pairs begin (16 bytes for the fitted length
-// lie last); INT64_MAX when too large.
-inline int64_t span_state_bytes(int B, int H, int D, int64_t P, int64_t* ml) {
-  if (P <= 1) return 0;
-  const int64_t rows = sat_mul(B, H, P), acc = sat_mul(rows, D * 4);
-  if (ml) *ml = acc;
-  return sat_add(sat_add(acc, sat_mul(rows, 8)), 16);
-}
+// Where in the workspace the (max, sum) pairs and, where parts are fitted, their keys and numbers
+// begin, and its bytes (INT64_MAX when too large; 0 when no row has parts).
+struct SpanLayout {
+  int64_t ml, fitted, numbers, end;
+
+  SpanLayout(const SpanArgs& a, int D) : ml(0), fitted(0), numbers(0), end(0) {
+    if (a.P <= 1) return;
+    const int64_t states = sat_mul(a.room ? a.states : sat_mul(a.B, a.P), a.H);
+    ml = sat_mul(states, D * 4);
+    fitted = sat_add(ml, sat_mul(states, 8));
+    numbers = sat_add(fitted, 16);
+    end = a.room ? sat_add(numbers, (int64_t)a.B * 8) : fitted;
+  }
+};
 
 void launch_span_merge(const SpanArgs& a, int D, hipStream_t stream);
 

@@ -189,31 +189,36 @@ __global__ __launch_bounds__(64 * kWaves) void span_merge_kernel(SpanArgs a) {
   __shared__ float sums[kWaves][kPer * 64], most[kWaves], totals[kWaves];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int64_t w = blockIdx.x;
-  const Span span(a, (int)(w / a.H));
-  const int n = span.parts(a.room ? *a.fitted : a.part);
+  const int b = (int)(w / a.H), h = (int)(w - (int64_t)b * a.H);
+  const int n = Span(a, b).parts(a.room ? *a.fitted : a.part);
   if (n <= 1) return;   // written already
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + w * a.P;
+  const int number = a.room ? a.numbers[2 * b] : 0, last = a.room ? a.numbers[2 * b + 1] : 0;
+  auto state = [&](int p) {
+    return a.room ? (int64_t)(p < n - 1 ? number + p : last) * a.H + h : w * a.P + p;
+  };
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
   const int each = (n + kWaves - 1) / kWaves, first = min(n, wv * each), end = min(n, first + each);
   float mm = kLowest;
-  for (int p = first + lane; p < end; p += 64) mm = fmaxf(mm, ml[p].x);
+  for (int p = first + lane; p < end; p += 64) mm = fmaxf(mm, ml[state(p)].x);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) mm = fmaxf(mm, __shfl_xor(mm, off));
   float acc[kPer] = {}, l = 0.0f;
   for (int p0 = first; p0 < end; p0 += 64) {
     const int here = min(64, end - p0);
-    const float2 st = lane < here ? ml[p0 + lane] : make_float2(kLowest, 0.0f);
+    const float2 st = lane < here ? ml[state(p0 + lane)] : make_float2(kLowest, 0.0f);
     const float wt = lane < here ? fast_exp2(st.x - mm) : 0.0f;
     l = fmaf(st.y, wt, l);
-    const float* pa = a.part_acc + (w * a.P + p0) * D;
     for (int p = 0; p < here; p += kBatch) {
       float v[kBatch][kPer];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u)
+      for (int u = 0; u < kBatch; ++u) {
+        const float* pa = a.part_acc + state(p0 + min(p + u, here - 1)) * D;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           const int d = lane + 64 * i;
-          v[u][i] = p + u < here && d < D ? pa[(p + u) * D + d] : 0.0f;
+          v[u][i] = p + u < here && d < D ? pa[d] : 0.0f;
         }
+      }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const float wu = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wt), min(p + u, 63)));

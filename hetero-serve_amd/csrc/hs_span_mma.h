@@ -57,6 +57,7 @@ __device__ inline int sum_up_to(int x) {
 // A wave's task.  `heads` query heads of a KV head a wave.
 struct Task {
   int wv, hw, np, hsub, ph;   // wave; heads side by side, phases; this wave's
+  uint32_t x;                 // number of the part among those of all rows
   int part, b, p, kvh, h0, gc;   // keys of a part; row, part; KV head, first query head, how many
   int64_t row0;               // head h0 of row b, of [B, H]
 
@@ -69,7 +70,7 @@ struct Task {
   // 55 us (79 with a workgroup for every part of the table), of 131072 69 (187).  us, parts of 512 keys / fitted, D 128, 32 / 8 heads, 4 bits: 64 rows of
   // 16..4096 keys 62 / 56, of 16..8192 97 / 88, of 8192 each 163 / 157, 16 of 8k..32k 117 / 103; 64 of
   // 500..4000, D 256, 85 / 61; over bf16, 64 of 64..4096 110 / 101.
-  __device__ bool fit(const SpanArgs& a, uint32_t x, int step) {
+  __device__ bool fit(const SpanArgs& a, int step) {
     const int lane = threadIdx.x & 63;
     int n[kDealt];                   // keys of row 64 r + lane; none behind the last row
     float sum = 0.0f;
@@ -148,17 +149,23 @@ struct Task {
     ph = wv / hw;
     const int group = a.H / a.Hkv, n_hc = (group + heads - 1) / heads, units = a.Hkv / hw * n_hc;
     // The heads of one part run on one XCD, one behind the other: they share lines of 128 bytes.
-    const uint32_t turn = blockIdx.x / kXcds, rp = turn / (uint32_t)units * kXcds + blockIdx.x % kXcds;
-    if (rp >= (uint32_t)a.tasks) return false;
+    const uint32_t turn = blockIdx.x / kXcds;
+    x = turn / (uint32_t)units * kXcds + blockIdx.x % kXcds;
+    if (x >= (uint32_t)a.tasks) return false;
     const int unit = turn % (uint32_t)units;
     part = a.part;
     if (a.room) {                    // uniform
-      if (!fit(a, rp, chunk * np)) return false;
+      if (!fit(a, chunk * np)) return false;
+      if (unit == 0 && threadIdx.x == 0) {
+        const int n = Span(a, b).parts(part), first = p - (a.P - n);
+        if (first == 0) a.numbers[2 * b] = (int)x;
+        if (first == n - 1) a.numbers[2 * b + 1] = (int)x;
+      }
     } else {
       // Parts of all rows next to each other, and a row's parts on every XCD in turn.
       const uint32_t B = a.B;
-      p = rp / B;
-      b = (rp - p * B + (B % 2 == 0 ? p : 0)) % B;
+      p = x / B;
+      b = (x - p * B + (B % 2 == 0 ? p : 0)) % B;
     }
     kvh = unit / n_hc * hw + hsub;
     const int hc = unit % n_hc;
@@ -185,15 +192,16 @@ __device__ inline void finish(const SpanArgs& a, const Task& t, bool whole, floa
                               float l, int jh, bool lead, Mine mine, Stage stage,
                               float2 (&states)[kWaves][kSlots]) {
   const int lane = threadIdx.x & 63, g = lane >> 4;
-  const int64_t pi = (t.row0 + jh) * a.P + t.p;
+  // The state of head h of this wave's: parts of fitted length lie by their number.
+  auto state = [&](int h) { return a.room ? (int64_t)t.x * a.H + t.h0 + h : (t.row0 + h) * a.P + t.p; };
   auto over = [&](float sum) { return !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum; };
   if (t.np == 1) {
     const float inv = over(l);
-    float* to = whole ? a.out + (t.row0 + jh) * D : a.part_acc + pi * D;
+    float* to = whole ? a.out + (t.row0 + jh) * D : a.part_acc + state(jh) * D;
 #pragma unroll
     for (int d = 0; d < D / 16; ++d)
       if (jh < t.gc && mine(d)) *reinterpret_cast<float4x*>(to + 16 * d + 4 * g) = o[d] * inv;
-    if (!whole && jh < t.gc && lead) reinterpret_cast<float2*>(a.part_ml)[pi] = make_float2(m, l);
+    if (!whole && jh < t.gc && lead) reinterpret_cast<float2*>(a.part_ml)[state(jh)] = make_float2(m, l);
     return;
   }
   lds_order();
@@ -211,14 +219,14 @@ __device__ inline void finish(const SpanArgs& a, const Task& t, bool whole, floa
   for (int d = 0; d < D / 16; ++d)
     if (mine(d)) *reinterpret_cast<float4x*>(stage(t.wv) + jh * (D + 4) + 16 * d + 4 * g) = o[d] * keep;
   if (!whole && t.ph == 0 && jh < t.gc && lead)
-    reinterpret_cast<float2*>(a.part_ml)[pi] = make_float2(mm, l);
+    reinterpret_cast<float2*>(a.part_ml)[state(jh)] = make_float2(mm, l);
   __syncthreads();
   for (int x = t.ph * 64 + lane; x < t.gc * (D / 4); x += t.np * 64) {
     const int h = x / (D / 4), d = x % (D / 4) * 4;
     float4x sum = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int i = 0; i < t.np; ++i)
       sum += *reinterpret_cast<const float4x*>(stage(t.hsub + t.hw * i) + h * (D + 4) + d);
-    float* to = whole ? a.out + (t.row0 + h) * D : a.part_acc + ((t.row0 + h) * a.P + t.p) * D;
+    float* to = whole ? a.out + (t.row0 + h) * D : a.part_acc + state(h) * D;
     *reinterpret_cast<float4x*>(to + d) = sum;
   }
 }
