@@ -406,13 +406,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
           if (d / 2 % kShare == i) o[d] *= times;
       }
     }
+    // (A chunk's sums are their own: fewer roundings where terms have one sign.)
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[i][e] = fast_exp2(fmaf(s[i][e], back, -m));
-        l += s[i][e];
+        sum += s[i][e];
       }
+    l += sum;
 #pragma unroll
     for (int i = 0; i < kShare; ++i) {   // group i of every share
       float4x ps[4];
@@ -427,12 +430,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : D == 128 ? 2 : 3) void 
           most = fmaxf(most, fabsf(ps[r][e % 4]));
         }
       }
+      float mids = 0.0f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float4x mid = *reinterpret_cast<const float4x*>(&w.vmid[js * kShare + i][16 * g + 4 * r]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) om[i] = fmaf(s[r][e], mid[e], om[i]);
+        for (int e = 0; e < 4; ++e) mids = fmaf(s[r][e], mid[e], mids);
       }
+      om[i] += mids;
       if (__builtin_amdgcn_ballot_w64(most * R[i] > ldexpf(1.0f, kMost)) != 0) {
         most = max_across_groups(most);
         if (most * R[i] > ldexpf(1.0f, kMost) && most < INFINITY) {
