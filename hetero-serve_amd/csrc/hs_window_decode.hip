@@ -245,8 +245,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_decode_kernel(SpanArgs 
 #pragma unroll
       for (int d = 0; d < kT; ++d) {
         const short8x vf = values(d);
+        float4x sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int n = 0; n < kTerms; ++n) o[d] = H::mma(vf, pf[n], o[d]);
+        for (int n = kTerms - 1; n >= 0; --n) sum = H::mma(vf, pf[n], sum);
+        o[d] += sum;
       }
     } else {
       bool more;
