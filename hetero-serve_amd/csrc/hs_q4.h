@@ -14,7 +14,8 @@
 // lie side by side so that they come in one load.
 //
 // Records are token-major like the rows of the other caches, so pages of them can be
-// copied, forked, packed and moved as bytes.  All offsets are multiples of D / 8 bytes.
+// copied, forked, packed and moved as bytes.  Records and their steps begin at multiples of
+// D / 8 bytes, lowest values half as much further on.
 #pragma once
 
 #include "hs_common.h"

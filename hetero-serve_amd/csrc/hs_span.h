@@ -15,6 +15,13 @@ namespace hs {
 
 constexpr int kSpanDealt = 256;   // rows at most whose parts are fitted and dealt by their number
 
+namespace span {
+constexpr int kWaves = 4;         // of a workgroup
+constexpr float kSlack = 8.0f;    // lazy raise of the running max, log2 units
+// Where running maxima start: no finite score lies below, so a row of one is never empty.
+constexpr float kLowest = -0x1.fffffep127f;
+}  // namespace span
+
 struct SpanArgs {
   const float* q;             // [B, H, D]
   const uint8_t *k, *v;       // [NB, BS, Hkv, row of one head]
@@ -33,7 +40,7 @@ struct SpanArgs {
   int64_t states;             // parts at most then
   int32_t* fitted;            // their keys
   int32_t* numbers;           // [B, 2]         of a row's first part, which the next ones follow, and of its last
-  int heads;                  // 4-bit cache: KV heads of a workgroup
+  int heads;                  // matrix cores: KV heads of a workgroup
   float qscale;               // scale * log2(e)
 };
 
@@ -78,9 +85,6 @@ struct Span {
   // As a row of the cache seen as [NB * BS] rows (below 2^31).
   __device__ static uint32_t slot(const SpanArgs& a, const Place& x) {
     return (uint32_t)safe_block(x.block, a.NB) * (uint32_t)a.BS + x.off;
-  }
-  __device__ uint32_t slot(const SpanArgs& a, const int32_t* bt, int i) const {
-    return slot(a, place(a, bt, i));
   }
 };
 

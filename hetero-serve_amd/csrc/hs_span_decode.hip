@@ -20,10 +20,7 @@ namespace hs {
 
 namespace {
 
-constexpr int kWaves = 4;         // of a workgroup
-constexpr float kSlack = 8.0f;    // lazy raise of the running max, log2 units
-// Where running maxima start: no finite score lies below, so a row of one is never empty.
-constexpr float kLowest = -0x1.fffffep127f;
+using namespace span;
 
 template <typename T, int D, int G>
 __global__ __launch_bounds__(64 * kWaves) void span_walk_kernel(SpanArgs a) {
@@ -190,12 +187,17 @@ __global__ __launch_bounds__(64 * kWaves) void span_merge_kernel(SpanArgs a) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int64_t w = blockIdx.x;
   const int b = (int)(w / a.H), h = (int)(w - (int64_t)b * a.H);
-  const int n = Span(a, b).parts(a.room ? *a.fitted : a.part);
+  int part = a.part, number = 0, last = 0;
+  if (a.room) {         // uniform; read with the row's length, not behind it
+    part = *a.fitted;
+    number = a.numbers[2 * b];
+    last = a.numbers[2 * b + 1];
+  }
+  const int n = Span(a, b).parts(part);
   if (n <= 1) return;   // written already
-  const int number = a.room ? a.numbers[2 * b] : 0, last = a.room ? a.numbers[2 * b + 1] : 0;
-  auto state = [&](int p) {
-    return a.room ? (int64_t)(p < n - 1 ? number + p : last) * a.H + h : w * a.P + p;
-  };
+  const int64_t base = a.room ? (int64_t)number * a.H + h : w * a.P, apart = a.room ? a.H : 1;
+  const int64_t end_state = a.room ? (int64_t)last * a.H + h : base + n - 1;
+  auto state = [&](int p) { return p < n - 1 ? base + p * apart : end_state; };
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
   const int each = (n + kWaves - 1) / kWaves, first = min(n, wv * each), end = min(n, first + each);
   float mm = kLowest;

@@ -11,16 +11,14 @@
 namespace hs {
 namespace span_mma {
 
+using namespace span;
+
 typedef float float4x __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 4;          // of a workgroup
 constexpr int kXcds = 8;           // workgroups are dealt to them in turn
 constexpr int kSlots = 16;         // columns of the products
 constexpr int kDealt = kSpanDealt / 64;   // rows of a lane
 constexpr int kLongest = 32;       // steps of a fitted part: what the matrix cores cut off adds up
-constexpr float kSlack = 8.0f;     // lazy raise of the running max, log2 units
-// Where running maxima start: no finite score lies below, so a row of one is never empty.
-constexpr float kLowest = -0x1.fffffep127f;
 
 // x of lanes l, l ^ 16, l ^ 32 and l ^ 48.
 __device__ inline float max_across_groups(float x) {

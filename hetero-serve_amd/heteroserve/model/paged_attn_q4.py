@@ -12,9 +12,11 @@ kv/quant.py and, if wanted, a window (paged_attn_window.py):
                         are seen; window 0: all of them
     ->                  [B, H, D]            float32
 
-The cache's values n s + lo are never written out: the products are taken with the whole
-numbers n on the matrix cores, the query and the probabilities in two fp16 terms each, and
-s and lo are applied in fp32, so the result is that of fp32 arithmetic on the values.
+The cache's values n s + lo are never written out.  The matrix cores multiply the whole
+numbers n - 8 by the query and by probability times step, each in two fp16 terms of 22
+bits that are scaled by head (and group), so what is lost is relative to the largest of
+them; the keys' steps and the values' middles lo + 8 s are applied in fp32.  The result is as near as
+fp32 arithmetic's on the values, relative to the range of their group of 32.
 A sequence without tokens gets a row of zeros.
 """
 
