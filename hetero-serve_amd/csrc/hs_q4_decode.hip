@@ -41,10 +41,11 @@
 // Waves share nothing before their states are put together, so the walk has no barriers.  Keys
 // past the part's end are read as its last one and count nothing: their scores are -inf.
 //
-// Times, D 128, 32 / 8 heads: 64 rows of 16..4096 keys, 168 MB, 56 us, of 2048 each 49, of 8192
-// each, 671 MB, 157 (4.3 TB/s; with parts of 512 keys 163, 152 of it without the arithmetic, 118
-// without the loads).  16 rows of 8k..32k, 419 MB, 103.  Loads two chunks ahead, three waves
-// a SIMD and waves' priorities gained nothing.
+// Times of a call in a graph, D 128, 32 / 8 heads: 64 rows of 16..4096 keys, 168 MB, 58 us (46 this
+// kernel), of 2048 each 51.5, of 8192 each, 671 MB, 159 (4.2 TB/s; with parts of 512 keys and
+// coarser sums 163, 152 of it without the arithmetic, 118 without the loads).  16 rows of 8k..32k, 419
+// MB, 107 (100).  Loads two chunks ahead, three waves a SIMD and waves' priorities gained
+// nothing.
 #include "hs_kernels.h"
 #include "hs_kvrows.h"
 #include "hs_q4.h"

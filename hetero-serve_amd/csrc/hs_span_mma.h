@@ -64,10 +64,11 @@ struct Task {
   // rows' last ones that are not whole, then the rows without keys: XCDs, to which
   // workgroups go in turn, have as many as each other, and long parts do not begin late.
   // Every wave finds all this by itself, in less than 1 us (which batches whose parts are few
-  // anyway do not pay), and the grid holds a.tasks: 64 rows of 16..4096 keys in tables of 32768 take
-  // 55 us (79 with a workgroup for every part of the table), of 131072 69 (187).  us, parts of 512 keys / fitted, D 128, 32 / 8 heads, 4 bits: 64 rows of
-  // 16..4096 keys 62 / 56, of 16..8192 97 / 88, of 8192 each 163 / 157, 16 of 8k..32k 117 / 103; 64 of
-  // 500..4000, D 256, 85 / 61; over bf16, 64 of 64..4096 110 / 101.
+  // anyway do not pay), and the grid holds a.tasks: 64 rows of 16..4096 keys in tables of 32768
+  // take 57.5 us (79 with a workgroup for every part of the table), of 131072 70 (187).
+  //   us, parts of 512 keys / fitted as it was added, D 128, 32 / 8 heads, 4 bits: 64 rows of 16..4096
+  // keys 62 / 56, of 16..8192 97 / 88, of 8192 each 163 / 157, 16 of 8k..32k 117 / 103; 64 of 500..4000,
+  // D 256, 85 / 61; over bf16, 64 of 64..4096 110 / 101.
   __device__ bool fit(const SpanArgs& a, int step) {
     const int lane = threadIdx.x & 63;
     int n[kDealt];                   // keys of row 64 r + lane; none behind the last row
