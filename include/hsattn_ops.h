@@ -195,7 +195,8 @@ int hs_q4_read(const void* k_cache, const void* v_cache, int NB, int BS, int Hkv
  * window 0: all of them.  What other tokens' slots hold never reaches a row,
  * infinities and NaN included.  hs_q4_decode reads a 4-bit cache, hs_window_decode
  * one of kv_dtype; scores, softmax and sums are fp32, products as near as fp32's (of
- * a 4-bit cache: relative to their group's range).
+ * a 4-bit cache: relative to their group's range), of a query's elements to 2^-22 or
+ * to 2^-35 of the largest of their head, whichever is larger.
  * A row that sees an infinity or a NaN may be NaN in the elements that it reaches.
  * A call repeated gives the same bits; how a row's sums are split, and so its last
  * bits, depends on the sizes and on the lengths of all rows.

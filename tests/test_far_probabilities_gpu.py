@@ -30,6 +30,7 @@ DEV = "cuda:0"
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 BS = 16
 SCALE = float(np.float32(math.log(2)))
+RISING = [3, 70, 140, 141, 270, 340, 500, 640], [12, 30, 41, 52, 70, 99, 110, 124]   # tokens, gaps
 RANGES = np.array([1.0, 2.0 ** -8, 2.0 ** -3, 2.0 ** -11, 1.0, 2.0 ** -6, 2.0, 2.0 ** -1])
 
 
@@ -38,11 +39,12 @@ def _f16(x):
 
 
 def _keys(rng, n, Hkv, D, odd, gap):
-    """(n, s, lo): elements of [-1/2, 1/2), and `gap` in all elements of the tokens `odd`."""
+    """(n, s, lo): elements of [-1/2, 1/2), and `gap` (one, or one for each) in all elements of the
+    tokens `odd`."""
     G = D // 32
     num = rng.integers(0, 16, (n, Hkv, G, 32))
     s, lo = np.full((n, Hkv, G), 2.0 ** -4), np.full((n, Hkv, G), -0.5)
-    num[odd], lo[odd] = 0, gap
+    num[odd], lo[odd] = 0, np.reshape(gap, (-1, 1, 1))
     return num, s, lo
 
 
@@ -100,7 +102,7 @@ def _case(kind, n, H, Hkv, D, odd, gap, size, rows, window, sinks, seed):
     for b in {0, rows // 2, rows - 1}:
         want, spread, _ = lc.decode(q[b], k[at], v[at], SCALE, sizes[0][at], sizes[1][at])
         err = np.sqrt(((got[b] - want) ** 2).reshape(H, -1, 32).mean(-1))
-        most = (abs(gap) + 4) * 2.0 ** -22 * np.sqrt((spread ** 2).reshape(H, -1, 32).mean(-1))
+        most = (np.abs(gap).max() + 4) * 2.0 ** -22 * np.sqrt((spread ** 2).reshape(H, -1, 32).mean(-1))
         assert (err <= most).all(), (b, (err / most).max(-1))
 
 
@@ -126,10 +128,12 @@ def test_huge_values_that_count_for_nothing_over_4_bits(H, Hkv, D, gap, where):
 
 @pytest.mark.parametrize("H,Hkv,D", GEOMETRIES)
 def test_maxima_that_rise_over_4_bits(H, Hkv, D):
-    """Tokens 40 log2 units above all before them, more and more of them, without values or with
-    small ones: what came before counts less and less."""
+    """Tokens 40 log2 units above the others here and there, and tokens that each lie 11 to 30 above
+    all before them, without values, with small or huge ones: what came before counts less and less."""
     for size in (0.0, 2.0 ** -8):
         _case("q4", 700, H, Hkv, D, [5, 130, 131, 400], 40, size, 2, 0, 0, D)
+    for size in (0.0, 2.0 ** -12, 2.0 ** 14):
+        _case("q4", 700, H, Hkv, D, *RISING, size, 2, 0, 0, D)
 
 
 TYPES = [F16, BF16, F32]
@@ -158,6 +162,8 @@ def test_huge_values_that_count_for_nothing_in_an_ordinary_cache(H, Hkv, D, dtyp
 def test_maxima_that_rise_in_an_ordinary_cache(H, Hkv, D, dtype):
     for size in (0.0, 2.0 ** -8):
         _case(dtype, 700, H, Hkv, D, [5, 130, 131, 400], 40, size, 2, 0, 0, D)
+    for size in (0.0, 2.0 ** -12, 2.0 ** 14):
+        _case(dtype, 700, H, Hkv, D, *RISING, size, 2, 0, 0, D)
 
 
 @pytest.mark.parametrize("H,Hkv,D", [x for x in GEOMETRIES if x[2] > 32])
