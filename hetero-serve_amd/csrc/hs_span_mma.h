@@ -249,7 +249,8 @@ inline int parts_on_chip(int B, int H, int Hkv, int heads, int side, int slots) 
 // that and they take two steps.  Longer rows are cut into parts of eight chunks, shorter ones
 // (of two steps) and fewer heads side by side while the parts are fewer than the CUs; of
 // sixteen where all waves are phases of one head and two workgroups a CU are left (64 rows of
-// 16..8192 keys, 4 bits, 16 heads over 1: 31 us, 33.5 of eight; 512 rows of 8192 168, 196).
+// 16..8192 keys, 4 bits, 16 heads over 1: 31 us, 33.5 of eight, as it was chosen, 33.3 since each group has
+// its own scale; 512 rows of 8192 168, 196).
 // Rows behind a window are as long as each other, so more of them are whole.  us, parts / whole,
 // windows of 1024: over 64 rows of 32 / 8 heads, bf16, D 128 55 / 46, D 64 33 / 25, 4 bits, D 128
 // 30 / 28; 8 heads, bf16, D 32 23.5 / 19; 8 rows of 32 heads, bf16, D 128 35 / 27.5.
